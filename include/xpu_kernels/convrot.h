@@ -216,8 +216,8 @@ int xpuint8_linear_dw_int8_stream(const void *stream, const void *dy, const int8
 int xpuint8_colquant_stream(const void *stream, const void *dy, const float *x_scale, int8_t *gq,
                             float *tg, int64_t M, int64_t N);
 
-/* The device fault words of the bounded waits (0 = none: the GEMM's, then the
- * wait probe's), read with a device synchronisation; reset != 0 clears them.
+/* The device fault words of the bounded waits (0 = none: the GEMM's, the MXFP4
+ * products', then the wait probe's), read with a device synchronisation; reset != 0 clears them.
  * A GEMM wait that gave up records its site here and the kernel returns. */
 int xpuint8_fault_status(int32_t reset);
 
@@ -295,6 +295,116 @@ int xpuint8_check_scale_math(int64_t *bad_scale, int64_t *bad_quant);
 int xpuint8_linear_noalloc_stream(const void *stream, const void *x, const int8_t *w8,
                                   const float *w_scale, const float *bias, void *out, int64_t M,
                                   int64_t N, int64_t K, int32_t activation);
+
+/* ---------------- MXFP4: 4-bit values in blocks of 32 with a power-of-two scale ----------------
+ *
+ * The OCP Microscaling format of 4 bits: a value is E2M1 (0, 0.5, 1, 1.5, 2, 3, 4, 6 and a sign),
+ * a block's scale is E8M0 (byte e stands for 2^(e - 127), 255 for NaN):
+ *   e = max(floor(log2 max|v|) - 2 + 127, 0), value = nearest E2M1 of v / 2^(e - 127), ties to the
+ *   even code, above 6 to 6.  A block that holds a NaN or an infinity gets e = 255.
+ * A matrix of R rows of K values is two buffers:
+ *   codes   [R][ceil(K / 32) * 16] bytes, the earlier value of a byte in its low half, zero past K;
+ *   scales  [ceil(R / 128)][ceil(K / 128)][32][16] bytes: row 32 j + l of a 128-row tile and its
+ *           block b at [l][4 j + b]; 0 for blocks past K, anything for rows past R.
+ * A stack of matrices has the codes of all rows after one another and whole scale tiles a matrix.
+ * `type`: 0 bf16, 1 fp16, 2 fp32.  codes, scales and the operands of products need 16-byte aligned
+ * bases, other pointers their element's alignment.  No counterpart in the reference. */
+
+/* x [rows, K] (row stride ldx elements) -> codes and scales along K, of a stack of rows /
+ * matrix_rows matrices.  With rotate (K % 256 == 0) behind the group-256 rotation, computed in 32
+ * bits and rounded to x's type; `rotated` (or NULL) then gets those values [rows, K], and codes and
+ * scales may both be NULL. */
+int xpuint8_mxfp4_quantize_stream(const void *stream, const void *x, int32_t type, int64_t ldx,
+                                  uint8_t *codes, uint8_t *scales, void *rotated, int64_t rows,
+                                  int64_t K, int64_t matrix_rows, int32_t rotate);
+
+/* Rows in the order of their experts (xpuint8_expert_sort_stream).  order NULL: x holds tokens, row
+ * t's codes go to the rows positions[t * fan ..] and its scales to the padded rows
+ * scale_rows[t * fan ..] (negative: no expert, not written).  order given (fan 1): x's rows are
+ * sorted already.  codes [rows * fan], scales of the padded rows: at most rows * fan / 128 +
+ * min(experts, rows * fan) tiles of 128. */
+int xpuint8_mxfp4_quantize_sorted_stream(const void *stream, const void *x, int32_t type,
+                                         int64_t ldx, uint8_t *codes, uint8_t *scales,
+                                         void *rotated, const int32_t *order,
+                                         const int32_t *positions, const int32_t *scale_rows,
+                                         int64_t rows, int64_t fan, int64_t K, int32_t rotate);
+
+/* x [rows, cols] -> codes and scales of x^T, along the rows: codes [cols][ceil(rows / 32) * 16] and
+ * scales of cols rows, for each of `matrices` matrices of `rows` rows after one another.  With
+ * offsets and tiles (of xpuint8_expert_sort_stream; matrices 1) the contraction is cut by expert,
+ * each expert's rows padded with zeros to whole 128-row tiles: codes [cols][max_tiles * 64]. */
+int xpuint8_mxfp4_quantize_columns_stream(const void *stream, const void *x, int32_t type,
+                                          int64_t ldx, uint8_t *codes, uint8_t *scales,
+                                          int64_t rows, int64_t cols, int64_t matrices,
+                                          const int32_t *offsets, const int32_t *tiles,
+                                          int64_t experts, int64_t max_tiles);
+
+/* The values that codes and scales stand for, out [rows, K] contiguous. */
+int xpuint8_mxfp4_dequantize_stream(const void *stream, const uint8_t *codes,
+                                    const uint8_t *scales, void *out, int32_t type, int64_t rows,
+                                    int64_t K, int64_t matrix_rows);
+
+/* out [M, N] (row stride ldo) = A B^T (+ bias [N] fp32, or NULL), A [M, K] and B [N, K] in MXFP4,
+ * summed in 32 bits and rounded once to `type`. */
+int xpuint8_mxfp4_mm_stream(const void *stream, const uint8_t *a_codes, const uint8_t *a_scales,
+                            const uint8_t *b_codes, const uint8_t *b_scales, const float *bias,
+                            void *out, int32_t type, int64_t ldo, int64_t M, int64_t N,
+                            int64_t K);
+
+/* Each expert's rows with its own B: A in sorted order (xpuint8_mxfp4_quantize_sorted_stream; max_tiles
+ * scale tiles), B a stack of `experts` matrices [N, K], out [rows, N]; rows from offsets[experts] on
+ * (of no expert) are zero. */
+int xpuint8_mxfp4_expert_mm_stream(const void *stream, const uint8_t *a_codes,
+                                   const uint8_t *a_scales, const uint8_t *b_codes,
+                                   const uint8_t *b_scales, void *out, int32_t type,
+                                   const int32_t *offsets, const int32_t *tiles, int64_t rows,
+                                   int64_t max_tiles, int64_t N, int64_t K, int64_t experts);
+
+/* One product an expert over its own rows: A [M] and B [N] rows of codes whose contraction is cut by
+ * expert (xpuint8_mxfp4_quantize_columns_stream with tiles), out [experts, M, N]; an expert without
+ * rows gets zeros. */
+int xpuint8_mxfp4_expert_dw_stream(const void *stream, const uint8_t *a_codes,
+                                   const uint8_t *a_scales, const uint8_t *b_codes,
+                                   const uint8_t *b_scales, void *out, int32_t type,
+                                   const int32_t *tiles, int64_t max_tiles, int64_t M, int64_t N,
+                                   int64_t experts);
+
+/* ---------------- experts: tokens sorted by expert and back ----------------
+ *
+ * ids [slots] (4 or 8 bytes each; a slot is a token's choice, token t's slots t * fan .. ) -> the
+ * stable order of the slots by expert, slots of no expert (an id outside [0, experts)) last:
+ * order [slots] (row -> slot), positions [slots] (slot -> row), offsets [experts + 1] (where each
+ * expert's rows begin; the last: where the rows of no expert begin), tiles [experts + 1] (the same
+ * in whole 128-row tiles), scale_rows [slots] (a slot's row among rows padded to those tiles, -1 for
+ * no expert).  At most 1024 experts.  The workspace holds xpuint8_expert_sort_workspace_bytes bytes
+ * (NULL where that is 0).  No counterpart in the reference. */
+int64_t xpuint8_expert_sort_workspace_bytes(int64_t slots, int64_t experts);
+int xpuint8_expert_sort_stream(const void *stream, const void *ids, int32_t id_bytes,
+                               int64_t slots, int64_t experts, int32_t *order,
+                               int32_t *positions, int32_t *scale_rows, int32_t *offsets,
+                               int32_t *tiles, void *workspace);
+
+/* x [tokens, width] (row stride ldx) -> out [tokens * fan, width] in sorted order; the rows of no
+ * expert are zero. */
+int xpuint8_expert_gather_stream(const void *stream, const void *x, int32_t type, int64_t ldx,
+                                 void *out, const int32_t *positions, const int32_t *scale_rows,
+                                 int64_t tokens, int64_t fan, int64_t width);
+
+/* out [tokens, width]: each token's rows (sorted order, row stride ld_rows) times its weights
+ * [tokens, fan] (NULL: 1), summed in 32 bits over the slots that an expert took.  Without weights
+ * it is the gradient of xpuint8_expert_gather_stream. */
+int xpuint8_expert_combine_stream(const void *stream, const void *rows, int32_t type,
+                                  int64_t ld_rows, const float *weights, void *out,
+                                  const int32_t *positions, const int32_t *scale_rows,
+                                  int64_t tokens, int64_t fan, int64_t width);
+
+/* The gradients of xpuint8_expert_combine_stream: grad_rows [tokens * fan, width] = weight * dy of the
+ * row's token, grad_weights [tokens, fan] = <dy, row>; zero for slots of no expert. */
+int xpuint8_expert_combine_grad_stream(const void *stream, const void *dy, int32_t type,
+                                       int64_t ld_dy, const void *rows, int64_t ld_rows,
+                                       const float *weights, void *grad_rows, float *grad_weights,
+                                       const int32_t *positions, const int32_t *scale_rows,
+                                       int64_t tokens, int64_t fan, int64_t width);
 
 #ifdef __cplusplus
 }

@@ -666,9 +666,10 @@ int xpuint8_rms_rope_stream(const void *stream, const void *x, int32_t x_is_int3
 
 int xpuint8_fault_status(int32_t reset) {
     const int g = gemm_fault_status(reset);
+    const int m = mx4_fault_status(reset);
     const int r = probe_fault_status(reset);
-    if (g < 0 || r < 0) return -1;
-    return g != 0 ? g : r;
+    if (g < 0 || m < 0 || r < 0) return -1;
+    return g != 0 ? g : m != 0 ? m : r;
 }
 
 int xpuint8_wait_probe(int64_t limit_ns, int32_t site, int64_t *elapsed_ns) {

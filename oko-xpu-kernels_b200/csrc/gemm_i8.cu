@@ -55,6 +55,7 @@
 #include "act.cuh"
 #include "common.cuh"
 #include "internal.h"
+#include "tmap.h"
 
 namespace xpuint8 {
 
@@ -629,51 +630,6 @@ __global__ void __launch_bounds__(Cfg<EPI>::kThreads, 1)
 }
 
 // -------------------------------------------------------------------------- host side
-using EncodeTiledFn = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *,
-                                   const cuuint64_t *, const cuuint64_t *, const cuuint32_t *,
-                                   const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle,
-                                   CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-EncodeTiledFn encode_fn() {
-    static EncodeTiledFn fn = nullptr;
-    static std::once_flag once;
-    std::call_once(once, [] {
-        void *p = nullptr;
-        cudaDriverEntryPointQueryResult q;
-        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) ==
-                cudaSuccess &&
-            q == cudaDriverEntryPointSuccess)
-            fn = reinterpret_cast<EncodeTiledFn>(p);
-    });
-    return fn;
-}
-
-// 2-D tensor map: `inner` contiguous elements per row, `outer` rows, row
-// stride `ld` bytes, swizzled boxes of box_inner x box_outer elements
-bool make_map(CUtensorMap *m, const void *base, uint64_t inner, uint64_t outer, uint64_t ld,
-              uint32_t box_inner, uint32_t box_outer,
-              CUtensorMapDataType dtype = CU_TENSOR_MAP_DATA_TYPE_UINT8,
-              CUtensorMapSwizzle swz = CU_TENSOR_MAP_SWIZZLE_128B) {
-    EncodeTiledFn enc = encode_fn();
-    if (!enc) {
-        set_error("cuTensorMapEncodeTiled is not available from the driver");
-        return false;
-    }
-    const cuuint64_t dims[2] = {inner, outer};
-    const cuuint64_t strides[1] = {ld};
-    const cuuint32_t box[2] = {box_inner, box_outer};
-    const cuuint32_t es[2] = {1, 1};
-    const CUresult r = enc(m, dtype, 2, const_cast<void *>(base), dims, strides, box, es,
-                           CU_TENSOR_MAP_INTERLEAVE_NONE, swz, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-    if (r != CUDA_SUCCESS) {
-        set_error("cuTensorMapEncodeTiled failed (error " + std::to_string(static_cast<int>(r)) +
-                  "): operands need 16-byte aligned bases and row strides");
-        return false;
-    }
-    return true;
-}
-
 // CTA pairs that can be resident at once for this kernel (cached per device;
 // launch_inst sets the shared-memory attribute on every launch, so a device
 // reset, which clears it, cannot leave a launch without it)

@@ -1,0 +1,1040 @@
+// MXFP4 products on the 5th-generation tensor cores (tcgen05, kind::mxf4 with block scales).
+//
+//   D[m, n] = sum over blocks b of sa[m, b] sb[n, b] sum over k in b of a[m, k] b[n, k]  (+ bias[n])
+//
+// A [M, K] and B [N, K] in MXFP4 (mx4.cuh), the sums in 32 bits, one rounding to the output's type.
+// The tensor cores multiply the codes and the scales exactly; what is rounded before the end is the
+// 32-bit running sum.
+//
+//   dense        D = A B^T
+//   rows         A's rows are grouped by expert (offsets), each expert has a B of its own
+//                (its matrices follow one another): D's rows are A's rows
+//   contraction  A and B hold all experts' contractions one after another, each padded to whole
+//                128-value tiles (tiles): D is one matrix an expert
+//
+// Two kernels.  pair_kernel: CTA pairs (one CTA an SM) walk 256 x bn output tiles, for many rows:
+// bound by the tensor cores.  few_kernel: for few rows a weight, where reading the weights counts:
+// the weight's rows are the MMA's 128 lanes and the tokens its columns, a cluster of CTAs splits
+// the contraction and adds its parts through distributed shared memory in a fixed order.
+//
+// Scales travel as stored: a TMA box of whole 512-byte tiles into shared memory, tcgen05.cp
+// (32x128b, the four-fold copy) into tensor memory: 128 rows x 4 blocks are 4 columns of 4 bytes a
+// lane.  An MMA takes 64 values of K, two blocks, whose scale bytes 0-1 or 2-3 of those columns its
+// instruction descriptor names.
+//
+// Every mbarrier wait is bounded (common.cuh: mbar_wait); on a timeout the kernel records the site
+// in g_mx4_fault, drains its own TMA loads and MMAs, frees its TMEM and returns.  No load uses
+// cluster multicast.
+#include <cuda.h>
+
+#include <algorithm>
+#include <atomic>
+#include <string>
+
+#include "internal.h"
+#include "mx4.cuh"
+#include "tmap.h"
+#include "xpu_kernels/convrot.h"
+
+namespace xpuint8 {
+
+__device__ int g_mx4_fault = 0;
+
+namespace {
+
+constexpr int kMaxExperts = 1024;
+enum Mode { kDense = 0, kRows = 1, kContraction = 2 };
+
+// -------------------------------------------------------------------- instructions and descriptors
+
+// kind::mxf4 instruction descriptor: bits 4-5 B's scale bytes (0 or 2), 7-9 and 10-11 the types
+// (1 = E2M1), 17-22 N >> 3, 23 the scales' type (1 = E8M0), 27-28 M >> 7, 29-30 A's scale bytes
+__host__ __device__ constexpr uint32_t idesc_mx4(int M, int N, int half) {
+    return (static_cast<uint32_t>(half * 2) << 4) | (1u << 7) | (1u << 10) | (static_cast<uint32_t>(N >> 3) << 17) |
+           (1u << 23) | (static_cast<uint32_t>(M >> 7) << 27) | (static_cast<uint32_t>(half * 2) << 29);
+}
+// shared-memory descriptor of a 512-byte scale tile: 32 rows of 16 bytes, no swizzle, 8-row groups
+// 128 bytes apart
+__device__ __forceinline__ uint64_t scale_desc(uint32_t saddr) {
+    return static_cast<uint64_t>((saddr & 0x3FFFFu) >> 4) | (static_cast<uint64_t>(128 >> 4) << 32) | (static_cast<uint64_t>(1) << 46);
+}
+template <int CTAS>
+__device__ __forceinline__ void copy_scales(uint32_t taddr, uint64_t desc) {
+    if constexpr (CTAS == 2) asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+    else asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+}
+template <int CTAS>
+__device__ __forceinline__ void umma_mx4(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sfa, uint32_t sfb, uint32_t accumulate) {
+    if constexpr (CTAS == 2)
+        asm volatile(
+            "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
+            "tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}\n" ::"r"(d),
+            "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
+            : "memory");
+    else
+        asm volatile(
+            "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
+            "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}\n" ::"r"(d),
+            "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
+            : "memory");
+}
+
+// bounded wait that ignores other threads' faults: only to drain this CTA's own asynchronous work
+__device__ __forceinline__ void drain_wait(uint32_t bar, uint32_t parity) {
+    const uint64_t t0 = global_timer_ns();
+    for (uint32_t it = 0; it < kWaitMaxIters; ++it) {
+        if (mbar_try_wait(bar, parity)) return;
+        if ((it & 255u) == 0u && global_timer_ns() - t0 > kWaitTimeoutNs) break;
+    }
+    atomicCAS(&g_mx4_fault, 0, 199);
+}
+
+// ------------------------------------------------------------------------------------- pair kernel
+
+constexpr int BK = 256;               // values of K a k-block: 128 bytes of codes a row
+constexpr int kCodeRow = 128;         // bytes
+constexpr int kScaleBlock = 1024;     // bytes of 128 rows' scales a k-block (two tiles)
+constexpr int kGroupM = 16;
+
+struct PairArgs {
+    void *out;
+    int64_t ldo;                      // elements
+    const float *bias;
+    int M, N;                         // of D, each matrix
+    int num_m, num_n;                 // 256-row and bn-column tiles of a matrix (dense, contraction)
+    int nk, last_steps;               // k-blocks; K = 64 steps in the last
+    int mode;
+    const int32_t *offsets, *tiles;   // experts
+    int experts;
+    int b_tiles;                      // rows: 128-row scale tiles of each expert's B
+    int64_t rows;                     // rows: D's rows, the ones of no expert among them
+    int tma_out;                      // D can be stored by the TMA unit
+    int vec_out;                      // D's rows are 16-byte aligned
+    int b_early;                      // B is not written by the kernel before this one
+};
+
+template <int BN>
+struct PairCfg {
+    static constexpr int kABytes = 128 * kCodeRow;
+    static constexpr int kBBytes = BN / 2 * kCodeRow;
+    static constexpr int kSfbBytes = BN / 128 * kScaleBlock;
+    static constexpr int kStageBytes = kABytes + kBBytes + kScaleBlock + kSfbBytes;
+    static constexpr int kStages = BN == 256 ? 5 : 7;
+    static constexpr int kEpiWarps = 8;
+    static constexpr int kThreads = 64 + 32 * kEpiWarps;
+    static constexpr int kEpiBytes = kEpiWarps * 2 * 2048;
+    static constexpr int kCumBytes = (kMaxExperts + 4) * 4;  // the experts' tiles, and up to 16 bytes
+    static constexpr int kBarAt = kStages * kStageBytes + kEpiBytes + kCumBytes;
+    static_assert(kBarAt % 16 == 0 && kStageBytes % 1024 == 0, "alignment of the barriers and tiles");
+    static constexpr size_t kSmemBytes = kBarAt + 256;
+    static_assert(kSmemBytes <= 232448, "over the 227 KB shared-memory limit of a CTA");
+    // TMEM: two accumulators and the scales of a k-block, 24 columns.  Two of 256 columns do not fit
+    // beside them, so the second begins 24 columns before the first ends; the drain of either takes
+    // the shared columns first and hands them over by themselves (OVER)
+    static constexpr int kScaleCol = 512 - 24;
+    static constexpr int kAccCol1 = BN == 256 ? kScaleCol - BN : BN;
+};
+
+struct Tile {
+    int a_row, a_sf, b_row, b_sf;  // first rows and scale tiles of A and B (the pair's)
+    int k_code, k_sf;              // first byte of a row of codes; first 4-byte word of a row of scale tiles
+    int nk, last_steps;
+    int64_t out_row;
+    int rows;                      // rows of D from out_row on that are this matrix's
+    int n0;
+};
+
+// the last i with cum[i] <= t, 0 <= i < n
+__device__ __forceinline__ int find_group(const int32_t *cum, int n, int t) {
+    int lo = 0, hi = n;
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (cum[mid] <= t) lo = mid;
+        else hi = mid;
+    }
+    return lo;
+}
+
+template <int BN>
+__device__ __forceinline__ Tile pair_tile(const PairArgs &a, const int32_t *s_cum, int tile) {
+    Tile t;
+    int mb, nb;
+    if (a.mode == kRows) {
+        const int e = find_group(s_cum, a.experts, tile / a.num_n);
+        const int local = tile - s_cum[e] * a.num_n, mt = s_cum[e + 1] - s_cum[e];
+        nb = local / mt;
+        mb = local - nb * mt;
+        const int begin = __ldg(a.offsets + e);
+        t.a_row = begin + mb * 256;
+        t.a_sf = __ldg(a.tiles + e) + mb * 2;
+        t.rows = __ldg(a.offsets + e + 1) - t.a_row;
+        t.out_row = t.a_row;
+        t.b_row = e * a.N + nb * BN;
+        t.b_sf = e * a.b_tiles + nb * (BN / 128);
+        t.k_code = t.k_sf = 0;
+        t.nk = a.nk;
+        t.last_steps = a.last_steps;
+        t.n0 = nb * BN;
+        return t;
+    }
+    int e = 0;
+    if (a.mode == kContraction) {
+        e = tile / (a.num_m * a.num_n);
+        tile -= e * a.num_m * a.num_n;
+    }
+    const int per_group = kGroupM * a.num_n;
+    const int group = tile / per_group;
+    const int first = group * kGroupM, size = min(kGroupM, a.num_m - first);
+    const int local = tile - group * per_group;
+    nb = local / size;
+    mb = first + local - nb * size;
+    t.a_row = mb * 256;
+    t.a_sf = mb * 2;
+    t.rows = a.M - t.a_row;
+    t.out_row = static_cast<int64_t>(e) * a.M + t.a_row;
+    t.b_row = nb * BN;
+    t.b_sf = nb * (BN / 128);
+    t.n0 = nb * BN;
+    if (a.mode == kContraction) {
+        const int k0 = __ldg(a.tiles + e), k1 = __ldg(a.tiles + e + 1);
+        t.k_code = k0 * 64;
+        t.k_sf = k0 * 128;
+        t.nk = (k1 - k0 + 1) / 2;
+        t.last_steps = ((k1 - k0) & 1) ? 2 : 4;
+    } else {
+        t.k_code = t.k_sf = 0;
+        t.nk = a.nk;
+        t.last_steps = a.last_steps;
+    }
+    return t;
+}
+
+// one row's 32 columns straight from registers: rows of a tile that the TMA store must not touch
+template <int T>
+__device__ __forceinline__ void store_row(const PairArgs &a, int64_t row, int n, const float (&v)[32]) {
+    uint8_t *p = static_cast<uint8_t *>(a.out) + (row * a.ldo + n) * mx_size(T);
+    if (a.vec_out && n + 32 <= a.N) {
+        if constexpr (T == kMxF32) {
+#pragma unroll
+            for (int q = 0; q < 8; ++q)
+                reinterpret_cast<uint4 *>(p)[q] = make_uint4(__float_as_uint(v[4 * q]), __float_as_uint(v[4 * q + 1]), __float_as_uint(v[4 * q + 2]), __float_as_uint(v[4 * q + 3]));
+        } else {
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+                reinterpret_cast<uint4 *>(p)[q] = make_uint4(mx_join<T>(v[8 * q], v[8 * q + 1]), mx_join<T>(v[8 * q + 2], v[8 * q + 3]), mx_join<T>(v[8 * q + 4], v[8 * q + 5]), mx_join<T>(v[8 * q + 6], v[8 * q + 7]));
+        }
+        return;
+    }
+#pragma unroll
+    for (int t = 0; t < 32; ++t)
+        if (n + t < a.N) mx_store1<T>(p, t, v[t]);
+}
+
+__device__ __forceinline__ uint32_t stage_addr(uint32_t buf, int row, int c) { return buf + row * 64 + ((c ^ ((row >> 1) & 3)) << 4); }
+
+// A CTA pair: each CTA holds 128 of the tile's 256 rows of A, half of its BN rows of B, its own
+// rows' scales and all of B's scales.
+//   warp 0     TMA producer of its CTA; both CTAs' bytes complete on the leader's FULL barrier
+//   warp 1     TMEM; in the leader the scale copies and MMAs of the pair
+//   warps 2-9  drain: TMEM lanes 32 (w % 4) .., half of the tile's columns each
+template <int BN, int T>
+__global__ void __launch_bounds__(PairCfg<BN>::kThreads, 1)
+    pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
+                const __grid_constant__ CUtensorMap tmSA, const __grid_constant__ CUtensorMap tmSB,
+                const __grid_constant__ CUtensorMap tmOut, const PairArgs args) {
+    using C = PairCfg<BN>;
+    constexpr int STAGES = C::kStages;
+    extern __shared__ __align__(1024) uint8_t smem[];
+    if (smem_u32(smem) & 1023u) {  // the 128-byte swizzle's alignment; the same in both CTAs
+        if (threadIdx.x == 0) atomicCAS(&g_mx4_fault, 0, 198);
+        return;
+    }
+    const uint32_t sA = smem_u32(smem);
+    const uint32_t sB = sA + STAGES * C::kABytes;
+    const uint32_t sSA = sB + STAGES * C::kBBytes;
+    const uint32_t sSB = sSA + STAGES * kScaleBlock;
+    const uint32_t sEpi = sSB + STAGES * C::kSfbBytes;
+    int32_t *s_cum = reinterpret_cast<int32_t *>(smem + STAGES * C::kStageBytes + C::kEpiBytes);
+    uint64_t *bars = reinterpret_cast<uint64_t *>(smem + C::kBarAt);
+    const uint32_t bar0 = smem_u32(bars);
+    auto FULL = [&](int s) { return bar0 + 8u * s; };
+    auto EMPTY = [&](int s) { return bar0 + 8u * (STAGES + s); };
+    auto TFULL = [&](int i) { return bar0 + 8u * (2 * STAGES + i); };
+    auto TEMPTY = [&](int i) { return bar0 + 8u * (2 * STAGES + 2 + i); };
+    auto OVER = [&](int i) { return bar0 + 8u * (2 * STAGES + 4 + i); };
+    const uint32_t final_bar = bar0 + 8u * (2 * STAGES + 6);
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 2 * STAGES + 7);
+    static_assert(8 * (2 * STAGES + 8) <= 256, "barriers");
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    int *fault = &g_mx4_fault;
+    const uint32_t rank = cluster_rank();
+    const bool leader = rank == 0;
+    const int pair = static_cast<int>(cluster_index()), npairs = static_cast<int>(cluster_count());
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < STAGES; ++s) {
+            mbar_init(FULL(s), 1);   // leader: its expect_tx + both CTAs' bytes
+            mbar_init(EMPTY(s), 1);  // the leader's commit
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(TFULL(i), 1);
+            mbar_init(TEMPTY(i), 2 * C::kEpiWarps);
+            mbar_init(OVER(i), C::kEpiWarps);  // the four warps of each CTA that hold the shared columns
+        }
+        mbar_init(final_bar, 1);
+        fence_mbar_init();
+        prefetch_tmap(&tmA);
+        prefetch_tmap(&tmB);
+        prefetch_tmap(&tmSA);
+        prefetch_tmap(&tmSB);
+        if (args.tma_out) prefetch_tmap(&tmOut);
+    }
+    cluster_sync();
+    if (warp == 1) {
+        tmem_alloc_pair(smem_u32(tmem_slot), 512);
+        tmem_relinquish_pair();
+    }
+    if (args.mode != kDense) pdl_wait();
+    if (args.mode == kRows && warp == 2) {
+        // s_cum[e]: 256-row tiles of the experts before e
+        int sum = 0;
+        for (int e0 = 0; e0 < args.experts; e0 += 32) {
+            const int e = e0 + lane;
+            const int v = e < args.experts ? (__ldg(args.offsets + e + 1) - __ldg(args.offsets + e) + 255) / 256 : 0;
+            int x = v;
+#pragma unroll
+            for (int d = 1; d < 32; d <<= 1) {
+                const int y = __shfl_up_sync(0xFFFFFFFFu, x, d);
+                if (lane >= d) x += y;
+            }
+            if (e < args.experts) s_cum[e] = sum + x - v;
+            sum += __shfl_sync(0xFFFFFFFFu, x, 31);
+        }
+        if (lane == 0) s_cum[args.experts] = sum;
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem_base = *tmem_slot;
+    const int num_tiles = args.mode == kRows ? s_cum[args.experts] * args.num_n
+                          : args.num_m * args.num_n * (args.mode == kContraction ? args.experts : 1);
+
+    if (warp == 0) {
+        if (lane == 0) {
+            // ------------------------------------------------ TMA producer (both CTAs)
+            int stage = 0;
+            uint32_t ph = 0, issued = 0;
+            constexpr uint32_t kTx = 2 * C::kStageBytes;
+            if (!args.b_early) pdl_wait();
+            auto load_b = [&](int st, const Tile &t, int kb) {
+                const uint32_t fb = peer_smem(FULL(st), 0);
+                tma_load_2d_pair(sB + st * C::kBBytes, &tmB, fb, t.k_code + kb * kCodeRow, t.b_row + static_cast<int>(rank) * (BN / 2));
+                tma_load_2d_pair(sSB + st * C::kSfbBytes, &tmSB, fb, t.k_sf + kb * 256, t.b_sf);
+            };
+            // b_early: the first pass over the ring takes B before the kernel before is done
+            uint32_t pre = 0;
+            if (args.b_early) {
+                int tile = pair, kb = 0;
+                for (; pre < static_cast<uint32_t>(STAGES) && tile < num_tiles; ++pre) {
+                    const Tile t = pair_tile<BN>(args, s_cum, tile);
+                    load_b(static_cast<int>(pre), t, kb);
+                    if (++kb == t.nk) { kb = 0; tile += npairs; }
+                }
+                pdl_wait();
+            }
+            bool ok = true;
+            for (int tile = pair; ok && tile < num_tiles; tile += npairs) {
+                const Tile t = pair_tile<BN>(args, s_cum, tile);
+                for (int kb = 0; kb < t.nk; ++kb) {
+                    if (!mbar_wait(EMPTY(stage), ph ^ 1u, fault, 101)) { ok = false; break; }
+                    if (leader) mbar_expect_tx(FULL(stage), kTx);
+                    const uint32_t fb = peer_smem(FULL(stage), 0);
+                    tma_load_2d_pair(sA + stage * C::kABytes, &tmA, fb, t.k_code + kb * kCodeRow, t.a_row + static_cast<int>(rank) * 128);
+                    tma_load_2d_pair(sSA + stage * kScaleBlock, &tmSA, fb, t.k_sf + kb * 256, t.a_sf + static_cast<int>(rank));
+                    if (issued >= pre) load_b(stage, t, kb);
+                    ++issued;
+                    if (++stage == STAGES) { stage = 0; ph ^= 1u; }
+                }
+            }
+            pdl_trigger();
+            // every load has landed once the MMAs that read it are done
+            for (uint32_t s = 0; s < static_cast<uint32_t>(STAGES) && s < issued; ++s) {
+                const uint32_t last = s + ((issued - 1 - s) / STAGES) * STAGES;
+                drain_wait(EMPTY(s), (last / STAGES) & 1u);
+            }
+        }
+    } else if (warp == 1) {
+        if (lane == 0 && leader) {
+            // ------------------------------------------------ scale copies and MMAs (leader)
+            constexpr uint32_t kIdesc[2] = {idesc_mx4(256, BN, 0), idesc_mx4(256, BN, 1)};
+            const uint32_t sfa = tmem_base + C::kScaleCol, sfb = sfa + 8;
+            int stage = 0, count = 0;
+            uint32_t ph = 0;
+            bool ok = true;
+            for (int tile = pair; ok && tile < num_tiles; tile += npairs) {
+                const Tile t = pair_tile<BN>(args, s_cum, tile);
+                if (t.nk == 0) continue;  // no contraction: the drain writes zeros
+                const int acc = count & 1;
+                if (!mbar_wait(TEMPTY(acc), ((count >> 1) & 1) ^ 1u, fault, 102)) break;
+                if (BN == 256 && count > 0 && !mbar_wait(OVER(acc ^ 1), ((count - 1) >> 1) & 1, fault, 103)) break;
+                tc_fence_after();
+                const uint32_t d = tmem_base + static_cast<uint32_t>(acc ? C::kAccCol1 : 0);
+                for (int kb = 0; kb < t.nk; ++kb) {
+                    if (!mbar_wait(FULL(stage), ph, fault, 104)) { ok = false; break; }
+                    tc_fence_after();
+                    const int steps = kb + 1 == t.nk ? t.last_steps : 4;
+#pragma unroll
+                    for (int kt = 0; kt < 2; ++kt) {
+                        copy_scales<2>(sfa + 4 * kt, scale_desc(sSA + stage * kScaleBlock + kt * kMxTileBytes));
+#pragma unroll
+                        for (int rt = 0; rt < BN / 128; ++rt)
+                            copy_scales<2>(sfb + kt * (BN / 32) + 4 * rt, scale_desc(sSB + stage * C::kSfbBytes + rt * kScaleBlock + kt * kMxTileBytes));
+                    }
+#pragma unroll
+                    for (int kk = 0; kk < 4; ++kk) {
+                        if (kk < steps)
+                            umma_mx4<2>(d, umma_sdesc_sw128(sA + stage * C::kABytes + kk * 32, 16, 1024),
+                                        umma_sdesc_sw128(sB + stage * C::kBBytes + kk * 32, 16, 1024), kIdesc[kk & 1],
+                                        sfa + 4 * (kk >> 1), sfb + (kk >> 1) * (BN / 32), (kb | kk) != 0 ? 1u : 0u);
+                    }
+                    umma_commit_pair(EMPTY(stage));
+                    umma_commit_pair(peer_smem(EMPTY(stage), 1));
+                    if (++stage == STAGES) { stage = 0; ph ^= 1u; }
+                }
+                if (!ok) break;
+                umma_commit_pair(TFULL(acc));
+                umma_commit_pair(peer_smem(TFULL(acc), 1));
+                ++count;
+            }
+            umma_commit_pair(final_bar);
+            drain_wait(final_bar, 0);
+        }
+    } else {
+        // ---------------------------------------------------------- drain (both CTAs)
+        const int quarter = warp & 3, half = (warp - 2) >> 2;
+        constexpr int kChunks = BN / 64;  // 32-column chunks of this warp's half
+        const uint32_t bufs = sEpi + (warp - 2) * 4096;
+        const uint32_t tempty0 = peer_smem(TEMPTY(0), 0), over0 = peer_smem(OVER(0), 0);
+        int bsel = 0, count = 0;
+        pdl_wait();
+        auto hand_over = [&](uint32_t local, uint32_t remote) {
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) {
+                if (leader) mbar_arrive(local);
+                else mbar_arrive_cluster(remote);
+            }
+        };
+        for (int tile = pair; tile < num_tiles; tile += npairs) {
+            const Tile t = pair_tile<BN>(args, s_cum, tile);
+            const int row0 = static_cast<int>(rank) * 128 + quarter * 32;  // of the tile
+            const int left = t.rows - row0;                                // rows of this warp that exist
+            const int acc = count & 1;
+            if (t.nk > 0) {
+                if (!mbar_wait(TFULL(acc), (count >> 1) & 1, fault, 105)) break;
+                tc_fence_after();
+            }
+            const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + static_cast<uint32_t>(acc ? C::kAccCol1 : 0);
+            // a whole 32-row strip (or dense, where the map ends with the matrix) leaves by TMA
+            const bool tma = args.tma_out && (args.mode == kDense || left >= 32);
+#pragma unroll 1
+            for (int i = 0; i < kChunks; ++i) {
+                // the columns that both accumulators use come first: the last of the first
+                // accumulator, the first of the second
+                const int c = half * (BN / 2) + 32 * (acc ? i : kChunks - 1 - i);
+                const int n = t.n0 + c;
+                float v[32];
+                if (t.nk > 0) {
+                    uint32_t r[32];
+                    tmem_ld32(taddr + c, r);
+                    tmem_wait_ld(r);
+                    if (BN == 256 && i == 0 && half == (acc ^ 1)) hand_over(OVER(acc), over0 + 8u * acc);
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) v[j] = 0.f;
+                }
+                if (n >= args.N || left <= 0) continue;
+                if (args.bias) {
+                    if (n + 32 <= args.N) {
+#pragma unroll
+                        for (int j = 0; j < 32; j += 4) {
+                            const float4 b = __ldg(reinterpret_cast<const float4 *>(args.bias + n + j));
+                            v[j] += b.x;
+                            v[j + 1] += b.y;
+                            v[j + 2] += b.z;
+                            v[j + 3] += b.w;
+                        }
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 32; ++j)
+                            if (n + j < args.N) v[j] += __ldg(args.bias + n + j);
+                    }
+                }
+                if (!tma) {
+                    if (lane < left) store_row<T>(args, t.out_row + row0 + lane, n, v);
+                    continue;
+                }
+                constexpr int kStores = T == kMxF32 ? 2 : 1;  // boxes of 64 bytes a row
+#pragma unroll
+                for (int h = 0; h < kStores; ++h) {
+                    if (lane == 0) bulk_wait_read<1>();  // the buffer's last store has read it
+                    __syncwarp();
+                    const uint32_t buf = bufs + bsel * 2048;
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        if constexpr (T == kMxF32)
+                            st_shared_v4(stage_addr(buf, lane, q), __float_as_uint(v[16 * h + 4 * q]), __float_as_uint(v[16 * h + 4 * q + 1]),
+                                         __float_as_uint(v[16 * h + 4 * q + 2]), __float_as_uint(v[16 * h + 4 * q + 3]));
+                        else
+                            st_shared_v4(stage_addr(buf, lane, q), mx_join<T>(v[8 * q], v[8 * q + 1]), mx_join<T>(v[8 * q + 2], v[8 * q + 3]),
+                                         mx_join<T>(v[8 * q + 4], v[8 * q + 5]), mx_join<T>(v[8 * q + 6], v[8 * q + 7]));
+                    }
+                    fence_async_smem();
+                    __syncwarp();
+                    if (lane == 0) {
+                        if (n + 16 * h < args.N || kStores == 1) tma_store_2d(&tmOut, buf, n + 16 * h, static_cast<int>(t.out_row + row0));
+                        bulk_commit();
+                    }
+                    bsel ^= 1;
+                }
+            }
+            if (t.nk > 0) {
+                hand_over(TEMPTY(acc), tempty0 + 8u * acc);
+                ++count;
+            }
+        }
+        // rows of no expert are zero
+        if (args.mode == kRows) {
+            const int64_t first = __ldg(args.offsets + args.experts);
+            const int64_t total = (args.rows - first) * args.N;
+            const int64_t step = static_cast<int64_t>(gridDim.x) * 32 * C::kEpiWarps;
+            for (int64_t i = static_cast<int64_t>(blockIdx.x) * 32 * C::kEpiWarps + threadIdx.x - 64; i < total; i += step) {
+                const int64_t r = i / args.N;
+                mx_store1<T>(args.out, (first + r) * args.ldo + (i - r * args.N), 0.f);
+            }
+        }
+        if (lane == 0) bulk_wait<0>();
+        __syncwarp();
+    }
+    tc_fence_before();
+    cluster_sync();
+    tc_fence_after();
+    if (warp == 1) tmem_dealloc_pair(tmem_base, 512);
+}
+
+// -------------------------------------------------------------------------------------- few kernel
+
+struct FewArgs {
+    void *out;
+    int64_t ldo;
+    const float *bias;
+    int M, N;                        // tokens (dense), weight rows of a matrix
+    int nk, last_steps;
+    int mode;                        // dense or rows
+    const int32_t *offsets, *tiles;
+    int experts;
+    int w_tiles;                     // 128-row scale tiles of each expert's weight
+    int64_t rows;
+    int w_early;                     // the weight is not written by the kernel before this one
+};
+
+constexpr int kFewThreads = 192;
+constexpr int kFewRing = 100 * 1024;                      // bytes of the ring: two CTAs an SM
+constexpr size_t kFewSmem = kFewRing + 1024;              // and the barriers
+constexpr int kFewMaxStages = 5;
+constexpr int kFewCols = 256;                             // TMEM columns: two CTAs an SM
+
+// One CTA: 128 rows of a weight x up to 128 tokens, over its cluster rank's share of K.
+//   warp 0     TMA producer   warp 1  TMEM, scale copies and MMAs   warps 2-5  drain
+struct FewMaps {
+    CUtensorMap x[4];  // boxes of 16, 32, 64, 128 tokens
+};
+template <int T>
+__global__ void __launch_bounds__(kFewThreads, 2)
+    few_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmSW,
+               const __grid_constant__ FewMaps tmX, const __grid_constant__ CUtensorMap tmSX, const FewArgs args) {
+    extern __shared__ __align__(1024) uint8_t smem[];
+    if (smem_u32(smem) & 1023u) {
+        if (threadIdx.x == 0) atomicCAS(&g_mx4_fault, 0, 197);
+        return;
+    }
+    uint32_t splits;
+    asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(splits));
+    const uint32_t rank = cluster_rank();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    int *fault = &g_mx4_fault;
+    const int nb = blockIdx.x / static_cast<int>(splits);
+    int e = 0, x_row, x_sf = blockIdx.y, count;
+    if (args.mode == kRows) {
+        pdl_wait();
+        const int64_t first = __ldg(args.offsets + args.experts), total = (args.rows - first) * args.N;
+        const int64_t step = static_cast<int64_t>(gridDim.x) * gridDim.y * kFewThreads;
+        for (int64_t i = (static_cast<int64_t>(blockIdx.y) * gridDim.x + blockIdx.x) * kFewThreads + threadIdx.x; i < total; i += step) {
+            const int64_t r = i / args.N;
+            mx_store1<T>(args.out, (first + r) * args.ldo + (i - r * args.N), 0.f);
+        }
+        if (x_sf >= __ldg(args.tiles + args.experts)) return;  // no rows: the cluster's CTAs all leave
+        e = find_group(args.tiles, args.experts, x_sf);
+        x_row = __ldg(args.offsets + e) + (x_sf - __ldg(args.tiles + e)) * 128;
+        count = min(128, __ldg(args.offsets + e + 1) - x_row);
+    } else {
+        x_row = x_sf * 128;
+        count = min(128, args.M - x_row);
+    }
+    const int box = count <= 16 ? 0 : count <= 32 ? 1 : count <= 64 ? 2 : 3;
+    const int nt = 16 << box;
+    const int k0 = static_cast<int>(rank) * args.nk / static_cast<int>(splits);
+    const int k1 = (static_cast<int>(rank) + 1) * args.nk / static_cast<int>(splits);
+
+    const uint32_t ring = smem_u32(smem);
+    const int w_bytes = 128 * kCodeRow, x_bytes = nt * kCodeRow;
+    const uint32_t stage_bytes = w_bytes + x_bytes + 2 * kScaleBlock;
+    const int stages = min(kFewMaxStages, static_cast<int>(kFewRing / stage_bytes));
+    uint64_t *bars = reinterpret_cast<uint64_t *>(smem + kFewRing);
+    const uint32_t bar0 = smem_u32(bars);
+    auto FULL = [&](int s) { return bar0 + 8u * s; };
+    auto EMPTY = [&](int s) { return bar0 + 8u * (kFewMaxStages + s); };
+    const uint32_t done = bar0 + 8u * (2 * kFewMaxStages);
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 2 * kFewMaxStages + 1);
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < kFewMaxStages; ++s) {
+            mbar_init(FULL(s), 1);
+            mbar_init(EMPTY(s), 1);
+        }
+        mbar_init(done, 1);
+        fence_mbar_init();
+        prefetch_tmap(&tmW);
+        prefetch_tmap(&tmSW);
+        prefetch_tmap(&tmX.x[box]);
+        prefetch_tmap(&tmSX);
+    }
+    if (warp == 1) {
+        tmem_alloc(smem_u32(tmem_slot), kFewCols);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+
+    if (warp == 0) {
+        if (lane == 0) {
+            const int w_row = e * args.N + nb * 128, w_sf = e * args.w_tiles + nb;
+            auto load_w = [&](int st, int kb) {
+                const uint32_t at = ring + st * stage_bytes;
+                tma_load_2d(at, &tmW, FULL(st), kb * kCodeRow, w_row);
+                tma_load_2d(at + w_bytes + x_bytes, &tmSW, FULL(st), kb * 256, w_sf);
+            };
+            int pre = 0;
+            if (args.mode == kDense) {
+                if (args.w_early)
+                    for (; pre < stages && k0 + pre < k1; ++pre) load_w(pre, k0 + pre);
+                pdl_wait();
+            }
+            int stage = 0;
+            uint32_t ph = 0, issued = 0;
+            for (int kb = k0; kb < k1; ++kb) {
+                if (!mbar_wait(EMPTY(stage), ph ^ 1u, fault, 111)) break;
+                mbar_expect_tx(FULL(stage), stage_bytes);
+                const uint32_t at = ring + stage * stage_bytes;
+                if (static_cast<int>(issued) >= pre) load_w(stage, kb);
+                tma_load_2d(at + w_bytes, &tmX.x[box], FULL(stage), kb * kCodeRow, x_row);
+                tma_load_2d(at + w_bytes + x_bytes + kScaleBlock, &tmSX, FULL(stage), kb * 256, x_sf);
+                ++issued;
+                if (++stage == stages) { stage = 0; ph ^= 1u; }
+            }
+            pdl_trigger();
+            const uint32_t n = static_cast<uint32_t>(stages);
+            for (uint32_t s = 0; s < n && s < issued; ++s) {
+                const uint32_t last = s + ((issued - 1 - s) / n) * n;
+                drain_wait(EMPTY(s), (last / n) & 1u);
+            }
+        }
+    } else if (warp == 1) {
+        if (lane == 0) {
+            const uint32_t idesc[2] = {idesc_mx4(128, nt, 0), idesc_mx4(128, nt, 1)};
+            const uint32_t sfa = tmem + 128, sfb = sfa + 8;
+            int stage = 0;
+            uint32_t ph = 0;
+            for (int kb = k0; kb < k1; ++kb) {
+                if (!mbar_wait(FULL(stage), ph, fault, 112)) break;
+                tc_fence_after();
+                const uint32_t at = ring + stage * stage_bytes;
+                const uint32_t sw = at + w_bytes + x_bytes, sx = sw + kScaleBlock;
+                const int steps = kb + 1 == args.nk ? args.last_steps : 4;
+#pragma unroll
+                for (int kt = 0; kt < 2; ++kt) {
+                    copy_scales<1>(sfa + 4 * kt, scale_desc(sw + kt * kMxTileBytes));
+                    copy_scales<1>(sfb + 4 * kt, scale_desc(sx + kt * kMxTileBytes));
+                }
+#pragma unroll
+                for (int kk = 0; kk < 4; ++kk) {
+                    if (kk < steps)
+                        umma_mx4<1>(tmem, umma_sdesc_sw128(at + kk * 32, 16, 1024), umma_sdesc_sw128(at + w_bytes + kk * 32, 16, 1024),
+                                    idesc[kk & 1], sfa + 4 * (kk >> 1), sfb + 4 * (kk >> 1), kb > k0 || kk > 0 ? 1u : 0u);
+                }
+                umma_commit(EMPTY(stage));
+                if (++stage == stages) { stage = 0; ph ^= 1u; }
+            }
+            umma_commit(done);
+            drain_wait(done, 0);
+        }
+    }
+    __syncthreads();  // every load has landed and every MMA is done: the ring is free
+    tc_fence_after();
+    // partial sums [token][128 rows] in this CTA's shared memory
+    float *part = reinterpret_cast<float *>(smem);
+    if (warp >= 2) {
+        const int quarter = warp & 3;
+        const uint32_t taddr = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
+        for (int c = 0; c < nt; c += 32) {
+            uint32_t r[32];
+            tmem_ld32(taddr + c, r);
+            tmem_wait_ld(r);
+#pragma unroll
+            for (int j = 0; j < 32; ++j)
+                if (c + j < count) part[(c + j) * 128 + quarter * 32 + lane] = k1 > k0 ? __uint_as_float(r[j]) : 0.f;
+        }
+    }
+    tc_fence_before();
+    if (splits > 1) cluster_sync();
+    else __syncthreads();
+    tc_fence_after();
+    if (warp == 1) tmem_dealloc(tmem, kFewCols);
+    pdl_wait();  // the output may be what the kernel before still reads
+    // this rank's share of the rows: all ranks' parts, in the order of the ranks
+    const int share = 128 / static_cast<int>(splits);
+    const uint32_t mine = smem_u32(part);
+    for (int i = threadIdx.x; i < count * share; i += kFewThreads) {
+        const int t = i / share, row = static_cast<int>(rank) * share + (i - t * share);
+        const int n = nb * 128 + row;
+        if (n >= args.N) continue;
+        float sum = 0.f;
+        for (uint32_t s = 0; s < splits; ++s) {
+            float v;
+            asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(peer_smem(mine + (t * 128 + row) * 4, s)));
+            sum = s == 0 ? v : __fadd_rn(sum, v);
+        }
+        if (args.bias) sum = __fadd_rn(sum, __ldg(args.bias + n));
+        mx_store1<T>(args.out, (x_row + t) * args.ldo + n, sum);
+    }
+    if (splits > 1) cluster_sync();  // the others have read this CTA's parts
+}
+
+// -------------------------------------------------------------------------------------------- host
+
+struct Operand {
+    const uint8_t *codes, *scales;
+    int64_t rows, K, tiles;  // rows of codes; 128-row scale tiles
+};
+
+bool code_map(CUtensorMap *m, const Operand &o, int box_rows) {
+    const int64_t bytes = (o.K + 31) / 32 * 16;
+    return make_map(m, o.codes, bytes, o.rows, bytes, kCodeRow, box_rows);
+}
+bool scale_map(CUtensorMap *m, const Operand &o, int box_tiles) {
+    const int64_t words = (o.K + 127) / 128 * 128;
+    return make_map(m, o.scales, words, o.tiles, words * 4, 256, box_tiles, CU_TENSOR_MAP_DATA_TYPE_UINT32, CU_TENSOR_MAP_SWIZZLE_NONE);
+}
+bool out_map(CUtensorMap *m, void *out, int type, int64_t rows, int64_t cols, int64_t ldo) {
+    const CUtensorMapDataType dt = type == kMxF32   ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                   : type == kMxF16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                                    : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+    return make_map(m, out, cols, rows, ldo * mx_size(type), type == kMxF32 ? 16 : 32, 32, dt, CU_TENSOR_MAP_SWIZZLE_64B);
+}
+
+template <int BN, int T>
+int resident_pairs(int dev) {
+    static std::atomic<int> cached[32] = {};
+    if (dev >= 0 && dev < 32) {
+        const int c = cached[dev].load(std::memory_order_relaxed);
+        if (c > 0) return c;
+    }
+    auto kern = pair_kernel<BN, T>;
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(PairCfg<BN>::kSmemBytes)) != cudaSuccess) return -1;
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 2;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.gridDim = dim3(2 * num_sms());
+    cfg.blockDim = dim3(PairCfg<BN>::kThreads);
+    cfg.dynamicSmemBytes = PairCfg<BN>::kSmemBytes;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    int n = 0;
+    if (cudaOccupancyMaxActiveClusters(&n, kern, &cfg) != cudaSuccess || n <= 0) return -1;
+    if (dev >= 0 && dev < 32) cached[dev].store(n, std::memory_order_relaxed);
+    return n;
+}
+
+struct PairMaps {
+    CUtensorMap a, b, sa, sb, out;
+};
+
+template <int BN, int T>
+int launch_pair(cudaStream_t s, const PairMaps &m, const PairArgs &a, int64_t tiles) {
+    int dev = 0;
+    cudaGetDevice(&dev);
+    const int resident = resident_pairs<BN, T>(dev);
+    if (resident <= 0) {
+        set_error("no CTA pair of the MXFP4 product fits on the device");
+        return 5;
+    }
+    auto kern = pair_kernel<BN, T>;
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(PairCfg<BN>::kSmemBytes)) != cudaSuccess)
+        return launch_status("mxfp4_mm (shared memory attribute)");
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 2;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.gridDim = dim3(2 * static_cast<uint32_t>(std::min<int64_t>(tiles, resident)));
+    cfg.blockDim = dim3(PairCfg<BN>::kThreads);
+    cfg.dynamicSmemBytes = PairCfg<BN>::kSmemBytes;
+    cfg.stream = s;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    cudaLaunchKernelEx(&cfg, kern, m.a, m.b, m.sa, m.sb, m.out, a);
+    return launch_status("mxfp4_mm");
+}
+
+template <int BN>
+int launch_pair_type(cudaStream_t s, const PairMaps &m, const PairArgs &a, int64_t tiles, int type) {
+    switch (type) {
+        case kMxBf16: return launch_pair<BN, kMxBf16>(s, m, a, tiles);
+        case kMxF16: return launch_pair<BN, kMxF16>(s, m, a, tiles);
+        default: return launch_pair<BN, kMxF32>(s, m, a, tiles);
+    }
+}
+
+// `a` complete but for the tile counts; max_m: 256-row tiles (rows: at most)
+int run_pair(cudaStream_t s, PairArgs a, const Operand &A, const Operand &B, int type, int64_t out_rows, int64_t max_m) {
+    // 256-column tiles where they fill the pairs; half as wide where they would leave pairs idle
+    const int64_t matrices = a.mode == kContraction ? a.experts : 1;
+    const int64_t pairs = num_sms() / 2;
+    auto cost = [&](int bn) {
+        const int64_t tiles = max_m * matrices * ((a.N + bn - 1) / bn);
+        return (tiles + pairs - 1) / pairs * (bn + 32);
+    };
+    const int bn = cost(128) < cost(256) ? 128 : 256;
+    a.num_n = (a.N + bn - 1) / bn;
+    const int64_t tiles = max_m * matrices * a.num_n;
+    if (tiles > 0x7FFFFFFF) {
+        set_error("mxfp4_mm: too many output tiles");
+        return 2;
+    }
+    const int es = mx_size(type);
+    a.vec_out = (reinterpret_cast<uintptr_t>(a.out) & 15) == 0 && (a.ldo * es) % 16 == 0;
+    a.tma_out = a.vec_out;
+    PairMaps m{};
+    if (!code_map(&m.a, A, 128) || !code_map(&m.b, B, bn / 2) || !scale_map(&m.sa, A, 1) || !scale_map(&m.sb, B, bn / 128)) return 2;
+    if (a.tma_out && !out_map(&m.out, a.out, type, out_rows, a.N, a.ldo)) return 2;
+    return bn == 256 ? launch_pair_type<256>(s, m, a, tiles, type) : launch_pair_type<128>(s, m, a, tiles, type);
+}
+
+template <int T>
+int launch_few(cudaStream_t s, const CUtensorMap &w, const CUtensorMap &sw, const FewMaps &x, const CUtensorMap &sx, const FewArgs &a, int splits, int64_t slots) {
+    auto kern = few_kernel<T>;
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kFewSmem)) != cudaSuccess)
+        return launch_status("mxfp4_mm (shared memory attribute)");
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = static_cast<uint32_t>(splits);
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.gridDim = dim3(static_cast<uint32_t>((a.N + 127) / 128 * splits), static_cast<uint32_t>(slots));
+    cfg.blockDim = dim3(kFewThreads);
+    cfg.dynamicSmemBytes = kFewSmem;
+    cfg.stream = s;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    cudaLaunchKernelEx(&cfg, kern, w, sw, x, sx, a);
+    return launch_status("mxfp4_mm");
+}
+
+// X tokens, W weight rows; slots: 128-token tiles (rows: at most)
+int run_few(cudaStream_t s, const FewArgs &a, const Operand &X, const Operand &W, int type, int64_t slots) {
+    if (slots > 65535) {
+        set_error("mxfp4_mm: too many token tiles");
+        return 2;
+    }
+    // the contraction is split while the CTAs do not fill the device twice and each part has two
+    // k-blocks at least
+    const int64_t tiles = (a.N + 127) / 128 * slots;
+    int splits = 1;
+    while (splits < 8 && tiles * splits * 2 <= 2 * num_sms() && a.nk >= splits * 4) splits *= 2;
+    CUtensorMap w, sw, sx;
+    FewMaps x{};
+    if (!code_map(&w, W, 128) || !scale_map(&sw, W, 1) || !scale_map(&sx, X, 1)) return 2;
+    for (int i = 0; i < 4; ++i)
+        if (!code_map(&x.x[i], X, 16 << i)) return 2;
+    switch (type) {
+        case kMxBf16: return launch_few<kMxBf16>(s, w, sw, x, sx, a, splits, slots);
+        case kMxF16: return launch_few<kMxF16>(s, w, sw, x, sx, a, splits, slots);
+        default: return launch_few<kMxF32>(s, w, sw, x, sx, a, splits, slots);
+    }
+}
+
+bool aligned(const void *p, int n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
+cudaStream_t as_stream(const void *s) { return static_cast<cudaStream_t>(const_cast<void *>(s)); }
+
+int check(const char *what, int32_t type, std::initializer_list<const void *> operands, const void *out, std::initializer_list<int64_t> sizes) {
+    if (type < 0 || type > 2) {
+        set_error(std::string(what) + ": the element type must be 0 (bf16), 1 (fp16) or 2 (fp32)");
+        return 2;
+    }
+    for (const void *p : operands)
+        if (!p || !aligned(p, 16)) {
+            set_error(std::string(what) + ": an operand is null or not 16-byte aligned");
+            return 2;
+        }
+    if (!out || !aligned(out, mx_size(type))) {
+        set_error(std::string(what) + ": the output is null or not aligned to its elements");
+        return 2;
+    }
+    for (int64_t n : sizes)
+        if (n <= 0 || n > 0x7FFFFF00ll) {
+            set_error(std::string(what) + ": sizes must be positive and fit in 31 bits");
+            return 2;
+        }
+    return 0;
+}
+
+void set_k(int64_t K, int &nk, int &last_steps) {
+    nk = static_cast<int>((K + BK - 1) / BK);
+    last_steps = static_cast<int>((K - static_cast<int64_t>(nk - 1) * BK + 63) / 64);
+}
+
+}  // namespace
+
+int mx4_fault_status(int reset) {
+    int v = 0;
+    if (cudaMemcpyFromSymbol(&v, g_mx4_fault, sizeof(int)) != cudaSuccess) {
+        set_error("could not read the MXFP4 product's fault word");
+        return -1;
+    }
+    if (reset && v) {
+        const int zero = 0;
+        cudaMemcpyToSymbol(g_mx4_fault, &zero, sizeof(int));
+    }
+    return v;
+}
+
+}  // namespace xpuint8
+
+using namespace xpuint8;
+
+extern "C" {
+
+int xpuint8_mxfp4_mm_stream(const void *stream, const uint8_t *a_codes, const uint8_t *a_scales,
+                            const uint8_t *b_codes, const uint8_t *b_scales, const float *bias,
+                            void *out, int32_t type, int64_t ldo, int64_t M, int64_t N,
+                            int64_t K) {
+    if (int rc = check("mxfp4_mm", type, {a_codes, a_scales, b_codes, b_scales}, out, {M, N, K})) return rc;
+    if (ldo < N || !aligned(bias, 16)) {
+        set_error("mxfp4_mm: the output's row stride must be at least N and the bias 16-byte aligned");
+        return 2;
+    }
+    const Operand A{a_codes, a_scales, M, K, (M + 127) / 128}, B{b_codes, b_scales, N, K, (N + 127) / 128};
+    if (M <= 128) {
+        FewArgs a{};
+        a.out = out;
+        a.ldo = ldo;
+        a.bias = bias;
+        a.M = static_cast<int>(M);
+        a.N = static_cast<int>(N);
+        set_k(K, a.nk, a.last_steps);
+        a.mode = kDense;
+        a.rows = M;
+        return run_few(as_stream(stream), a, A, B, type, 1);
+    }
+    PairArgs a{};
+    a.out = out;
+    a.ldo = ldo;
+    a.bias = bias;
+    a.M = static_cast<int>(M);
+    a.N = static_cast<int>(N);
+    a.num_m = static_cast<int>((M + 255) / 256);
+    set_k(K, a.nk, a.last_steps);
+    a.mode = kDense;
+    return run_pair(as_stream(stream), a, A, B, type, M, a.num_m);
+}
+
+int xpuint8_mxfp4_expert_mm_stream(const void *stream, const uint8_t *a_codes,
+                                   const uint8_t *a_scales, const uint8_t *b_codes,
+                                   const uint8_t *b_scales, void *out, int32_t type,
+                                   const int32_t *offsets, const int32_t *tiles, int64_t rows,
+                                   int64_t max_tiles, int64_t N, int64_t K, int64_t experts) {
+    if (int rc = check("mxfp4_expert_mm", type, {a_codes, a_scales, b_codes, b_scales}, out, {rows, max_tiles, N, K, experts})) return rc;
+    if (!offsets || !tiles || experts > kMaxExperts || experts * N > 0x7FFFFF00ll || max_tiles > 65535) {
+        set_error("mxfp4_expert_mm: offsets and tiles, 1 to 1024 experts, experts x N below 2^31, at most 65535 tiles");
+        return 2;
+    }
+    const Operand A{a_codes, a_scales, rows, K, max_tiles};
+    const Operand B{b_codes, b_scales, experts * N, K, experts * ((N + 127) / 128)};
+    if (rows <= experts * 64) {
+        FewArgs a{};
+        a.out = out;
+        a.ldo = N;
+        a.M = static_cast<int>(rows);
+        a.N = static_cast<int>(N);
+        set_k(K, a.nk, a.last_steps);
+        a.mode = kRows;
+        a.offsets = offsets;
+        a.tiles = tiles;
+        a.experts = static_cast<int>(experts);
+        a.w_tiles = static_cast<int>((N + 127) / 128);
+        a.rows = rows;
+        return run_few(as_stream(stream), a, A, B, type, max_tiles);
+    }
+    PairArgs a{};
+    a.out = out;
+    a.ldo = N;
+    a.M = static_cast<int>(rows);
+    a.N = static_cast<int>(N);
+    set_k(K, a.nk, a.last_steps);
+    a.mode = kRows;
+    a.offsets = offsets;
+    a.tiles = tiles;
+    a.experts = static_cast<int>(experts);
+    a.b_tiles = static_cast<int>((N + 127) / 128);
+    a.rows = rows;
+    // 256-row tiles: no more than the 128-row ones
+    const int64_t max_m = std::min(max_tiles, rows / 256 + std::min(experts, rows));
+    return run_pair(as_stream(stream), a, A, B, type, rows, max_m);
+}
+
+int xpuint8_mxfp4_expert_dw_stream(const void *stream, const uint8_t *a_codes,
+                                   const uint8_t *a_scales, const uint8_t *b_codes,
+                                   const uint8_t *b_scales, void *out, int32_t type,
+                                   const int32_t *tiles, int64_t max_tiles, int64_t M, int64_t N,
+                                   int64_t experts) {
+    if (int rc = check("mxfp4_expert_dw", type, {a_codes, a_scales, b_codes, b_scales}, out, {max_tiles, M, N, experts})) return rc;
+    if (!tiles || experts > kMaxExperts || max_tiles > 65535 || experts * M > 0x7FFFFF00ll) {
+        set_error("mxfp4_expert_dw: tiles, 1 to 1024 experts, at most 65535 tiles, experts x M below 2^31");
+        return 2;
+    }
+    const Operand A{a_codes, a_scales, M, max_tiles * 128, (M + 127) / 128};
+    const Operand B{b_codes, b_scales, N, max_tiles * 128, (N + 127) / 128};
+    PairArgs a{};
+    a.out = out;
+    a.ldo = N;
+    a.M = static_cast<int>(M);
+    a.N = static_cast<int>(N);
+    a.num_m = static_cast<int>((M + 255) / 256);
+    a.mode = kContraction;
+    a.tiles = tiles;
+    a.experts = static_cast<int>(experts);
+    return run_pair(as_stream(stream), a, A, B, type, experts * M, a.num_m);
+}
+
+}  // extern "C"

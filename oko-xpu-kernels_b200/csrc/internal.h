@@ -80,6 +80,7 @@ struct GemmCall {
 };
 int launch_gemm(cudaStream_t s, const GemmCall &c);
 int gemm_fault_status(int reset);  // device fault word of the GEMM waits
+int mx4_fault_status(int reset);   // of the MXFP4 products' waits (gemm_mx4.cu)
 
 // RMS norm + rotary embedding of attention heads (rope.cu), from bf16 heads or
 // from the int32 accumulator with its dequant

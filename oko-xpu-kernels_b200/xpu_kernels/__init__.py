@@ -58,6 +58,26 @@ from .capture import (
     prepare_for_capture,
     require_capture_ready,
 )
+from .mxfp4 import (
+    MXFP4,
+    Mxfp4Linear,
+    TrainableMxfp4Linear,
+    dequantize_mxfp4,
+    linear_mxfp4,
+    mxfp4_linear,
+    mxfp4_mm,
+    prepare_weight_mxfp4,
+    quantize_mxfp4,
+)
+from .experts import (
+    ExpertPlan,
+    expert_combine,
+    expert_ffn_mxfp4,
+    expert_gather,
+    expert_linear_mxfp4,
+    expert_sort,
+    mxfp4_expert_linear,
+)
 from . import int8
 
 __version__ = "0.4.0+b200"
@@ -71,4 +91,8 @@ __all__ = [
     "linear_dx", "linear_dx_int8", "load", "prepare_for_capture", "prepare_weight",
     "prepare_weight_fused", "quantize", "quantize_act", "quantize_row", "quantize_row_torch",
     "require_capture_ready", "rotate", "selftest", "unsupported_reason", "int8",
+    "MXFP4", "Mxfp4Linear", "TrainableMxfp4Linear", "dequantize_mxfp4", "linear_mxfp4",
+    "mxfp4_linear", "mxfp4_mm", "prepare_weight_mxfp4", "quantize_mxfp4",
+    "ExpertPlan", "expert_combine", "expert_ffn_mxfp4", "expert_gather", "expert_linear_mxfp4",
+    "expert_sort", "mxfp4_expert_linear",
 ]

@@ -94,6 +94,19 @@ def _signatures():
         "xpuint8_ipc_close": [vp],
         "xpuint8_ipc_free": [vp],
         "xpuint8_linear_noalloc_stream": [vp] * 6 + [i64] * 3 + [i32],
+        "xpuint8_mxfp4_quantize_stream": [vp, vp, i32, i64] + [vp] * 3 + [i64] * 3 + [i32],
+        "xpuint8_mxfp4_quantize_sorted_stream": [vp, vp, i32, i64] + [vp] * 6 + [i64] * 3 + [i32],
+        "xpuint8_mxfp4_quantize_columns_stream": [vp, vp, i32, i64, vp, vp] + [i64] * 3 + [vp] * 2
+                                                 + [i64] * 2,
+        "xpuint8_mxfp4_dequantize_stream": [vp] * 4 + [i32] + [i64] * 3,
+        "xpuint8_mxfp4_mm_stream": [vp] * 7 + [i32] + [i64] * 4,
+        "xpuint8_mxfp4_expert_mm_stream": [vp] * 6 + [i32, vp, vp] + [i64] * 5,
+        "xpuint8_mxfp4_expert_dw_stream": [vp] * 6 + [i32, vp] + [i64] * 4,
+        "xpuint8_expert_sort_workspace_bytes": [i64] * 2,
+        "xpuint8_expert_sort_stream": [vp, vp, i32, i64, i64] + [vp] * 6,
+        "xpuint8_expert_gather_stream": [vp, vp, i32, i64] + [vp] * 3 + [i64] * 3,
+        "xpuint8_expert_combine_stream": [vp, vp, i32, i64] + [vp] * 4 + [i64] * 3,
+        "xpuint8_expert_combine_grad_stream": [vp, vp, i32, i64, vp, i64] + [vp] * 5 + [i64] * 3,
     }
 
 
