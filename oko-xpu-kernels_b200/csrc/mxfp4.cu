@@ -10,6 +10,7 @@
 #include <cuda_runtime.h>
 
 #include <string>
+#include <type_traits>
 
 #include "internal.h"
 #include "mx4.cuh"
@@ -238,24 +239,30 @@ __global__ void __launch_bounds__(128) quantize_columns_kernel(const ColumnArgs 
     const uint32_t r0 = begin + warp * 32;
     const uint8_t *x = static_cast<const uint8_t *>(a.x) + blockIdx.z * a.matrix_stride * mx_size(T);
     float v[2][32];
-    const bool both = VEC && c + 1 < a.cols;
+    if (VEC && c + 1 < a.cols) {
+        // all loads before the first use: two columns of a 16-bit type are one word
+        using Word = typename std::conditional<T == kMxF32, float2, uint32_t>::type;
+        Word w[32];
 #pragma unroll
-    for (int i = 0; i < 32; ++i) {
-        v[0][i] = v[1][i] = 0.f;
-        if (r0 + i < end) {
-            const int64_t at = static_cast<int64_t>(r0 + i) * a.ldx + c;
-            if (both) {
-                if constexpr (T == kMxF32) {
-                    const float2 w = __ldg(reinterpret_cast<const float2 *>(x + at * 4));
-                    v[0][i] = w.x;
-                    v[1][i] = w.y;
-                } else {
-                    mx_split<T>(__ldg(reinterpret_cast<const uint32_t *>(x + at * 2)), v[0][i], v[1][i]);
-                }
+        for (int i = 0; i < 32; ++i) {
+            w[i] = Word{};
+            if (r0 + i < end) w[i] = __ldg(reinterpret_cast<const Word *>(x + (static_cast<int64_t>(r0 + i) * a.ldx + c) * mx_size(T)));
+        }
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+            if constexpr (T == kMxF32) {
+                v[0][i] = w[i].x;
+                v[1][i] = w[i].y;
             } else {
-                if (c < a.cols) v[0][i] = mx_load1<T>(x, at);
-                if (c + 1 < a.cols) v[1][i] = mx_load1<T>(x, at + 1);
+                mx_split<T>(w[i], v[0][i], v[1][i]);
             }
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+            const int64_t at = static_cast<int64_t>(r0 + i) * a.ldx + c;
+            v[0][i] = r0 + i < end && c < a.cols ? mx_load1<T>(x, at) : 0.f;
+            v[1][i] = r0 + i < end && c + 1 < a.cols ? mx_load1<T>(x, at + 1) : 0.f;
         }
     }
 #pragma unroll
