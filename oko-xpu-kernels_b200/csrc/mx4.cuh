@@ -60,10 +60,15 @@ __device__ __forceinline__ uint32_t mx_pack8(const float *v) {
         : "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]));
     return r;
 }
+// the value of a code in the low four bits: its exponent and mantissa bits at those of an fp32 number
+// are the value times 2^-126, the smallest step (0.5) a subnormal number
+__device__ __forceinline__ float mx_value(uint32_t code) {
+    return __fmul_rn(__uint_as_float(((code & 7u) << 22) | ((code & 8u) << 28)), 8.507059173023462e37f);
+}
 // the two values of a byte of codes
 __device__ __forceinline__ void mx_unpack2(uint32_t byte, float &lo, float &hi) {
     uint32_t h;
-    asm("{\n\t.reg .b8 a, z;\n\tmov.b32 {a, z, z, z}, %1;\n\tcvt.rn.f16x2.e2m1x2 %0, a;\n\t}" : "=r"(h) : "r"(byte));
+    asm("{\n\t.reg .b8 a, x, y, z;\n\tmov.b32 {a, x, y, z}, %1;\n\tcvt.rn.f16x2.e2m1x2 %0, a;\n\t}" : "=r"(h) : "r"(byte));
     asm("{\n\t.reg .f16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.f32.f16 %0, a;\n\tcvt.f32.f16 %1, b;\n\t}"
         : "=f"(lo), "=f"(hi) : "r"(h));
 }

@@ -28,150 +28,231 @@ struct RowArgs {
     uint32_t groups;             // rows * G
     uint32_t K, G, KB, KT;       // 256-groups, 32-blocks and 128-tiles of a row
     uint32_t matrix_rows;        // rows of each matrix of a stack
-    uint32_t matrix_tiles;       // its 128-row tiles
+    uint32_t matrix_tiles;       // its 128-row tiles (0: one matrix)
     const int32_t *order;        // sorted rows: row r of x is the slot order[r]
     const int32_t *positions;    // [slots] the row of codes that a slot's row goes to
     const int32_t *scale_rows;   // [slots] the row of scales; negative: no expert takes it
     uint32_t fan;                // slots of a token
 };
 
-// 16 consecutive values of a row from column c on, zero past K
+// A lane's run of 16 consecutive values of a row, as loaded: 8 words of two 16-bit values, or 16 words
+// of fp32.
+template <int T>
+struct Run {
+    static constexpr int kWords = 4 * mx_size(T);
+    uint32_t w[kWords];
+};
+
+// from column c on, zero past `cols`
 template <int T, bool VEC>
-__device__ __forceinline__ void load16(const RowArgs &a, const void *row, uint32_t c, float (&v)[16]) {
-    if (VEC && c + 16 <= a.K) {
+__device__ __forceinline__ Run<T> load_run(const void *row, uint32_t c, uint32_t cols) {
+    Run<T> r;
+    if (VEC && c + 16 <= cols) {
         const uint4 *p = reinterpret_cast<const uint4 *>(static_cast<const uint8_t *>(row) + static_cast<int64_t>(c) * mx_size(T));
+#pragma unroll
+        for (int j = 0; j < Run<T>::kWords / 4; ++j) {
+            const uint4 q = __ldg(p + j);
+            r.w[4 * j] = q.x;
+            r.w[4 * j + 1] = q.y;
+            r.w[4 * j + 2] = q.z;
+            r.w[4 * j + 3] = q.w;
+        }
+    } else if constexpr (T == kMxF32) {
+#pragma unroll
+        for (int t = 0; t < 16; ++t) r.w[t] = c + t < cols ? __ldg(static_cast<const uint32_t *>(row) + c + t) : 0u;
+    } else {
+#pragma unroll
+        for (int t = 0; t < 8; ++t) {
+            const uint32_t lo = c + 2 * t < cols ? __ldg(static_cast<const uint16_t *>(row) + c + 2 * t) : 0u;
+            const uint32_t hi = c + 2 * t + 1 < cols ? __ldg(static_cast<const uint16_t *>(row) + c + 2 * t + 1) : 0u;
+            r.w[t] = lo | (hi << 16);
+        }
+    }
+    return r;
+}
+template <int T>
+__device__ __forceinline__ Run<T> zero_run() {
+    Run<T> r;
+#pragma unroll
+    for (int j = 0; j < Run<T>::kWords; ++j) r.w[j] = 0u;
+    return r;
+}
+
+// per half, the maximum of two unsigned 16-bit values
+__device__ __forceinline__ uint32_t max_u16x2(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("max.u16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+}
+// the fp32 bits of a 16-bit magnitude
+template <int T>
+__device__ __forceinline__ uint32_t widen_bits(uint32_t h) {
+    if constexpr (T == kMxBf16) return h << 16;
+    float lo, hi;
+    mx_split<T>(h, lo, hi);
+    return __float_as_uint(lo);
+}
+
+// the pair (v0, v1) times (s0, s1)
+__device__ __forceinline__ void scale2(float &v0, float &v1, f2 s) { un2(mul2(mk2(v0, v1), s), v0, v1); }
+
+// Codes of a lane's 16 values, its neighbour (lane ^ 1) holding the block's other 16: 8 bytes, and
+// the block's scale byte.
+template <int T>
+__device__ __forceinline__ uint2 quantize_run(const Run<T> &r, uint32_t &e) {
+    uint32_t m = 0;
+    if constexpr (T == kMxF32) {
+#pragma unroll
+        for (int t = 0; t < 16; ++t) m = max(m, r.w[t] & 0x7FFFFFFFu);
+        m = max(m, __shfl_xor_sync(0xFFFFFFFFu, m, 1));
+    } else {
+#pragma unroll
+        for (int t = 0; t < 8; ++t) m = max_u16x2(m, r.w[t] & 0x7FFF7FFFu);
+        m = max_u16x2(m, __shfl_xor_sync(0xFFFFFFFFu, m, 1));
+        m = widen_bits<T>(max(m & 0xFFFFu, m >> 16));
+    }
+    e = mx_exponent(m);
+    const float inv = mx_inverse(e);
+    const f2 s = mk2(inv, inv);
+    float v[16];
+#pragma unroll
+    for (int t = 0; t < 8; ++t) {
         if constexpr (T == kMxF32) {
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const uint4 w = __ldg(p + j);
-                v[4 * j] = __uint_as_float(w.x);
-                v[4 * j + 1] = __uint_as_float(w.y);
-                v[4 * j + 2] = __uint_as_float(w.z);
-                v[4 * j + 3] = __uint_as_float(w.w);
-            }
+            v[2 * t] = __uint_as_float(r.w[2 * t]);
+            v[2 * t + 1] = __uint_as_float(r.w[2 * t + 1]);
         } else {
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                const uint4 w = __ldg(p + j);
-                mx_split<T>(w.x, v[8 * j], v[8 * j + 1]);
-                mx_split<T>(w.y, v[8 * j + 2], v[8 * j + 3]);
-                mx_split<T>(w.z, v[8 * j + 4], v[8 * j + 5]);
-                mx_split<T>(w.w, v[8 * j + 6], v[8 * j + 7]);
-            }
+            mx_split<T>(r.w[t], v[2 * t], v[2 * t + 1]);
         }
-        return;
+        scale2(v[2 * t], v[2 * t + 1], s);
     }
-#pragma unroll
-    for (int t = 0; t < 16; ++t) v[t] = c + t < a.K ? mx_load1<T>(row, c + t) : 0.f;
+    return make_uint2(mx_pack8(v), mx_pack8(v + 8));
 }
 
-template <int T>
-__device__ __forceinline__ void store16(void *row, uint32_t c, const float (&v)[16]) {
-    uint4 *p = reinterpret_cast<uint4 *>(static_cast<uint8_t *>(row) + static_cast<int64_t>(c) * mx_size(T));
-    if constexpr (T == kMxF32) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-            p[j] = make_uint4(__float_as_uint(v[4 * j]), __float_as_uint(v[4 * j + 1]),
-                              __float_as_uint(v[4 * j + 2]), __float_as_uint(v[4 * j + 3]));
-    } else {
-#pragma unroll
-        for (int j = 0; j < 2; ++j)
-            p[j] = make_uint4(mx_join<T>(v[8 * j], v[8 * j + 1]), mx_join<T>(v[8 * j + 2], v[8 * j + 3]),
-                              mx_join<T>(v[8 * j + 4], v[8 * j + 5]), mx_join<T>(v[8 * j + 6], v[8 * j + 7]));
-    }
+// Lanes 0, 2, 4, 6 (8, 10, 12, 14) of a half-warp hold the scale bytes of a tile's four blocks: the
+// word of them, on lanes 0 and 8.
+__device__ __forceinline__ uint32_t join_scales(uint32_t e) {
+    const uint32_t two = e | (__shfl_down_sync(0xFFFFFFFFu, e, 2) << 8);
+    return two | (__shfl_down_sync(0xFFFFFFFFu, two, 4) << 16);
 }
 
-// The rotated pair P[w] = (A[16 w + l], B[16 w + l]) (x16), scaled, rounded to the type, and
-// turned so that lane l holds values 16 l .. 16 l + 15 of both groups.
+// A pair of 256-value groups A and B on a half-warp's lanes, turned to pairs: value c of both at
+// pair_at(c) of the slot's shared memory, as a word (16-bit types) or two (fp32).  The pitches put
+// the words of a column and those of a run into different banks, with every address a base and a
+// constant.
+constexpr int kSlotBytes = 16 * 144;
 template <int T>
-__device__ __forceinline__ void settle_pair(f2 (&P)[16], uint32_t tile, int l, float (&A)[16], float (&B)[16]) {
-    if constexpr (T == kMxF32) {
-        // 8-byte words, row w of 128 bytes, 16-byte chunk c at c ^ (w & 7)
+__device__ __forceinline__ constexpr uint32_t pair_at(int w, int l) { return T == kMxF32 ? w * 144 + l * 8 : w * 80 + l * 4; }
+
+// The rotation of the pair, scaled and rounded to the type, left in shared memory.  Lane l brings
+// values 16 l .. 16 l + 15 of both groups: two radix-4 steps in registers (accumulation chains), the
+// turn through shared memory, two more (butterflies): the association of rotate(), so the same bits.
+template <int T>
+__device__ __forceinline__ void rotate_to_shared(const Run<T> &A, const Run<T> &B, uint32_t slot, int l) {
+    f2 P[16];
 #pragma unroll
-        for (int w = 0; w < 16; ++w) {
-            const f2 s = mul2(P[w], mk2(0.0625f, 0.0625f));
-            asm volatile("st.shared.b64 [%0], %1;" ::"r"(tile + w * 128 + ((((l >> 1) ^ w) & 7) << 4) + ((l & 1) << 3)), "l"(s.v) : "memory");
+    for (int t = 0; t < 8; ++t) {
+        float a0, a1, b0, b1;
+        if constexpr (T == kMxF32) {
+            a0 = __uint_as_float(A.w[2 * t]);
+            a1 = __uint_as_float(A.w[2 * t + 1]);
+            b0 = __uint_as_float(B.w[2 * t]);
+            b1 = __uint_as_float(B.w[2 * t + 1]);
+        } else {
+            mx_split<T>(A.w[t], a0, a1);
+            mx_split<T>(B.w[t], b0, b1);
         }
-        __syncwarp();
+        P[2 * t] = mk2(a0, b0);
+        P[2 * t + 1] = mk2(a1, b1);
+    }
 #pragma unroll
-        for (int c = 0; c < 8; ++c) {
-            uint32_t x, y, z, u;
-            asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(x), "=r"(y), "=r"(z), "=r"(u) : "r"(tile + l * 128 + ((c ^ (l & 7)) << 4)));
-            A[2 * c] = __uint_as_float(x);
-            B[2 * c] = __uint_as_float(y);
-            A[2 * c + 1] = __uint_as_float(z);
-            B[2 * c + 1] = __uint_as_float(u);
-        }
-    } else {
-        // 4-byte words (A, B), row w of 64 bytes, 16-byte chunk c at c ^ ((w >> 1) & 3)
+    for (int j = 0; j < 4; ++j) seq2(P[4 * j], P[4 * j + 1], P[4 * j + 2], P[4 * j + 3]);
 #pragma unroll
-        for (int w = 0; w < 16; ++w) {
+    for (int j = 0; j < 4; ++j) seq2(P[j], P[j + 4], P[j + 8], P[j + 12]);
+    const uint32_t mine = slot + l * 144, column = slot + l * 8;
+#pragma unroll
+    for (int c = 0; c < 8; ++c)
+        asm volatile("st.shared.v2.b64 [%0], {%1, %2};" ::"r"(mine + c * 16), "l"(P[2 * c].v), "l"(P[2 * c + 1].v) : "memory");
+    __syncwarp();
+#pragma unroll
+    for (int w = 0; w < 16; ++w) asm volatile("ld.shared.b64 %0, [%1];" : "=l"(P[w].v) : "r"(column + w * 144));
+    __syncwarp();
+#pragma unroll
+    for (int j = 0; j < 4; ++j) bfly2(P[4 * j], P[4 * j + 1], P[4 * j + 2], P[4 * j + 3]);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) bfly2(P[j], P[j + 4], P[j + 8], P[j + 12]);
+#pragma unroll
+    for (int w = 0; w < 16; ++w) {
+        const f2 s = mul2(P[w], mk2(0.0625f, 0.0625f));
+        if constexpr (T == kMxF32) {
+            asm volatile("st.shared.b64 [%0], %1;" ::"r"(slot + pair_at<T>(w, 0) + l * 8), "l"(s.v) : "memory");
+        } else {
             float p, q;
-            un2(mul2(P[w], mk2(0.0625f, 0.0625f)), p, q);
-            asm volatile("st.shared.b32 [%0], %1;" ::"r"(tile + w * 64 + (((l >> 2) ^ ((w >> 1) & 3)) << 4) + ((l & 3) << 2)), "r"(mx_join<T>(p, q)) : "memory");
+            un2(s, p, q);
+            asm volatile("st.shared.b32 [%0], %1;" ::"r"(slot + pair_at<T>(w, 0) + l * 4), "r"(mx_join<T>(p, q)) : "memory");
         }
-        __syncwarp();
+    }
+    __syncwarp();
+}
+
+// both runs of lane l back from the pairs
+template <int T>
+__device__ __forceinline__ void runs_from_shared(Run<T> &A, Run<T> &B, uint32_t slot, int l) {
+    const uint32_t at = slot + pair_at<T>(1, 0) * l;
+    if constexpr (T == kMxF32) {
+#pragma unroll
+        for (int c = 0; c < 8; ++c)
+            asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(A.w[2 * c]), "=r"(B.w[2 * c]), "=r"(A.w[2 * c + 1]), "=r"(B.w[2 * c + 1]) : "r"(at + c * 16));
+    } else {
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
             uint32_t w[4];
-            asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(tile + l * 64 + ((c ^ ((l >> 1) & 3)) << 4)));
-#pragma unroll
-            for (int t = 0; t < 4; ++t) mx_split<T>(w[t], A[4 * c + t], B[4 * c + t]);
+            asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(at + c * 16));
+            A.w[2 * c] = __byte_perm(w[0], w[1], 0x5410);
+            B.w[2 * c] = __byte_perm(w[0], w[1], 0x7632);
+            A.w[2 * c + 1] = __byte_perm(w[2], w[3], 0x5410);
+            B.w[2 * c + 1] = __byte_perm(w[2], w[3], 0x7632);
         }
     }
 }
 
-// 16 values of this lane and the 16 of its neighbour (lane ^ 1) are a block: its codes (8 bytes a
-// lane) and, on lanes 0 and 8 of the half-warp, the word of four scales that starts there.
-__device__ __forceinline__ void quantize16(const float (&v)[16], int l, uint2 &code, uint32_t &word) {
-    uint32_t m = 0;
+template <int T>
+__device__ __forceinline__ void store_run(void *row, uint32_t c, const Run<T> &r) {
+    uint4 *p = reinterpret_cast<uint4 *>(static_cast<uint8_t *>(row) + static_cast<int64_t>(c) * mx_size(T));
 #pragma unroll
-    for (int t = 0; t < 16; ++t) m = max(m, __float_as_uint(v[t]) & 0x7FFFFFFFu);
-    m = max(m, __shfl_xor_sync(0xFFFFFFFFu, m, 1));
-    const uint32_t e = mx_exponent(m);
-    const float inv = mx_inverse(e);
-    float s[16];
-#pragma unroll
-    for (int t = 0; t < 16; ++t) s[t] = __fmul_rn(v[t], inv);
-    code = make_uint2(mx_pack8(s), mx_pack8(s + 8));
-    // lanes 0, 2, 4, 6 (8, 10, 12, 14) hold the bytes of a word
-    const uint32_t two = e | (__shfl_down_sync(0xFFFFFFFFu, e, 2) << 8);
-    word = two | (__shfl_down_sync(0xFFFFFFFFu, two, 4) << 16);
+    for (int j = 0; j < Run<T>::kWords / 4; ++j) p[j] = make_uint4(r.w[4 * j], r.w[4 * j + 1], r.w[4 * j + 2], r.w[4 * j + 3]);
 }
 
 // One half-warp ("slot") quantizes a pair of 256-value groups: a lane holds 16 consecutive values
 // of each, so a block of 32 is two lanes, codes leave as 8 bytes a lane (128 consecutive bytes a
-// group) and scales as one 4-byte word a 128-wide tile.
+// group) and scales as one 4-byte word a 128-wide tile.  Instructions bound it before memory does:
+// 16-bit values stay packed up to the conversion (the maximum is an integer one of two at a time),
+// the rotation and the scaling are packed fp32x2.
 template <int T, bool ROT, bool VEC>
 __global__ void __launch_bounds__(128) quantize_rows_kernel(const RowArgs a) {
-    __shared__ __align__(128) uint8_t tiles[ROT ? 8 * 2048 : 16];
+    __shared__ __align__(128) uint8_t tiles[ROT ? 8 * kSlotBytes : 16];
     const int slot = threadIdx.x >> 4, l = threadIdx.x & 15;
     const uint32_t f0 = (blockIdx.x * 8u + slot) * 2u;
     const uint32_t r0 = f0 / a.G, g0 = f0 - r0 * a.G;
     const uint32_t r1 = g0 + 1 == a.G ? r0 + 1 : r0, g1 = g0 + 1 == a.G ? 0 : g0 + 1;
     const bool ok0 = f0 < a.groups, ok1 = f0 + 1 < a.groups;
     const uint8_t *base = static_cast<const uint8_t *>(a.x);
-    float A[16] = {}, B[16] = {};
-    if (ok0) load16<T, VEC>(a, base + r0 * a.ldx * mx_size(T), g0 * 256 + l * 16, A);
-    if (ok1) load16<T, VEC>(a, base + r1 * a.ldx * mx_size(T), g1 * 256 + l * 16, B);
+    Run<T> A = zero_run<T>(), B = zero_run<T>();
+    if (ok0) A = load_run<T, VEC>(base + r0 * a.ldx * mx_size(T), g0 * 256 + l * 16, a.K);
+    if (ok1) B = load_run<T, VEC>(base + r1 * a.ldx * mx_size(T), g1 * 256 + l * 16, a.K);
     if constexpr (ROT) {
-        f2 P[16];
-#pragma unroll
-        for (int t = 0; t < 16; ++t) P[t] = mk2(A[t], B[t]);
-        const uint32_t tile = smem_u32(tiles) + slot * 2048;
-        rotate_pair(P, tile, l);
-        settle_pair<T>(P, tile, l, A, B);
+        const uint32_t tile = smem_u32(tiles) + slot * kSlotBytes;
+        rotate_to_shared<T>(A, B, tile, l);
+        runs_from_shared<T>(A, B, tile, l);
         if (a.rotated) {
             uint8_t *out = static_cast<uint8_t *>(a.rotated);
-            if (ok0) store16<T>(out + static_cast<int64_t>(r0) * a.K * mx_size(T), g0 * 256 + l * 16, A);
-            if (ok1) store16<T>(out + static_cast<int64_t>(r1) * a.K * mx_size(T), g1 * 256 + l * 16, B);
+            if (ok0) store_run<T>(out + static_cast<int64_t>(r0) * a.K * mx_size(T), g0 * 256 + l * 16, A);
+            if (ok1) store_run<T>(out + static_cast<int64_t>(r1) * a.K * mx_size(T), g1 * 256 + l * 16, B);
         }
         if (!a.codes) return;
     }
-    uint2 c0, c1;
-    uint32_t w0, w1;
-    quantize16(A, l, c0, w0);
-    quantize16(B, l, c1, w1);
+    uint32_t e0, e1;
+    const uint2 c0 = quantize_run<T>(A, e0), c1 = quantize_run<T>(B, e1);
+    const uint32_t w0 = join_scales(e0), w1 = join_scales(e1);
     auto put = [&](uint32_t r, uint32_t g, const uint2 &code, uint32_t word) {
         const uint32_t c = g * 256 + l * 16, kt = g * 2 + (l >> 3);
         const bool has_code = c < a.KB * 32, has_word = (l & 7) == 0 && kt < a.KT;
@@ -182,6 +263,8 @@ __global__ void __launch_bounds__(128) quantize_rows_kernel(const RowArgs a) {
                 sr = __ldg(a.scale_rows + at);
                 if (sr < 0) continue;
                 if (!a.order) cr = __ldg(a.positions + at);
+            } else if (a.matrix_tiles == 0) {
+                sr = r;
             } else {
                 const uint32_t b = r / a.matrix_rows;
                 sr = static_cast<int64_t>(b) * a.matrix_tiles * 128 + (r - b * a.matrix_rows);
@@ -238,46 +321,67 @@ __global__ void __launch_bounds__(128) quantize_columns_kernel(const ColumnArgs 
     const uint32_t c = blockIdx.x * 64 + lane * 2;
     const uint32_t r0 = begin + warp * 32;
     const uint8_t *x = static_cast<const uint8_t *>(a.x) + blockIdx.z * a.matrix_stride * mx_size(T);
-    float v[2][32];
+    // all loads before the first use; the two columns of a 16-bit type are one word
+    using Word = typename std::conditional<T == kMxF32, float2, uint32_t>::type;
+    Word w[32];
     if (VEC && c + 1 < a.cols) {
-        // all loads before the first use: two columns of a 16-bit type are one word
-        using Word = typename std::conditional<T == kMxF32, float2, uint32_t>::type;
-        Word w[32];
 #pragma unroll
         for (int i = 0; i < 32; ++i) {
             w[i] = Word{};
             if (r0 + i < end) w[i] = __ldg(reinterpret_cast<const Word *>(x + (static_cast<int64_t>(r0 + i) * a.ldx + c) * mx_size(T)));
         }
-#pragma unroll
-        for (int i = 0; i < 32; ++i) {
-            if constexpr (T == kMxF32) {
-                v[0][i] = w[i].x;
-                v[1][i] = w[i].y;
-            } else {
-                mx_split<T>(w[i], v[0][i], v[1][i]);
-            }
-        }
     } else {
 #pragma unroll
         for (int i = 0; i < 32; ++i) {
             const int64_t at = static_cast<int64_t>(r0 + i) * a.ldx + c;
-            v[0][i] = r0 + i < end && c < a.cols ? mx_load1<T>(x, at) : 0.f;
-            v[1][i] = r0 + i < end && c + 1 < a.cols ? mx_load1<T>(x, at + 1) : 0.f;
+            const bool in0 = r0 + i < end && c < a.cols, in1 = r0 + i < end && c + 1 < a.cols;
+            if constexpr (T == kMxF32) {
+                const float *p = reinterpret_cast<const float *>(x);
+                w[i] = make_float2(in0 ? __ldg(p + at) : 0.f, in1 ? __ldg(p + at + 1) : 0.f);
+            } else {
+                const uint16_t *p = reinterpret_cast<const uint16_t *>(x);
+                w[i] = (in0 ? __ldg(p + at) : 0u) | (static_cast<uint32_t>(in1 ? __ldg(p + at + 1) : 0u) << 16);
+            }
         }
     }
+    uint32_t m0 = 0, m1 = 0;
+    if constexpr (T == kMxF32) {
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
+        for (int i = 0; i < 32; ++i) {
+            m0 = max(m0, __float_as_uint(w[i].x) & 0x7FFFFFFFu);
+            m1 = max(m1, __float_as_uint(w[i].y) & 0x7FFFFFFFu);
+        }
+    } else {
         uint32_t m = 0;
 #pragma unroll
-        for (int i = 0; i < 32; ++i) m = max(m, __float_as_uint(v[h][i]) & 0x7FFFFFFFu);
-        const uint32_t e = mx_exponent(m);
-        const float inv = mx_inverse(e);
-#pragma unroll
-        for (int i = 0; i < 32; ++i) v[h][i] = __fmul_rn(v[h][i], inv);
-        uint4 code = make_uint4(mx_pack8(v[h]), mx_pack8(v[h] + 8), mx_pack8(v[h] + 16), mx_pack8(v[h] + 24));
-        *reinterpret_cast<uint4 *>(&s_code[lane * 2 + h][warp * 4]) = code;
-        s_scale[lane * 2 + h][warp] = static_cast<uint8_t>(e);
+        for (int i = 0; i < 32; ++i) m = max_u16x2(m, w[i] & 0x7FFF7FFFu);
+        m0 = widen_bits<T>(m & 0xFFFFu);
+        m1 = widen_bits<T>(m >> 16);
     }
+    const uint32_t e0 = mx_exponent(m0), e1 = mx_exponent(m1);
+    const f2 inv = mk2(mx_inverse(e0), mx_inverse(e1));
+    uint32_t code[2][4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+        float v0[8], v1[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            if constexpr (T == kMxF32) {
+                v0[i] = w[8 * q + i].x;
+                v1[i] = w[8 * q + i].y;
+            } else {
+                mx_split<T>(w[8 * q + i], v0[i], v1[i]);
+            }
+            scale2(v0[i], v1[i], inv);
+        }
+        code[0][q] = mx_pack8(v0);
+        code[1][q] = mx_pack8(v1);
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+        *reinterpret_cast<uint4 *>(&s_code[lane * 2 + h][warp * 4]) = make_uint4(code[h][0], code[h][1], code[h][2], code[h][3]);
+    s_scale[lane * 2][warp] = static_cast<uint8_t>(e0);
+    s_scale[lane * 2 + 1][warp] = static_cast<uint8_t>(e1);
     __syncthreads();
     uint8_t *codes = a.codes + blockIdx.z * a.matrix_codes;
     uint8_t *scales = a.scales + blockIdx.z * a.matrix_scales;
@@ -298,38 +402,58 @@ __global__ void __launch_bounds__(128) quantize_columns_kernel(const ColumnArgs 
 struct ValueArgs {
     const uint8_t *codes, *scales;
     void *out;
-    uint32_t K, KB, KT, halves;  // halves: runs of 16 values of a row
-    int64_t total;               // rows * halves
+    uint32_t K, KB, KT, units;  // units: of a row, runs of 16 values or of eight blocks
+    int64_t total;              // rows * units
     uint32_t matrix_rows, matrix_tiles;
 };
 
-// 16 values a thread: 8 bytes of codes, a scale byte, 32 (64) bytes out
-template <int T, bool VEC>
+// Rows that are 16-byte aligned: 16 values a thread, 8 bytes of codes, a scale byte, 32 (64) bytes out.
+template <int T>
 __global__ void __launch_bounds__(256) values_kernel(const ValueArgs a) {
     const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
     if (i >= a.total) return;
-    const int64_t r = i / a.halves;
-    const uint32_t h = static_cast<uint32_t>(i - r * a.halves);
+    const int64_t r = i / a.units;
+    const uint32_t h = static_cast<uint32_t>(i - r * a.units);
     const int64_t b = r / a.matrix_rows;
     const int64_t sr = b * a.matrix_tiles * 128 + (r - b * a.matrix_rows);
     const uint2 code = __ldg(reinterpret_cast<const uint2 *>(a.codes + r * a.KB * 16 + h * 8));
     const float s = mx_scale(__ldg(a.scales + mx_scale_word(sr, h >> 3, a.KT) + ((h >> 1) & 3)));
-    float v[16];
+    Run<T> out;
 #pragma unroll
     for (int t = 0; t < 8; ++t) {
-        const uint32_t w = t < 4 ? code.x : code.y;
-        mx_unpack2((w >> (8 * (t & 3))) & 0xFFu, v[2 * t], v[2 * t + 1]);
-        v[2 * t] = __fmul_rn(v[2 * t], s);
-        v[2 * t + 1] = __fmul_rn(v[2 * t + 1], s);
+        float v0, v1;
+        mx_unpack2(((t < 4 ? code.x : code.y) >> (8 * (t & 3))) & 0xFFu, v0, v1);
+        scale2(v0, v1, mk2(s, s));
+        if constexpr (T == kMxF32) {
+            out.w[2 * t] = __float_as_uint(v0);
+            out.w[2 * t + 1] = __float_as_uint(v1);
+        } else {
+            out.w[t] = mx_join<T>(v0, v1);
+        }
     }
-    uint8_t *row = static_cast<uint8_t *>(a.out) + r * a.K * mx_size(T);
-    const uint32_t c = h * 16;
-    if (VEC && c + 16 <= a.K) {
-        store16<T>(row, c, v);
-    } else {
+    store_run<T>(static_cast<uint8_t *>(a.out) + r * a.K * mx_size(T), h * 16, out);
+}
+
+// Rows of any length: a warp reads eight blocks of a row one after another, a value a lane, so that
+// neighbouring lanes write neighbouring values.
+template <int T>
+__global__ void __launch_bounds__(256) odd_values_kernel(const ValueArgs a) {
+    const int64_t i = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
+    const int lane = threadIdx.x & 31;
+    if (i >= a.total) return;
+    const int64_t r = i / a.units;
+    const uint32_t b0 = static_cast<uint32_t>(i - r * a.units) * 8;
+    const int64_t m = r / a.matrix_rows;
+    const int64_t sr = m * a.matrix_tiles * 128 + (r - m * a.matrix_rows);
+    const uint8_t *codes = a.codes + r * a.KB * 16;
 #pragma unroll
-        for (int t = 0; t < 16; ++t)
-            if (c + t < a.K) mx_store1<T>(row, c + t, v[t]);
+    for (int j = 0; j < 8; ++j) {
+        const uint32_t b = b0 + j, c = b * 32 + lane;
+        if (c < a.K) {
+            const uint32_t byte = __ldg(codes + c / 2), code = lane & 1 ? byte >> 4 : byte & 15u;
+            const float s = mx_scale(__ldg(a.scales + mx_scale_word(sr, b >> 2, a.KT) + (b & 3)));
+            mx_store1<T>(a.out, r * a.K + c, __fmul_rn(mx_value(code), s));
+        }
     }
 }
 
@@ -440,7 +564,7 @@ int xpuint8_mxfp4_quantize_stream(const void *stream, const void *x, int32_t typ
     a.scales = scales;
     a.rotated = rotated;
     a.matrix_rows = static_cast<uint32_t>(matrix_rows);
-    a.matrix_tiles = static_cast<uint32_t>((matrix_rows + 127) / 128);
+    a.matrix_tiles = matrix_rows == rows ? 0 : static_cast<uint32_t>((matrix_rows + 127) / 128);
     a.fan = 1;
     return quantize_rows(as_stream(stream), a, type, rows, K, ldx, rotate != 0);
 }
@@ -538,25 +662,25 @@ int xpuint8_mxfp4_dequantize_stream(const void *stream, const uint8_t *codes,
     a.K = static_cast<uint32_t>(K);
     a.KB = static_cast<uint32_t>((K + 31) / 32);
     a.KT = (a.KB + 3) / 4;
-    a.halves = static_cast<uint32_t>((K + 15) / 16);
-    a.total = rows * a.halves;
     a.matrix_rows = static_cast<uint32_t>(matrix_rows);
     a.matrix_tiles = static_cast<uint32_t>((matrix_rows + 127) / 128);
-    const int64_t blocks = (a.total + 255) / 256;
+    const bool vec = aligned(out, 16) && (K * mx_size(type)) % 16 == 0 && K % 16 == 0;
+    a.units = static_cast<uint32_t>(vec ? K / 16 : (K + 255) / 256);
+    a.total = rows * a.units;
+    const int64_t blocks = vec ? (a.total + 255) / 256 : (a.total + 7) / 8;
     if (blocks > 0x7FFFFFFFll) {
         set_error("mxfp4: too many values");
         return 2;
     }
-    const bool vec = aligned(out, 16) && (K * mx_size(type)) % 16 == 0;
     cudaStream_t s = as_stream(stream);
     const uint32_t grid = static_cast<uint32_t>(blocks);
     switch (type * 2 + (vec ? 1 : 0)) {
-        case 0: values_kernel<kMxBf16, false><<<grid, 256, 0, s>>>(a); break;
-        case 1: values_kernel<kMxBf16, true><<<grid, 256, 0, s>>>(a); break;
-        case 2: values_kernel<kMxF16, false><<<grid, 256, 0, s>>>(a); break;
-        case 3: values_kernel<kMxF16, true><<<grid, 256, 0, s>>>(a); break;
-        case 4: values_kernel<kMxF32, false><<<grid, 256, 0, s>>>(a); break;
-        default: values_kernel<kMxF32, true><<<grid, 256, 0, s>>>(a); break;
+        case 0: odd_values_kernel<kMxBf16><<<grid, 256, 0, s>>>(a); break;
+        case 1: values_kernel<kMxBf16><<<grid, 256, 0, s>>>(a); break;
+        case 2: odd_values_kernel<kMxF16><<<grid, 256, 0, s>>>(a); break;
+        case 3: values_kernel<kMxF16><<<grid, 256, 0, s>>>(a); break;
+        case 4: odd_values_kernel<kMxF32><<<grid, 256, 0, s>>>(a); break;
+        default: values_kernel<kMxF32><<<grid, 256, 0, s>>>(a); break;
     }
     return launch_status("mxfp4_dequantize");
 }
