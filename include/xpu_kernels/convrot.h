@@ -369,6 +369,70 @@ int xpuint8_mxfp4_expert_dw_stream(const void *stream, const uint8_t *a_codes,
                                    const int32_t *tiles, int64_t max_tiles, int64_t M, int64_t N,
                                    int64_t experts);
 
+/* The MXFP4 linear in one call: x [M, K] (row stride ldx) quantised along K, behind the rotation or
+ * not, times the weight [N, K] in MXFP4, bias fp32 [N] or NULL, out [M, N].  Up to 16 rows whose
+ * stride and base are multiples of 16 bytes are quantised inside the product (the workspace may be
+ * NULL); others use xpuint8_mxfp4_linear_workspace_bytes bytes. */
+int64_t xpuint8_mxfp4_linear_workspace_bytes(int64_t M, int64_t K);
+int xpuint8_mxfp4_linear_stream(const void *stream, const void *x, int32_t type, int64_t ldx,
+                                const uint8_t *w_codes, const uint8_t *w_scales, const float *bias,
+                                void *out, void *workspace, int64_t M, int64_t N, int64_t K,
+                                int32_t rotate);
+
+/* The MXFP4 linear with both operands quantised in the call, and its gradients.  `want` bit 0: dx will
+ * be asked for, bit 1: dw; `saved` (xpuint8_mxfp4_train_saved_workspace_bytes) is kept from the forward
+ * call to the backward one, both called with the same sizes, rotate and want.  dx [M, K] of `type`,
+ * dw [N, K] of `w_type`, contiguous; NULL where not wanted. */
+int64_t xpuint8_mxfp4_train_saved_workspace_bytes(int64_t M, int64_t N, int64_t K, int32_t want);
+int64_t xpuint8_mxfp4_train_workspace_bytes(int64_t M, int64_t N, int64_t K);
+int xpuint8_mxfp4_train_stream(const void *stream, const void *x, int32_t type, int64_t ldx,
+                               const void *w, int32_t w_type, int64_t ldw, const float *bias,
+                               void *out, void *saved, void *workspace, int64_t M, int64_t N,
+                               int64_t K, int32_t rotate, int32_t want);
+int64_t xpuint8_mxfp4_grad_workspace_bytes(int64_t M, int64_t N, int64_t K, int32_t w_type,
+                                           int32_t rotate, int32_t want);
+int xpuint8_mxfp4_grad_stream(const void *stream, const void *dy, int32_t type, int64_t ld_dy,
+                              const void *saved, void *dx, void *dw, int32_t w_type,
+                              void *workspace, int64_t M, int64_t N, int64_t K, int32_t rotate,
+                              int32_t want);
+
+/* The same by expert: rows in the order of xpuint8_expert_sort_stream, whose arrays order .. tiles
+ * are; x holds tokens [tokens, K], or with `sorted` the plan's rows [tokens * fan, K]; w is a stack
+ * [experts, N, K]; max_tiles as in xpuint8_mxfp4_quantize_sorted_stream.  Up to 128 rows are quantised
+ * inside the product where their stride and base are multiples of 16 bytes. */
+int64_t xpuint8_mxfp4_expert_linear_workspace_bytes(int64_t rows, int64_t max_tiles, int64_t K);
+int xpuint8_mxfp4_expert_linear_stream(const void *stream, const void *x, int32_t type,
+                                       int64_t ldx, const uint8_t *w_codes,
+                                       const uint8_t *w_scales, void *out, void *workspace,
+                                       const int32_t *order, const int32_t *positions,
+                                       const int32_t *scale_rows, const int32_t *offsets,
+                                       const int32_t *tiles, int64_t tokens, int64_t fan,
+                                       int64_t max_tiles, int64_t N, int64_t K, int64_t experts,
+                                       int32_t rotate, int32_t sorted);
+int64_t xpuint8_mxfp4_expert_train_saved_workspace_bytes(int64_t max_tiles, int64_t N, int64_t K,
+                                                         int64_t experts, int32_t want);
+int64_t xpuint8_mxfp4_expert_train_workspace_bytes(int64_t rows, int64_t max_tiles, int64_t N,
+                                                   int64_t K, int64_t experts);
+int xpuint8_mxfp4_expert_train_stream(const void *stream, const void *x, int32_t type,
+                                      int64_t ldx, const void *w, int32_t w_type, void *out,
+                                      void *saved, void *workspace, const int32_t *order,
+                                      const int32_t *positions, const int32_t *scale_rows,
+                                      const int32_t *offsets, const int32_t *tiles,
+                                      int64_t tokens, int64_t fan, int64_t max_tiles, int64_t N,
+                                      int64_t K, int64_t experts, int32_t rotate, int32_t sorted,
+                                      int32_t want);
+int64_t xpuint8_mxfp4_expert_grad_workspace_bytes(int64_t rows, int64_t max_tiles, int64_t N,
+                                                  int64_t K, int64_t experts, int32_t w_type,
+                                                  int32_t rotate, int32_t sorted, int32_t want);
+int xpuint8_mxfp4_expert_grad_stream(const void *stream, const void *dy, int32_t type,
+                                     int64_t ld_dy, const void *saved, void *dx, void *dw,
+                                     int32_t w_type, void *workspace, const int32_t *order,
+                                     const int32_t *positions, const int32_t *scale_rows,
+                                     const int32_t *offsets, const int32_t *tiles, int64_t tokens,
+                                     int64_t fan, int64_t max_tiles, int64_t N, int64_t K,
+                                     int64_t experts, int32_t rotate, int32_t sorted,
+                                     int32_t want);
+
 /* ---------------- experts: tokens sorted by expert and back ----------------
  *
  * ids [slots] (4 or 8 bytes each; a slot is a token's choice, token t's slots t * fan .. ) -> the

@@ -32,7 +32,8 @@
 #include <string>
 
 #include "internal.h"
-#include "mx4.cuh"
+#include "mx4.h"
+#include "mx4quant.cuh"
 #include "tmap.h"
 #include "xpu_kernels/convrot.h"
 
@@ -539,23 +540,43 @@ struct FewArgs {
     int w_tiles;                     // 128-row scale tiles of each expert's weight
     int64_t rows;
     int w_early;                     // the weight is not written by the kernel before this one
+    const void *x;                   // FUSE: the tokens themselves, K values a row
+    int64_t ldx;
+    int K;
+    const int32_t *order;            // FUSE, rows: row r is slot order[r]'s token (fan > 0) or x's row r
+    int fan;
 };
 
+enum Fuse { kFuseNone = 0, kFusePlain = 1, kFuseRotate = 2 };
+
 constexpr int kFewThreads = 192;
-constexpr int kFewRing = 100 * 1024;                      // bytes of the ring: two CTAs an SM
-constexpr size_t kFewSmem = kFewRing + 1024;              // and the barriers
 constexpr int kFewMaxStages = 5;
 constexpr int kFewCols = 256;                             // TMEM columns: two CTAs an SM
+template <int FUSE>
+struct FewCfg {
+    static constexpr int kRing = FUSE == kFuseNone ? 100 * 1024 : 80 * 1024;  // two CTAs an SM
+    static constexpr int kSlots = FUSE == kFuseRotate ? 8 * kSlotBytes : 0;   // the rotations' turns
+    static constexpr int kBarAt = kRing + kSlots;
+    static constexpr size_t kSmem = kBarAt + 256;
+    static_assert(kBarAt % 16 == 0 && 2 * (kSmem + 1024) <= 228 * 1024, "two CTAs an SM");
+};
 
-// One CTA: 128 rows of a weight x up to 128 tokens, over its cluster rank's share of K.
-//   warp 0     TMA producer   warp 1  TMEM, scale copies and MMAs   warps 2-5  drain
 struct FewMaps {
     CUtensorMap x[4];  // boxes of 16, 32, 64, 128 tokens
 };
-template <int T>
+
+// One CTA: 128 rows of a weight x up to 128 tokens, over its cluster rank's share of K.
+//   warp 0     TMA producer   warp 1  TMEM, scale copies and MMAs   warps 2-5  drain
+// FUSE: the drain's warps first make the tokens' operand themselves: eight half-warps take pairs of
+// rows of a k-block (a 256-value group), quantize them, behind the rotation or not, straight into
+// the swizzled stage and its scale tiles, and arrive on the stage's FULL barrier beside the TMA
+// unit's bytes.  Every CTA repeats that for its share of K, which the weight's bytes hide while the
+// tokens are few, and one launch and the operand's way through memory are saved.
+template <int T, int FUSE>
 __global__ void __launch_bounds__(kFewThreads, 2)
     few_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmSW,
                const __grid_constant__ FewMaps tmX, const __grid_constant__ CUtensorMap tmSX, const FewArgs args) {
+    using C = FewCfg<FUSE>;
     extern __shared__ __align__(1024) uint8_t smem[];
     if (smem_u32(smem) & 1023u) {
         if (threadIdx.x == 0) atomicCAS(&g_mx4_fault, 0, 197);
@@ -592,25 +613,28 @@ __global__ void __launch_bounds__(kFewThreads, 2)
     const uint32_t ring = smem_u32(smem);
     const int w_bytes = 128 * kCodeRow, x_bytes = nt * kCodeRow;
     const uint32_t stage_bytes = w_bytes + x_bytes + 2 * kScaleBlock;
-    const int stages = min(kFewMaxStages, static_cast<int>(kFewRing / stage_bytes));
-    uint64_t *bars = reinterpret_cast<uint64_t *>(smem + kFewRing);
+    const int stages = min(kFewMaxStages, static_cast<int>(C::kRing / stage_bytes));
+    uint64_t *bars = reinterpret_cast<uint64_t *>(smem + C::kBarAt);
     const uint32_t bar0 = smem_u32(bars);
     auto FULL = [&](int s) { return bar0 + 8u * s; };
     auto EMPTY = [&](int s) { return bar0 + 8u * (kFewMaxStages + s); };
     const uint32_t done = bar0 + 8u * (2 * kFewMaxStages);
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 2 * kFewMaxStages + 1);
+    const int pairs = (count + 1) / 2;  // FUSE: row pairs of a k-block
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < kFewMaxStages; ++s) {
-            mbar_init(FULL(s), 1);
+            mbar_init(FULL(s), FUSE == kFuseNone ? 1 : 1 + pairs);
             mbar_init(EMPTY(s), 1);
         }
         mbar_init(done, 1);
         fence_mbar_init();
         prefetch_tmap(&tmW);
         prefetch_tmap(&tmSW);
-        prefetch_tmap(&tmX.x[box]);
-        prefetch_tmap(&tmSX);
+        if (FUSE == kFuseNone) {
+            prefetch_tmap(&tmX.x[box]);
+            prefetch_tmap(&tmSX);
+        }
     }
     if (warp == 1) {
         tmem_alloc(smem_u32(tmem_slot), kFewCols);
@@ -639,11 +663,13 @@ __global__ void __launch_bounds__(kFewThreads, 2)
             uint32_t ph = 0, issued = 0;
             for (int kb = k0; kb < k1; ++kb) {
                 if (!mbar_wait(EMPTY(stage), ph ^ 1u, fault, 111)) break;
-                mbar_expect_tx(FULL(stage), stage_bytes);
+                mbar_expect_tx(FULL(stage), FUSE == kFuseNone ? stage_bytes : w_bytes + kScaleBlock);
                 const uint32_t at = ring + stage * stage_bytes;
                 if (static_cast<int>(issued) >= pre) load_w(stage, kb);
-                tma_load_2d(at + w_bytes, &tmX.x[box], FULL(stage), kb * kCodeRow, x_row);
-                tma_load_2d(at + w_bytes + x_bytes + kScaleBlock, &tmSX, FULL(stage), kb * 256, x_sf);
+                if (FUSE == kFuseNone) {
+                    tma_load_2d(at + w_bytes, &tmX.x[box], FULL(stage), kb * kCodeRow, x_row);
+                    tma_load_2d(at + w_bytes + x_bytes + kScaleBlock, &tmSX, FULL(stage), kb * 256, x_sf);
+                }
                 ++issued;
                 if (++stage == stages) { stage = 0; ph ^= 1u; }
             }
@@ -683,6 +709,66 @@ __global__ void __launch_bounds__(kFewThreads, 2)
             umma_commit(done);
             drain_wait(done, 0);
         }
+    } else if constexpr (FUSE != kFuseNone) {
+        // task t: k-block k0 + t / pairs, rows 2 (t % pairs) and the next; eight slots, task by task,
+        // so every stage is freed by k-blocks whose tasks come earlier
+        const int slot = (warp - 2) * 2 + (lane >> 4), l = lane & 15;
+        const int tasks = (k1 - k0) * pairs;
+        if (args.mode == kDense) pdl_wait();  // x
+        auto bring = [&](int r, int kb) {
+            if (r >= count) return zero_run<T>();
+            int64_t row = x_row + r;
+            if (args.fan > 0) row = __ldg(args.order + row) / args.fan;
+            const uint8_t *p = static_cast<const uint8_t *>(args.x) + row * args.ldx * mx_size(T);
+            return load_run<T, true>(p, kb * 256 + l * 16, args.K);
+        };
+        int t = slot, rp = 0, kb = k0;
+        Run<T> A = zero_run<T>(), B = zero_run<T>();
+        if (t < tasks) {
+            kb = k0 + t / pairs;
+            rp = t % pairs;
+            A = bring(2 * rp, kb);
+            B = bring(2 * rp + 1, kb);
+        }
+        bool ok = true;
+        for (int it = 0; ok && it < tasks; it += 8) {
+            const bool mine = t < tasks;
+            if constexpr (FUSE == kFuseRotate) {
+                const uint32_t tile = ring + C::kRing + slot * kSlotBytes;
+                rotate_to_shared<T>(A, B, tile, l);
+                runs_from_shared<T>(A, B, tile, l);
+                __syncwarp();
+            }
+            uint32_t e0, e1;
+            const uint2 c0 = quantize_run<T>(A, e0), c1 = quantize_run<T>(B, e1);
+            const uint32_t w0 = join_scales(e0), w1 = join_scales(e1);
+            const int r = 2 * rp, local = kb - k0, stage = local % stages;
+            t += 8;
+            if (t < tasks) {  // the next task's loads, before this one's wait
+                kb = k0 + t / pairs;
+                rp = t % pairs;
+                A = bring(2 * rp, kb);
+                B = bring(2 * rp + 1, kb);
+            }
+            if (mine) ok = mbar_wait(EMPTY(stage), ((local / stages) & 1) ^ 1u, fault, 113);
+            ok = __all_sync(0xFFFFFFFFu, ok);
+            if (mine && ok) {
+                const uint32_t at = ring + stage * stage_bytes + w_bytes, sx = at + x_bytes + kScaleBlock;
+                // K-major rows of 128 bytes, 16-byte chunk c of row r at c ^ (r & 7)
+                const uint32_t a0 = at + r * 128 + (((l >> 1) ^ (r & 7)) << 4) + (l & 1) * 8;
+                asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(a0), "r"(c0.x), "r"(c0.y) : "memory");
+                const uint32_t a1 = at + (r + 1) * 128 + (((l >> 1) ^ ((r + 1) & 7)) << 4) + (l & 1) * 8;
+                asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(a1), "r"(c1.x), "r"(c1.y) : "memory");
+                if ((l & 7) == 0) {
+                    const uint32_t s0 = sx + (l >> 3) * kMxTileBytes + (r & 31) * 16 + (r >> 5) * 4;
+                    asm volatile("st.shared.b32 [%0], %1;" ::"r"(s0), "r"(w0) : "memory");
+                    asm volatile("st.shared.b32 [%0], %1;" ::"r"(s0 + 16), "r"(w1) : "memory");
+                }
+                fence_async_smem();
+            }
+            __syncwarp();
+            if (mine && ok && l == 0) mbar_arrive(FULL(stage));
+        }
     }
     __syncthreads();  // every load has landed and every MMA is done: the ring is free
     tc_fence_after();
@@ -707,18 +793,21 @@ __global__ void __launch_bounds__(kFewThreads, 2)
     if (warp == 1) tmem_dealloc(tmem, kFewCols);
     pdl_wait();  // the output may be what the kernel before still reads
     // this rank's share of the rows: all ranks' parts, in the order of the ranks
-    const int share = 128 / static_cast<int>(splits);
+    const int share = 128 / static_cast<int>(splits), shift = 31 - __clz(share);
     const uint32_t mine = smem_u32(part);
+#pragma unroll 4
     for (int i = threadIdx.x; i < count * share; i += kFewThreads) {
-        const int t = i / share, row = static_cast<int>(rank) * share + (i - t * share);
+        const int t = i >> shift, row = static_cast<int>(rank) * share + (i & (share - 1));
         const int n = nb * 128 + row;
         if (n >= args.N) continue;
-        float sum = 0.f;
-        for (uint32_t s = 0; s < splits; ++s) {
-            float v;
-            asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(peer_smem(mine + (t * 128 + row) * 4, s)));
-            sum = s == 0 ? v : __fadd_rn(sum, v);
-        }
+        float v[8];
+#pragma unroll
+        for (uint32_t s = 0; s < 8; ++s)
+            if (s < splits) asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v[s]) : "r"(peer_smem(mine + (t * 128 + row) * 4, s)));
+        float sum = v[0];
+#pragma unroll
+        for (uint32_t s = 1; s < 8; ++s)
+            if (s < splits) sum = __fadd_rn(sum, v[s]);
         if (args.bias) sum = __fadd_rn(sum, __ldg(args.bias + n));
         mx_store1<T>(args.out, (x_row + t) * args.ldo + n, sum);
     }
@@ -839,10 +928,10 @@ int run_pair(cudaStream_t s, PairArgs a, const Operand &A, const Operand &B, int
     return bn == 256 ? launch_pair_type<256>(s, m, a, tiles, type) : launch_pair_type<128>(s, m, a, tiles, type);
 }
 
-template <int T>
+template <int T, int FUSE>
 int launch_few(cudaStream_t s, const CUtensorMap &w, const CUtensorMap &sw, const FewMaps &x, const CUtensorMap &sx, const FewArgs &a, int splits, int64_t slots) {
-    auto kern = few_kernel<T>;
-    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kFewSmem)) != cudaSuccess)
+    auto kern = few_kernel<T, FUSE>;
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(FewCfg<FUSE>::kSmem)) != cudaSuccess)
         return launch_status("mxfp4_mm (shared memory attribute)");
     cudaLaunchConfig_t cfg = {};
     cudaLaunchAttribute attr[2];
@@ -853,7 +942,7 @@ int launch_few(cudaStream_t s, const CUtensorMap &w, const CUtensorMap &sw, cons
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.gridDim = dim3(static_cast<uint32_t>((a.N + 127) / 128 * splits), static_cast<uint32_t>(slots));
     cfg.blockDim = dim3(kFewThreads);
-    cfg.dynamicSmemBytes = kFewSmem;
+    cfg.dynamicSmemBytes = FewCfg<FUSE>::kSmem;
     cfg.stream = s;
     cfg.attrs = attr;
     cfg.numAttrs = 2;
@@ -861,8 +950,18 @@ int launch_few(cudaStream_t s, const CUtensorMap &w, const CUtensorMap &sw, cons
     return launch_status("mxfp4_mm");
 }
 
-// X tokens, W weight rows; slots: 128-token tiles (rows: at most)
-int run_few(cudaStream_t s, const FewArgs &a, const Operand &X, const Operand &W, int type, int64_t slots) {
+template <int T>
+int launch_few(cudaStream_t s, const CUtensorMap &w, const CUtensorMap &sw, const FewMaps &x, const CUtensorMap &sx, const FewArgs &a, int splits, int64_t slots, int fuse) {
+    switch (fuse) {
+        case kFuseNone: return launch_few<T, kFuseNone>(s, w, sw, x, sx, a, splits, slots);
+        case kFusePlain: return launch_few<T, kFusePlain>(s, w, sw, x, sx, a, splits, slots);
+        default: return launch_few<T, kFuseRotate>(s, w, sw, x, sx, a, splits, slots);
+    }
+}
+
+// X tokens (null where they are quantised in the kernel), W weight rows; slots: 128-token tiles (rows:
+// at most)
+int run_few(cudaStream_t s, const FewArgs &a, const Operand *X, const Operand &W, int type, int64_t slots, int fuse) {
     if (slots > 65535) {
         set_error("mxfp4_mm: too many token tiles");
         return 2;
@@ -872,15 +971,20 @@ int run_few(cudaStream_t s, const FewArgs &a, const Operand &X, const Operand &W
     const int64_t tiles = (a.N + 127) / 128 * slots;
     int splits = 1;
     while (splits < 8 && tiles * splits * 2 <= 2 * num_sms() && a.nk >= splits * 4) splits *= 2;
-    CUtensorMap w, sw, sx;
+    CUtensorMap w, sw, sx{};
     FewMaps x{};
-    if (!code_map(&w, W, 128) || !scale_map(&sw, W, 1) || !scale_map(&sx, X, 1)) return 2;
-    for (int i = 0; i < 4; ++i)
-        if (!code_map(&x.x[i], X, 16 << i)) return 2;
+    if (!code_map(&w, W, 128) || !scale_map(&sw, W, 1)) return 2;
+    if (X) {
+        if (!scale_map(&sx, *X, 1)) return 2;
+        // dense: the one box that this many tokens take; rows: each expert's count picks its own
+        const int box = a.M <= 16 ? 0 : a.M <= 32 ? 1 : a.M <= 64 ? 2 : 3;
+        for (int i = 0; i < 4; ++i)
+            if ((a.mode == kRows || i == box) && !code_map(&x.x[i], *X, 16 << i)) return 2;
+    }
     switch (type) {
-        case kMxBf16: return launch_few<kMxBf16>(s, w, sw, x, sx, a, splits, slots);
-        case kMxF16: return launch_few<kMxF16>(s, w, sw, x, sx, a, splits, slots);
-        default: return launch_few<kMxF32>(s, w, sw, x, sx, a, splits, slots);
+        case kMxBf16: return launch_few<kMxBf16>(s, w, sw, x, sx, a, splits, slots, fuse);
+        case kMxF16: return launch_few<kMxF16>(s, w, sw, x, sx, a, splits, slots, fuse);
+        default: return launch_few<kMxF32>(s, w, sw, x, sx, a, splits, slots, fuse);
     }
 }
 
@@ -914,7 +1018,116 @@ void set_k(int64_t K, int &nk, int &last_steps) {
     last_steps = static_cast<int>((K - static_cast<int64_t>(nk - 1) * BK + 63) / 64);
 }
 
+FewArgs few_args(void *out, int64_t ldo, int64_t M, int64_t N, int64_t K) {
+    FewArgs a{};
+    a.out = out;
+    a.ldo = ldo;
+    a.M = static_cast<int>(M);
+    a.N = static_cast<int>(N);
+    a.K = static_cast<int>(K);
+    set_k(K, a.nk, a.last_steps);
+    a.rows = M;
+    a.w_tiles = static_cast<int>((N + 127) / 128);
+    return a;
+}
+
 }  // namespace
+
+int mx4_mm(cudaStream_t s, const uint8_t *a_codes, const uint8_t *a_scales, const uint8_t *b_codes, const uint8_t *b_scales,
+           const float *bias, void *out, int type, int64_t ldo, int64_t M, int64_t N, int64_t K, bool b_early) {
+    const Operand A{a_codes, a_scales, M, K, (M + 127) / 128}, B{b_codes, b_scales, N, K, (N + 127) / 128};
+    if (M <= 128) {
+        FewArgs a = few_args(out, ldo, M, N, K);
+        a.bias = bias;
+        a.mode = kDense;
+        a.w_early = b_early;
+        return run_few(s, a, &A, B, type, 1, kFuseNone);
+    }
+    PairArgs a{};
+    a.out = out;
+    a.ldo = ldo;
+    a.bias = bias;
+    a.M = static_cast<int>(M);
+    a.N = static_cast<int>(N);
+    a.num_m = static_cast<int>((M + 255) / 256);
+    set_k(K, a.nk, a.last_steps);
+    a.mode = kDense;
+    a.b_early = b_early;
+    return run_pair(s, a, A, B, type, M, a.num_m);
+}
+
+int mx4_token_mm(cudaStream_t s, const void *x, int64_t ldx, const uint8_t *b_codes, const uint8_t *b_scales, const float *bias, void *out,
+                 int type, int64_t M, int64_t N, int64_t K, bool rotate) {
+    FewArgs a = few_args(out, N, M, N, K);
+    a.bias = bias;
+    a.mode = kDense;
+    a.w_early = 1;
+    a.x = x;
+    a.ldx = ldx;
+    return run_few(s, a, nullptr, Operand{b_codes, b_scales, N, K, (N + 127) / 128}, type, 1, rotate ? kFuseRotate : kFusePlain);
+}
+
+int mx4_expert_token_mm(cudaStream_t s, const void *x, int64_t ldx, const int32_t *order, int64_t fan, const uint8_t *b_codes,
+                        const uint8_t *b_scales, void *out, int type, const int32_t *offsets, const int32_t *tiles, int64_t rows,
+                        int64_t max_tiles, int64_t N, int64_t K, int64_t experts, bool rotate) {
+    FewArgs a = few_args(out, N, rows, N, K);
+    a.mode = kRows;
+    a.offsets = offsets;
+    a.tiles = tiles;
+    a.experts = static_cast<int>(experts);
+    a.x = x;
+    a.ldx = ldx;
+    a.order = order;
+    a.fan = static_cast<int>(fan);
+    return run_few(s, a, nullptr, Operand{b_codes, b_scales, experts * N, K, experts * ((N + 127) / 128)}, type, max_tiles,
+                   rotate ? kFuseRotate : kFusePlain);
+}
+
+int mx4_expert_mm(cudaStream_t s, const uint8_t *a_codes, const uint8_t *a_scales, const uint8_t *b_codes, const uint8_t *b_scales,
+                  void *out, int type, const int32_t *offsets, const int32_t *tiles, int64_t rows, int64_t max_tiles, int64_t N,
+                  int64_t K, int64_t experts) {
+    const Operand A{a_codes, a_scales, rows, K, max_tiles};
+    const Operand B{b_codes, b_scales, experts * N, K, experts * ((N + 127) / 128)};
+    if (rows <= experts * 64) {
+        FewArgs a = few_args(out, N, rows, N, K);
+        a.mode = kRows;
+        a.offsets = offsets;
+        a.tiles = tiles;
+        a.experts = static_cast<int>(experts);
+        return run_few(s, a, &A, B, type, max_tiles, kFuseNone);
+    }
+    PairArgs a{};
+    a.out = out;
+    a.ldo = N;
+    a.M = static_cast<int>(rows);
+    a.N = static_cast<int>(N);
+    set_k(K, a.nk, a.last_steps);
+    a.mode = kRows;
+    a.offsets = offsets;
+    a.tiles = tiles;
+    a.experts = static_cast<int>(experts);
+    a.b_tiles = static_cast<int>((N + 127) / 128);
+    a.rows = rows;
+    // 256-row tiles: no more than the 128-row ones
+    const int64_t max_m = std::min(max_tiles, rows / 256 + std::min(experts, rows));
+    return run_pair(s, a, A, B, type, rows, max_m);
+}
+
+int mx4_expert_dw(cudaStream_t s, const uint8_t *a_codes, const uint8_t *a_scales, const uint8_t *b_codes, const uint8_t *b_scales,
+                  void *out, int type, const int32_t *tiles, int64_t max_tiles, int64_t M, int64_t N, int64_t experts) {
+    const Operand A{a_codes, a_scales, M, max_tiles * 128, (M + 127) / 128};
+    const Operand B{b_codes, b_scales, N, max_tiles * 128, (N + 127) / 128};
+    PairArgs a{};
+    a.out = out;
+    a.ldo = N;
+    a.M = static_cast<int>(M);
+    a.N = static_cast<int>(N);
+    a.num_m = static_cast<int>((M + 255) / 256);
+    a.mode = kContraction;
+    a.tiles = tiles;
+    a.experts = static_cast<int>(experts);
+    return run_pair(s, a, A, B, type, experts * M, a.num_m);
+}
 
 int mx4_fault_status(int reset) {
     int v = 0;
@@ -944,29 +1157,7 @@ int xpuint8_mxfp4_mm_stream(const void *stream, const uint8_t *a_codes, const ui
         set_error("mxfp4_mm: the output's row stride must be at least N and the bias 16-byte aligned");
         return 2;
     }
-    const Operand A{a_codes, a_scales, M, K, (M + 127) / 128}, B{b_codes, b_scales, N, K, (N + 127) / 128};
-    if (M <= 128) {
-        FewArgs a{};
-        a.out = out;
-        a.ldo = ldo;
-        a.bias = bias;
-        a.M = static_cast<int>(M);
-        a.N = static_cast<int>(N);
-        set_k(K, a.nk, a.last_steps);
-        a.mode = kDense;
-        a.rows = M;
-        return run_few(as_stream(stream), a, A, B, type, 1);
-    }
-    PairArgs a{};
-    a.out = out;
-    a.ldo = ldo;
-    a.bias = bias;
-    a.M = static_cast<int>(M);
-    a.N = static_cast<int>(N);
-    a.num_m = static_cast<int>((M + 255) / 256);
-    set_k(K, a.nk, a.last_steps);
-    a.mode = kDense;
-    return run_pair(as_stream(stream), a, A, B, type, M, a.num_m);
+    return mx4_mm(as_stream(stream), a_codes, a_scales, b_codes, b_scales, bias, out, type, ldo, M, N, K, false);
 }
 
 int xpuint8_mxfp4_expert_mm_stream(const void *stream, const uint8_t *a_codes,
@@ -979,38 +1170,7 @@ int xpuint8_mxfp4_expert_mm_stream(const void *stream, const uint8_t *a_codes,
         set_error("mxfp4_expert_mm: offsets and tiles, 1 to 1024 experts, experts x N below 2^31, at most 65535 tiles");
         return 2;
     }
-    const Operand A{a_codes, a_scales, rows, K, max_tiles};
-    const Operand B{b_codes, b_scales, experts * N, K, experts * ((N + 127) / 128)};
-    if (rows <= experts * 64) {
-        FewArgs a{};
-        a.out = out;
-        a.ldo = N;
-        a.M = static_cast<int>(rows);
-        a.N = static_cast<int>(N);
-        set_k(K, a.nk, a.last_steps);
-        a.mode = kRows;
-        a.offsets = offsets;
-        a.tiles = tiles;
-        a.experts = static_cast<int>(experts);
-        a.w_tiles = static_cast<int>((N + 127) / 128);
-        a.rows = rows;
-        return run_few(as_stream(stream), a, A, B, type, max_tiles);
-    }
-    PairArgs a{};
-    a.out = out;
-    a.ldo = N;
-    a.M = static_cast<int>(rows);
-    a.N = static_cast<int>(N);
-    set_k(K, a.nk, a.last_steps);
-    a.mode = kRows;
-    a.offsets = offsets;
-    a.tiles = tiles;
-    a.experts = static_cast<int>(experts);
-    a.b_tiles = static_cast<int>((N + 127) / 128);
-    a.rows = rows;
-    // 256-row tiles: no more than the 128-row ones
-    const int64_t max_m = std::min(max_tiles, rows / 256 + std::min(experts, rows));
-    return run_pair(as_stream(stream), a, A, B, type, rows, max_m);
+    return mx4_expert_mm(as_stream(stream), a_codes, a_scales, b_codes, b_scales, out, type, offsets, tiles, rows, max_tiles, N, K, experts);
 }
 
 int xpuint8_mxfp4_expert_dw_stream(const void *stream, const uint8_t *a_codes,
@@ -1023,18 +1183,7 @@ int xpuint8_mxfp4_expert_dw_stream(const void *stream, const uint8_t *a_codes,
         set_error("mxfp4_expert_dw: tiles, 1 to 1024 experts, at most 65535 tiles, experts x M below 2^31");
         return 2;
     }
-    const Operand A{a_codes, a_scales, M, max_tiles * 128, (M + 127) / 128};
-    const Operand B{b_codes, b_scales, N, max_tiles * 128, (N + 127) / 128};
-    PairArgs a{};
-    a.out = out;
-    a.ldo = N;
-    a.M = static_cast<int>(M);
-    a.N = static_cast<int>(N);
-    a.num_m = static_cast<int>((M + 255) / 256);
-    a.mode = kContraction;
-    a.tiles = tiles;
-    a.experts = static_cast<int>(experts);
-    return run_pair(as_stream(stream), a, A, B, type, experts * M, a.num_m);
+    return mx4_expert_dw(as_stream(stream), a_codes, a_scales, b_codes, b_scales, out, type, tiles, max_tiles, M, N, experts);
 }
 
 }  // extern "C"

@@ -13,8 +13,8 @@
 #include <type_traits>
 
 #include "internal.h"
-#include "mx4.cuh"
-#include "rotpair.cuh"
+#include "mx4.h"
+#include "mx4quant.cuh"
 #include "xpu_kernels/convrot.h"
 
 namespace xpuint8 {
@@ -34,186 +34,6 @@ struct RowArgs {
     const int32_t *scale_rows;   // [slots] the row of scales; negative: no expert takes it
     uint32_t fan;                // slots of a token
 };
-
-// A lane's run of 16 consecutive values of a row, as loaded: 8 words of two 16-bit values, or 16 words
-// of fp32.
-template <int T>
-struct Run {
-    static constexpr int kWords = 4 * mx_size(T);
-    uint32_t w[kWords];
-};
-
-// from column c on, zero past `cols`
-template <int T, bool VEC>
-__device__ __forceinline__ Run<T> load_run(const void *row, uint32_t c, uint32_t cols) {
-    Run<T> r;
-    if (VEC && c + 16 <= cols) {
-        const uint4 *p = reinterpret_cast<const uint4 *>(static_cast<const uint8_t *>(row) + static_cast<int64_t>(c) * mx_size(T));
-#pragma unroll
-        for (int j = 0; j < Run<T>::kWords / 4; ++j) {
-            const uint4 q = __ldg(p + j);
-            r.w[4 * j] = q.x;
-            r.w[4 * j + 1] = q.y;
-            r.w[4 * j + 2] = q.z;
-            r.w[4 * j + 3] = q.w;
-        }
-    } else if constexpr (T == kMxF32) {
-#pragma unroll
-        for (int t = 0; t < 16; ++t) r.w[t] = c + t < cols ? __ldg(static_cast<const uint32_t *>(row) + c + t) : 0u;
-    } else {
-#pragma unroll
-        for (int t = 0; t < 8; ++t) {
-            const uint32_t lo = c + 2 * t < cols ? __ldg(static_cast<const uint16_t *>(row) + c + 2 * t) : 0u;
-            const uint32_t hi = c + 2 * t + 1 < cols ? __ldg(static_cast<const uint16_t *>(row) + c + 2 * t + 1) : 0u;
-            r.w[t] = lo | (hi << 16);
-        }
-    }
-    return r;
-}
-template <int T>
-__device__ __forceinline__ Run<T> zero_run() {
-    Run<T> r;
-#pragma unroll
-    for (int j = 0; j < Run<T>::kWords; ++j) r.w[j] = 0u;
-    return r;
-}
-
-// per half, the maximum of two unsigned 16-bit values
-__device__ __forceinline__ uint32_t max_u16x2(uint32_t a, uint32_t b) {
-    uint32_t r;
-    asm("max.u16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
-    return r;
-}
-// the fp32 bits of a 16-bit magnitude
-template <int T>
-__device__ __forceinline__ uint32_t widen_bits(uint32_t h) {
-    if constexpr (T == kMxBf16) return h << 16;
-    float lo, hi;
-    mx_split<T>(h, lo, hi);
-    return __float_as_uint(lo);
-}
-
-// the pair (v0, v1) times (s0, s1)
-__device__ __forceinline__ void scale2(float &v0, float &v1, f2 s) { un2(mul2(mk2(v0, v1), s), v0, v1); }
-
-// Codes of a lane's 16 values, its neighbour (lane ^ 1) holding the block's other 16: 8 bytes, and
-// the block's scale byte.
-template <int T>
-__device__ __forceinline__ uint2 quantize_run(const Run<T> &r, uint32_t &e) {
-    uint32_t m = 0;
-    if constexpr (T == kMxF32) {
-#pragma unroll
-        for (int t = 0; t < 16; ++t) m = max(m, r.w[t] & 0x7FFFFFFFu);
-        m = max(m, __shfl_xor_sync(0xFFFFFFFFu, m, 1));
-    } else {
-#pragma unroll
-        for (int t = 0; t < 8; ++t) m = max_u16x2(m, r.w[t] & 0x7FFF7FFFu);
-        m = max_u16x2(m, __shfl_xor_sync(0xFFFFFFFFu, m, 1));
-        m = widen_bits<T>(max(m & 0xFFFFu, m >> 16));
-    }
-    e = mx_exponent(m);
-    const float inv = mx_inverse(e);
-    const f2 s = mk2(inv, inv);
-    float v[16];
-#pragma unroll
-    for (int t = 0; t < 8; ++t) {
-        if constexpr (T == kMxF32) {
-            v[2 * t] = __uint_as_float(r.w[2 * t]);
-            v[2 * t + 1] = __uint_as_float(r.w[2 * t + 1]);
-        } else {
-            mx_split<T>(r.w[t], v[2 * t], v[2 * t + 1]);
-        }
-        scale2(v[2 * t], v[2 * t + 1], s);
-    }
-    return make_uint2(mx_pack8(v), mx_pack8(v + 8));
-}
-
-// Lanes 0, 2, 4, 6 (8, 10, 12, 14) of a half-warp hold the scale bytes of a tile's four blocks: the
-// word of them, on lanes 0 and 8.
-__device__ __forceinline__ uint32_t join_scales(uint32_t e) {
-    const uint32_t two = e | (__shfl_down_sync(0xFFFFFFFFu, e, 2) << 8);
-    return two | (__shfl_down_sync(0xFFFFFFFFu, two, 4) << 16);
-}
-
-// A pair of 256-value groups A and B on a half-warp's lanes, turned to pairs: value c of both at
-// pair_at(c) of the slot's shared memory, as a word (16-bit types) or two (fp32).  The pitches put
-// the words of a column and those of a run into different banks, with every address a base and a
-// constant.
-constexpr int kSlotBytes = 16 * 144;
-template <int T>
-__device__ __forceinline__ constexpr uint32_t pair_at(int w, int l) { return T == kMxF32 ? w * 144 + l * 8 : w * 80 + l * 4; }
-
-// The rotation of the pair, scaled and rounded to the type, left in shared memory.  Lane l brings
-// values 16 l .. 16 l + 15 of both groups: two radix-4 steps in registers (accumulation chains), the
-// turn through shared memory, two more (butterflies): the association of rotate(), so the same bits.
-template <int T>
-__device__ __forceinline__ void rotate_to_shared(const Run<T> &A, const Run<T> &B, uint32_t slot, int l) {
-    f2 P[16];
-#pragma unroll
-    for (int t = 0; t < 8; ++t) {
-        float a0, a1, b0, b1;
-        if constexpr (T == kMxF32) {
-            a0 = __uint_as_float(A.w[2 * t]);
-            a1 = __uint_as_float(A.w[2 * t + 1]);
-            b0 = __uint_as_float(B.w[2 * t]);
-            b1 = __uint_as_float(B.w[2 * t + 1]);
-        } else {
-            mx_split<T>(A.w[t], a0, a1);
-            mx_split<T>(B.w[t], b0, b1);
-        }
-        P[2 * t] = mk2(a0, b0);
-        P[2 * t + 1] = mk2(a1, b1);
-    }
-#pragma unroll
-    for (int j = 0; j < 4; ++j) seq2(P[4 * j], P[4 * j + 1], P[4 * j + 2], P[4 * j + 3]);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) seq2(P[j], P[j + 4], P[j + 8], P[j + 12]);
-    const uint32_t mine = slot + l * 144, column = slot + l * 8;
-#pragma unroll
-    for (int c = 0; c < 8; ++c)
-        asm volatile("st.shared.v2.b64 [%0], {%1, %2};" ::"r"(mine + c * 16), "l"(P[2 * c].v), "l"(P[2 * c + 1].v) : "memory");
-    __syncwarp();
-#pragma unroll
-    for (int w = 0; w < 16; ++w) asm volatile("ld.shared.b64 %0, [%1];" : "=l"(P[w].v) : "r"(column + w * 144));
-    __syncwarp();
-#pragma unroll
-    for (int j = 0; j < 4; ++j) bfly2(P[4 * j], P[4 * j + 1], P[4 * j + 2], P[4 * j + 3]);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) bfly2(P[j], P[j + 4], P[j + 8], P[j + 12]);
-#pragma unroll
-    for (int w = 0; w < 16; ++w) {
-        const f2 s = mul2(P[w], mk2(0.0625f, 0.0625f));
-        if constexpr (T == kMxF32) {
-            asm volatile("st.shared.b64 [%0], %1;" ::"r"(slot + pair_at<T>(w, 0) + l * 8), "l"(s.v) : "memory");
-        } else {
-            float p, q;
-            un2(s, p, q);
-            asm volatile("st.shared.b32 [%0], %1;" ::"r"(slot + pair_at<T>(w, 0) + l * 4), "r"(mx_join<T>(p, q)) : "memory");
-        }
-    }
-    __syncwarp();
-}
-
-// both runs of lane l back from the pairs
-template <int T>
-__device__ __forceinline__ void runs_from_shared(Run<T> &A, Run<T> &B, uint32_t slot, int l) {
-    const uint32_t at = slot + pair_at<T>(1, 0) * l;
-    if constexpr (T == kMxF32) {
-#pragma unroll
-        for (int c = 0; c < 8; ++c)
-            asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(A.w[2 * c]), "=r"(B.w[2 * c]), "=r"(A.w[2 * c + 1]), "=r"(B.w[2 * c + 1]) : "r"(at + c * 16));
-    } else {
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-            uint32_t w[4];
-            asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(at + c * 16));
-            A.w[2 * c] = __byte_perm(w[0], w[1], 0x5410);
-            B.w[2 * c] = __byte_perm(w[0], w[1], 0x7632);
-            A.w[2 * c + 1] = __byte_perm(w[2], w[3], 0x5410);
-            B.w[2 * c + 1] = __byte_perm(w[2], w[3], 0x7632);
-        }
-    }
-}
 
 template <int T>
 __device__ __forceinline__ void store_run(void *row, uint32_t c, const Run<T> &r) {
@@ -399,6 +219,183 @@ __global__ void __launch_bounds__(128) quantize_columns_kernel(const ColumnArgs 
     }
 }
 
+struct BothArgs {
+    const void *x;
+    int64_t ldx, matrix_stride;            // elements
+    uint8_t *row_codes, *row_scales;       // null: not wanted
+    uint8_t *col_codes, *col_scales;
+    uint32_t rows, cols;                   // of a matrix
+    uint32_t KB, KT;                       // blocks and tiles along the columns
+    int64_t row_matrix_codes, row_matrix_scales;
+    int64_t col_pitch, col_matrix_codes, col_matrix_scales;
+    uint32_t col_blocks, col_KT;           // along the rows
+    const int32_t *offsets, *tiles, *order;  // experts: rows are sorted rows, taken from slot order[row]'s token
+    int experts;
+    uint32_t fan;                          // slots of a token; 0: x's rows are sorted already
+};
+
+constexpr int kBothThreads = 256, kBothSlots = 16, kCodePitch = 80;
+constexpr int kBothSmem = kBothSlots * kSlotBytes + 256 * kCodePitch + 256 * 4;
+
+// Codes along the rows and along the columns in one read: a CTA takes 128 rows (a tile of scales
+// along the rows) x 256 columns (a group of the rotation), 32 rows at a time.  A slot brings two
+// neighbouring rows, rotates them, quantizes them along the columns and leaves them in shared memory
+// as pairs; a thread a column then takes the 32 rows from there.
+template <int T, bool ROT, bool VEC>
+__global__ void __launch_bounds__(kBothThreads) quantize_both_kernel(const BothArgs a) {
+    extern __shared__ __align__(128) uint8_t smem[];
+    const uint32_t slots = smem_u32(smem);
+    uint8_t *s_code = smem + kBothSlots * kSlotBytes;
+    uint8_t *s_scale = s_code + 256 * kCodePitch;
+    const int slot = threadIdx.x >> 4, l = threadIdx.x & 15, kt = blockIdx.y;
+    const uint32_t mine = slots + slot * kSlotBytes;
+    pdl_trigger();
+    uint32_t begin = kt * 128u, end = a.rows;
+    if (a.offsets) {
+        if (kt >= __ldg(a.tiles + a.experts)) return;
+        const int e = find_tile(a.tiles, a.experts, kt);
+        begin = __ldg(a.offsets + e) + (kt - __ldg(a.tiles + e)) * 128;
+        end = __ldg(a.offsets + e + 1);
+    }
+    const uint32_t c = blockIdx.x * 256 + l * 16;
+    const uint8_t *x = static_cast<const uint8_t *>(a.x) + blockIdx.z * a.matrix_stride * mx_size(T);
+    auto bring = [&](uint32_t i) {
+        if (begin + i >= end) return zero_run<T>();
+        uint32_t r = begin + i;
+        if (a.fan) r = static_cast<uint32_t>(__ldg(a.order + r)) / a.fan;
+        return load_run<T, VEC>(x + static_cast<int64_t>(r) * a.ldx * mx_size(T), c, a.cols);
+    };
+    Run<T> A = bring(2 * slot), B = bring(2 * slot + 1);
+#pragma unroll 1
+    for (int sub = 0; sub < 4; ++sub) {
+        if constexpr (ROT) {
+            rotate_to_shared<T>(A, B, mine, l);
+            runs_from_shared<T>(A, B, mine, l);
+        } else {
+            runs_to_shared<T>(A, B, mine, l);
+        }
+        __syncwarp();
+        if (a.row_codes) {
+            uint32_t e0, e1;
+            const uint2 c0 = quantize_run<T>(A, e0), c1 = quantize_run<T>(B, e1);
+            const uint32_t w0 = join_scales(e0), w1 = join_scales(e1);
+            const uint32_t i = sub * 32 + 2 * slot, tile = blockIdx.x * 2 + (l >> 3);
+            const bool has_code = c < a.KB * 32, has_word = (l & 7) == 0 && tile < a.KT;
+            uint8_t *codes = a.row_codes + blockIdx.z * a.row_matrix_codes;
+            uint8_t *scales = a.row_scales + blockIdx.z * a.row_matrix_scales;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                if (begin + i + h >= end) continue;
+                if (has_code) *reinterpret_cast<uint2 *>(codes + static_cast<int64_t>(begin + i + h) * a.KB * 16 + c / 2) = h ? c1 : c0;
+                if (has_word) *reinterpret_cast<uint32_t *>(scales + mx_scale_word(kt * 128ll + i + h, tile, a.KT)) = h ? w1 : w0;
+            }
+        }
+        if (sub < 3) {
+            A = bring(sub * 32 + 32 + 2 * slot);
+            B = bring(sub * 32 + 33 + 2 * slot);
+        }
+        if (!a.col_codes) continue;
+        __syncthreads();
+        const uint32_t at = slots + pair_at<T>(1, 0) * (threadIdx.x >> 4) + (T == kMxF32 ? 8 : 4) * (threadIdx.x & 15);
+        uint32_t e;
+        float v[32];
+        if constexpr (T == kMxF32) {
+            uint32_t m = 0;
+#pragma unroll
+            for (int s = 0; s < 16; ++s) {
+                asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(v[2 * s]), "=f"(v[2 * s + 1]) : "r"(at + s * kSlotBytes));
+                m = max(m, max(__float_as_uint(v[2 * s]) & 0x7FFFFFFFu, __float_as_uint(v[2 * s + 1]) & 0x7FFFFFFFu));
+            }
+            e = mx_exponent(m);
+        } else {
+            uint32_t w[16], m = 0;
+#pragma unroll
+            for (int s = 0; s < 16; ++s) asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w[s]) : "r"(at + s * kSlotBytes));
+#pragma unroll
+            for (int s = 0; s < 16; ++s) m = max_u16x2(m, w[s] & 0x7FFF7FFFu);
+            e = mx_exponent(widen_bits<T>(max(m & 0xFFFFu, m >> 16)));
+#pragma unroll
+            for (int s = 0; s < 16; ++s) mx_split<T>(w[s], v[2 * s], v[2 * s + 1]);
+        }
+        const float inv = mx_inverse(e);
+#pragma unroll
+        for (int s = 0; s < 16; ++s) scale2(v[2 * s], v[2 * s + 1], mk2(inv, inv));
+        *reinterpret_cast<uint4 *>(s_code + threadIdx.x * kCodePitch + sub * 16) = make_uint4(mx_pack8(v), mx_pack8(v + 8), mx_pack8(v + 16), mx_pack8(v + 24));
+        s_scale[threadIdx.x * 4 + sub] = static_cast<uint8_t>(e);
+        __syncthreads();
+    }
+    if (!a.col_codes) return;
+    uint8_t *codes = a.col_codes + blockIdx.z * a.col_matrix_codes;
+    uint8_t *scales = a.col_scales + blockIdx.z * a.col_matrix_scales;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const uint32_t col = (threadIdx.x >> 2) + 64 * i, part = threadIdx.x & 3, n = blockIdx.x * 256 + col;
+        if (n < a.cols && kt * 4u + part < a.col_blocks)
+            *reinterpret_cast<uint4 *>(codes + n * a.col_pitch + (kt * 4 + part) * 16) = *reinterpret_cast<const uint4 *>(s_code + col * kCodePitch + part * 16);
+    }
+    const uint32_t n = blockIdx.x * 256 + threadIdx.x;
+    if (n < a.cols) *reinterpret_cast<uint32_t *>(scales + mx_scale_word(n, kt, a.col_KT)) = *reinterpret_cast<const uint32_t *>(s_scale + threadIdx.x * 4);
+}
+
+struct TurnArgs {
+    const float *x;              // [rows, K], or the experts' rows that are summed
+    void *out;                   // [rows, K]
+    uint32_t groups, G, K;
+    const int32_t *positions, *scale_rows;  // experts: [rows, fan], or null
+    uint32_t fan;
+};
+
+// fp32 rows, or the sums of each token's rows, turned back by the rotation and rounded once.
+template <int T, bool ROT, bool VEC>
+__global__ void __launch_bounds__(128) turn_kernel(const TurnArgs a) {
+    __shared__ __align__(128) uint8_t tiles[ROT ? 8 * kSlotBytes : 16];
+    const int slot = threadIdx.x >> 4, l = threadIdx.x & 15;
+    const uint32_t f0 = (blockIdx.x * 8u + slot) * 2u;
+    const uint32_t r0 = f0 / a.G, g0 = f0 - r0 * a.G;
+    const uint32_t r1 = g0 + 1 == a.G ? r0 + 1 : r0, g1 = g0 + 1 == a.G ? 0 : g0 + 1;
+    auto bring = [&](bool ok, uint32_t r, uint32_t g) {
+        Run<kMxF32> v = zero_run<kMxF32>();
+        if (!ok) return v;
+        const uint32_t c = g * 256 + l * 16;
+        if (!a.positions) return load_run<kMxF32, VEC>(a.x + static_cast<int64_t>(r) * a.K, c, a.K);
+#pragma unroll 2
+        for (uint32_t j = 0; j < a.fan; ++j) {
+            const int64_t at = static_cast<int64_t>(r) * a.fan + j;
+            if (__ldg(a.scale_rows + at) < 0) continue;
+            const Run<kMxF32> u = load_run<kMxF32, VEC>(a.x + static_cast<int64_t>(__ldg(a.positions + at)) * a.K, c, a.K);
+#pragma unroll
+            for (int t = 0; t < 16; ++t) v.w[t] = __float_as_uint(__fadd_rn(__uint_as_float(v.w[t]), __uint_as_float(u.w[t])));
+        }
+        return v;
+    };
+    const bool ok0 = f0 < a.groups, ok1 = f0 + 1 < a.groups;
+    Run<kMxF32> A = bring(ok0, r0, g0), B = bring(ok1, r1, g1);
+    if constexpr (ROT) {
+        const uint32_t tile = smem_u32(tiles) + slot * kSlotBytes;
+        rotate_to_shared<kMxF32>(A, B, tile, l);
+        runs_from_shared<kMxF32>(A, B, tile, l);
+    }
+    auto put = [&](uint32_t r, uint32_t g, const Run<kMxF32> &v) {
+        uint8_t *row = static_cast<uint8_t *>(a.out) + static_cast<int64_t>(r) * a.K * mx_size(T);
+        const uint32_t c = g * 256 + l * 16;
+        if (VEC && c + 16 <= a.K) {
+            Run<T> o;
+#pragma unroll
+            for (int t = 0; t < Run<T>::kWords; ++t) {
+                if constexpr (T == kMxF32) o.w[t] = v.w[t];
+                else o.w[t] = mx_join<T>(__uint_as_float(v.w[2 * t]), __uint_as_float(v.w[2 * t + 1]));
+            }
+            store_run<T>(row, c, o);
+        } else {
+#pragma unroll
+            for (int t = 0; t < 16; ++t)
+                if (c + t < a.K) mx_store1<T>(row, c + t, __uint_as_float(v.w[t]));
+        }
+    };
+    if (ok0) put(r0, g0, A);
+    if (ok1) put(r1, g1, B);
+}
+
 struct ValueArgs {
     const uint8_t *codes, *scales;
     void *out;
@@ -492,6 +489,164 @@ int quantize_rows(cudaStream_t s, RowArgs &a, int type, int64_t rows, int64_t K,
     return launch_status("mxfp4_quantize");
 }
 
+template <int T, bool ROT, bool VEC>
+int launch_both(cudaStream_t s, const BothArgs &a, dim3 grid) {
+    auto kern = quantize_both_kernel<T, ROT, VEC>;
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kBothSmem) != cudaSuccess)
+        return launch_status("mxfp4_quantize (shared memory attribute)");
+    kern<<<grid, kBothThreads, kBothSmem, s>>>(a);
+    return launch_status("mxfp4_quantize");
+}
+template <int T>
+int launch_both(cudaStream_t s, const BothArgs &a, dim3 grid, bool rotate, bool vec) {
+    if (rotate) return vec ? launch_both<T, true, true>(s, a, grid) : launch_both<T, true, false>(s, a, grid);
+    return vec ? launch_both<T, false, true>(s, a, grid) : launch_both<T, false, false>(s, a, grid);
+}
+
+template <int T>
+void launch_turn(cudaStream_t s, const TurnArgs &a, bool rotate, bool vec) {
+    const uint32_t grid = (a.groups + 15) / 16;
+    if (rotate) turn_kernel<T, true, true><<<grid, 128, 0, s>>>(a);  // K % 256 == 0: rows are aligned
+    else if (vec) turn_kernel<T, false, true><<<grid, 128, 0, s>>>(a);
+    else turn_kernel<T, false, false><<<grid, 128, 0, s>>>(a);
+}
+
+}  // namespace
+
+int mx4_quantize_rows(cudaStream_t s, const void *x, int type, int64_t ldx, uint8_t *codes, uint8_t *scales, void *rotated, int64_t rows,
+                      int64_t K, int64_t matrix_rows, bool rotate) {
+    RowArgs a{};
+    a.x = x;
+    a.codes = codes;
+    a.scales = scales;
+    a.rotated = rotated;
+    a.matrix_rows = static_cast<uint32_t>(matrix_rows);
+    a.matrix_tiles = matrix_rows == rows ? 0 : static_cast<uint32_t>((matrix_rows + 127) / 128);
+    a.fan = 1;
+    return quantize_rows(s, a, type, rows, K, ldx, rotate);
+}
+
+int mx4_quantize_sorted(cudaStream_t s, const void *x, int type, int64_t ldx, uint8_t *codes, uint8_t *scales, void *rotated,
+                        const int32_t *order, const int32_t *positions, const int32_t *scale_rows, int64_t rows, int64_t fan,
+                        int64_t K, bool rotate) {
+    RowArgs a{};
+    a.x = x;
+    a.codes = codes;
+    a.scales = scales;
+    a.rotated = rotated;
+    a.order = order;
+    a.positions = positions;
+    a.scale_rows = scale_rows;
+    a.matrix_rows = 1;
+    a.fan = static_cast<uint32_t>(fan);
+    return quantize_rows(s, a, type, rows, K, ldx, rotate);
+}
+
+int mx4_quantize_columns(cudaStream_t s, const void *x, int type, int64_t ldx, uint8_t *codes, uint8_t *scales, int64_t rows,
+                         int64_t cols, int64_t matrices, const int32_t *offsets, const int32_t *tiles, int64_t experts, int64_t max_tiles) {
+    const bool sorted = offsets != nullptr;
+    ColumnArgs a{};
+    a.x = x;
+    a.ldx = ldx;
+    a.matrix_stride = rows * ldx;
+    a.codes = codes;
+    a.scales = scales;
+    a.rows = static_cast<uint32_t>(rows);
+    a.cols = static_cast<uint32_t>(cols);
+    a.code_blocks = static_cast<uint32_t>(sorted ? max_tiles * 4 : (rows + 31) / 32);
+    a.KT = static_cast<uint32_t>(sorted ? max_tiles : (rows + 127) / 128);
+    a.pitch = static_cast<int64_t>(a.code_blocks) * 16;
+    a.matrix_codes = a.pitch * cols;
+    a.matrix_scales = (cols + 127) / 128 * a.KT * static_cast<int64_t>(kMxTileBytes);
+    a.offsets = offsets;
+    a.tiles = tiles;
+    a.experts = static_cast<int>(experts);
+    if (a.KT > 65535u) {
+        set_error("mxfp4: at most 8388480 rows along the contraction");
+        return 2;
+    }
+    const int es = mx_size(type);
+    const bool vec = aligned(x, 2 * es) && ldx % 2 == 0;
+    const dim3 grid(static_cast<uint32_t>((cols + 63) / 64), a.KT, static_cast<uint32_t>(matrices));
+    switch (type * 2 + (vec ? 1 : 0)) {
+        case 0: quantize_columns_kernel<kMxBf16, false><<<grid, 128, 0, s>>>(a); break;
+        case 1: quantize_columns_kernel<kMxBf16, true><<<grid, 128, 0, s>>>(a); break;
+        case 2: quantize_columns_kernel<kMxF16, false><<<grid, 128, 0, s>>>(a); break;
+        case 3: quantize_columns_kernel<kMxF16, true><<<grid, 128, 0, s>>>(a); break;
+        case 4: quantize_columns_kernel<kMxF32, false><<<grid, 128, 0, s>>>(a); break;
+        default: quantize_columns_kernel<kMxF32, true><<<grid, 128, 0, s>>>(a); break;
+    }
+    return launch_status("mxfp4_quantize_columns");
+}
+
+int mx4_quantize_both(cudaStream_t s, const Mx4Both &b) {
+    const bool sorted = b.offsets != nullptr;
+    // columns alone of what is not rotated nor gathered: the kernel made for them
+    if (!b.row_codes && !b.rotate && !b.fan)
+        return mx4_quantize_columns(s, b.x, b.type, b.ldx, b.col_codes, b.col_scales, b.rows, b.cols, b.matrices, b.offsets, b.tiles, b.experts, b.max_tiles);
+    BothArgs a{};
+    a.x = b.x;
+    a.ldx = b.ldx;
+    a.matrix_stride = b.rows * b.ldx;
+    a.row_codes = b.row_codes;
+    a.row_scales = b.row_scales;
+    a.col_codes = b.col_codes;
+    a.col_scales = b.col_scales;
+    a.rows = static_cast<uint32_t>(b.rows);
+    a.cols = static_cast<uint32_t>(b.cols);
+    a.KB = static_cast<uint32_t>((b.cols + 31) / 32);
+    a.KT = (a.KB + 3) / 4;
+    a.row_matrix_codes = b.rows * a.KB * 16;
+    a.row_matrix_scales = (b.rows + 127) / 128 * a.KT * static_cast<int64_t>(kMxTileBytes);
+    a.col_blocks = static_cast<uint32_t>(sorted ? b.max_tiles * 4 : (b.rows + 31) / 32);
+    a.col_KT = static_cast<uint32_t>(sorted ? b.max_tiles : (b.rows + 127) / 128);
+    a.col_pitch = static_cast<int64_t>(a.col_blocks) * 16;
+    a.col_matrix_codes = a.col_pitch * b.cols;
+    a.col_matrix_scales = (b.cols + 127) / 128 * a.col_KT * static_cast<int64_t>(kMxTileBytes);
+    a.offsets = b.offsets;
+    a.tiles = b.tiles;
+    a.order = b.order;
+    a.experts = static_cast<int>(b.experts);
+    a.fan = static_cast<uint32_t>(b.fan);
+    if (a.col_KT > 65535u || b.matrices > 65535) {
+        set_error("mxfp4: at most 8388480 rows along the contraction and 65535 matrices");
+        return 2;
+    }
+    const bool vec = aligned(b.x, 16) && (b.ldx * mx_size(b.type)) % 16 == 0;
+    const dim3 grid(static_cast<uint32_t>((b.cols + 255) / 256), a.col_KT, static_cast<uint32_t>(b.matrices));
+    switch (b.type) {
+        case kMxBf16: return launch_both<kMxBf16>(s, a, grid, b.rotate, vec);
+        case kMxF16: return launch_both<kMxF16>(s, a, grid, b.rotate, vec);
+        default: return launch_both<kMxF32>(s, a, grid, b.rotate, vec);
+    }
+}
+
+int mx4_turn(cudaStream_t s, const float *x, void *out, int type, int64_t rows, int64_t K, const int32_t *positions,
+             const int32_t *scale_rows, int64_t fan, bool rotate) {
+    TurnArgs a{};
+    a.x = x;
+    a.out = out;
+    a.G = static_cast<uint32_t>((K + 255) / 256);
+    a.K = static_cast<uint32_t>(K);
+    if (rows * a.G > 0x7FFFFFF0ll) {
+        set_error("mxfp4: rows x 256-groups must be below 2^31");
+        return 2;
+    }
+    a.groups = static_cast<uint32_t>(rows * a.G);
+    a.positions = positions;
+    a.scale_rows = scale_rows;
+    a.fan = static_cast<uint32_t>(fan);
+    const bool vec = aligned(x, 16) && aligned(out, 16) && (K * mx_size(type)) % 16 == 0 && K % 4 == 0;
+    switch (type) {
+        case kMxBf16: launch_turn<kMxBf16>(s, a, rotate, vec); break;
+        case kMxF16: launch_turn<kMxF16>(s, a, rotate, vec); break;
+        default: launch_turn<kMxF32>(s, a, rotate, vec); break;
+    }
+    return launch_status("mxfp4_turn");
+}
+
+namespace {
+
 int check_type(int32_t type) {
     if (type >= 0 && type <= 2) return 0;
     set_error("mxfp4: the element type must be 0 (bf16), 1 (fp16) or 2 (fp32)");
@@ -558,15 +713,7 @@ int xpuint8_mxfp4_quantize_stream(const void *stream, const void *x, int32_t typ
         set_error("mxfp4: ldx must be at least K and rows a multiple of matrix_rows");
         return 2;
     }
-    RowArgs a{};
-    a.x = x;
-    a.codes = codes;
-    a.scales = scales;
-    a.rotated = rotated;
-    a.matrix_rows = static_cast<uint32_t>(matrix_rows);
-    a.matrix_tiles = matrix_rows == rows ? 0 : static_cast<uint32_t>((matrix_rows + 127) / 128);
-    a.fan = 1;
-    return quantize_rows(as_stream(stream), a, type, rows, K, ldx, rotate != 0);
+    return mx4_quantize_rows(as_stream(stream), x, type, ldx, codes, scales, rotated, rows, K, matrix_rows, rotate != 0);
 }
 
 int xpuint8_mxfp4_quantize_sorted_stream(const void *stream, const void *x, int32_t type,
@@ -583,17 +730,7 @@ int xpuint8_mxfp4_quantize_sorted_stream(const void *stream, const void *x, int3
         set_error("mxfp4: sorted rows need positions, scale_rows, a positive fan (1 with order) and ldx >= K");
         return 2;
     }
-    RowArgs a{};
-    a.x = x;
-    a.codes = codes;
-    a.scales = scales;
-    a.rotated = rotated;
-    a.order = order;
-    a.positions = positions;
-    a.scale_rows = scale_rows;
-    a.matrix_rows = a.matrix_tiles = 1;
-    a.fan = static_cast<uint32_t>(fan);
-    return quantize_rows(as_stream(stream), a, type, rows, K, ldx, rotate != 0);
+    return mx4_quantize_sorted(as_stream(stream), x, type, ldx, codes, scales, rotated, order, positions, scale_rows, rows, fan, K, rotate != 0);
 }
 
 int xpuint8_mxfp4_quantize_columns_stream(const void *stream, const void *x, int32_t type,
@@ -610,39 +747,7 @@ int xpuint8_mxfp4_quantize_columns_stream(const void *stream, const void *x, int
         set_error("mxfp4: ldx must be at least cols, 1 to 65535 matrices, and experts need tiles");
         return 2;
     }
-    ColumnArgs a{};
-    a.x = x;
-    a.ldx = ldx;
-    a.matrix_stride = rows * ldx;
-    a.codes = codes;
-    a.scales = scales;
-    a.rows = static_cast<uint32_t>(rows);
-    a.cols = static_cast<uint32_t>(cols);
-    a.code_blocks = static_cast<uint32_t>(sorted ? max_tiles * 4 : (rows + 31) / 32);
-    a.KT = static_cast<uint32_t>(sorted ? max_tiles : (rows + 127) / 128);
-    a.pitch = static_cast<int64_t>(a.code_blocks) * 16;
-    a.matrix_codes = a.pitch * cols;
-    a.matrix_scales = (cols + 127) / 128 * a.KT * static_cast<int64_t>(kMxTileBytes);
-    a.offsets = offsets;
-    a.tiles = tiles;
-    a.experts = static_cast<int>(experts);
-    if (a.KT > 65535u) {
-        set_error("mxfp4: at most 8388480 rows along the contraction");
-        return 2;
-    }
-    const int es = mx_size(type);
-    const bool vec = aligned(x, 2 * es) && ldx % 2 == 0;
-    const dim3 grid(static_cast<uint32_t>((cols + 63) / 64), a.KT, static_cast<uint32_t>(matrices));
-    cudaStream_t s = as_stream(stream);
-    switch (type * 2 + (vec ? 1 : 0)) {
-        case 0: quantize_columns_kernel<kMxBf16, false><<<grid, 128, 0, s>>>(a); break;
-        case 1: quantize_columns_kernel<kMxBf16, true><<<grid, 128, 0, s>>>(a); break;
-        case 2: quantize_columns_kernel<kMxF16, false><<<grid, 128, 0, s>>>(a); break;
-        case 3: quantize_columns_kernel<kMxF16, true><<<grid, 128, 0, s>>>(a); break;
-        case 4: quantize_columns_kernel<kMxF32, false><<<grid, 128, 0, s>>>(a); break;
-        default: quantize_columns_kernel<kMxF32, true><<<grid, 128, 0, s>>>(a); break;
-    }
-    return launch_status("mxfp4_quantize_columns");
+    return mx4_quantize_columns(as_stream(stream), x, type, ldx, codes, scales, rows, cols, matrices, offsets, tiles, experts, max_tiles);
 }
 
 int xpuint8_mxfp4_dequantize_stream(const void *stream, const uint8_t *codes,

@@ -16,19 +16,7 @@ from __future__ import annotations
 
 import torch
 
-from .int8._lib import _lib
-from .mxfp4 import (
-    MXFP4,
-    _TYPES,
-    _check_rotate,
-    _empty,
-    _launch,
-    _quantize,
-    _quantize_columns,
-    _rotate,
-    _rows,
-    _type,
-)
+from .mxfp4 import _TYPES, _check_rotate, _entry, _launch, _rows, _scratch, _type
 
 
 class ExpertPlan:
@@ -37,15 +25,35 @@ class ExpertPlan:
     ``order`` [T * k]: the slot of each row; ``positions`` [T, k]: the row of each slot; ``offsets``
     [E + 1]: where each expert's rows begin, the last where the rows of no expert begin;
     ``scale_rows`` [T, k]: a slot's row among rows padded to whole 128-row tiles an expert (-1: no
-    expert), ``tiles`` [E + 1]: where each expert's tiles begin.
+    expert), ``tiles`` [E + 1]: where each expert's tiles begin.  ``max_tiles`` bounds the tiles of any
+    routing of these sizes.
     """
 
-    __slots__ = ("order", "positions", "scale_rows", "offsets", "tiles", "num_experts", "tokens", "top",
-                 "max_tiles")
+    __slots__ = ("num_experts", "tokens", "top", "rows", "max_tiles", "_buffer", "_at", "_index")
+
+    # the arrays follow one another in one buffer and become tensors when asked for
+    @property
+    def order(self):
+        return self._buffer[:self.rows]
 
     @property
-    def rows(self):
-        return self.tokens * self.top
+    def positions(self):
+        n = self.rows
+        return self._buffer[n:2 * n].view(self.tokens, self.top)
+
+    @property
+    def scale_rows(self):
+        n = self.rows
+        return self._buffer[2 * n:3 * n].view(self.tokens, self.top)
+
+    @property
+    def offsets(self):
+        return self._buffer[3 * self.rows:3 * self.rows + self.num_experts + 1]
+
+    @property
+    def tiles(self):
+        at = 3 * self.rows + self.num_experts + 1
+        return self._buffer[at:at + self.num_experts + 1]
 
     def __repr__(self):
         return f"ExpertPlan(tokens={self.tokens}, top={self.top}, experts={self.num_experts})"
@@ -54,64 +62,65 @@ class ExpertPlan:
 def expert_sort(ids, num_experts):
     """``ids`` [T, k] or [T] (int32 or int64, on the GPU) -> :class:`ExpertPlan`: a stable sort of the
     slots by expert, in one or two launches."""
+    size = ids.element_size()
     if ids.dtype not in (torch.int32, torch.int64):
         raise TypeError(f"ids must be int32 or int64, got {ids.dtype}")
-    if not ids.is_cuda:
+    index = ids.get_device()
+    if index < 0:
         raise TypeError(f"ids must be a CUDA tensor, got {ids.device}")
-    if ids.dim() not in (1, 2):
-        raise ValueError(f"ids must be [T, k] or [T], got {tuple(ids.shape)}")
+    shape = ids.shape
+    if len(shape) not in (1, 2):
+        raise ValueError(f"ids must be [T, k] or [T], got {tuple(shape)}")
     if not 1 <= num_experts <= 1024:
         raise ValueError(f"num_experts must be 1 to 1024, got {num_experts}")
-    ids = ids.contiguous()
-    n, e = ids.numel(), num_experts
+    if not ids.is_contiguous():
+        ids = ids.contiguous()
+    e = num_experts
     plan = ExpertPlan()
-    plan.num_experts, plan.tokens = e, ids.shape[0]
-    plan.top = ids.shape[1] if ids.dim() == 2 else 1
+    plan.num_experts, plan.tokens, plan._index = e, shape[0], index
+    plan.top = shape[1] if len(shape) == 2 else 1
+    n = plan.rows = plan.tokens * plan.top
     plan.max_tiles = n // 128 + min(e, n)
-    lib = _lib()
-    work = lib.xpuint8_expert_sort_workspace_bytes(n, e)
+    work = _entry("expert_sort_workspace_bytes")(n, e)
     if work < 0:
         raise ValueError(f"expert_sort: too many slots ({n})")
-    buffer = torch.empty(3 * n + 2 * (e + 1) + work // 4, dtype=torch.int32, device=ids.device)
-    order, positions, scale_rows, offsets, tiles, work = buffer.split([n, n, n, e + 1, e + 1, work // 4])
-    plan.order, plan.offsets, plan.tiles = order, offsets, tiles
-    plan.positions, plan.scale_rows = positions.view(plan.tokens, plan.top), scale_rows.view(plan.tokens, plan.top)
+    buffer = plan._buffer = torch.empty(3 * n + 2 * (e + 1) + work // 4, dtype=torch.int32, device=ids.device)
+    at = buffer.data_ptr()
+    p, o = at + 12 * n, 4 * (e + 1)
+    plan._at = (at, at + 4 * n, at + 8 * n, p, p + o)
     if n:
-        at = buffer.data_ptr()
-        _launch(lib, "xpuint8_expert_sort_stream", ids.device, ids.data_ptr(), ids.element_size(), n, e,
-                at, at + 4 * n, at + 8 * n, at + 12 * n, at + 12 * n + 4 * (e + 1),
-                at + 12 * n + 8 * (e + 1))
+        _launch("expert_sort", index, ids.data_ptr(), size, n, e, *plan._at, p + 2 * o)
     else:
-        offsets.zero_()
-        tiles.zero_()
+        buffer.zero_()
     return plan
 
 
-def _same_device(x, plan, what):
-    if x.device != plan.order.device:
-        raise ValueError(f"{what} is on {x.device} and the plan on {plan.order.device}")
+def _same_device(index, plan, x, what):
+    if index != plan._index:
+        raise ValueError(f"{what} is on {x.device} and the plan on {plan._buffer.device}")
 
 
 def _gather(x, plan):
     t = _type(x, "x")
     x, ldx = _rows(x)
-    out = torch.empty((plan.rows, x.shape[1]), dtype=x.dtype, device=x.device)
-    if out.numel():
-        _launch(_lib(), "xpuint8_expert_gather_stream", x.device, x.data_ptr(), t, ldx, out.data_ptr(),
-                plan.positions.data_ptr(), plan.scale_rows.data_ptr(), plan.tokens, plan.top, x.shape[1])
+    w = x.shape[1]
+    out = x.new_empty((plan.rows, w))
+    if w and plan.rows:
+        _launch("expert_gather", plan._index, x.data_ptr(), t, ldx, out.data_ptr(), plan._at[1], plan._at[2],
+                plan.tokens, plan.top, w)
     return out
 
 
 def _combine(y, weights, plan):
     t = _type(y, "y")
     y, ldy = _rows(y)
-    out = torch.empty((plan.tokens, y.shape[1]), dtype=y.dtype, device=y.device)
-    if not plan.top:
+    w = y.shape[1]
+    out = y.new_empty((plan.tokens, w))
+    if w and plan.rows:
+        _launch("expert_combine", plan._index, y.data_ptr(), t, ldy, None if weights is None else weights.data_ptr(),
+                out.data_ptr(), plan._at[1], plan._at[2], plan.tokens, plan.top, w)
+    else:
         out.zero_()
-    elif out.numel():
-        _launch(_lib(), "xpuint8_expert_combine_stream", y.device, y.data_ptr(), t, ldy,
-                None if weights is None else weights.data_ptr(), out.data_ptr(),
-                plan.positions.data_ptr(), plan.scale_rows.data_ptr(), plan.tokens, plan.top, y.shape[1])
     return out
 
 
@@ -139,13 +148,13 @@ class _CombineFn(torch.autograd.Function):
         plan = ctx.plan
         dy, ld_dy = _rows(dy)
         y, ld_y = _rows(y)
-        grad_y = torch.empty((plan.rows, y.shape[1]), dtype=y.dtype, device=y.device)
-        grad_w = torch.empty((plan.tokens, plan.top), dtype=torch.float32, device=y.device)
-        if grad_y.numel():
-            _launch(_lib(), "xpuint8_expert_combine_grad_stream", y.device, dy.data_ptr(), _type(y, "y"),
-                    ld_dy, y.data_ptr(), ld_y, weights.data_ptr(), grad_y.data_ptr(), grad_w.data_ptr(),
-                    plan.positions.data_ptr(), plan.scale_rows.data_ptr(), plan.tokens, plan.top,
-                    y.shape[1])
+        w = y.shape[1]
+        grad_y = y.new_empty((plan.rows, w))
+        grad_w = weights.new_empty((plan.tokens, plan.top))
+        if w and plan.rows:
+            _launch("expert_combine_grad", plan._index, dy.data_ptr(), _TYPES[y.dtype], ld_dy, y.data_ptr(), ld_y,
+                    weights.data_ptr(), grad_y.data_ptr(), grad_w.data_ptr(), plan._at[1], plan._at[2], plan.tokens,
+                    plan.top, w)
         else:
             grad_w.zero_()
         return grad_y, grad_w, None
@@ -156,8 +165,9 @@ def expert_gather(x, plan):
     Differentiable: the gradient of a token is the sum of its rows'."""
     if x.dim() != 2 or x.shape[0] != plan.tokens:
         raise ValueError(f"x must be [{plan.tokens}, W], got {tuple(x.shape)}")
-    _same_device(x, plan, "x")
+    _same_device(x.get_device(), plan, x, "x")
     if x.requires_grad and torch.is_grad_enabled():
+        _type(x, "x")
         return _GatherFn.apply(x, plan)
     return _gather(x, plan)
 
@@ -167,61 +177,22 @@ def expert_combine(y, weights, plan):
     its weights, summed in 32 bits.  Differentiable in both."""
     if y.dim() != 2 or y.shape[0] != plan.rows:
         raise ValueError(f"y must be [{plan.rows}, W], got {tuple(y.shape)}")
-    if tuple(weights.shape) != (plan.tokens, plan.top) and weights.numel() != plan.rows:
+    shape = (plan.tokens, plan.top)
+    if weights.shape != shape and weights.numel() != plan.rows:
         raise ValueError(f"weights must be [{plan.tokens}, {plan.top}], got {tuple(weights.shape)}")
-    _same_device(y, plan, "y")
-    _same_device(weights, plan, "weights")
+    _same_device(y.get_device(), plan, y, "y")
+    _same_device(weights.get_device(), plan, weights, "weights")
     if not weights.is_floating_point():
         raise TypeError(f"weights must be floating point, got {weights.dtype}")
-    if weights.dtype != torch.float32 or weights.dim() != 2 or not weights.is_contiguous():
-        weights = weights.to(torch.float32).reshape(plan.tokens, plan.top).contiguous()
-    if torch.is_grad_enabled() and (y.requires_grad or weights.requires_grad):
+    if weights.dtype != torch.float32 or weights.shape != shape or not weights.is_contiguous():
+        weights = weights.to(torch.float32).reshape(shape).contiguous()
+    if (y.requires_grad or weights.requires_grad) and torch.is_grad_enabled():
+        _type(y, "y")
         return _CombineFn.apply(y, weights, plan)
     return _combine(y, weights, plan)
 
 
 # ------------------------------------------------------------------------------ the experts' product
-
-def _quantize_sorted(x, plan, rotate, in_order, keep=False):
-    """(codes of the plan's rows, scales in padded tiles, x's rotated values): x holds tokens, or the
-    plan's rows (in_order)."""
-    t = _type(x, "x")
-    x, ldx = _rows(x)
-    k = x.shape[1]
-    codes = torch.empty((plan.rows, (k + 31) // 32 * 16), dtype=torch.uint8, device=x.device)
-    scales = torch.empty((plan.max_tiles, (k + 127) // 128, 32, 16), dtype=torch.uint8, device=x.device)
-    rotated = torch.empty(x.shape, dtype=x.dtype, device=x.device) if keep and rotate else None
-    _launch(_lib(), "xpuint8_mxfp4_quantize_sorted_stream", x.device, x.data_ptr(), t, ldx,
-            codes.data_ptr(), scales.data_ptr(), None if rotated is None else rotated.data_ptr(),
-            plan.order.data_ptr() if in_order else None, plan.positions.data_ptr(),
-            plan.scale_rows.data_ptr(), x.shape[0], 1 if in_order else plan.top, k, 1 if rotate else 0)
-    return codes, scales, (rotated if rotate else x)
-
-
-def _quantize_sorted_columns(x, plan):
-    """x's rows (in the plan's order) quantised along the rows, each expert's padded to whole tiles:
-    codes [W, max_tiles * 64], scales."""
-    t = _type(x, "x")
-    x, ldx = _rows(x)
-    w, tiles = x.shape[1], plan.max_tiles
-    codes = torch.empty((w, tiles * 64), dtype=torch.uint8, device=x.device)
-    scales = torch.empty(((w + 127) // 128, tiles, 32, 16), dtype=torch.uint8, device=x.device)
-    _launch(_lib(), "xpuint8_mxfp4_quantize_columns_stream", x.device, x.data_ptr(), t, ldx,
-            codes.data_ptr(), scales.data_ptr(), x.shape[0], w, 1, plan.offsets.data_ptr(),
-            plan.tiles.data_ptr(), plan.num_experts, tiles)
-    return codes, scales
-
-
-def _expert_mm(codes, scales, w, plan, dtype):
-    n, k = w.shape[1:]
-    out = torch.empty((plan.rows, n), dtype=dtype, device=codes.device)
-    if out.numel():
-        _launch(_lib(), "xpuint8_mxfp4_expert_mm_stream", out.device, codes.data_ptr(), scales.data_ptr(),
-                w.codes.data_ptr(), w.scales.data_ptr(), out.data_ptr(), _TYPES[dtype],
-                plan.offsets.data_ptr(), plan.tiles.data_ptr(), plan.rows, plan.max_tiles, n, k,
-                plan.num_experts)
-    return out
-
 
 def _check_product(x, shape, plan, rotate, in_order):
     if len(shape) != 3 or shape[0] != plan.num_experts or x.dim() != 2 or x.shape[1] != shape[2]:
@@ -233,8 +204,9 @@ def _check_product(x, shape, plan, rotate, in_order):
                          f"got {x.shape[0]}")
     if shape[2] == 0:
         raise ValueError("the experts' weight needs K of at least 1")
-    _same_device(x, plan, "x")
-    _check_rotate(shape[2], rotate)
+    _same_device(x.get_device(), plan, x, "x")
+    if rotate and shape[2] % 256:
+        _check_rotate(shape[2], rotate)
 
 
 def expert_linear_mxfp4(x, w, plan, *, rotate=True, sorted=False):
@@ -245,12 +217,25 @@ def expert_linear_mxfp4(x, w, plan, *, rotate=True, sorted=False):
     Rows of no expert are zero.
     """
     _check_product(x, w.shape, plan, rotate, sorted)
-    _same_device(w, plan, "the weight")
-    x = x.detach()
-    if plan.rows == 0:
-        return torch.empty((0, w.shape[1]), dtype=x.dtype, device=x.device)
-    codes, scales, _ = _quantize_sorted(x, plan, rotate, sorted)
-    return _expert_mm(codes, scales, w, plan, x.dtype)
+    t = _type(x, "x")
+    if w._index != plan._index:
+        raise ValueError(f"the weight is on {w.device} and the plan on {plan._buffer.device}")
+    if x.requires_grad:
+        x = x.detach()
+    e, n, k = w.shape
+    rows = plan.rows
+    x, ldx = _rows(x)
+    out = x.new_empty((rows, n))
+    if rows and n:
+        p = x.data_ptr()
+        # up to 128 aligned rows are quantised inside the product, without scratch
+        work = None
+        if rows > 128 or p % 16 or ldx * x.element_size() % 16:
+            work = _scratch(_entry("mxfp4_expert_linear_workspace_bytes")(rows, plan.max_tiles, k), x.device)
+        _launch("mxfp4_expert_linear", plan._index, p, t, ldx, w._cp, w._sp, out.data_ptr(),
+                None if work is None else work.data_ptr(), *plan._at, plan.tokens, plan.top, plan.max_tiles, n, k, e,
+                1 if rotate else 0, 1 if sorted else 0)
+    return out
 
 
 class _ExpertLinearFn(torch.autograd.Function):
@@ -259,34 +244,45 @@ class _ExpertLinearFn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, w, plan, rotate, in_order):
-        codes, scales, xr = _quantize_sorted(x, plan, rotate, in_order, keep=True)
-        wq, wr = _quantize(w, rotate, keep=True)
-        ctx.save_for_backward(xr, wr)
-        ctx.plan, ctx.rotate, ctx.in_order = plan, rotate, in_order
-        return _expert_mm(codes, scales, wq, plan, x.dtype)
+        e, n, k = w.shape
+        w = w.contiguous()
+        x2, ldx = _rows(x)
+        rows, device = plan.rows, x.device
+        need = ctx.needs_input_grad
+        want = (1 if need[0] else 0) | (2 if need[1] else 0)
+        y = x2.new_empty((rows, n))
+        flags = (1 if rotate else 0, 1 if in_order else 0)
+        if n:
+            saved = _scratch(_entry("mxfp4_expert_train_saved_workspace_bytes")(plan.max_tiles, n, k, e, want), device)
+            work = _scratch(_entry("mxfp4_expert_train_workspace_bytes")(rows, plan.max_tiles, n, k, e), device)
+            _launch("mxfp4_expert_train", plan._index, x2.data_ptr(), _TYPES[x.dtype], ldx, w.data_ptr(), _TYPES[w.dtype],
+                    y.data_ptr(), saved.data_ptr() if want else None, work.data_ptr(), *plan._at, plan.tokens, plan.top,
+                    plan.max_tiles, n, k, e, *flags, want)
+            ctx.save_for_backward(saved)
+        ctx.plan, ctx.sizes, ctx.like = plan, (e, n, k, want, flags), (x.dtype, w.dtype)
+        return y
 
     @staticmethod
     def backward(ctx, dy):
-        xr, wr = ctx.saved_tensors
         plan = ctx.plan
-        dx = dw = None
-        dy = dy.contiguous()
-        if ctx.needs_input_grad[0]:
-            codes, scales, _ = _quantize_sorted(dy, plan, False, True)
-            dx = _expert_mm(codes, scales, _quantize_columns(wr), plan, xr.dtype)
-            if not ctx.in_order:
-                dx = _combine(dx, None, plan)
-            dx = _rotate(dx) if ctx.rotate else dx
-        if ctx.needs_input_grad[1]:
-            e, n, k = wr.shape
-            a = _quantize_sorted_columns(dy, plan)
-            b = _quantize_sorted_columns(xr if ctx.in_order else _gather(xr, plan), plan)
-            dw = torch.empty((e, n, k), dtype=wr.dtype, device=wr.device)
-            if dw.numel():
-                _launch(_lib(), "xpuint8_mxfp4_expert_dw_stream", dw.device, a[0].data_ptr(),
-                        a[1].data_ptr(), b[0].data_ptr(), b[1].data_ptr(), dw.data_ptr(),
-                        _TYPES[dw.dtype], plan.tiles.data_ptr(), plan.max_tiles, n, k, e)
-            dw = _rotate(dw) if ctx.rotate else dw
+        e, n, k, want, flags = ctx.sizes
+        x_type, w_type = ctx.like
+        need = ctx.needs_input_grad
+        dy, ld = _rows(dy)
+        device = dy.device
+        rows = plan.rows
+        dx = torch.empty((rows if flags[1] else plan.tokens, k), dtype=x_type, device=device) if need[0] else None
+        dw = torch.empty((e, n, k), dtype=w_type, device=device) if need[1] else None
+        if n and (need[0] or need[1]):
+            saved, = ctx.saved_tensors
+            have = (1 if need[0] else 0) | (2 if need[1] else 0)
+            w_code = _TYPES[w_type]
+            work = _scratch(_entry("mxfp4_expert_grad_workspace_bytes")(rows, plan.max_tiles, n, k, e, w_code, *flags, have), device)
+            _launch("mxfp4_expert_grad", plan._index, dy.data_ptr(), _TYPES[x_type], ld, saved.data_ptr(),
+                    dx.data_ptr() if need[0] else None, dw.data_ptr() if need[1] else None, w_code, work.data_ptr(),
+                    *plan._at, plan.tokens, plan.top, plan.max_tiles, n, k, e, *flags, want)
+        elif need[0]:
+            dx.zero_()
         return dx, dw, None, None, None
 
 
@@ -296,7 +292,7 @@ def mxfp4_expert_linear(x, w, plan, *, rotate=True, sorted=False):
     _check_product(x, w.shape, plan, rotate, sorted)
     _type(x, "x")
     _type(w, "w")
-    _same_device(w, plan, "w")
+    _same_device(w.get_device(), plan, w, "w")
     if plan.rows == 0:
         return x.reshape(0, x.shape[1]) @ w.sum(0).to(x.dtype).T
     return _ExpertLinearFn.apply(x, w, plan, rotate, sorted)

@@ -102,6 +102,21 @@ def _signatures():
         "xpuint8_mxfp4_mm_stream": [vp] * 7 + [i32] + [i64] * 4,
         "xpuint8_mxfp4_expert_mm_stream": [vp] * 6 + [i32, vp, vp] + [i64] * 5,
         "xpuint8_mxfp4_expert_dw_stream": [vp] * 6 + [i32, vp] + [i64] * 4,
+        "xpuint8_mxfp4_linear_workspace_bytes": [i64] * 2,
+        "xpuint8_mxfp4_linear_stream": [vp, vp, i32, i64] + [vp] * 5 + [i64] * 3 + [i32],
+        "xpuint8_mxfp4_train_saved_workspace_bytes": [i64] * 3 + [i32],
+        "xpuint8_mxfp4_train_workspace_bytes": [i64] * 3,
+        "xpuint8_mxfp4_train_stream": [vp, vp, i32, i64, vp, i32, i64] + [vp] * 4 + [i64] * 3 + [i32] * 2,
+        "xpuint8_mxfp4_grad_workspace_bytes": [i64] * 3 + [i32] * 3,
+        "xpuint8_mxfp4_grad_stream": [vp, vp, i32, i64, vp, vp, vp, i32, vp] + [i64] * 3 + [i32] * 2,
+        "xpuint8_mxfp4_expert_linear_workspace_bytes": [i64] * 3,
+        "xpuint8_mxfp4_expert_linear_stream": [vp, vp, i32, i64] + [vp] * 9 + [i64] * 6 + [i32] * 2,
+        "xpuint8_mxfp4_expert_train_saved_workspace_bytes": [i64] * 4 + [i32],
+        "xpuint8_mxfp4_expert_train_workspace_bytes": [i64] * 5,
+        "xpuint8_mxfp4_expert_train_stream": [vp, vp, i32, i64, vp, i32] + [vp] * 8 + [i64] * 6 + [i32] * 3,
+        "xpuint8_mxfp4_expert_grad_workspace_bytes": [i64] * 5 + [i32] * 4,
+        "xpuint8_mxfp4_expert_grad_stream": [vp, vp, i32, i64, vp, vp, vp, i32] + [vp] * 6 + [i64] * 6
+                                            + [i32] * 3,
         "xpuint8_expert_sort_workspace_bytes": [i64] * 2,
         "xpuint8_expert_sort_stream": [vp, vp, i32, i64, i64] + [vp] * 6,
         "xpuint8_expert_gather_stream": [vp, vp, i32, i64] + [vp] * 3 + [i64] * 3,

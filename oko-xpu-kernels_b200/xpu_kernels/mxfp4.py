@@ -22,21 +22,31 @@ from .int8._lib import _err, _lib
 
 _TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 _raw_stream = torch._C._cuda_getCurrentRawStream
+_current = torch._C._cuda_getDevice
+_entries = {}
 
 
-def _launch(lib, entry, device, *args):
-    """One C entry on the current stream of `device`; raises what it reports."""
-    index = device.index
-    if index == torch.cuda.current_device():
-        rc = getattr(lib, entry)(_raw_stream(index), *args)
+def _entry(name):
+    fn = _entries.get(name)
+    if fn is None:
+        fn = _entries[name] = getattr(_lib(), "xpuint8_" + name)
+    return fn
+
+
+def _launch(name, index, *args):
+    """The C entry xpuint8_<name>_stream on the current stream of device `index`; raises what it reports."""
+    fn = _entry(name + "_stream")
+    if index == _current():
+        rc = fn(_raw_stream(index), *args)
     else:
         with torch.cuda.device(index):
-            rc = getattr(lib, entry)(_raw_stream(index), *args)
-    if rc != 0:
-        _err(lib, entry[len("xpuint8_"):-len("_stream")])
+            rc = fn(_raw_stream(index), *args)
+    if rc:
+        _err(_lib(), name)
 
 
 def _type(x, what):
+    """x's type for the C entries; raises where there is none or x is not on a GPU."""
     t = _TYPES.get(x.dtype)
     if t is None:
         raise TypeError(f"{what} must be bfloat16, float16 or float32, got {x.dtype}")
@@ -47,9 +57,16 @@ def _type(x, what):
 
 def _rows(x):
     """x [R, K] with unit column stride (a copy where it has none), and its row stride."""
-    if x.stride(1) != 1 and x.shape[1] != 1 or x.shape[0] > 1 and x.stride(0) < x.shape[1]:
-        x = x.contiguous()
-    return x, (x.stride(0) if x.shape[0] > 1 else x.shape[1])
+    if x.is_contiguous():
+        return x, x.shape[1]
+    r, k = x.shape
+    if k != 1 and x.stride(1) != 1 or r > 1 and x.stride(0) < k:
+        return x.contiguous(), k
+    return x, (x.stride(0) if r > 1 else k)
+
+
+def _scratch(n, device):
+    return torch.empty(n, dtype=torch.uint8, device=device)
 
 
 def _check_rotate(k, rotate):
@@ -66,26 +83,60 @@ class MXFP4:
     aligned, so they can be saved and loaded as they are.
     """
 
-    __slots__ = ("codes", "scales", "shape")
+    __slots__ = ("shape", "_codes", "_scales", "_buffer", "_at", "_cp", "_sp", "_index")
 
     def __init__(self, codes, scales, shape):
-        shape = tuple(int(n) for n in shape)
-        if len(shape) not in (2, 3):
-            raise ValueError(f"an MXFP4 matrix has the shape [R, K] or [E, R, K], got {shape}")
-        r, k = shape[-2:]
-        lead = shape[:-2]
-        want_codes = (*lead, r, (k + 31) // 32 * 16)
-        want_scales = (*lead, (r + 127) // 128, (k + 127) // 128, 32, 16)
+        if len(shape) == 2:
+            r, k = shape
+            want_codes, want_scales = (r, (k + 31) // 32 * 16), ((r + 127) // 128, (k + 127) // 128, 32, 16)
+        elif len(shape) == 3:
+            n, r, k = shape
+            want_codes = (n, r, (k + 31) // 32 * 16)
+            want_scales = (n, (r + 127) // 128, (k + 127) // 128, 32, 16)
+        else:
+            raise ValueError(f"an MXFP4 matrix has the shape [R, K] or [E, R, K], got {tuple(shape)}")
         if codes.dtype != torch.uint8 or scales.dtype != torch.uint8:
             raise TypeError(f"codes and scales must be uint8, got {codes.dtype} and {scales.dtype}")
-        if tuple(codes.shape) != want_codes or tuple(scales.shape) != want_scales:
-            raise ValueError(f"an MXFP4 matrix {shape} has codes {want_codes} and scales {want_scales}, "
+        if codes.shape != want_codes or scales.shape != want_scales:
+            raise ValueError(f"an MXFP4 matrix {tuple(shape)} has codes {want_codes} and scales {want_scales}, "
                              f"got {tuple(codes.shape)} and {tuple(scales.shape)}")
-        if codes.device != scales.device:
+        index = codes.get_device()
+        if index != scales.get_device():
             raise ValueError(f"codes are on {codes.device} and scales on {scales.device}")
         if not codes.is_contiguous() or not scales.is_contiguous():
             raise ValueError("codes and scales must be contiguous")
-        self.codes, self.scales, self.shape = codes, scales, shape
+        self.shape = tuple(shape)
+        self._codes, self._scales, self._index = codes, scales, index
+        self._cp, self._sp = codes.data_ptr(), scales.data_ptr()
+
+    @classmethod
+    def _empty(cls, shape, device, index):
+        """An unwritten matrix: codes and scales in one buffer, made into tensors when asked for."""
+        r, k = shape[-2:]
+        n = shape[0] if len(shape) == 3 else 1
+        at = (n * r * ((k + 31) // 32 * 16) + 255) // 256 * 256
+        q = cls.__new__(cls)
+        q._buffer = torch.empty(at + n * ((r + 127) // 128) * ((k + 127) // 128) * 512, dtype=torch.uint8,
+                                device=device)
+        q.shape, q._codes, q._scales, q._at, q._index = tuple(shape), None, None, at, index
+        q._cp = q._buffer.data_ptr()
+        q._sp = q._cp + at
+        return q
+
+    @property
+    def codes(self):
+        if self._codes is None:
+            *lead, r, k = self.shape
+            row = (k + 31) // 32 * 16
+            self._codes = self._buffer[:(lead[0] if lead else 1) * r * row].view(*lead, r, row)
+        return self._codes
+
+    @property
+    def scales(self):
+        if self._scales is None:
+            *lead, r, k = self.shape
+            self._scales = self._buffer[self._at:].view(*lead, (r + 127) // 128, (k + 127) // 128, 32, 16)
+        return self._scales
 
     @property
     def device(self):
@@ -95,78 +146,39 @@ class MXFP4:
         return f"MXFP4({self.shape}, device={self.device})"
 
 
-def _empty(shape, device):
-    *lead, r, k = shape
-    q = MXFP4.__new__(MXFP4)
-    q.codes = torch.empty((*lead, r, (k + 31) // 32 * 16), dtype=torch.uint8, device=device)
-    q.scales = torch.empty((*lead, (r + 127) // 128, (k + 127) // 128, 32, 16), dtype=torch.uint8,
-                           device=device)
-    q.shape = tuple(shape)
-    return q
-
-
-def _quantize(x, rotate=False, keep=False):
-    """(MXFP4 of x [R, K] or [E, R, K], the rotated values where `keep` asks for them)."""
-    t = _type(x, "x")
-    k = x.shape[-1]
-    if x.dim() == 2:
-        x, ldx = _rows(x)
-        each = x.shape[0]
-    else:
-        x, ldx, each = x.contiguous(), k, x.shape[-2]
-    q = _empty(x.shape, x.device)
-    rotated = torch.empty(x.shape, dtype=x.dtype, device=x.device) if keep and rotate else None
-    rows = x.numel() // k if k else 0
-    if rows:
-        _launch(_lib(), "xpuint8_mxfp4_quantize_stream", x.device, x.data_ptr(), t, ldx,
-                q.codes.data_ptr(), q.scales.data_ptr(), rotated.data_ptr() if keep and rotate else None,
-                rows, k, each, 1 if rotate else 0)
-    return q, (rotated if rotate else x)
-
-
-def _quantize_columns(x):
-    """MXFP4 of x's transpose: [R, C] -> [C, R], [E, R, C] -> [E, C, R]."""
-    t = _type(x, "x")
-    rows, cols = x.shape[-2:]
-    if x.dim() == 2:
-        x, ldx = _rows(x)
-        matrices, shape = 1, (cols, rows)
-    else:
-        x, ldx, matrices = x.contiguous(), cols, x.shape[0]
-        shape = (matrices, cols, rows)
-    q = _empty(shape, x.device)
-    if x.numel():
-        _launch(_lib(), "xpuint8_mxfp4_quantize_columns_stream", x.device, x.data_ptr(), t, ldx,
-                q.codes.data_ptr(), q.scales.data_ptr(), rows, cols, matrices, None, None, 0, 0)
-    return q
-
-
-def _rotate(x):
-    """The rotation alone, of x's type, along the last axis."""
-    x = x.contiguous()
-    out = torch.empty_like(x)
-    k = x.shape[-1]
-    if x.numel():
-        rows = x.numel() // k
-        _launch(_lib(), "xpuint8_mxfp4_quantize_stream", x.device, x.data_ptr(), _type(x, "x"), k, None,
-                None, out.data_ptr(), rows, k, rows, 1)
-    return out
-
-
 def quantize_mxfp4(x, *, rotate=False, transpose=False):
     """``x`` [R, K] or a stack [E, R, K] (bf16, fp16, fp32; any K) -> :class:`MXFP4` along K.
 
     ``rotate`` puts the group-256 rotation in front (K a multiple of 256), its result rounded to x's
     type.  ``transpose`` gives the MXFP4 of ``x``'s transpose instead, blocks along R.
     """
-    if x.dim() not in (2, 3):
-        raise ValueError(f"x must be [R, K] or [E, R, K], got {tuple(x.shape)}")
+    shape = x.shape
+    if len(shape) == 2:
+        r, k = shape
+        n = 1
+    elif len(shape) == 3:
+        n, r, k = shape
+    else:
+        raise ValueError(f"x must be [R, K] or [E, R, K], got {tuple(shape)}")
+    if transpose and rotate:
+        raise ValueError("rotate goes along K: transpose quantises along the other axis")
+    if rotate and k % 256:
+        _check_rotate(k, rotate)
+    t = _type(x, "x")
+    if len(shape) == 2:
+        x, ldx = _rows(x)
+    else:
+        x, ldx = x.contiguous(), k
+    index = x.get_device()
     if transpose:
-        if rotate:
-            raise ValueError("rotate goes along K: transpose quantises along the other axis")
-        return _quantize_columns(x)
-    _check_rotate(x.shape[-1], rotate)
-    return _quantize(x, rotate)[0]
+        q = MXFP4._empty((*shape[:-2], k, r), x.device, index)
+        if n and r and k:
+            _launch("mxfp4_quantize_columns", index, x.data_ptr(), t, ldx, q._cp, q._sp, r, k, n, None, None, 0, 0)
+    else:
+        q = MXFP4._empty(shape, x.device, index)
+        if n and r and k:
+            _launch("mxfp4_quantize", index, x.data_ptr(), t, ldx, q._cp, q._sp, None, n * r, k, r, 1 if rotate else 0)
+    return q
 
 
 def dequantize_mxfp4(q, dtype=torch.bfloat16):
@@ -174,11 +186,11 @@ def dequantize_mxfp4(q, dtype=torch.bfloat16):
     t = _TYPES.get(dtype)
     if t is None:
         raise TypeError(f"dtype must be bfloat16, float16 or float32, got {dtype}")
-    out = torch.empty(q.shape, dtype=dtype, device=q.device)
-    if out.numel():
+    out = torch.empty(q.shape, dtype=dtype, device=q._buffer.device if q._codes is None else q._codes.device)
+    n = out.numel()
+    if n:
         r, k = q.shape[-2:]
-        _launch(_lib(), "xpuint8_mxfp4_dequantize_stream", out.device, q.codes.data_ptr(),
-                q.scales.data_ptr(), out.data_ptr(), t, out.numel() // k, k, r)
+        _launch("mxfp4_dequantize", q._index, q._cp, q._sp, out.data_ptr(), t, n // k, k, r)
     return out
 
 
@@ -192,31 +204,31 @@ def _bias(bias, n, device):
         return None
     if bias.numel() != n:
         raise ValueError(f"bias has {bias.numel()} values; expected N={n}")
-    b = bias.detach().reshape(-1).to(device=device, dtype=torch.float32).contiguous()
+    b = bias.detach()
+    if b.dtype != torch.float32 or b.device != device or not b.is_contiguous():
+        b = b.to(device=device, dtype=torch.float32).contiguous()
     return b.clone() if b.data_ptr() % 16 else b
-
-
-def _mm(a, b, bias, dtype):
-    m, n, k = a.shape[0], b.shape[0], a.shape[1]
-    out = torch.empty((m, n), dtype=dtype, device=a.codes.device)
-    if m and n:
-        _launch(_lib(), "xpuint8_mxfp4_mm_stream", out.device, a.codes.data_ptr(), a.scales.data_ptr(),
-                b.codes.data_ptr(), b.scales.data_ptr(), None if bias is None else bias.data_ptr(),
-                out.data_ptr(), _TYPES[dtype], n, m, n, k)
-    return out
 
 
 def mxfp4_mm(a, b, bias=None, dtype=torch.bfloat16):
     """``a @ b.T (+ bias)`` of two MXFP4 matrices [M, K] and [N, K]: summed in 32 bits, rounded once."""
     if len(a.shape) != 2 or len(b.shape) != 2 or a.shape[1] != b.shape[1]:
         raise ValueError(f"mxfp4_mm takes [M, K] and [N, K], got {a.shape} and {b.shape}")
-    if a.shape[1] == 0:
+    (m, k), n = a.shape, b.shape[0]
+    if k == 0:
         raise ValueError("mxfp4_mm needs K of at least 1")
-    if dtype not in _TYPES:
+    t = _TYPES.get(dtype)
+    if t is None:
         raise TypeError(f"dtype must be bfloat16, float16 or float32, got {dtype}")
-    if a.device != b.device:
+    if a._index != b._index:
         raise ValueError(f"a is on {a.device} and b on {b.device}")
-    return _mm(a, b, _bias(bias, b.shape[0], a.device), dtype)
+    device = a.device
+    bias = _bias(bias, n, device)
+    out = torch.empty((m, n), dtype=dtype, device=device)
+    if m and n:
+        _launch("mxfp4_mm", a._index, a._cp, a._sp, b._cp, b._sp, None if bias is None else bias.data_ptr(),
+                out.data_ptr(), t, n, m, n, k)
+    return out
 
 
 def linear_mxfp4(x, w, bias=None, *, rotate=True):
@@ -225,50 +237,87 @@ def linear_mxfp4(x, w, bias=None, *, rotate=True):
     ``w`` is the :class:`MXFP4` weight [N, K] of :func:`prepare_weight_mxfp4`, ``rotate`` what it was
     prepared with.  ``bias`` is added in 32 bits before the one rounding.
     """
-    if len(w.shape) != 2 or x.shape[-1] != w.shape[1]:
-        raise ValueError(f"x has {x.shape[-1]} columns and the weight is {w.shape}")
-    if x.device != w.codes.device:
+    shape = x.shape
+    if len(w.shape) != 2 or shape[-1] != w.shape[1]:
+        raise ValueError(f"x has {shape[-1]} columns and the weight is {w.shape}")
+    index = x.get_device()
+    if index != w._index:
         raise ValueError(f"x is on {x.device} and the weight on {w.device}")
     n, k = w.shape
-    _check_rotate(k, rotate)
-    x2 = x.detach().reshape(-1, k)
-    q, _ = _quantize(x2, rotate)
-    out = _mm(q, w, _bias(bias, n, x.device), x.dtype)
-    return out if x.dim() == 2 else out.reshape(*x.shape[:-1], n)
+    if rotate and k % 256:
+        _check_rotate(k, rotate)
+    t = _type(x, "x")
+    if x.requires_grad:
+        x = x.detach()
+    x2, ldx = _rows(x if len(shape) == 2 else x.reshape(-1, k))
+    m = x2.shape[0]
+    if bias is not None:
+        bias = _bias(bias, n, x.device)
+    out = x2.new_empty((m, n))
+    if m and n:
+        p = x2.data_ptr()
+        # up to 16 aligned rows are quantised inside the product, without scratch
+        work = None
+        if m > 16 or p % 16 or ldx * x2.element_size() % 16:
+            work = _scratch(_entry("mxfp4_linear_workspace_bytes")(m, k), x.device)
+        _launch("mxfp4_linear", index, p, t, ldx, w._cp, w._sp, None if bias is None else bias.data_ptr(),
+                out.data_ptr(), None if work is None else work.data_ptr(), m, n, k, 1 if rotate else 0)
+    return out if len(shape) == 2 else out.reshape(*shape[:-1], n)
 
 
 class _Mxfp4LinearFn(torch.autograd.Function):
     """y = Q(x) Q(w)^T with both operands quantised along K; the gradients' products quantise their
     operands along their own contractions, dy and w along N for dx, dy and x along the rows for dw
-    (straight through the roundings)."""
+    (straight through the roundings).  What is kept is in 4 bits: x and w along those axes, where
+    their gradient is wanted."""
 
     @staticmethod
     def forward(ctx, x, w, bias, rotate):
-        k = x.shape[-1]
-        xq, xr = _quantize(x.reshape(-1, k), rotate, keep=True)
-        wq, wr = _quantize(w, rotate, keep=True)
-        ctx.save_for_backward(xr, wr)
-        ctx.rotate, ctx.shape = rotate, x.shape
-        ctx.bias_type = None if bias is None else bias.dtype
-        return _mm(xq, wq, _bias(bias, w.shape[0], x.device), x.dtype).reshape(*x.shape[:-1], w.shape[0])
+        n, k = w.shape
+        x2, ldx = _rows(x.reshape(-1, k))
+        w2, ldw = _rows(w)
+        m, device, index = x2.shape[0], x.device, x.get_device()
+        need = ctx.needs_input_grad
+        want = (1 if need[0] else 0) | (2 if need[1] else 0)
+        y = x2.new_empty((m, n))
+        saved = None
+        if m and n:
+            if want:
+                saved = _scratch(_entry("mxfp4_train_saved_workspace_bytes")(m, n, k, want), device)
+            work = _scratch(_entry("mxfp4_train_workspace_bytes")(m, n, k), device)
+            b = _bias(bias, n, device)
+            _launch("mxfp4_train", index, x2.data_ptr(), _TYPES[x.dtype], ldx, w2.data_ptr(), _TYPES[w.dtype], ldw,
+                    None if b is None else b.data_ptr(), y.data_ptr(), None if saved is None else saved.data_ptr(),
+                    work.data_ptr(), m, n, k, 1 if rotate else 0, want)
+        if saved is not None:
+            ctx.save_for_backward(saved)
+        ctx.sizes = (m, n, k, want, rotate)
+        ctx.like = (x.dtype, w.dtype, None if bias is None else bias.dtype, x.shape)
+        return y.reshape(*x.shape[:-1], n)
 
     @staticmethod
     def backward(ctx, dy):
-        xr, wr = ctx.saved_tensors
-        dy = dy.reshape(-1, dy.shape[-1])
-        dx = dw = db = None
-        if ctx.needs_input_grad[0]:
-            dx = _mm(_quantize(dy)[0], _quantize_columns(wr), None, xr.dtype)
-            dx = (_rotate(dx) if ctx.rotate else dx).reshape(ctx.shape)
-        if ctx.needs_input_grad[1]:
-            if dy.shape[0]:
-                dw = _mm(_quantize_columns(dy), _quantize_columns(xr), None, wr.dtype)
-                dw = _rotate(dw) if ctx.rotate else dw
-            else:
-                dw = torch.zeros_like(wr)
-        if ctx.needs_input_grad[2]:
-            db = dy.sum(dim=0, dtype=torch.float32).to(ctx.bias_type)
-        return dx, dw, db, None
+        m, n, k, want, rotate = ctx.sizes
+        x_type, w_type, bias_type, shape = ctx.like
+        need = ctx.needs_input_grad
+        dy2, ld = _rows(dy.reshape(-1, n))
+        device = dy.device
+        dx = torch.empty((m, k), dtype=x_type, device=device) if need[0] else None
+        dw = torch.empty((n, k), dtype=w_type, device=device) if need[1] else None
+        if m and n and (need[0] or need[1]):
+            saved, = ctx.saved_tensors
+            have = (1 if need[0] else 0) | (2 if need[1] else 0)
+            w_code = _TYPES[w_type]
+            work = _scratch(_entry("mxfp4_grad_workspace_bytes")(m, n, k, w_code, 1 if rotate else 0, have), device)
+            _launch("mxfp4_grad", dy.get_device(), dy2.data_ptr(), _TYPES[x_type], ld, saved.data_ptr(),
+                    dx.data_ptr() if need[0] else None, dw.data_ptr() if need[1] else None, w_code, work.data_ptr(),
+                    m, n, k, 1 if rotate else 0, want)
+        else:
+            for g in (dx, dw):
+                if g is not None:
+                    g.zero_()
+        db = dy2.sum(dim=0, dtype=torch.float32).to(bias_type) if need[2] else None
+        return (None if dx is None else dx.reshape(shape)), dw, db, None
 
 
 def mxfp4_linear(x, w, bias=None, *, rotate=True):
@@ -278,8 +327,10 @@ def mxfp4_linear(x, w, bias=None, *, rotate=True):
         raise ValueError(f"x has {x.shape[-1]} columns and the weight is {tuple(w.shape)}")
     _type(x, "x")
     _type(w, "w")
-    if x.device != w.device:
+    if x.get_device() != w.get_device():
         raise ValueError(f"x is on {x.device} and the weight on {w.device}")
+    if w.shape[1] == 0:
+        raise ValueError("mxfp4_linear needs K of at least 1")
     _check_rotate(w.shape[1], rotate)
     return _Mxfp4LinearFn.apply(x, w, bias, rotate)
 
