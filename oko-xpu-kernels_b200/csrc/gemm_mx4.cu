@@ -545,6 +545,7 @@ struct FewArgs {
     int K;
     const int32_t *order;            // FUSE, rows: row r is slot order[r]'s token (fan > 0) or x's row r
     int fan;
+    int vec_out;                     // four neighbouring outputs are aligned to their bytes
 };
 
 enum Fuse { kFuseNone = 0, kFusePlain = 1, kFuseRotate = 2 };
@@ -733,15 +734,15 @@ __global__ void __launch_bounds__(kFewThreads, 2)
         bool ok = true;
         for (int it = 0; ok && it < tasks; it += 8) {
             const bool mine = t < tasks;
+            PairCodes q;
             if constexpr (FUSE == kFuseRotate) {
                 const uint32_t tile = ring + C::kRing + slot * kSlotBytes;
                 rotate_to_shared<T>(A, B, tile, l);
-                runs_from_shared<T>(A, B, tile, l);
+                q = quantize_pairs<T>(pairs_from_shared<T>(tile, l));
                 __syncwarp();
+            } else {
+                q = quantize_runs<T>(A, B);
             }
-            uint32_t e0, e1;
-            const uint2 c0 = quantize_run<T>(A, e0), c1 = quantize_run<T>(B, e1);
-            const uint32_t w0 = join_scales(e0), w1 = join_scales(e1);
             const int r = 2 * rp, local = kb - k0, stage = local % stages;
             t += 8;
             if (t < tasks) {  // the next task's loads, before this one's wait
@@ -756,13 +757,13 @@ __global__ void __launch_bounds__(kFewThreads, 2)
                 const uint32_t at = ring + stage * stage_bytes + w_bytes, sx = at + x_bytes + kScaleBlock;
                 // K-major rows of 128 bytes, 16-byte chunk c of row r at c ^ (r & 7)
                 const uint32_t a0 = at + r * 128 + (((l >> 1) ^ (r & 7)) << 4) + (l & 1) * 8;
-                asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(a0), "r"(c0.x), "r"(c0.y) : "memory");
+                asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(a0), "r"(q.c0.x), "r"(q.c0.y) : "memory");
                 const uint32_t a1 = at + (r + 1) * 128 + (((l >> 1) ^ ((r + 1) & 7)) << 4) + (l & 1) * 8;
-                asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(a1), "r"(c1.x), "r"(c1.y) : "memory");
+                asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(a1), "r"(q.c1.x), "r"(q.c1.y) : "memory");
                 if ((l & 7) == 0) {
                     const uint32_t s0 = sx + (l >> 3) * kMxTileBytes + (r & 31) * 16 + (r >> 5) * 4;
-                    asm volatile("st.shared.b32 [%0], %1;" ::"r"(s0), "r"(w0) : "memory");
-                    asm volatile("st.shared.b32 [%0], %1;" ::"r"(s0 + 16), "r"(w1) : "memory");
+                    asm volatile("st.shared.b32 [%0], %1;" ::"r"(s0), "r"(q.w0) : "memory");
+                    asm volatile("st.shared.b32 [%0], %1;" ::"r"(s0 + 16), "r"(q.w1) : "memory");
                 }
                 fence_async_smem();
             }
@@ -772,6 +773,31 @@ __global__ void __launch_bounds__(kFewThreads, 2)
     }
     __syncthreads();  // every load has landed and every MMA is done: the ring is free
     tc_fence_after();
+    if (splits == 1) {
+        // a lane is a row of the weight: for each token a warp stores 32 neighbouring outputs
+        pdl_wait();  // the output may be what the kernel before still reads
+        if (warp >= 2) {
+            const int quarter = warp & 3, n = nb * 128 + quarter * 32 + lane;
+            const uint32_t taddr = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
+            const float bias = args.bias && n < args.N ? __ldg(args.bias + n) : 0.f;
+            for (int c = 0; c < nt; c += 32) {
+                uint32_t r[32];
+                tmem_ld32(taddr + c, r);
+                tmem_wait_ld(r);
+#pragma unroll
+                for (int j = 0; j < 32; ++j)
+                    if (c + j < count && n < args.N) {
+                        const float v = __uint_as_float(r[j]);
+                        mx_store1<T>(args.out, (x_row + c + j) * args.ldo + n, args.bias ? __fadd_rn(v, bias) : v);
+                    }
+            }
+        }
+        tc_fence_before();
+        __syncthreads();
+        tc_fence_after();
+        if (warp == 1) tmem_dealloc(tmem, kFewCols);
+        return;
+    }
     // partial sums [token][128 rows] in this CTA's shared memory
     float *part = reinterpret_cast<float *>(smem);
     if (warp >= 2) {
@@ -787,31 +813,42 @@ __global__ void __launch_bounds__(kFewThreads, 2)
         }
     }
     tc_fence_before();
-    if (splits > 1) cluster_sync();
-    else __syncthreads();
+    cluster_sync();
     tc_fence_after();
     if (warp == 1) tmem_dealloc(tmem, kFewCols);
-    pdl_wait();  // the output may be what the kernel before still reads
-    // this rank's share of the rows: all ranks' parts, in the order of the ranks
-    const int share = 128 / static_cast<int>(splits), shift = 31 - __clz(share);
+    pdl_wait();
+    // this rank's share of the rows, four at a time: all ranks' parts, in the order of the ranks
+    const int share = 128 / static_cast<int>(splits), shift = 29 - __clz(share);  // log2(share / 4)
     const uint32_t mine = smem_u32(part);
-#pragma unroll 4
-    for (int i = threadIdx.x; i < count * share; i += kFewThreads) {
-        const int t = i >> shift, row = static_cast<int>(rank) * share + (i & (share - 1));
+    for (int i = threadIdx.x; i < (count << shift); i += kFewThreads) {
+        const int t = i >> shift, row = static_cast<int>(rank) * share + 4 * (i & ((1 << shift) - 1));
         const int n = nb * 128 + row;
         if (n >= args.N) continue;
-        float v[8];
+        float v[8][4];
 #pragma unroll
         for (uint32_t s = 0; s < 8; ++s)
-            if (s < splits) asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v[s]) : "r"(peer_smem(mine + (t * 128 + row) * 4, s)));
-        float sum = v[0];
+            if (s < splits)
+                asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v[s][0]), "=f"(v[s][1]), "=f"(v[s][2]), "=f"(v[s][3]) : "r"(peer_smem(mine + (t * 128 + row) * 4, s)));
 #pragma unroll
-        for (uint32_t s = 1; s < 8; ++s)
-            if (s < splits) sum = __fadd_rn(sum, v[s]);
-        if (args.bias) sum = __fadd_rn(sum, __ldg(args.bias + n));
-        mx_store1<T>(args.out, (x_row + t) * args.ldo + n, sum);
+        for (int q = 0; q < 4; ++q) {
+            float sum = v[0][q];
+#pragma unroll
+            for (uint32_t s = 1; s < 8; ++s)
+                if (s < splits) sum = __fadd_rn(sum, v[s][q]);
+            if (args.bias && n + q < args.N) sum = __fadd_rn(sum, __ldg(args.bias + n + q));
+            v[0][q] = sum;
+        }
+        const int64_t at = (x_row + t) * args.ldo + n;
+        if (args.vec_out && n + 4 <= args.N) {
+            if constexpr (T == kMxF32) *reinterpret_cast<float4 *>(static_cast<float *>(args.out) + at) = make_float4(v[0][0], v[0][1], v[0][2], v[0][3]);
+            else *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(args.out) + at) = make_uint2(mx_join<T>(v[0][0], v[0][1]), mx_join<T>(v[0][2], v[0][3]));
+        } else {
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+                if (n + q < args.N) mx_store1<T>(args.out, at + q, v[0][q]);
+        }
     }
-    if (splits > 1) cluster_sync();  // the others have read this CTA's parts
+    cluster_sync();  // the others have read this CTA's parts
 }
 
 // -------------------------------------------------------------------------------------------- host
@@ -961,13 +998,14 @@ int launch_few(cudaStream_t s, const CUtensorMap &w, const CUtensorMap &sw, cons
 
 // X tokens (null where they are quantised in the kernel), W weight rows; slots: 128-token tiles (rows:
 // at most)
-int run_few(cudaStream_t s, const FewArgs &a, const Operand *X, const Operand &W, int type, int64_t slots, int fuse) {
+int run_few(cudaStream_t s, FewArgs a, const Operand *X, const Operand &W, int type, int64_t slots, int fuse) {
     if (slots > 65535) {
         set_error("mxfp4_mm: too many token tiles");
         return 2;
     }
     // the contraction is split while the CTAs do not fill the device twice and each part has two
     // k-blocks at least
+    a.vec_out = a.ldo % 4 == 0 && (reinterpret_cast<uintptr_t>(a.out) & 15) == 0;
     const int64_t tiles = (a.N + 127) / 128 * slots;
     int splits = 1;
     while (splits < 8 && tiles * splits * 2 <= 2 * num_sms() && a.nk >= splits * 4) splits *= 2;
@@ -1061,7 +1099,7 @@ int mx4_token_mm(cudaStream_t s, const void *x, int64_t ldx, const uint8_t *b_co
     FewArgs a = few_args(out, N, M, N, K);
     a.bias = bias;
     a.mode = kDense;
-    a.w_early = 1;
+    a.w_early = 0;  // the kernel before may be the one that wrote the weight
     a.x = x;
     a.ldx = ldx;
     return run_few(s, a, nullptr, Operand{b_codes, b_scales, N, K, (N + 127) / 128}, type, 1, rotate ? kFuseRotate : kFusePlain);

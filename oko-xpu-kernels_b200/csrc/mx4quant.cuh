@@ -67,43 +67,68 @@ __device__ __forceinline__ uint32_t widen_bits(uint32_t h) {
 // the pair (v0, v1) times (s0, s1)
 __device__ __forceinline__ void scale2(float &v0, float &v1, f2 s) { un2(mul2(mk2(v0, v1), s), v0, v1); }
 
-// Codes of a lane's 16 values, its neighbour (lane ^ 1) holding the block's other 16: 8 bytes, and
-// the block's scale byte.
+// What a lane makes of its 16 values of two rows: 8 bytes of codes each and, on lanes 0 and 8 of the
+// half-warp, the words of four scales that start there.
+struct PairCodes {
+    uint2 c0, c1;
+    uint32_t w0, w1;
+};
+
+// the scale words of both rows from the lanes' scale bytes (lanes 0, 2, 4, 6 and 8, 10, 12, 14 hold a
+// tile's four blocks)
+__device__ __forceinline__ void join_scales(uint32_t e0, uint32_t e1, uint32_t &w0, uint32_t &w1) {
+    const uint32_t both = e0 | (e1 << 16);
+    const uint32_t two = both | (__shfl_down_sync(0xFFFFFFFFu, both, 2) << 8);
+    const uint32_t next = __shfl_down_sync(0xFFFFFFFFu, two, 4);
+    w0 = __byte_perm(two, next, 0x5410);
+    w1 = __byte_perm(two, next, 0x7632);
+}
+
+// Two runs of 16, the neighbouring lane (lane ^ 1) holding each block's other 16 values.
 template <int T>
-__device__ __forceinline__ uint2 quantize_run(const Run<T> &r, uint32_t &e) {
-    uint32_t m = 0;
+__device__ __forceinline__ PairCodes quantize_runs(const Run<T> &A, const Run<T> &B) {
+    uint32_t mA = 0, mB = 0;
     if constexpr (T == kMxF32) {
 #pragma unroll
-        for (int t = 0; t < 16; ++t) m = max(m, r.w[t] & 0x7FFFFFFFu);
-        m = max(m, __shfl_xor_sync(0xFFFFFFFFu, m, 1));
+        for (int t = 0; t < 16; ++t) {
+            mA = max(mA, A.w[t] & 0x7FFFFFFFu);
+            mB = max(mB, B.w[t] & 0x7FFFFFFFu);
+        }
+        mA = max(mA, __shfl_xor_sync(0xFFFFFFFFu, mA, 1));
+        mB = max(mB, __shfl_xor_sync(0xFFFFFFFFu, mB, 1));
     } else {
 #pragma unroll
-        for (int t = 0; t < 8; ++t) m = max_u16x2(m, r.w[t] & 0x7FFF7FFFu);
+        for (int t = 0; t < 8; ++t) {
+            mA = max_u16x2(mA, A.w[t] & 0x7FFF7FFFu);
+            mB = max_u16x2(mB, B.w[t] & 0x7FFF7FFFu);
+        }
+        uint32_t m = max_u16x2(__byte_perm(mA, mB, 0x5410), __byte_perm(mA, mB, 0x7632));  // (A, B)
         m = max_u16x2(m, __shfl_xor_sync(0xFFFFFFFFu, m, 1));
-        m = widen_bits<T>(max(m & 0xFFFFu, m >> 16));
+        mA = widen_bits<T>(m & 0xFFFFu);
+        mB = widen_bits<T>(m >> 16);
     }
-    e = mx_exponent(m);
-    const float inv = mx_inverse(e);
-    const f2 s = mk2(inv, inv);
-    float v[16];
+    const uint32_t e0 = mx_exponent(mA), e1 = mx_exponent(mB);
+    const f2 s0 = mk2(mx_inverse(e0), mx_inverse(e0)), s1 = mk2(mx_inverse(e1), mx_inverse(e1));
+    float a[16], b[16];
 #pragma unroll
     for (int t = 0; t < 8; ++t) {
         if constexpr (T == kMxF32) {
-            v[2 * t] = __uint_as_float(r.w[2 * t]);
-            v[2 * t + 1] = __uint_as_float(r.w[2 * t + 1]);
+            a[2 * t] = __uint_as_float(A.w[2 * t]);
+            a[2 * t + 1] = __uint_as_float(A.w[2 * t + 1]);
+            b[2 * t] = __uint_as_float(B.w[2 * t]);
+            b[2 * t + 1] = __uint_as_float(B.w[2 * t + 1]);
         } else {
-            mx_split<T>(r.w[t], v[2 * t], v[2 * t + 1]);
+            mx_split<T>(A.w[t], a[2 * t], a[2 * t + 1]);
+            mx_split<T>(B.w[t], b[2 * t], b[2 * t + 1]);
         }
-        scale2(v[2 * t], v[2 * t + 1], s);
+        scale2(a[2 * t], a[2 * t + 1], s0);
+        scale2(b[2 * t], b[2 * t + 1], s1);
     }
-    return make_uint2(mx_pack8(v), mx_pack8(v + 8));
-}
-
-// Lanes 0, 2, 4, 6 (8, 10, 12, 14) of a half-warp hold the scale bytes of a tile's four blocks: the
-// word of them, on lanes 0 and 8.
-__device__ __forceinline__ uint32_t join_scales(uint32_t e) {
-    const uint32_t two = e | (__shfl_down_sync(0xFFFFFFFFu, e, 2) << 8);
-    return two | (__shfl_down_sync(0xFFFFFFFFu, two, 4) << 16);
+    PairCodes p;
+    p.c0 = make_uint2(mx_pack8(a), mx_pack8(a + 8));
+    p.c1 = make_uint2(mx_pack8(b), mx_pack8(b + 8));
+    join_scales(e0, e1, p.w0, p.w1);
+    return p;
 }
 
 // A pair of 256-value groups A and B on a half-warp's lanes, turned to pairs: value c of both at
@@ -180,25 +205,89 @@ __device__ __forceinline__ void runs_to_shared(const Run<T> &A, const Run<T> &B,
     }
 }
 
-// both runs of lane l back from the pairs
+// lane l's 16 values of both groups from the pairs, as they lie there: words (A, B) of a 16-bit type,
+// or fp32 pairs
 template <int T>
-__device__ __forceinline__ void runs_from_shared(Run<T> &A, Run<T> &B, uint32_t slot, int l) {
+struct Pairs {
+    static constexpr int kWords = 8 * mx_size(T);
+    uint32_t w[kWords];
+};
+template <int T>
+__device__ __forceinline__ Pairs<T> pairs_from_shared(uint32_t slot, int l) {
+    Pairs<T> p;
     const uint32_t at = slot + pair_at<T>(1, 0) * l;
+#pragma unroll
+    for (int c = 0; c < Pairs<T>::kWords / 4; ++c)
+        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(p.w[4 * c]), "=r"(p.w[4 * c + 1]), "=r"(p.w[4 * c + 2]), "=r"(p.w[4 * c + 3]) : "r"(at + c * 16));
+    return p;
+}
+// as two runs
+template <int T>
+__device__ __forceinline__ void split_pairs(const Pairs<T> &p, Run<T> &A, Run<T> &B) {
     if constexpr (T == kMxF32) {
 #pragma unroll
-        for (int c = 0; c < 8; ++c)
-            asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(A.w[2 * c]), "=r"(B.w[2 * c]), "=r"(A.w[2 * c + 1]), "=r"(B.w[2 * c + 1]) : "r"(at + c * 16));
+        for (int t = 0; t < 16; ++t) {
+            A.w[t] = p.w[2 * t];
+            B.w[t] = p.w[2 * t + 1];
+        }
     } else {
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-            uint32_t w[4];
-            asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(at + c * 16));
-            A.w[2 * c] = __byte_perm(w[0], w[1], 0x5410);
-            B.w[2 * c] = __byte_perm(w[0], w[1], 0x7632);
-            A.w[2 * c + 1] = __byte_perm(w[2], w[3], 0x5410);
-            B.w[2 * c + 1] = __byte_perm(w[2], w[3], 0x7632);
+        for (int t = 0; t < 8; ++t) {
+            A.w[t] = __byte_perm(p.w[2 * t], p.w[2 * t + 1], 0x5410);
+            B.w[t] = __byte_perm(p.w[2 * t], p.w[2 * t + 1], 0x7632);
         }
     }
 }
+// quantize_runs on the pairs: one maximum and one scaling serve both groups
+template <int T>
+__device__ __forceinline__ PairCodes quantize_pairs(const Pairs<T> &p) {
+    uint32_t mA = 0, mB = 0;
+    if constexpr (T == kMxF32) {
+#pragma unroll
+        for (int t = 0; t < 16; ++t) {
+            mA = max(mA, p.w[2 * t] & 0x7FFFFFFFu);
+            mB = max(mB, p.w[2 * t + 1] & 0x7FFFFFFFu);
+        }
+        mA = max(mA, __shfl_xor_sync(0xFFFFFFFFu, mA, 1));
+        mB = max(mB, __shfl_xor_sync(0xFFFFFFFFu, mB, 1));
+    } else {
+        uint32_t m = 0;
+#pragma unroll
+        for (int t = 0; t < 16; ++t) m = max_u16x2(m, p.w[t] & 0x7FFF7FFFu);
+        m = max_u16x2(m, __shfl_xor_sync(0xFFFFFFFFu, m, 1));
+        mA = widen_bits<T>(m & 0xFFFFu);
+        mB = widen_bits<T>(m >> 16);
+    }
+    const uint32_t e0 = mx_exponent(mA), e1 = mx_exponent(mB);
+    const f2 s = mk2(mx_inverse(e0), mx_inverse(e1));
+    float a[16], b[16];
+#pragma unroll
+    for (int t = 0; t < 16; ++t) {
+        if constexpr (T == kMxF32) {
+            a[t] = __uint_as_float(p.w[2 * t]);
+            b[t] = __uint_as_float(p.w[2 * t + 1]);
+        } else {
+            mx_split<T>(p.w[t], a[t], b[t]);
+        }
+        scale2(a[t], b[t], s);
+    }
+    PairCodes r;
+    r.c0 = make_uint2(mx_pack8(a), mx_pack8(a + 8));
+    r.c1 = make_uint2(mx_pack8(b), mx_pack8(b + 8));
+    join_scales(e0, e1, r.w0, r.w1);
+    return r;
+}
+
+// n / d for 0 <= n < 2^31 by one high multiply, an add and a shift: the invariant-divisor method of
+// Granlund & Montgomery (PLDI 1994, section 4), l = ceil(log2 d), m = floor(2^32 (2^l - d) / d) + 1
+struct Divisor {
+    uint32_t d, m, l;
+    static Divisor of(uint32_t d) {
+        uint32_t l = 0;
+        while ((uint64_t{1} << l) < d) ++l;
+        return {d, static_cast<uint32_t>(((uint64_t{1} << 32) * ((uint64_t{1} << l) - d)) / d + 1), l};
+    }
+    __device__ __forceinline__ uint32_t operator()(uint32_t n) const { return (__umulhi(n, m) + n) >> l; }
+};
 
 }  // namespace xpuint8

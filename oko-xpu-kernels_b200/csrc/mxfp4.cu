@@ -25,8 +25,10 @@ struct RowArgs {
     int64_t ldx;                 // elements between rows of x
     uint8_t *codes, *scales;     // codes may be null: only the rotated values are wanted
     void *rotated;               // [rows, K] of x's type, or null
-    uint32_t groups;             // rows * G
-    uint32_t K, G, KB, KT;       // 256-groups, 32-blocks and 128-tiles of a row
+    uint32_t tasks;              // row pairs * G
+    uint32_t rows;
+    uint32_t K, KB, KT;          // values, 32-blocks and 128-tiles of a row
+    Divisor G;                   // 256-groups of a row
     uint32_t matrix_rows;        // rows of each matrix of a stack
     uint32_t matrix_tiles;       // its 128-row tiles (0: one matrix)
     const int32_t *order;        // sorted rows: row r of x is the slot order[r]
@@ -42,59 +44,75 @@ __device__ __forceinline__ void store_run(void *row, uint32_t c, const Run<T> &r
     for (int j = 0; j < Run<T>::kWords / 4; ++j) p[j] = make_uint4(r.w[4 * j], r.w[4 * j + 1], r.w[4 * j + 2], r.w[4 * j + 3]);
 }
 
-// One half-warp ("slot") quantizes a pair of 256-value groups: a lane holds 16 consecutive values
-// of each, so a block of 32 is two lanes, codes leave as 8 bytes a lane (128 consecutive bytes a
-// group) and scales as one 4-byte word a 128-wide tile.  Instructions bound it before memory does:
-// 16-bit values stay packed up to the conversion (the maximum is an integer one of two at a time),
-// the rotation and the scaling are packed fp32x2.
-template <int T, bool ROT, bool VEC>
+enum Where { kOneMatrix = 0, kStack = 1, kExperts = 2 };
+
+// One half-warp ("slot") quantizes the same 256-value group of two neighbouring rows: a lane holds 16
+// consecutive values of each, so a block of 32 is two lanes, codes leave as 8 bytes a lane (128
+// consecutive bytes a group) and scales as one 4-byte word a 128-wide tile.  Instructions bound it
+// before memory does: 16-bit values stay packed up to the conversion (the maximum is an integer one of
+// two at a time), the rotation and the scaling are packed fp32x2, and the second row's addresses are
+// the first's and a constant.
+template <int T, bool ROT, bool VEC, int WHERE>
 __global__ void __launch_bounds__(128) quantize_rows_kernel(const RowArgs a) {
     __shared__ __align__(128) uint8_t tiles[ROT ? 8 * kSlotBytes : 16];
     const int slot = threadIdx.x >> 4, l = threadIdx.x & 15;
-    const uint32_t f0 = (blockIdx.x * 8u + slot) * 2u;
-    const uint32_t r0 = f0 / a.G, g0 = f0 - r0 * a.G;
-    const uint32_t r1 = g0 + 1 == a.G ? r0 + 1 : r0, g1 = g0 + 1 == a.G ? 0 : g0 + 1;
-    const bool ok0 = f0 < a.groups, ok1 = f0 + 1 < a.groups;
-    const uint8_t *base = static_cast<const uint8_t *>(a.x);
-    Run<T> A = zero_run<T>(), B = zero_run<T>();
-    if (ok0) A = load_run<T, VEC>(base + r0 * a.ldx * mx_size(T), g0 * 256 + l * 16, a.K);
-    if (ok1) B = load_run<T, VEC>(base + r1 * a.ldx * mx_size(T), g1 * 256 + l * 16, a.K);
+    const uint32_t task = min(blockIdx.x * 8u + slot, a.tasks - 1);  // the last slots repeat a task: their warp's other half needs their lanes
+    const uint32_t rp = a.G(task), g = task - rp * a.G.d, r = 2 * rp, c = g * 256 + l * 16;
+    const bool two = r + 1 < a.rows;
+    const uint8_t *row = static_cast<const uint8_t *>(a.x) + r * a.ldx * mx_size(T);
+    const Run<T> A = load_run<T, VEC>(row, c, a.K);
+    const Run<T> B = two ? load_run<T, VEC>(row + a.ldx * mx_size(T), c, a.K) : zero_run<T>();
+    pdl_trigger();
+    PairCodes q;
     if constexpr (ROT) {
         const uint32_t tile = smem_u32(tiles) + slot * kSlotBytes;
         rotate_to_shared<T>(A, B, tile, l);
-        runs_from_shared<T>(A, B, tile, l);
+        const Pairs<T> p = pairs_from_shared<T>(tile, l);
         if (a.rotated) {
-            uint8_t *out = static_cast<uint8_t *>(a.rotated);
-            if (ok0) store_run<T>(out + static_cast<int64_t>(r0) * a.K * mx_size(T), g0 * 256 + l * 16, A);
-            if (ok1) store_run<T>(out + static_cast<int64_t>(r1) * a.K * mx_size(T), g1 * 256 + l * 16, B);
+            Run<T> u, v;
+            split_pairs<T>(p, u, v);
+            uint8_t *out = static_cast<uint8_t *>(a.rotated) + static_cast<int64_t>(r) * a.K * mx_size(T);
+            store_run<T>(out, c, u);
+            if (two) store_run<T>(out + static_cast<int64_t>(a.K) * mx_size(T), c, v);
         }
         if (!a.codes) return;
+        q = quantize_pairs<T>(p);
+    } else {
+        q = quantize_runs<T>(A, B);
     }
-    uint32_t e0, e1;
-    const uint2 c0 = quantize_run<T>(A, e0), c1 = quantize_run<T>(B, e1);
-    const uint32_t w0 = join_scales(e0), w1 = join_scales(e1);
-    auto put = [&](uint32_t r, uint32_t g, const uint2 &code, uint32_t word) {
-        const uint32_t c = g * 256 + l * 16, kt = g * 2 + (l >> 3);
-        const bool has_code = c < a.KB * 32, has_word = (l & 7) == 0 && kt < a.KT;
-        for (uint32_t j = 0; j < a.fan; ++j) {
-            int64_t cr = r, sr;
-            if (a.scale_rows) {
-                const uint32_t at = a.order ? static_cast<uint32_t>(__ldg(a.order + r)) : r * a.fan + j;
-                sr = __ldg(a.scale_rows + at);
-                if (sr < 0) continue;
-                if (!a.order) cr = __ldg(a.positions + at);
-            } else if (a.matrix_tiles == 0) {
-                sr = r;
-            } else {
-                const uint32_t b = r / a.matrix_rows;
-                sr = static_cast<int64_t>(b) * a.matrix_tiles * 128 + (r - b * a.matrix_rows);
-            }
-            if (has_code) *reinterpret_cast<uint2 *>(a.codes + cr * a.KB * 16 + c / 2) = code;
-            if (has_word) *reinterpret_cast<uint32_t *>(a.scales + mx_scale_word(sr, kt, a.KT)) = word;
+    const uint32_t kt = g * 2 + (l >> 3);
+    const bool has_code = c < a.KB * 32, has_word = (l & 7) == 0 && kt < a.KT;
+    if constexpr (WHERE == kOneMatrix) {
+        uint8_t *codes = a.codes + static_cast<int64_t>(r) * a.KB * 16 + c / 2;
+        uint8_t *scales = a.scales + mx_scale_word(r, kt, a.KT);
+        if (has_code) {
+            *reinterpret_cast<uint2 *>(codes) = q.c0;
+            if (two) *reinterpret_cast<uint2 *>(codes + a.KB * 16) = q.c1;
         }
-    };
-    if (ok0) put(r0, g0, c0, w0);
-    if (ok1) put(r1, g1, c1, w1);
+        if (has_word) {  // r is even: the next row is the next 16 bytes of the tile
+            *reinterpret_cast<uint32_t *>(scales) = q.w0;
+            if (two) *reinterpret_cast<uint32_t *>(scales + 16) = q.w1;
+        }
+    } else {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            if (h && !two) break;
+            for (uint32_t j = 0; j < (WHERE == kExperts ? a.fan : 1u); ++j) {
+                int64_t cr = r + h, sr;
+                if constexpr (WHERE == kExperts) {
+                    const uint32_t at = a.order ? static_cast<uint32_t>(__ldg(a.order + r + h)) : (r + h) * a.fan + j;
+                    sr = __ldg(a.scale_rows + at);
+                    if (sr < 0) continue;
+                    if (!a.order) cr = __ldg(a.positions + at);
+                } else {
+                    const uint32_t b = (r + h) / a.matrix_rows;
+                    sr = static_cast<int64_t>(b) * a.matrix_tiles * 128 + (r + h - b * a.matrix_rows);
+                }
+                if (has_code) *reinterpret_cast<uint2 *>(a.codes + cr * a.KB * 16 + c / 2) = h ? q.c1 : q.c0;
+                if (has_word) *reinterpret_cast<uint32_t *>(a.scales + mx_scale_word(sr, kt, a.KT)) = h ? q.w1 : q.w0;
+            }
+        }
+    }
 }
 
 struct ColumnArgs {
@@ -268,28 +286,27 @@ __global__ void __launch_bounds__(kBothThreads) quantize_both_kernel(const BothA
     Run<T> A = bring(2 * slot), B = bring(2 * slot + 1);
 #pragma unroll 1
     for (int sub = 0; sub < 4; ++sub) {
-        if constexpr (ROT) {
-            rotate_to_shared<T>(A, B, mine, l);
-            runs_from_shared<T>(A, B, mine, l);
-        } else {
-            runs_to_shared<T>(A, B, mine, l);
-        }
-        __syncwarp();
+        if constexpr (ROT) rotate_to_shared<T>(A, B, mine, l);
+        else runs_to_shared<T>(A, B, mine, l);
         if (a.row_codes) {
-            uint32_t e0, e1;
-            const uint2 c0 = quantize_run<T>(A, e0), c1 = quantize_run<T>(B, e1);
-            const uint32_t w0 = join_scales(e0), w1 = join_scales(e1);
+            PairCodes q;
+            if constexpr (ROT) q = quantize_pairs<T>(pairs_from_shared<T>(mine, l));
+            else q = quantize_runs<T>(A, B);
             const uint32_t i = sub * 32 + 2 * slot, tile = blockIdx.x * 2 + (l >> 3);
             const bool has_code = c < a.KB * 32, has_word = (l & 7) == 0 && tile < a.KT;
-            uint8_t *codes = a.row_codes + blockIdx.z * a.row_matrix_codes;
-            uint8_t *scales = a.row_scales + blockIdx.z * a.row_matrix_scales;
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                if (begin + i + h >= end) continue;
-                if (has_code) *reinterpret_cast<uint2 *>(codes + static_cast<int64_t>(begin + i + h) * a.KB * 16 + c / 2) = h ? c1 : c0;
-                if (has_word) *reinterpret_cast<uint32_t *>(scales + mx_scale_word(kt * 128ll + i + h, tile, a.KT)) = h ? w1 : w0;
+            const bool one = begin + i < end, two = begin + i + 1 < end;
+            uint8_t *codes = a.row_codes + blockIdx.z * a.row_matrix_codes + static_cast<int64_t>(begin + i) * a.KB * 16 + c / 2;
+            uint8_t *scales = a.row_scales + blockIdx.z * a.row_matrix_scales + mx_scale_word(kt * 128ll + i, tile, a.KT);
+            if (has_code) {
+                if (one) *reinterpret_cast<uint2 *>(codes) = q.c0;
+                if (two) *reinterpret_cast<uint2 *>(codes + a.KB * 16) = q.c1;
+            }
+            if (has_word) {  // i is even: the next row is the next 16 bytes of the tile
+                if (one) *reinterpret_cast<uint32_t *>(scales) = q.w0;
+                if (two) *reinterpret_cast<uint32_t *>(scales + 16) = q.w1;
             }
         }
+        __syncwarp();
         if (sub < 3) {
             A = bring(sub * 32 + 32 + 2 * slot);
             B = bring(sub * 32 + 33 + 2 * slot);
@@ -373,7 +390,7 @@ __global__ void __launch_bounds__(128) turn_kernel(const TurnArgs a) {
     if constexpr (ROT) {
         const uint32_t tile = smem_u32(tiles) + slot * kSlotBytes;
         rotate_to_shared<kMxF32>(A, B, tile, l);
-        runs_from_shared<kMxF32>(A, B, tile, l);
+        split_pairs<kMxF32>(pairs_from_shared<kMxF32>(tile, l), A, B);
     }
     auto put = [&](uint32_t r, uint32_t g, const Run<kMxF32> &v) {
         uint8_t *row = static_cast<uint8_t *>(a.out) + static_cast<int64_t>(r) * a.K * mx_size(T);
@@ -443,44 +460,54 @@ __global__ void __launch_bounds__(256) odd_values_kernel(const ValueArgs a) {
     const int64_t m = r / a.matrix_rows;
     const int64_t sr = m * a.matrix_tiles * 128 + (r - m * a.matrix_rows);
     const uint8_t *codes = a.codes + r * a.KB * 16;
+    // lane j holds the scale of block j (of eight)
+    const uint32_t mine = min(b0 + (lane & 7), a.KB - 1);
+    const float scale = mx_scale(__ldg(a.scales + mx_scale_word(sr, mine >> 2, a.KT) + (mine & 3)));
+    codes += b0 * 16 + (lane >> 1);
+    const int shift = (lane & 1) * 4;
+    const int64_t at = r * a.K + b0 * 32 + lane;
+    const uint32_t left = a.K - b0 * 32;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-        const uint32_t b = b0 + j, c = b * 32 + lane;
-        if (c < a.K) {
-            const uint32_t byte = __ldg(codes + c / 2), code = lane & 1 ? byte >> 4 : byte & 15u;
-            const float s = mx_scale(__ldg(a.scales + mx_scale_word(sr, b >> 2, a.KT) + (b & 3)));
-            mx_store1<T>(a.out, r * a.K + c, __fmul_rn(mx_value(code), s));
-        }
+        const float s = __shfl_sync(0xFFFFFFFFu, scale, j);
+        if (j * 32 + lane < left) mx_store1<T>(a.out, at + j * 32, __fmul_rn(mx_value(__ldg(codes + j * 16) >> shift), s));
     }
 }
 
 bool aligned(const void *p, int n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
 
+template <int T, int WHERE>
+void launch_rows(cudaStream_t s, const RowArgs &a, bool rotate, bool vec) {
+    const uint32_t grid = (a.tasks + 7) / 8;
+    if (rotate) {
+        if (vec) quantize_rows_kernel<T, true, true, WHERE><<<grid, 128, 0, s>>>(a);
+        else quantize_rows_kernel<T, true, false, WHERE><<<grid, 128, 0, s>>>(a);
+    } else {
+        if (vec) quantize_rows_kernel<T, false, true, WHERE><<<grid, 128, 0, s>>>(a);
+        else quantize_rows_kernel<T, false, false, WHERE><<<grid, 128, 0, s>>>(a);
+    }
+}
 template <int T>
 void launch_rows(cudaStream_t s, const RowArgs &a, bool rotate, bool vec) {
-    const uint32_t grid = (a.groups + 15) / 16;
-    if (rotate) {
-        if (vec) quantize_rows_kernel<T, true, true><<<grid, 128, 0, s>>>(a);
-        else quantize_rows_kernel<T, true, false><<<grid, 128, 0, s>>>(a);
-    } else {
-        if (vec) quantize_rows_kernel<T, false, true><<<grid, 128, 0, s>>>(a);
-        else quantize_rows_kernel<T, false, false><<<grid, 128, 0, s>>>(a);
-    }
+    if (a.scale_rows) launch_rows<T, kExperts>(s, a, rotate, vec);
+    else if (a.matrix_tiles) launch_rows<T, kStack>(s, a, rotate, vec);
+    else launch_rows<T, kOneMatrix>(s, a, rotate, vec);
 }
 
 int quantize_rows(cudaStream_t s, RowArgs &a, int type, int64_t rows, int64_t K, int64_t ldx, bool rotate) {
+    const int64_t G = (K + 255) / 256;
+    if ((rows + 1) / 2 * G > 0x7FFFFFF0ll) {
+        set_error("mxfp4: rows x 256-groups must be below 2^32");
+        return 2;
+    }
+    a.rows = static_cast<uint32_t>(rows);
     a.K = static_cast<uint32_t>(K);
-    a.G = static_cast<uint32_t>((K + 255) / 256);
+    a.G = Divisor::of(static_cast<uint32_t>(G));
     a.KB = static_cast<uint32_t>((K + 31) / 32);
     a.KT = (a.KB + 3) / 4;
     a.ldx = ldx;
-    if (rows * a.G > 0x7FFFFFF0ll) {
-        set_error("mxfp4: rows x 256-groups must be below 2^31");
-        return 2;
-    }
-    a.groups = static_cast<uint32_t>(rows * a.G);
-    const int es = mx_size(type);
-    const bool vec = aligned(a.x, 16) && (ldx * es) % 16 == 0;
+    a.tasks = static_cast<uint32_t>((rows + 1) / 2 * G);
+    const bool vec = aligned(a.x, 16) && (ldx * mx_size(type)) % 16 == 0;
     switch (type) {
         case kMxBf16: launch_rows<kMxBf16>(s, a, rotate, vec); break;
         case kMxF16: launch_rows<kMxF16>(s, a, rotate, vec); break;
