@@ -370,7 +370,7 @@ int xpuint8_mxfp4_expert_dw_stream(const void *stream, const uint8_t *a_codes,
                                    int64_t experts);
 
 /* The MXFP4 linear in one call: x [M, K] (row stride ldx) quantised along K, behind the rotation or
- * not, times the weight [N, K] in MXFP4, bias fp32 [N] or NULL, out [M, N].  Up to 16 rows whose
+ * not, times the weight [N, K] in MXFP4, bias fp32 [N] or NULL, out [M, N].  Up to 8 rows whose
  * stride and base are multiples of 16 bytes are quantised inside the product (the workspace may be
  * NULL); others use xpuint8_mxfp4_linear_workspace_bytes bytes. */
 int64_t xpuint8_mxfp4_linear_workspace_bytes(int64_t M, int64_t K);

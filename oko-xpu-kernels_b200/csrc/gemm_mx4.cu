@@ -90,6 +90,17 @@ __device__ __forceinline__ void drain_wait(uint32_t bar, uint32_t parity) {
     atomicCAS(&g_mx4_fault, 0, 199);
 }
 
+// one lane of a converged warp
+__device__ __forceinline__ bool elect_one() {
+    uint32_t p;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xFFFFFFFF;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+    return p != 0;
+}
+// mbar_wait by a whole warp: the same answer in every lane
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, int *fault, int site) {
+    return __all_sync(0xFFFFFFFFu, mbar_wait(bar, parity, fault, site));
+}
+
 // ------------------------------------------------------------------------------------- pair kernel
 
 constexpr int BK = 256;               // values of K a k-block: 128 bytes of codes a row
@@ -322,52 +333,63 @@ __global__ void __launch_bounds__(PairCfg<BN>::kThreads, 1)
                           : args.num_m * args.num_n * (args.mode == kContraction ? args.experts : 1);
 
     if (warp == 0) {
-        if (lane == 0) {
-            // ------------------------------------------------ TMA producer (both CTAs)
-            int stage = 0;
-            uint32_t ph = 0, issued = 0;
-            constexpr uint32_t kTx = 2 * C::kStageBytes;
-            if (!args.b_early) pdl_wait();
-            auto load_b = [&](int st, const Tile &t, int kb) {
-                const uint32_t fb = peer_smem(FULL(st), 0);
-                tma_load_2d_pair(sB + st * C::kBBytes, &tmB, fb, t.k_code + kb * kCodeRow, t.b_row + static_cast<int>(rank) * (BN / 2));
-                tma_load_2d_pair(sSB + st * C::kSfbBytes, &tmSB, fb, t.k_sf + kb * 256, t.b_sf);
-            };
-            // b_early: the first pass over the ring takes B before the kernel before is done
-            uint32_t pre = 0;
-            if (args.b_early) {
-                int tile = pair, kb = 0;
-                for (; pre < static_cast<uint32_t>(STAGES) && tile < num_tiles; ++pre) {
-                    const Tile t = pair_tile<BN>(args, s_cum, tile);
-                    load_b(static_cast<int>(pre), t, kb);
-                    if (++kb == t.nk) { kb = 0; tile += npairs; }
-                }
-                pdl_wait();
-            }
-            bool ok = true;
-            for (int tile = pair; ok && tile < num_tiles; tile += npairs) {
+        // ------------------------------------------------ TMA producer (both CTAs)
+        int stage = 0;
+        uint32_t ph = 0, issued = 0;
+        constexpr uint32_t kTx = 2 * C::kStageBytes;
+        if (!args.b_early) pdl_wait();
+        // B's half and scales of k-block kb into stage st (one lane)
+        auto load_b = [&](int st, int b_row, int b_sf, int k_code, int k_sf) {
+            const uint32_t fb = peer_smem(FULL(st), 0);
+            tma_load_2d_pair(sB + st * C::kBBytes, &tmB, fb, k_code, b_row);
+            tma_load_2d_pair(sSB + st * C::kSfbBytes, &tmSB, fb, k_sf, b_sf);
+        };
+        // b_early: the first pass over the ring takes B before the kernel before is done
+        uint32_t pre = 0;
+        if (args.b_early) {
+            int tile = pair, kb = 0;
+            for (; pre < static_cast<uint32_t>(STAGES) && tile < num_tiles; ++pre) {
                 const Tile t = pair_tile<BN>(args, s_cum, tile);
-                for (int kb = 0; kb < t.nk; ++kb) {
-                    if (!mbar_wait(EMPTY(stage), ph ^ 1u, fault, 101)) { ok = false; break; }
+                if (lane == 0) load_b(static_cast<int>(pre), t.b_row + static_cast<int>(rank) * (BN / 2), t.b_sf, t.k_code + kb * kCodeRow, t.k_sf + kb * 256);
+                if (++kb == t.nk) { kb = 0; tile += npairs; }
+            }
+            __syncwarp();
+            pdl_wait();
+        }
+        bool ok = true;
+        for (int tile = pair; ok && tile < num_tiles; tile += npairs) {
+            const Tile t = pair_tile<BN>(args, s_cum, tile);
+            const int nk = __shfl_sync(0xFFFFFFFFu, t.nk, 0);
+            int k_code = __shfl_sync(0xFFFFFFFFu, t.k_code, 0), k_sf = __shfl_sync(0xFFFFFFFFu, t.k_sf, 0);
+            const int a_row = __shfl_sync(0xFFFFFFFFu, t.a_row, 0) + static_cast<int>(rank) * 128, a_sf = __shfl_sync(0xFFFFFFFFu, t.a_sf, 0) + static_cast<int>(rank);
+            const int b_row = __shfl_sync(0xFFFFFFFFu, t.b_row, 0) + static_cast<int>(rank) * (BN / 2), b_sf = __shfl_sync(0xFFFFFFFFu, t.b_sf, 0);
+            for (int kb = 0; kb < nk; ++kb, k_code += kCodeRow, k_sf += 256) {
+                if (!warp_wait(EMPTY(stage), ph ^ 1u, fault, 101)) { ok = false; break; }
+                if (elect_one()) {
                     if (leader) mbar_expect_tx(FULL(stage), kTx);
                     const uint32_t fb = peer_smem(FULL(stage), 0);
-                    tma_load_2d_pair(sA + stage * C::kABytes, &tmA, fb, t.k_code + kb * kCodeRow, t.a_row + static_cast<int>(rank) * 128);
-                    tma_load_2d_pair(sSA + stage * kScaleBlock, &tmSA, fb, t.k_sf + kb * 256, t.a_sf + static_cast<int>(rank));
-                    if (issued >= pre) load_b(stage, t, kb);
-                    ++issued;
-                    if (++stage == STAGES) { stage = 0; ph ^= 1u; }
+                    tma_load_2d_pair(sA + stage * C::kABytes, &tmA, fb, k_code, a_row);
+                    tma_load_2d_pair(sSA + stage * kScaleBlock, &tmSA, fb, k_sf, a_sf);
+                    if (issued >= pre) load_b(stage, b_row, b_sf, k_code, k_sf);
                 }
-            }
-            pdl_trigger();
-            // every load has landed once the MMAs that read it are done
-            for (uint32_t s = 0; s < static_cast<uint32_t>(STAGES) && s < issued; ++s) {
-                const uint32_t last = s + ((issued - 1 - s) / STAGES) * STAGES;
-                drain_wait(EMPTY(s), (last / STAGES) & 1u);
+                __syncwarp();
+                ++issued;
+                if (++stage == STAGES) { stage = 0; ph ^= 1u; }
             }
         }
+        pdl_trigger();
+        // every load has landed once the MMAs that read it are done
+        for (uint32_t s = 0; s < static_cast<uint32_t>(STAGES) && s < issued; ++s) {
+            const uint32_t last = s + ((issued - 1 - s) / STAGES) * STAGES;
+            drain_wait(EMPTY(s), (last / STAGES) & 1u);
+        }
     } else if (warp == 1) {
-        if (lane == 0 && leader) {
+        if (leader) {
             // ------------------------------------------------ scale copies and MMAs (leader)
+            // the whole warp walks the loop and one elected lane issues: the addresses and descriptors
+            // then live in uniform registers, where these instructions take them from; in a branch of
+            // one lane each operand is moved there first, and the issue itself bounds the main loop
+            // (8192 x 14336 x 4096: 264 us so, against the figure above)
             constexpr uint32_t kIdesc[2] = {idesc_mx4(256, BN, 0), idesc_mx4(256, BN, 1)};
             const uint32_t sfa = tmem_base + C::kScaleCol, sfb = sfa + 8;
             int stage = 0, count = 0;
@@ -375,40 +397,47 @@ __global__ void __launch_bounds__(PairCfg<BN>::kThreads, 1)
             bool ok = true;
             for (int tile = pair; ok && tile < num_tiles; tile += npairs) {
                 const Tile t = pair_tile<BN>(args, s_cum, tile);
-                if (t.nk == 0) continue;  // no contraction: the drain writes zeros
+                const int nk = __shfl_sync(0xFFFFFFFFu, t.nk, 0), last_steps = __shfl_sync(0xFFFFFFFFu, t.last_steps, 0);
+                if (nk == 0) continue;  // no contraction: the drain writes zeros
                 const int acc = count & 1;
-                if (!mbar_wait(TEMPTY(acc), ((count >> 1) & 1) ^ 1u, fault, 102)) break;
-                if (BN == 256 && count > 0 && !mbar_wait(OVER(acc ^ 1), ((count - 1) >> 1) & 1, fault, 103)) break;
+                if (!warp_wait(TEMPTY(acc), ((count >> 1) & 1) ^ 1u, fault, 102)) break;
+                if (BN == 256 && count > 0 && !warp_wait(OVER(acc ^ 1), ((count - 1) >> 1) & 1, fault, 103)) break;
                 tc_fence_after();
                 const uint32_t d = tmem_base + static_cast<uint32_t>(acc ? C::kAccCol1 : 0);
-                for (int kb = 0; kb < t.nk; ++kb) {
-                    if (!mbar_wait(FULL(stage), ph, fault, 104)) { ok = false; break; }
+                for (int kb = 0; kb < nk; ++kb) {
+                    if (!warp_wait(FULL(stage), ph, fault, 104)) { ok = false; break; }
                     tc_fence_after();
-                    const int steps = kb + 1 == t.nk ? t.last_steps : 4;
+                    const int steps = kb + 1 == nk ? last_steps : 4;
+                    if (elect_one()) {
 #pragma unroll
-                    for (int kt = 0; kt < 2; ++kt) {
-                        copy_scales<2>(sfa + 4 * kt, scale_desc(sSA + stage * kScaleBlock + kt * kMxTileBytes));
+                        for (int kt = 0; kt < 2; ++kt) {
+                            copy_scales<2>(sfa + 4 * kt, scale_desc(sSA + stage * kScaleBlock + kt * kMxTileBytes));
 #pragma unroll
-                        for (int rt = 0; rt < BN / 128; ++rt)
-                            copy_scales<2>(sfb + kt * (BN / 32) + 4 * rt, scale_desc(sSB + stage * C::kSfbBytes + rt * kScaleBlock + kt * kMxTileBytes));
+                            for (int rt = 0; rt < BN / 128; ++rt)
+                                copy_scales<2>(sfb + kt * (BN / 32) + 4 * rt, scale_desc(sSB + stage * C::kSfbBytes + rt * kScaleBlock + kt * kMxTileBytes));
+                        }
+#pragma unroll
+                        for (int kk = 0; kk < 4; ++kk) {
+                            if (kk < steps)
+                                umma_mx4<2>(d, umma_sdesc_sw128(sA + stage * C::kABytes + kk * 32, 16, 1024),
+                                            umma_sdesc_sw128(sB + stage * C::kBBytes + kk * 32, 16, 1024), kIdesc[kk & 1],
+                                            sfa + 4 * (kk >> 1), sfb + (kk >> 1) * (BN / 32), (kb | kk) != 0 ? 1u : 0u);
+                        }
+                        umma_commit_pair(EMPTY(stage));
+                        umma_commit_pair(peer_smem(EMPTY(stage), 1));
+                        if (kb + 1 == nk) {
+                            umma_commit_pair(TFULL(acc));
+                            umma_commit_pair(peer_smem(TFULL(acc), 1));
+                        }
                     }
-#pragma unroll
-                    for (int kk = 0; kk < 4; ++kk) {
-                        if (kk < steps)
-                            umma_mx4<2>(d, umma_sdesc_sw128(sA + stage * C::kABytes + kk * 32, 16, 1024),
-                                        umma_sdesc_sw128(sB + stage * C::kBBytes + kk * 32, 16, 1024), kIdesc[kk & 1],
-                                        sfa + 4 * (kk >> 1), sfb + (kk >> 1) * (BN / 32), (kb | kk) != 0 ? 1u : 0u);
-                    }
-                    umma_commit_pair(EMPTY(stage));
-                    umma_commit_pair(peer_smem(EMPTY(stage), 1));
+                    __syncwarp();
                     if (++stage == STAGES) { stage = 0; ph ^= 1u; }
                 }
                 if (!ok) break;
-                umma_commit_pair(TFULL(acc));
-                umma_commit_pair(peer_smem(TFULL(acc), 1));
                 ++count;
             }
-            umma_commit_pair(final_bar);
+            if (elect_one()) umma_commit_pair(final_bar);
+            __syncwarp();
             drain_wait(final_bar, 0);
         }
     } else {
@@ -647,52 +676,56 @@ __global__ void __launch_bounds__(kFewThreads, 2)
     const uint32_t tmem = *tmem_slot;
 
     if (warp == 0) {
-        if (lane == 0) {
-            const int w_row = e * args.N + nb * 128, w_sf = e * args.w_tiles + nb;
-            auto load_w = [&](int st, int kb) {
-                const uint32_t at = ring + st * stage_bytes;
-                tma_load_2d(at, &tmW, FULL(st), kb * kCodeRow, w_row);
-                tma_load_2d(at + w_bytes + x_bytes, &tmSW, FULL(st), kb * 256, w_sf);
-            };
-            int pre = 0;
-            if (args.mode == kDense) {
-                if (args.w_early)
-                    for (; pre < stages && k0 + pre < k1; ++pre) load_w(pre, k0 + pre);
-                pdl_wait();
-            }
-            int stage = 0;
-            uint32_t ph = 0, issued = 0;
-            for (int kb = k0; kb < k1; ++kb) {
-                if (!mbar_wait(EMPTY(stage), ph ^ 1u, fault, 111)) break;
+        const int w_row = __shfl_sync(0xFFFFFFFFu, e, 0) * args.N + nb * 128, w_sf = __shfl_sync(0xFFFFFFFFu, e, 0) * args.w_tiles + nb;
+        const int row0 = __shfl_sync(0xFFFFFFFFu, x_row, 0);
+        auto load_w = [&](int st, int kb) {
+            const uint32_t at = ring + st * stage_bytes;
+            tma_load_2d(at, &tmW, FULL(st), kb * kCodeRow, w_row);
+            tma_load_2d(at + w_bytes + x_bytes, &tmSW, FULL(st), kb * 256, w_sf);
+        };
+        int pre = 0;
+        if (args.mode == kDense) {
+            if (args.w_early)
+                for (; pre < stages && k0 + pre < k1; ++pre)
+                    if (elect_one()) load_w(pre, k0 + pre);
+            __syncwarp();
+            pdl_wait();
+        }
+        int stage = 0;
+        uint32_t ph = 0, issued = 0;
+        for (int kb = k0; kb < k1; ++kb) {
+            if (!warp_wait(EMPTY(stage), ph ^ 1u, fault, 111)) break;
+            if (elect_one()) {
                 mbar_expect_tx(FULL(stage), FUSE == kFuseNone ? stage_bytes : w_bytes + kScaleBlock);
                 const uint32_t at = ring + stage * stage_bytes;
                 if (static_cast<int>(issued) >= pre) load_w(stage, kb);
                 if (FUSE == kFuseNone) {
-                    tma_load_2d(at + w_bytes, &tmX.x[box], FULL(stage), kb * kCodeRow, x_row);
+                    tma_load_2d(at + w_bytes, &tmX.x[box], FULL(stage), kb * kCodeRow, row0);
                     tma_load_2d(at + w_bytes + x_bytes + kScaleBlock, &tmSX, FULL(stage), kb * 256, x_sf);
                 }
-                ++issued;
-                if (++stage == stages) { stage = 0; ph ^= 1u; }
             }
-            pdl_trigger();
-            const uint32_t n = static_cast<uint32_t>(stages);
-            for (uint32_t s = 0; s < n && s < issued; ++s) {
-                const uint32_t last = s + ((issued - 1 - s) / n) * n;
-                drain_wait(EMPTY(s), (last / n) & 1u);
-            }
+            __syncwarp();
+            ++issued;
+            if (++stage == stages) { stage = 0; ph ^= 1u; }
+        }
+        pdl_trigger();
+        const uint32_t n = static_cast<uint32_t>(stages);
+        for (uint32_t s = 0; s < n && s < issued; ++s) {
+            const uint32_t last = s + ((issued - 1 - s) / n) * n;
+            drain_wait(EMPTY(s), (last / n) & 1u);
         }
     } else if (warp == 1) {
-        if (lane == 0) {
-            const uint32_t idesc[2] = {idesc_mx4(128, nt, 0), idesc_mx4(128, nt, 1)};
-            const uint32_t sfa = tmem + 128, sfb = sfa + 8;
-            int stage = 0;
-            uint32_t ph = 0;
-            for (int kb = k0; kb < k1; ++kb) {
-                if (!mbar_wait(FULL(stage), ph, fault, 112)) break;
-                tc_fence_after();
-                const uint32_t at = ring + stage * stage_bytes;
-                const uint32_t sw = at + w_bytes + x_bytes, sx = sw + kScaleBlock;
-                const int steps = kb + 1 == args.nk ? args.last_steps : 4;
+        const uint32_t idesc[2] = {idesc_mx4(128, nt, 0), idesc_mx4(128, nt, 1)};
+        const uint32_t sfa = tmem + 128, sfb = sfa + 8;
+        int stage = 0;
+        uint32_t ph = 0;
+        for (int kb = k0; kb < k1; ++kb) {
+            if (!warp_wait(FULL(stage), ph, fault, 112)) break;
+            tc_fence_after();
+            const uint32_t at = ring + stage * stage_bytes;
+            const uint32_t sw = at + w_bytes + x_bytes, sx = sw + kScaleBlock;
+            const int steps = kb + 1 == args.nk ? args.last_steps : 4;
+            if (elect_one()) {
 #pragma unroll
                 for (int kt = 0; kt < 2; ++kt) {
                     copy_scales<1>(sfa + 4 * kt, scale_desc(sw + kt * kMxTileBytes));
@@ -705,11 +738,13 @@ __global__ void __launch_bounds__(kFewThreads, 2)
                                     idesc[kk & 1], sfa + 4 * (kk >> 1), sfb + 4 * (kk >> 1), kb > k0 || kk > 0 ? 1u : 0u);
                 }
                 umma_commit(EMPTY(stage));
-                if (++stage == stages) { stage = 0; ph ^= 1u; }
             }
-            umma_commit(done);
-            drain_wait(done, 0);
+            __syncwarp();
+            if (++stage == stages) { stage = 0; ph ^= 1u; }
         }
+        if (elect_one()) umma_commit(done);
+        __syncwarp();
+        drain_wait(done, 0);
     } else if constexpr (FUSE != kFuseNone) {
         // task t: k-block k0 + t / pairs, rows 2 (t % pairs) and the next; eight slots, task by task,
         // so every stage is freed by k-blocks whose tasks come earlier

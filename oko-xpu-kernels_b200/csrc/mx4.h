@@ -46,7 +46,7 @@ int mx4_expert_mm(cudaStream_t s, const uint8_t *a_codes, const uint8_t *a_scale
 int mx4_expert_dw(cudaStream_t s, const uint8_t *a_codes, const uint8_t *a_scales, const uint8_t *b_codes, const uint8_t *b_scales,
                   void *out, int type, const int32_t *tiles, int64_t max_tiles, int64_t M, int64_t N, int64_t experts);
 // few tokens quantised inside the product: x [M, K] of the output's type, M <= kMx4Tokens
-constexpr int64_t kMx4Tokens = 16;
+constexpr int64_t kMx4Tokens = 8;
 int mx4_token_mm(cudaStream_t s, const void *x, int64_t ldx, const uint8_t *b_codes, const uint8_t *b_scales, const float *bias, void *out,
                  int type, int64_t M, int64_t N, int64_t K, bool rotate);
 // the same by expert, rows <= kMx4ExpertRows: row r comes from x's row r (fan 0) or token order[r] / fan

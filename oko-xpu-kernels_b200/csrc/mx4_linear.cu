@@ -1,7 +1,7 @@
 // The MXFP4 linears as one C call each: the quantizers and products of mxfp4.cu and gemm_mx4.cu in
 // order on the caller's stream, over caller scratch.
 //
-//   linear         y = Q(x) Wq^T (+ bias): up to 16 tokens in one launch (quantised inside the product)
+//   linear         y = Q(x) Wq^T (+ bias): up to 8 tokens in one launch (quantised inside the product)
 //   train          y = Q(x) Q(w)^T (+ bias), and what the gradients need later: x and w quantised along
 //                  the other axis, in the same read
 //   grad           dx = Q(dy) Q(w^T)^T, dw = Q(dy^T) Q(x^T)^T, each turned back where x and w were rotated

@@ -256,9 +256,9 @@ def linear_mxfp4(x, w, bias=None, *, rotate=True):
     out = x2.new_empty((m, n))
     if m and n:
         p = x2.data_ptr()
-        # up to 16 aligned rows are quantised inside the product, without scratch
+        # up to 8 aligned rows are quantised inside the product, without scratch
         work = None
-        if m > 16 or p % 16 or ldx * x2.element_size() % 16:
+        if m > 8 or p % 16 or ldx * x2.element_size() % 16:
             work = _scratch(_entry("mxfp4_linear_workspace_bytes")(m, k), x.device)
         _launch("mxfp4_linear", index, p, t, ldx, w._cp, w._sp, None if bias is None else bias.data_ptr(),
                 out.data_ptr(), None if work is None else work.data_ptr(), m, n, k, 1 if rotate else 0)
