@@ -389,7 +389,7 @@ __global__ void __launch_bounds__(PairCfg<BN>::kThreads, 1)
             // the whole warp walks the loop and one elected lane issues: the addresses and descriptors
             // then live in uniform registers, where these instructions take them from; in a branch of
             // one lane each operand is moved there first, and the issue itself bounds the main loop
-            // (8192 x 14336 x 4096: 264 us so, against the figure above)
+            // (8192 x 14336 x 4096: 264 us so, 188 us this way)
             constexpr uint32_t kIdesc[2] = {idesc_mx4(256, BN, 0), idesc_mx4(256, BN, 1)};
             const uint32_t sfa = tmem_base + C::kScaleCol, sfb = sfa + 8;
             int stage = 0, count = 0;
@@ -977,12 +977,18 @@ int launch_pair_type(cudaStream_t s, const PairMaps &m, const PairArgs &a, int64
 
 // `a` complete but for the tile counts; max_m: 256-row tiles (rows: at most)
 int run_pair(cudaStream_t s, PairArgs a, const Operand &A, const Operand &B, int type, int64_t out_rows, int64_t max_m) {
-    // 256-column tiles where they fill the pairs; half as wide where they would leave pairs idle
+    // 256 or 128 columns a tile, by the rounds that the pairs take.  A k-block takes 0.32 us at 256
+    // columns and nearly as long at 128 (0.9 of it: an MMA's time hardly depends on its columns), and a
+    // tile costs its hand-over and the end of its drain, 7.5 k-blocks' time at 256 columns and 5 at
+    // 128 (measured at 8192 x 14336 and 18944 x 128 to 256, K 1024 to 16384).  So the narrow tile wins
+    // where it turns one round of few tiles into one of more: 1000 x 1024 x 1024 5.8 us against 7.3,
+    // 4096 x 1280 x 5120 25.5 us wide against 30 narrow.
     const int64_t matrices = a.mode == kContraction ? a.experts : 1;
     const int64_t pairs = num_sms() / 2;
+    const int64_t nk = a.mode == kContraction ? std::max<int64_t>(1, A.K / BK / a.experts) : a.nk;
     auto cost = [&](int bn) {
         const int64_t tiles = max_m * matrices * ((a.N + bn - 1) / bn);
-        return (tiles + pairs - 1) / pairs * (bn + 32);
+        return (tiles + pairs - 1) / pairs * (bn == 256 ? 10 * nk + 75 : 9 * nk + 50);
     };
     const int bn = cost(128) < cost(256) ? 128 : 256;
     a.num_n = (a.N + bn - 1) / bn;
