@@ -756,7 +756,7 @@ __global__ void __launch_bounds__(kFewThreads, 2)
             int64_t row = x_row + r;
             if (args.fan > 0) row = __ldg(args.order + row) / args.fan;
             const uint8_t *p = static_cast<const uint8_t *>(args.x) + row * args.ldx * mx_size(T);
-            return load_run<T, true>(p, kb * 256 + l * 16, args.K);
+            return load_run<T, true>(p, kb * 256 + l * 16, args.K, false);
         };
         int t = slot, rp = 0, kb = k0;
         Run<T> A = zero_run<T>(), B = zero_run<T>();

@@ -14,12 +14,32 @@ struct Run {
     uint32_t w[kWords];
 };
 
-// from column c on, zero past `cols`
+// eight words by one 32-byte access
+__device__ __forceinline__ void load_v8(const void *p, uint32_t *w) {
+    asm("ld.global.nc.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+        : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7])
+        : "l"(p));
+}
+__device__ __forceinline__ void store_v8(void *p, const uint32_t *w) {
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]),
+                 "r"(w[5]), "r"(w[6]), "r"(w[7])
+                 : "memory");
+}
+
+// from column c on, zero past `cols`.  VEC: rows are 16-byte aligned; wide: 32-byte, so that a lane's
+// run of a 16-bit type is one access and a warp's are whole lines (as two of 16 bytes they take twice
+// the shared-memory pipe's time, which bounds the rotated quantizer)
 template <int T, bool VEC>
-__device__ __forceinline__ Run<T> load_run(const void *row, uint32_t c, uint32_t cols) {
+__device__ __forceinline__ Run<T> load_run(const void *row, uint32_t c, uint32_t cols, bool wide) {
     Run<T> r;
     if (VEC && c + 16 <= cols) {
-        const uint4 *p = reinterpret_cast<const uint4 *>(static_cast<const uint8_t *>(row) + static_cast<int64_t>(c) * mx_size(T));
+        const uint8_t *q = static_cast<const uint8_t *>(row) + static_cast<int64_t>(c) * mx_size(T);
+        if (wide) {
+#pragma unroll
+            for (int j = 0; j < Run<T>::kWords / 8; ++j) load_v8(q + 32 * j, r.w + 8 * j);
+            return r;
+        }
+        const uint4 *p = reinterpret_cast<const uint4 *>(q);
 #pragma unroll
         for (int j = 0; j < Run<T>::kWords / 4; ++j) {
             const uint4 q = __ldg(p + j);
@@ -134,8 +154,8 @@ __device__ __forceinline__ PairCodes quantize_runs(const Run<T> &A, const Run<T>
 // A pair of 256-value groups A and B on a half-warp's lanes, turned to pairs: value c of both at
 // pair_at(c) of the slot's shared memory, as a word (16-bit types) or two (fp32).  The pitches put
 // the words of a column and those of a run into different banks, with every address a base and a
-// constant.
-constexpr int kSlotBytes = 16 * 144;
+// constant; the slots of a warp's two halves lie 16 banks apart.
+constexpr int kSlotBytes = 16 * 144 + 64;
 template <int T>
 __device__ __forceinline__ constexpr uint32_t pair_at(int w, int l) { return T == kMxF32 ? w * 144 + l * 8 : w * 80 + l * 4; }
 

@@ -35,11 +35,19 @@ struct RowArgs {
     const int32_t *positions;    // [slots] the row of codes that a slot's row goes to
     const int32_t *scale_rows;   // [slots] the row of scales; negative: no expert takes it
     uint32_t fan;                // slots of a token
+    bool wide, wide_out;         // rows of x and of the rotated values are 32-byte aligned
 };
 
+// a run to a row that is 16-byte aligned (wide: 32)
 template <int T>
-__device__ __forceinline__ void store_run(void *row, uint32_t c, const Run<T> &r) {
-    uint4 *p = reinterpret_cast<uint4 *>(static_cast<uint8_t *>(row) + static_cast<int64_t>(c) * mx_size(T));
+__device__ __forceinline__ void store_run(void *row, uint32_t c, const Run<T> &r, bool wide) {
+    uint8_t *q = static_cast<uint8_t *>(row) + static_cast<int64_t>(c) * mx_size(T);
+    if (wide) {
+#pragma unroll
+        for (int j = 0; j < Run<T>::kWords / 8; ++j) store_v8(q + 32 * j, r.w + 8 * j);
+        return;
+    }
+    uint4 *p = reinterpret_cast<uint4 *>(q);
 #pragma unroll
     for (int j = 0; j < Run<T>::kWords / 4; ++j) p[j] = make_uint4(r.w[4 * j], r.w[4 * j + 1], r.w[4 * j + 2], r.w[4 * j + 3]);
 }
@@ -60,8 +68,8 @@ __global__ void __launch_bounds__(128) quantize_rows_kernel(const RowArgs a) {
     const uint32_t rp = a.G(task), g = task - rp * a.G.d, r = 2 * rp, c = g * 256 + l * 16;
     const bool two = r + 1 < a.rows;
     const uint8_t *row = static_cast<const uint8_t *>(a.x) + r * a.ldx * mx_size(T);
-    const Run<T> A = load_run<T, VEC>(row, c, a.K);
-    const Run<T> B = two ? load_run<T, VEC>(row + a.ldx * mx_size(T), c, a.K) : zero_run<T>();
+    const Run<T> A = load_run<T, VEC>(row, c, a.K, a.wide);
+    const Run<T> B = two ? load_run<T, VEC>(row + a.ldx * mx_size(T), c, a.K, a.wide) : zero_run<T>();
     pdl_trigger();
     PairCodes q;
     if constexpr (ROT) {
@@ -72,8 +80,8 @@ __global__ void __launch_bounds__(128) quantize_rows_kernel(const RowArgs a) {
             Run<T> u, v;
             split_pairs<T>(p, u, v);
             uint8_t *out = static_cast<uint8_t *>(a.rotated) + static_cast<int64_t>(r) * a.K * mx_size(T);
-            store_run<T>(out, c, u);
-            if (two) store_run<T>(out + static_cast<int64_t>(a.K) * mx_size(T), c, v);
+            store_run<T>(out, c, u, a.wide_out);
+            if (two) store_run<T>(out + static_cast<int64_t>(a.K) * mx_size(T), c, v, a.wide_out);
         }
         if (!a.codes) return;
         q = quantize_pairs<T>(p);
@@ -250,6 +258,8 @@ struct BothArgs {
     const int32_t *offsets, *tiles, *order;  // experts: rows are sorted rows, taken from slot order[row]'s token
     int experts;
     uint32_t fan;                          // slots of a token; 0: x's rows are sorted already
+    int subs;                              // 32-row steps of a CTA: 4, or 2 or 1 where that fills the device
+    bool wide;                             // rows of x are 32-byte aligned
 };
 
 constexpr int kBothThreads = 256, kBothSlots = 16, kCodePitch = 80;
@@ -265,7 +275,8 @@ __global__ void __launch_bounds__(kBothThreads) quantize_both_kernel(const BothA
     const uint32_t slots = smem_u32(smem);
     uint8_t *s_code = smem + kBothSlots * kSlotBytes;
     uint8_t *s_scale = s_code + 256 * kCodePitch;
-    const int slot = threadIdx.x >> 4, l = threadIdx.x & 15, kt = blockIdx.y;
+    const int slot = threadIdx.x >> 4, l = threadIdx.x & 15;
+    const int row0 = blockIdx.y * 32 * a.subs, kt = row0 >> 7, sub0 = (row0 >> 5) & 3;
     const uint32_t mine = slots + slot * kSlotBytes;
     pdl_trigger();
     uint32_t begin = kt * 128u, end = a.rows;
@@ -281,11 +292,11 @@ __global__ void __launch_bounds__(kBothThreads) quantize_both_kernel(const BothA
         if (begin + i >= end) return zero_run<T>();
         uint32_t r = begin + i;
         if (a.fan) r = static_cast<uint32_t>(__ldg(a.order + r)) / a.fan;
-        return load_run<T, VEC>(x + static_cast<int64_t>(r) * a.ldx * mx_size(T), c, a.cols);
+        return load_run<T, VEC>(x + static_cast<int64_t>(r) * a.ldx * mx_size(T), c, a.cols, a.wide);
     };
-    Run<T> A = bring(2 * slot), B = bring(2 * slot + 1);
+    Run<T> A = bring(sub0 * 32 + 2 * slot), B = bring(sub0 * 32 + 2 * slot + 1);
 #pragma unroll 1
-    for (int sub = 0; sub < 4; ++sub) {
+    for (int sub = sub0; sub < sub0 + a.subs; ++sub) {
         if constexpr (ROT) rotate_to_shared<T>(A, B, mine, l);
         else runs_to_shared<T>(A, B, mine, l);
         if (a.row_codes) {
@@ -307,7 +318,7 @@ __global__ void __launch_bounds__(kBothThreads) quantize_both_kernel(const BothA
             }
         }
         __syncwarp();
-        if (sub < 3) {
+        if (sub + 1 < sub0 + a.subs) {
             A = bring(sub * 32 + 32 + 2 * slot);
             B = bring(sub * 32 + 33 + 2 * slot);
         }
@@ -344,14 +355,19 @@ __global__ void __launch_bounds__(kBothThreads) quantize_both_kernel(const BothA
     if (!a.col_codes) return;
     uint8_t *codes = a.col_codes + blockIdx.z * a.col_matrix_codes;
     uint8_t *scales = a.col_scales + blockIdx.z * a.col_matrix_scales;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const uint32_t col = (threadIdx.x >> 2) + 64 * i, part = threadIdx.x & 3, n = blockIdx.x * 256 + col;
+    const int shift = a.subs >> 1;  // log2
+    for (int i = threadIdx.x; i < 256 << shift; i += kBothThreads) {
+        const uint32_t col = i >> shift, part = sub0 + (i & (a.subs - 1)), n = blockIdx.x * 256 + col;
         if (n < a.cols && kt * 4u + part < a.col_blocks)
             *reinterpret_cast<uint4 *>(codes + n * a.col_pitch + (kt * 4 + part) * 16) = *reinterpret_cast<const uint4 *>(s_code + col * kCodePitch + part * 16);
     }
     const uint32_t n = blockIdx.x * 256 + threadIdx.x;
-    if (n < a.cols) *reinterpret_cast<uint32_t *>(scales + mx_scale_word(n, kt, a.col_KT)) = *reinterpret_cast<const uint32_t *>(s_scale + threadIdx.x * 4);
+    if (n < a.cols) {
+        uint8_t *to = scales + mx_scale_word(n, kt, a.col_KT), *from = s_scale + threadIdx.x * 4;
+        if (a.subs == 4) *reinterpret_cast<uint32_t *>(to) = *reinterpret_cast<const uint32_t *>(from);
+        else
+            for (int q = sub0; q < sub0 + a.subs; ++q) to[q] = from[q];
+    }
 }
 
 struct TurnArgs {
@@ -360,6 +376,7 @@ struct TurnArgs {
     uint32_t groups, G, K;
     const int32_t *positions, *scale_rows;  // experts: [rows, fan], or null
     uint32_t fan;
+    bool wide, wide_out;         // rows of x and out are 32-byte aligned
 };
 
 // fp32 rows, or the sums of each token's rows, turned back by the rotation and rounded once.
@@ -374,12 +391,12 @@ __global__ void __launch_bounds__(128) turn_kernel(const TurnArgs a) {
         Run<kMxF32> v = zero_run<kMxF32>();
         if (!ok) return v;
         const uint32_t c = g * 256 + l * 16;
-        if (!a.positions) return load_run<kMxF32, VEC>(a.x + static_cast<int64_t>(r) * a.K, c, a.K);
+        if (!a.positions) return load_run<kMxF32, VEC>(a.x + static_cast<int64_t>(r) * a.K, c, a.K, a.wide);
 #pragma unroll 2
         for (uint32_t j = 0; j < a.fan; ++j) {
             const int64_t at = static_cast<int64_t>(r) * a.fan + j;
             if (__ldg(a.scale_rows + at) < 0) continue;
-            const Run<kMxF32> u = load_run<kMxF32, VEC>(a.x + static_cast<int64_t>(__ldg(a.positions + at)) * a.K, c, a.K);
+            const Run<kMxF32> u = load_run<kMxF32, VEC>(a.x + static_cast<int64_t>(__ldg(a.positions + at)) * a.K, c, a.K, a.wide);
 #pragma unroll
             for (int t = 0; t < 16; ++t) v.w[t] = __float_as_uint(__fadd_rn(__uint_as_float(v.w[t]), __uint_as_float(u.w[t])));
         }
@@ -402,7 +419,7 @@ __global__ void __launch_bounds__(128) turn_kernel(const TurnArgs a) {
                 if constexpr (T == kMxF32) o.w[t] = v.w[t];
                 else o.w[t] = mx_join<T>(__uint_as_float(v.w[2 * t]), __uint_as_float(v.w[2 * t + 1]));
             }
-            store_run<T>(row, c, o);
+            store_run<T>(row, c, o, a.wide_out);
         } else {
 #pragma unroll
             for (int t = 0; t < 16; ++t)
@@ -419,6 +436,7 @@ struct ValueArgs {
     uint32_t K, KB, KT, units;  // units: of a row, runs of 16 values or of eight blocks
     int64_t total;              // rows * units
     uint32_t matrix_rows, matrix_tiles;
+    bool wide;                  // rows of out are 32-byte aligned
 };
 
 // Rows that are 16-byte aligned: 16 values a thread, 8 bytes of codes, a scale byte, 32 (64) bytes out.
@@ -445,7 +463,7 @@ __global__ void __launch_bounds__(256) values_kernel(const ValueArgs a) {
             out.w[t] = mx_join<T>(v0, v1);
         }
     }
-    store_run<T>(static_cast<uint8_t *>(a.out) + r * a.K * mx_size(T), h * 16, out);
+    store_run<T>(static_cast<uint8_t *>(a.out) + r * a.K * mx_size(T), h * 16, out, a.wide);
 }
 
 // Rows of any length: a warp reads eight blocks of a row one after another, a value a lane, so that
@@ -508,6 +526,8 @@ int quantize_rows(cudaStream_t s, RowArgs &a, int type, int64_t rows, int64_t K,
     a.ldx = ldx;
     a.tasks = static_cast<uint32_t>((rows + 1) / 2 * G);
     const bool vec = aligned(a.x, 16) && (ldx * mx_size(type)) % 16 == 0;
+    a.wide = aligned(a.x, 32) && (ldx * mx_size(type)) % 32 == 0;
+    a.wide_out = aligned(a.rotated, 32);
     switch (type) {
         case kMxBf16: launch_rows<kMxBf16>(s, a, rotate, vec); break;
         case kMxF16: launch_rows<kMxF16>(s, a, rotate, vec); break;
@@ -640,7 +660,13 @@ int mx4_quantize_both(cudaStream_t s, const Mx4Both &b) {
         return 2;
     }
     const bool vec = aligned(b.x, 16) && (b.ldx * mx_size(b.type)) % 16 == 0;
-    const dim3 grid(static_cast<uint32_t>((b.cols + 255) / 256), a.col_KT, static_cast<uint32_t>(b.matrices));
+    a.wide = aligned(b.x, 32) && (b.ldx * mx_size(b.type)) % 32 == 0;
+    // 128 rows a CTA write each column's 64 bytes together; fewer rows where the CTAs would not fill the
+    // device twice (three fit an SM): [4096, 1280] takes 12.7 us in 160 CTAs of four steps
+    const int64_t ctas = (b.cols + 255) / 256 * a.col_KT * b.matrices;
+    a.subs = 4;
+    while (a.subs > 1 && ctas * (4 / a.subs) < 6 * num_sms() && a.col_KT * (8 / a.subs) <= 65535) a.subs /= 2;
+    const dim3 grid(static_cast<uint32_t>((b.cols + 255) / 256), a.col_KT * (4 / a.subs), static_cast<uint32_t>(b.matrices));
     switch (b.type) {
         case kMxBf16: return launch_both<kMxBf16>(s, a, grid, b.rotate, vec);
         case kMxF16: return launch_both<kMxF16>(s, a, grid, b.rotate, vec);
@@ -663,6 +689,8 @@ int mx4_turn(cudaStream_t s, const float *x, void *out, int type, int64_t rows, 
     a.positions = positions;
     a.scale_rows = scale_rows;
     a.fan = static_cast<uint32_t>(fan);
+    a.wide = aligned(x, 32) && K % 8 == 0;
+    a.wide_out = aligned(out, 32) && (K * mx_size(type)) % 32 == 0;
     const bool vec = aligned(x, 16) && aligned(out, 16) && (K * mx_size(type)) % 16 == 0 && K % 4 == 0;
     switch (type) {
         case kMxBf16: launch_turn<kMxBf16>(s, a, rotate, vec); break;
@@ -797,6 +825,7 @@ int xpuint8_mxfp4_dequantize_stream(const void *stream, const uint8_t *codes,
     a.matrix_rows = static_cast<uint32_t>(matrix_rows);
     a.matrix_tiles = static_cast<uint32_t>((matrix_rows + 127) / 128);
     const bool vec = aligned(out, 16) && (K * mx_size(type)) % 16 == 0 && K % 16 == 0;
+    a.wide = aligned(out, 32) && (K * mx_size(type)) % 32 == 0;
     a.units = static_cast<uint32_t>(vec ? K / 16 : (K + 255) / 256);
     a.total = rows * a.units;
     const int64_t blocks = vec ? (a.total + 255) / 256 : (a.total + 7) / 8;
