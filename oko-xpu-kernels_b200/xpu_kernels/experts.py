@@ -15,8 +15,9 @@ them have the largest size they can need.
 from __future__ import annotations
 
 import torch
+from torch.autograd.function import once_differentiable
 
-from .mxfp4 import _TYPES, _check_rotate, _entry, _launch, _rows, _scratch, _type
+from .mxfp4 import _TYPES, _check_rotate, _entry, _launch, _rows, _scratch, _type, _wanted
 
 
 class ExpertPlan:
@@ -131,6 +132,7 @@ class _GatherFn(torch.autograd.Function):
         return _gather(x, plan)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dy):
         return _combine(dy, None, ctx.plan), None
 
@@ -143,6 +145,7 @@ class _CombineFn(torch.autograd.Function):
         return _combine(y, weights, plan)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dy):
         y, weights = ctx.saved_tensors
         plan = ctx.plan
@@ -243,26 +246,26 @@ class _ExpertLinearFn(torch.autograd.Function):
     along each expert's own rows."""
 
     @staticmethod
-    def forward(ctx, x, w, plan, rotate, in_order):
+    def forward(ctx, x, w, plan, rotate, in_order, want):
         e, n, k = w.shape
         w = w.contiguous()
         x2, ldx = _rows(x)
         rows, device = plan.rows, x.device
-        need = ctx.needs_input_grad
-        want = (1 if need[0] else 0) | (2 if need[1] else 0)
         y = x2.new_empty((rows, n))
         flags = (1 if rotate else 0, 1 if in_order else 0)
         if n:
-            saved = _scratch(_entry("mxfp4_expert_train_saved_workspace_bytes")(plan.max_tiles, n, k, e, want), device)
+            saved = _scratch(_entry("mxfp4_expert_train_saved_workspace_bytes")(plan.max_tiles, n, k, e, want), device) if want else None
             work = _scratch(_entry("mxfp4_expert_train_workspace_bytes")(rows, plan.max_tiles, n, k, e), device)
             _launch("mxfp4_expert_train", plan._index, x2.data_ptr(), _TYPES[x.dtype], ldx, w.data_ptr(), _TYPES[w.dtype],
-                    y.data_ptr(), saved.data_ptr() if want else None, work.data_ptr(), *plan._at, plan.tokens, plan.top,
+                    y.data_ptr(), None if saved is None else saved.data_ptr(), work.data_ptr(), *plan._at, plan.tokens, plan.top,
                     plan.max_tiles, n, k, e, *flags, want)
-            ctx.save_for_backward(saved)
+            if saved is not None:
+                ctx.save_for_backward(saved)
         ctx.plan, ctx.sizes, ctx.like = plan, (e, n, k, want, flags), (x.dtype, w.dtype)
         return y
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dy):
         plan = ctx.plan
         e, n, k, want, flags = ctx.sizes
@@ -283,7 +286,7 @@ class _ExpertLinearFn(torch.autograd.Function):
                     *plan._at, plan.tokens, plan.top, plan.max_tiles, n, k, e, *flags, want)
         elif need[0]:
             dx.zero_()
-        return dx, dw, None, None, None
+        return dx, dw, None, None, None, None
 
 
 def mxfp4_expert_linear(x, w, plan, *, rotate=True, sorted=False):
@@ -295,7 +298,7 @@ def mxfp4_expert_linear(x, w, plan, *, rotate=True, sorted=False):
     _same_device(w.get_device(), plan, w, "w")
     if plan.rows == 0:
         return x.reshape(0, x.shape[1]) @ w.sum(0).to(x.dtype).T
-    return _ExpertLinearFn.apply(x, w, plan, rotate, sorted)
+    return _ExpertLinearFn.apply(x, w, plan, rotate, sorted, _wanted(x, w))
 
 
 def expert_ffn_mxfp4(x, ids, weights, up, down, *, rotate=True):

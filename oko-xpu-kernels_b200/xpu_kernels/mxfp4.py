@@ -17,6 +17,7 @@ The kernels run on torch's current stream; nothing here synchronises.
 from __future__ import annotations
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from .int8._lib import _err, _lib
 
@@ -186,6 +187,8 @@ def dequantize_mxfp4(q, dtype=torch.bfloat16):
     t = _TYPES.get(dtype)
     if t is None:
         raise TypeError(f"dtype must be bfloat16, float16 or float32, got {dtype}")
+    if q._index < 0:
+        raise TypeError(f"q must be on a CUDA device, got {q.device}")
     out = torch.empty(q.shape, dtype=dtype, device=q._buffer.device if q._codes is None else q._codes.device)
     n = out.numel()
     if n:
@@ -222,6 +225,8 @@ def mxfp4_mm(a, b, bias=None, dtype=torch.bfloat16):
         raise TypeError(f"dtype must be bfloat16, float16 or float32, got {dtype}")
     if a._index != b._index:
         raise ValueError(f"a is on {a.device} and b on {b.device}")
+    if a._index < 0:
+        raise TypeError(f"a and b must be on a CUDA device, got {a.device}")
     device = a.device
     bias = _bias(bias, n, device)
     out = torch.empty((m, n), dtype=dtype, device=device)
@@ -272,13 +277,11 @@ class _Mxfp4LinearFn(torch.autograd.Function):
     their gradient is wanted."""
 
     @staticmethod
-    def forward(ctx, x, w, bias, rotate):
+    def forward(ctx, x, w, bias, rotate, want):
         n, k = w.shape
         x2, ldx = _rows(x.reshape(-1, k))
         w2, ldw = _rows(w)
         m, device, index = x2.shape[0], x.device, x.get_device()
-        need = ctx.needs_input_grad
-        want = (1 if need[0] else 0) | (2 if need[1] else 0)
         y = x2.new_empty((m, n))
         saved = None
         if m and n:
@@ -296,6 +299,7 @@ class _Mxfp4LinearFn(torch.autograd.Function):
         return y.reshape(*x.shape[:-1], n)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dy):
         m, n, k, want, rotate = ctx.sizes
         x_type, w_type, bias_type, shape = ctx.like
@@ -317,7 +321,7 @@ class _Mxfp4LinearFn(torch.autograd.Function):
                 if g is not None:
                     g.zero_()
         db = dy2.sum(dim=0, dtype=torch.float32).to(bias_type) if need[2] else None
-        return (None if dx is None else dx.reshape(shape)), dw, db, None
+        return (None if dx is None else dx.reshape(shape)), dw, db, None, None
 
 
 def mxfp4_linear(x, w, bias=None, *, rotate=True):
@@ -332,7 +336,12 @@ def mxfp4_linear(x, w, bias=None, *, rotate=True):
     if w.shape[1] == 0:
         raise ValueError("mxfp4_linear needs K of at least 1")
     _check_rotate(w.shape[1], rotate)
-    return _Mxfp4LinearFn.apply(x, w, bias, rotate)
+    return _Mxfp4LinearFn.apply(x, w, bias, rotate, _wanted(x, w))
+
+
+def _wanted(x, w):
+    """Which gradients a backward call may ask for: bit 0 x's, bit 1 w's."""
+    return (1 if x.requires_grad else 0) | (2 if w.requires_grad else 0) if torch.is_grad_enabled() else 0
 
 
 class Mxfp4Linear(torch.nn.Module):

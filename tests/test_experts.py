@@ -273,6 +273,40 @@ def test_rotated_expert_gradients_are_the_plain_ones_turned(gpu, in_order):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("rotate", [False, True])
+def test_one_gradient_alone_is_the_same(gpu, rotate):
+    plan = xk.expert_sort(torch.from_numpy(routing(200, 2, 3, 8, 0.1)).to(DEV), 3)
+    x, w, dy = rand((200, 256), 1).to(DEV), rand((3, 96, 256), 2).to(DEV), rand((400, 96), 3).to(DEV)
+    xg, wg = x.clone().requires_grad_(), w.clone().requires_grad_()
+    y = xk.mxfp4_expert_linear(xg, wg, plan, rotate=rotate)
+    dx, dw = torch.autograd.grad(y, (xg, wg), dy)
+    assert torch.equal(torch.autograd.grad(xk.mxfp4_expert_linear(xg, w, plan, rotate=rotate), xg, dy)[0], dx)
+    assert torch.equal(torch.autograd.grad(xk.mxfp4_expert_linear(x, wg, plan, rotate=rotate), wg, dy)[0], dw)
+    with torch.no_grad():
+        assert torch.equal(xk.mxfp4_expert_linear(xg, wg, plan, rotate=rotate), y)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("tokens,top", [(1, 1), (1, 4), (30, 4), (32, 4), (33, 4), (128, 1), (300, 2)])
+def test_rows_quantised_in_the_product_are_the_quantiser_s(gpu, tokens, top):
+    """Up to 128 rows are quantised inside the product, others before it: each row is its token's times
+    its expert's weight, whichever it is."""
+    ids = routing(tokens, top, 5, 3)
+    plan = xk.expert_sort(torch.from_numpy(ids).to(DEV), 5)
+    order, _, offsets, _, _ = X.sort(ids, 5)
+    x, w = rand((tokens, 512), 1).to(DEV), rand((5, 140, 512), 2).to(DEV)
+    wq = xk.prepare_weight_mxfp4(w)
+    got = xk.expert_linear_mxfp4(x, wq, plan)
+    sorted_rows = xk.expert_gather(x, plan)
+    assert torch.equal(got, xk.expert_linear_mxfp4(sorted_rows, wq, plan, sorted=True))
+    for e in range(5):
+        rows = slice(int(offsets[e]), int(offsets[e + 1]))
+        if rows.start < rows.stop:
+            one = xk.MXFP4(wq.codes[e], wq.scales[e], (140, 512))
+            assert torch.equal(got[rows], xk.linear_mxfp4(sorted_rows[rows], one))
+
+
+@pytest.mark.gpu
 def test_the_network(gpu):
     """The whole path against the same steps in 64 bits between its 4-bit roundings, within what
     codes that move at bf16 roundings of the intermediate can change (a step is at most a third of a

@@ -279,6 +279,54 @@ def test_gradients_against_differences(gpu, m, n, k):
         assert (loss(x, w + v) - loss(x, w - v)) / 2 == float((dw.double() * v).sum())
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("rotate", [False, True])
+def test_one_gradient_alone_is_the_same(gpu, rotate):
+    x, w, dy = rand((140, 256), 1).to(DEV), rand((96, 256), 2).to(DEV), rand((140, 96), 3).to(DEV)
+    xg, wg = x.clone().requires_grad_(), w.clone().requires_grad_()
+    y = xk.mxfp4_linear(xg, wg, rotate=rotate)
+    dx, dw = torch.autograd.grad(y, (xg, wg), dy)
+    xg, wg = x.clone().requires_grad_(), w.clone().requires_grad_()
+    assert torch.equal(torch.autograd.grad(xk.mxfp4_linear(xg, w, rotate=rotate), xg, dy)[0], dx)
+    assert torch.equal(torch.autograd.grad(xk.mxfp4_linear(x, wg, rotate=rotate), wg, dy)[0], dw)
+    both = xk.mxfp4_linear(xg, wg, rotate=rotate)
+    assert torch.equal(torch.autograd.grad(both, wg, dy, retain_graph=True)[0], dw)
+    assert torch.equal(torch.autograd.grad(both, xg, dy)[0], dx)
+    with torch.no_grad():
+        assert torch.equal(xk.mxfp4_linear(xg, wg, rotate=rotate), y)
+
+
+@pytest.mark.gpu
+def test_a_second_derivative_is_refused(gpu):
+    x, w = rand((4, 32), 1, torch.float32).to(DEV).requires_grad_(), rand((8, 32), 2, torch.float32).to(DEV)
+    dx, = torch.autograd.grad(xk.mxfp4_linear(x, w, rotate=False).square().sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        dx.sum().backward()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m", [1, 3, 8, 9, 130])
+@pytest.mark.parametrize("rotate", [False, True])
+def test_a_nan_in_x_reaches_its_row_only(gpu, m, rotate):
+    x, w = rand((m, 512), 1), rand((300, 512), 2)
+    x[m // 2, 7] = float("nan")
+    y = f64(xk.linear_mxfp4(x.to(DEV), xk.prepare_weight_mxfp4(w.to(DEV), rotate=rotate), rotate=rotate))
+    want = np.zeros((m, 300), dtype=bool)
+    want[m // 2] = True
+    assert np.array_equal(np.isnan(y), want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m", [1, 2, 5, 8])
+def test_tokens_quantised_in_the_product_are_the_quantiser_s(gpu, m):
+    for dtype in TYPES:
+        for k, rotate in ((512, True), (100, False), (2816, True)):
+            x, w = rand((m, k), m, dtype).to(DEV), rand((140, k), 2, dtype).to(DEV)
+            wq = xk.prepare_weight_mxfp4(w, rotate=rotate)
+            want = xk.mxfp4_mm(xk.quantize_mxfp4(x, rotate=rotate), wq, dtype=dtype)
+            assert torch.equal(xk.linear_mxfp4(x, wq, rotate=rotate), want)
+
+
 # ------------------------------------------------------------------------------ streams and graphs
 
 @pytest.mark.gpu
@@ -344,6 +392,10 @@ def test_arguments_are_checked_before_the_device():
         xk.quantize_mxfp4(x.double())
     with pytest.raises(TypeError, match="dtype"):
         xk.dequantize_mxfp4(w, dtype=torch.float64)
+    with pytest.raises(TypeError, match="CUDA"):
+        xk.dequantize_mxfp4(w)
+    with pytest.raises(TypeError, match="CUDA"):
+        xk.mxfp4_mm(w, w)
     with pytest.raises(ValueError, match="columns"):
         xk.linear_mxfp4(x[:, :32], w, rotate=False)
     with pytest.raises(ValueError, match="256"):
