@@ -1055,10 +1055,11 @@ int run_few(cudaStream_t s, FewArgs a, const Operand *X, const Operand &W, int t
     if (!code_map(&w, W, 128) || !scale_map(&sw, W, 1)) return 2;
     if (X) {
         if (!scale_map(&sx, *X, 1)) return 2;
-        // dense: the one box that this many tokens take; rows: each expert's count picks its own
-        const int box = a.M <= 16 ? 0 : a.M <= 32 ? 1 : a.M <= 64 ? 2 : 3;
+        // the boxes that some tile's tokens take: a dense tile's, or any where an expert's count picks it
+        const auto box = [](int n) { return n <= 16 ? 0 : n <= 32 ? 1 : n <= 64 ? 2 : 3; };
+        const int last = box((a.M - 1) % 128 + 1);
         for (int i = 0; i < 4; ++i)
-            if ((a.mode == kRows || i == box) && !code_map(&x.x[i], *X, 16 << i)) return 2;
+            if ((a.mode == kRows || i == last || (i == 3 && a.M > 128)) && !code_map(&x.x[i], *X, 16 << i)) return 2;
     }
     switch (type) {
         case kMxBf16: return launch_few<kMxBf16>(s, w, sw, x, sx, a, splits, slots, fuse);
@@ -1115,12 +1116,17 @@ FewArgs few_args(void *out, int64_t ldo, int64_t M, int64_t N, int64_t K) {
 int mx4_mm(cudaStream_t s, const uint8_t *a_codes, const uint8_t *a_scales, const uint8_t *b_codes, const uint8_t *b_scales,
            const float *bias, void *out, int type, int64_t ldo, int64_t M, int64_t N, int64_t K, bool b_early) {
     const Operand A{a_codes, a_scales, M, K, (M + 127) / 128}, B{b_codes, b_scales, N, K, (N + 127) / 128};
-    if (M <= 128) {
+    // The few-row kernel reads a weight once for up to 64 rows with less to start than the pairs' (4096 x
+    // 4096: 6.3 us at 16 rows against 8.8, 8.4 against 8.8 at 64, 11.7 against 9.1 at 128).  Beyond that
+    // it wins only where a long contraction is left to fewer tiles than there are pairs, which it splits:
+    // N 4096, K 14336: 12.6 us at 64 rows against 21.8, 18.2 at 256 against 22.5, 25.9 at 384 against 23.2.
+    const int64_t nk = (K + BK - 1) / BK;
+    if (M <= 64 || (M <= 256 && nk > 24 && (N + 127) / 128 < num_sms() / 2)) {
         FewArgs a = few_args(out, ldo, M, N, K);
         a.bias = bias;
         a.mode = kDense;
         a.w_early = b_early;
-        return run_few(s, a, &A, B, type, 1, kFuseNone);
+        return run_few(s, a, &A, B, type, (M + 127) / 128, kFuseNone);
     }
     PairArgs a{};
     a.out = out;
@@ -1167,7 +1173,10 @@ int mx4_expert_mm(cudaStream_t s, const uint8_t *a_codes, const uint8_t *a_scale
                   int64_t K, int64_t experts) {
     const Operand A{a_codes, a_scales, rows, K, max_tiles};
     const Operand B{b_codes, b_scales, experts * N, K, experts * ((N + 127) / 128)};
-    if (rows <= experts * 64) {
+    // by the mean rows of an expert: 64 experts of 2816 x 2048 take 50 us at 32 rows against the pairs'
+    // 57, 56 against 57 at 48, 63 against 57 at 64; 8 of 5632 x 2048 13.8 against 18.2, 15.9 against
+    // 18.4, 19.2 against 18.5
+    if (rows <= experts * 48) {
         FewArgs a = few_args(out, N, rows, N, K);
         a.mode = kRows;
         a.offsets = offsets;
