@@ -286,15 +286,22 @@ __global__ void __launch_bounds__(kBothThreads) quantize_both_kernel(const BothA
         begin = __ldg(a.offsets + e) + (kt - __ldg(a.tiles + e)) * 128;
         end = __ldg(a.offsets + e + 1);
     }
-    const uint32_t c = blockIdx.x * 256 + l * 16;
+    const uint32_t c = blockIdx.x * 256 + l * 16, tile = blockIdx.x * 2 + (l >> 3);
     const uint8_t *x = static_cast<const uint8_t *>(a.x) + blockIdx.z * a.matrix_stride * mx_size(T);
-    auto bring = [&](uint32_t i) {
-        if (begin + i >= end) return zero_run<T>();
-        uint32_t r = begin + i;
-        if (a.fan) r = static_cast<uint32_t>(__ldg(a.order + r)) / a.fan;
-        return load_run<T, VEC>(x + static_cast<int64_t>(r) * a.ldx * mx_size(T), c, a.cols, a.wide);
+    const int64_t pitch = a.ldx * mx_size(T);
+    // this slot's rows of a step are `row` and the next; they move on by 32 a step
+    uint32_t row = begin + sub0 * 32 + 2 * slot;
+    const uint8_t *at_x = x + row * pitch;
+    uint8_t *codes = a.row_codes + blockIdx.z * a.row_matrix_codes + static_cast<int64_t>(row) * a.KB * 16 + c / 2;
+    // row 2 slot of 32-row step j of the tile is at 32 slot + 4 j of its 512 bytes, the next 16 bytes on
+    uint8_t *scales = a.row_scales + blockIdx.z * a.row_matrix_scales + (static_cast<int64_t>(kt) * a.KT + tile) * kMxTileBytes + slot * 32 + sub0 * 4;
+    const bool has_code = c < a.KB * 32, has_word = (l & 7) == 0 && tile < a.KT;
+    auto bring = [&](uint32_t r, const uint8_t *from) {
+        if (r >= end) return zero_run<T>();
+        if (a.fan) from = x + static_cast<uint32_t>(__ldg(a.order + r)) / a.fan * pitch;
+        return load_run<T, VEC>(from, c, a.cols, a.wide);
     };
-    Run<T> A = bring(sub0 * 32 + 2 * slot), B = bring(sub0 * 32 + 2 * slot + 1);
+    Run<T> A = bring(row, at_x), B = bring(row + 1, at_x + pitch);
 #pragma unroll 1
     for (int sub = sub0; sub < sub0 + a.subs; ++sub) {
         if constexpr (ROT) rotate_to_shared<T>(A, B, mine, l);
@@ -303,24 +310,24 @@ __global__ void __launch_bounds__(kBothThreads) quantize_both_kernel(const BothA
             PairCodes q;
             if constexpr (ROT) q = quantize_pairs<T>(pairs_from_shared<T>(mine, l));
             else q = quantize_runs<T>(A, B);
-            const uint32_t i = sub * 32 + 2 * slot, tile = blockIdx.x * 2 + (l >> 3);
-            const bool has_code = c < a.KB * 32, has_word = (l & 7) == 0 && tile < a.KT;
-            const bool one = begin + i < end, two = begin + i + 1 < end;
-            uint8_t *codes = a.row_codes + blockIdx.z * a.row_matrix_codes + static_cast<int64_t>(begin + i) * a.KB * 16 + c / 2;
-            uint8_t *scales = a.row_scales + blockIdx.z * a.row_matrix_scales + mx_scale_word(kt * 128ll + i, tile, a.KT);
+            const bool one = row < end, two = row + 1 < end;
             if (has_code) {
                 if (one) *reinterpret_cast<uint2 *>(codes) = q.c0;
                 if (two) *reinterpret_cast<uint2 *>(codes + a.KB * 16) = q.c1;
             }
-            if (has_word) {  // i is even: the next row is the next 16 bytes of the tile
+            if (has_word) {
                 if (one) *reinterpret_cast<uint32_t *>(scales) = q.w0;
                 if (two) *reinterpret_cast<uint32_t *>(scales + 16) = q.w1;
             }
+            codes += a.KB * 512;
+            scales += 4;
         }
         __syncwarp();
+        row += 32;
+        at_x += 32 * pitch;
         if (sub + 1 < sub0 + a.subs) {
-            A = bring(sub * 32 + 32 + 2 * slot);
-            B = bring(sub * 32 + 33 + 2 * slot);
+            A = bring(row, at_x);
+            B = bring(row + 1, at_x + pitch);
         }
         if (!a.col_codes) continue;
         __syncthreads();
@@ -353,17 +360,17 @@ __global__ void __launch_bounds__(kBothThreads) quantize_both_kernel(const BothA
         __syncthreads();
     }
     if (!a.col_codes) return;
-    uint8_t *codes = a.col_codes + blockIdx.z * a.col_matrix_codes;
-    uint8_t *scales = a.col_scales + blockIdx.z * a.col_matrix_scales;
+    uint8_t *col_codes = a.col_codes + blockIdx.z * a.col_matrix_codes;
+    uint8_t *col_scales = a.col_scales + blockIdx.z * a.col_matrix_scales;
     const int shift = a.subs >> 1;  // log2
     for (int i = threadIdx.x; i < 256 << shift; i += kBothThreads) {
         const uint32_t col = i >> shift, part = sub0 + (i & (a.subs - 1)), n = blockIdx.x * 256 + col;
         if (n < a.cols && kt * 4u + part < a.col_blocks)
-            *reinterpret_cast<uint4 *>(codes + n * a.col_pitch + (kt * 4 + part) * 16) = *reinterpret_cast<const uint4 *>(s_code + col * kCodePitch + part * 16);
+            *reinterpret_cast<uint4 *>(col_codes + n * a.col_pitch + (kt * 4 + part) * 16) = *reinterpret_cast<const uint4 *>(s_code + col * kCodePitch + part * 16);
     }
     const uint32_t n = blockIdx.x * 256 + threadIdx.x;
     if (n < a.cols) {
-        uint8_t *to = scales + mx_scale_word(n, kt, a.col_KT), *from = s_scale + threadIdx.x * 4;
+        uint8_t *to = col_scales + mx_scale_word(n, kt, a.col_KT), *from = s_scale + threadIdx.x * 4;
         if (a.subs == 4) *reinterpret_cast<uint32_t *>(to) = *reinterpret_cast<const uint32_t *>(from);
         else
             for (int q = sub0; q < sub0 + a.subs; ++q) to[q] = from[q];
