@@ -69,10 +69,18 @@ __device__ __forceinline__ Run<T> zero_run() {
     return r;
 }
 
-// per half, the maximum of two unsigned 16-bit values
-__device__ __forceinline__ uint32_t max_u16x2(uint32_t a, uint32_t b) {
+// per half, the larger magnitude of two 16-bit values, its sign anything; a NaN is the largest
+template <int T>
+__device__ __forceinline__ uint32_t max_abs2(uint32_t a, uint32_t b) {
     uint32_t r;
-    asm("max.u16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    if constexpr (T == kMxBf16) asm("max.NaN.xorsign.abs.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    else asm("max.NaN.xorsign.abs.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+}
+// the largest of m and two magnitudes; a NaN is the largest
+__device__ __forceinline__ float max_abs3(float m, uint32_t a, uint32_t b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(m), "f"(fabsf(__uint_as_float(a))), "f"(fabsf(__uint_as_float(b))));
     return r;
 }
 // the fp32 bits of a 16-bit magnitude
@@ -109,21 +117,24 @@ template <int T>
 __device__ __forceinline__ PairCodes quantize_runs(const Run<T> &A, const Run<T> &B) {
     uint32_t mA = 0, mB = 0;
     if constexpr (T == kMxF32) {
+        float a = 0.f, b = 0.f;
 #pragma unroll
-        for (int t = 0; t < 16; ++t) {
-            mA = max(mA, A.w[t] & 0x7FFFFFFFu);
-            mB = max(mB, B.w[t] & 0x7FFFFFFFu);
+        for (int t = 0; t < 16; t += 2) {
+            a = max_abs3(a, A.w[t], A.w[t + 1]);
+            b = max_abs3(b, B.w[t], B.w[t + 1]);
         }
+        mA = __float_as_uint(a);
+        mB = __float_as_uint(b);
         mA = max(mA, __shfl_xor_sync(0xFFFFFFFFu, mA, 1));
         mB = max(mB, __shfl_xor_sync(0xFFFFFFFFu, mB, 1));
     } else {
 #pragma unroll
         for (int t = 0; t < 8; ++t) {
-            mA = max_u16x2(mA, A.w[t] & 0x7FFF7FFFu);
-            mB = max_u16x2(mB, B.w[t] & 0x7FFF7FFFu);
+            mA = max_abs2<T>(mA, A.w[t]);
+            mB = max_abs2<T>(mB, B.w[t]);
         }
-        uint32_t m = max_u16x2(__byte_perm(mA, mB, 0x5410), __byte_perm(mA, mB, 0x7632));  // (A, B)
-        m = max_u16x2(m, __shfl_xor_sync(0xFFFFFFFFu, m, 1));
+        uint32_t m = max_abs2<T>(__byte_perm(mA, mB, 0x5410), __byte_perm(mA, mB, 0x7632));  // (A, B)
+        m = max_abs2<T>(m, __shfl_xor_sync(0xFFFFFFFFu, m, 1)) & 0x7FFF7FFFu;
         mA = widen_bits<T>(m & 0xFFFFu);
         mB = widen_bits<T>(m >> 16);
     }
@@ -263,18 +274,21 @@ template <int T>
 __device__ __forceinline__ PairCodes quantize_pairs(const Pairs<T> &p) {
     uint32_t mA = 0, mB = 0;
     if constexpr (T == kMxF32) {
+        float a = 0.f, b = 0.f;
 #pragma unroll
-        for (int t = 0; t < 16; ++t) {
-            mA = max(mA, p.w[2 * t] & 0x7FFFFFFFu);
-            mB = max(mB, p.w[2 * t + 1] & 0x7FFFFFFFu);
+        for (int t = 0; t < 16; t += 2) {
+            a = max_abs3(a, p.w[2 * t], p.w[2 * t + 2]);
+            b = max_abs3(b, p.w[2 * t + 1], p.w[2 * t + 3]);
         }
+        mA = __float_as_uint(a);
+        mB = __float_as_uint(b);
         mA = max(mA, __shfl_xor_sync(0xFFFFFFFFu, mA, 1));
         mB = max(mB, __shfl_xor_sync(0xFFFFFFFFu, mB, 1));
     } else {
         uint32_t m = 0;
 #pragma unroll
-        for (int t = 0; t < 16; ++t) m = max_u16x2(m, p.w[t] & 0x7FFF7FFFu);
-        m = max_u16x2(m, __shfl_xor_sync(0xFFFFFFFFu, m, 1));
+        for (int t = 0; t < 16; ++t) m = max_abs2<T>(m, p.w[t]);
+        m = max_abs2<T>(m, __shfl_xor_sync(0xFFFFFFFFu, m, 1)) & 0x7FFF7FFFu;
         mA = widen_bits<T>(m & 0xFFFFu);
         mB = widen_bits<T>(m >> 16);
     }

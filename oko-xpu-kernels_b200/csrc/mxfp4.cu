@@ -193,14 +193,15 @@ __global__ void __launch_bounds__(128) quantize_columns_kernel(const ColumnArgs 
     uint32_t m0 = 0, m1 = 0;
     if constexpr (T == kMxF32) {
 #pragma unroll
-        for (int i = 0; i < 32; ++i) {
-            m0 = max(m0, __float_as_uint(w[i].x) & 0x7FFFFFFFu);
-            m1 = max(m1, __float_as_uint(w[i].y) & 0x7FFFFFFFu);
+        for (int i = 0; i < 32; i += 2) {
+            m0 = __float_as_uint(max_abs3(__uint_as_float(m0), __float_as_uint(w[i].x), __float_as_uint(w[i + 1].x)));
+            m1 = __float_as_uint(max_abs3(__uint_as_float(m1), __float_as_uint(w[i].y), __float_as_uint(w[i + 1].y)));
         }
     } else {
         uint32_t m = 0;
 #pragma unroll
-        for (int i = 0; i < 32; ++i) m = max_u16x2(m, w[i] & 0x7FFF7FFFu);
+        for (int i = 0; i < 32; ++i) m = max_abs2<T>(m, w[i]);
+        m &= 0x7FFF7FFFu;
         m0 = widen_bits<T>(m & 0xFFFFu);
         m1 = widen_bits<T>(m >> 16);
     }
@@ -262,19 +263,27 @@ struct BothArgs {
     bool wide;                             // rows of x are 32-byte aligned
 };
 
-constexpr int kBothThreads = 256, kBothSlots = 16, kCodePitch = 80;
-constexpr int kBothSmem = kBothSlots * kSlotBytes + 256 * kCodePitch + 256 * 4;
+constexpr int kBothThreads = 256, kBothSlots = 16;
+// the columns' codes: the 16 bytes of 32 rows in a column's 64 bytes, by columns into different banks.
+// Four CTAs an SM behind the rotation, whose arithmetic they hide; three without it, padded: four take
+// 70 us for 16384 x 5632 bf16, three 67.
+template <bool ROT>
+constexpr int kBothSmem = kBothSlots * kSlotBytes + 256 * (ROT ? 64 : 80) + 256 * 4;
+template <bool ROT>
+__device__ __forceinline__ uint32_t code_at(uint32_t col, uint32_t part) {
+    return ROT ? col * 64 + ((part ^ ((col >> 1) & 3)) << 4) : col * 80 + part * 16;
+}
 
 // Codes along the rows and along the columns in one read: a CTA takes 128 rows (a tile of scales
 // along the rows) x 256 columns (a group of the rotation), 32 rows at a time.  A slot brings two
 // neighbouring rows, rotates them, quantizes them along the columns and leaves them in shared memory
 // as pairs; a thread a column then takes the 32 rows from there.
 template <int T, bool ROT, bool VEC>
-__global__ void __launch_bounds__(kBothThreads) quantize_both_kernel(const BothArgs a) {
+__global__ void __launch_bounds__(kBothThreads, T == kMxF32 ? 2 : ROT ? 4 : 3) quantize_both_kernel(const BothArgs a) {
     extern __shared__ __align__(128) uint8_t smem[];
     const uint32_t slots = smem_u32(smem);
     uint8_t *s_code = smem + kBothSlots * kSlotBytes;
-    uint8_t *s_scale = s_code + 256 * kCodePitch;
+    uint8_t *s_scale = s_code + 256 * (ROT ? 64 : 80);
     const int slot = threadIdx.x >> 4, l = threadIdx.x & 15;
     const int row0 = blockIdx.y * 32 * a.subs, kt = row0 >> 7, sub0 = (row0 >> 5) & 3;
     const uint32_t mine = slots + slot * kSlotBytes;
@@ -339,7 +348,7 @@ __global__ void __launch_bounds__(kBothThreads) quantize_both_kernel(const BothA
 #pragma unroll
             for (int s = 0; s < 16; ++s) {
                 asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(v[2 * s]), "=f"(v[2 * s + 1]) : "r"(at + s * kSlotBytes));
-                m = max(m, max(__float_as_uint(v[2 * s]) & 0x7FFFFFFFu, __float_as_uint(v[2 * s + 1]) & 0x7FFFFFFFu));
+                m = __float_as_uint(max_abs3(__uint_as_float(m), __float_as_uint(v[2 * s]), __float_as_uint(v[2 * s + 1])));
             }
             e = mx_exponent(m);
         } else {
@@ -347,7 +356,8 @@ __global__ void __launch_bounds__(kBothThreads) quantize_both_kernel(const BothA
 #pragma unroll
             for (int s = 0; s < 16; ++s) asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w[s]) : "r"(at + s * kSlotBytes));
 #pragma unroll
-            for (int s = 0; s < 16; ++s) m = max_u16x2(m, w[s] & 0x7FFF7FFFu);
+            for (int s = 0; s < 16; ++s) m = max_abs2<T>(m, w[s]);
+            m &= 0x7FFF7FFFu;
             e = mx_exponent(widen_bits<T>(max(m & 0xFFFFu, m >> 16)));
 #pragma unroll
             for (int s = 0; s < 16; ++s) mx_split<T>(w[s], v[2 * s], v[2 * s + 1]);
@@ -355,7 +365,7 @@ __global__ void __launch_bounds__(kBothThreads) quantize_both_kernel(const BothA
         const float inv = mx_inverse(e);
 #pragma unroll
         for (int s = 0; s < 16; ++s) scale2(v[2 * s], v[2 * s + 1], mk2(inv, inv));
-        *reinterpret_cast<uint4 *>(s_code + threadIdx.x * kCodePitch + sub * 16) = make_uint4(mx_pack8(v), mx_pack8(v + 8), mx_pack8(v + 16), mx_pack8(v + 24));
+        *reinterpret_cast<uint4 *>(s_code + code_at<ROT>(threadIdx.x, sub)) = make_uint4(mx_pack8(v), mx_pack8(v + 8), mx_pack8(v + 16), mx_pack8(v + 24));
         s_scale[threadIdx.x * 4 + sub] = static_cast<uint8_t>(e);
         __syncthreads();
     }
@@ -366,7 +376,7 @@ __global__ void __launch_bounds__(kBothThreads) quantize_both_kernel(const BothA
     for (int i = threadIdx.x; i < 256 << shift; i += kBothThreads) {
         const uint32_t col = i >> shift, part = sub0 + (i & (a.subs - 1)), n = blockIdx.x * 256 + col;
         if (n < a.cols && kt * 4u + part < a.col_blocks)
-            *reinterpret_cast<uint4 *>(col_codes + n * a.col_pitch + (kt * 4 + part) * 16) = *reinterpret_cast<const uint4 *>(s_code + col * kCodePitch + part * 16);
+            *reinterpret_cast<uint4 *>(col_codes + n * a.col_pitch + (kt * 4 + part) * 16) = *reinterpret_cast<const uint4 *>(s_code + code_at<ROT>(col, part));
     }
     const uint32_t n = blockIdx.x * 256 + threadIdx.x;
     if (n < a.cols) {
@@ -546,9 +556,9 @@ int quantize_rows(cudaStream_t s, RowArgs &a, int type, int64_t rows, int64_t K,
 template <int T, bool ROT, bool VEC>
 int launch_both(cudaStream_t s, const BothArgs &a, dim3 grid) {
     auto kern = quantize_both_kernel<T, ROT, VEC>;
-    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kBothSmem) != cudaSuccess)
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kBothSmem<ROT>) != cudaSuccess)
         return launch_status("mxfp4_quantize (shared memory attribute)");
-    kern<<<grid, kBothThreads, kBothSmem, s>>>(a);
+    kern<<<grid, kBothThreads, kBothSmem<ROT>, s>>>(a);
     return launch_status("mxfp4_quantize");
 }
 template <int T>
@@ -669,7 +679,7 @@ int mx4_quantize_both(cudaStream_t s, const Mx4Both &b) {
     const bool vec = aligned(b.x, 16) && (b.ldx * mx_size(b.type)) % 16 == 0;
     a.wide = aligned(b.x, 32) && (b.ldx * mx_size(b.type)) % 32 == 0;
     // 128 rows a CTA write each column's 64 bytes together; fewer rows where the CTAs would not fill the
-    // device twice (three fit an SM): [4096, 1280] takes 12.7 us in 160 CTAs of four steps
+    // device twice (three or four fit an SM): [4096, 1280] takes 12.7 us in 160 CTAs of four steps, 10.5 in 640
     const int64_t ctas = (b.cols + 255) / 256 * a.col_KT * b.matrices;
     a.subs = 4;
     while (a.subs > 1 && ctas * (4 / a.subs) < 6 * num_sms() && a.col_KT * (8 / a.subs) <= 65535) a.subs /= 2;
