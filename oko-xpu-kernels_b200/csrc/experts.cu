@@ -19,7 +19,7 @@
 #include <type_traits>
 
 #include "internal.h"
-#include "mx4.cuh"
+#include "mx4quant.cuh"
 #include "xpu_kernels/convrot.h"
 
 namespace xpuint8 {
@@ -196,16 +196,24 @@ struct MoveArgs {
     const float *weights;      // combine: [tokens, fan] or null
     const int32_t *positions, *scale_rows;
     int64_t total;             // tokens * units
-    uint32_t units, fan, W;    // units: vectors of a row
+    Divisor units;             // vectors of a row
+    uint32_t fan, W;
 };
+
+// vector i: its token and place in the row
+__device__ __forceinline__ void place(const MoveArgs &a, int64_t i, int64_t &t, uint32_t &u) {
+    t = a.total < 0x7FFFFFFF ? a.units(static_cast<uint32_t>(i)) : i / a.units.d;
+    u = static_cast<uint32_t>(i - t * a.units.d);
+}
 
 // One thread: one vector of VEC elements of a token, read once and written to the token's rows.
 template <int T, int VEC>
 __global__ void __launch_bounds__(256) gather_kernel(const MoveArgs a) {
     const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
     if (i >= a.total) return;
-    const int64_t t = i / a.units;
-    const uint32_t u = static_cast<uint32_t>(i - t * a.units);
+    int64_t t;
+    uint32_t u;
+    place(a, i, t, u);
     constexpr int kBytes = VEC * mx_size(T);
     using Word = typename std::conditional<kBytes == 16, uint4, typename std::conditional<kBytes == 4, uint32_t, uint16_t>::type>::type;
     const Word v = __ldg(reinterpret_cast<const Word *>(static_cast<const uint8_t *>(a.in) + (t * a.ld_in + static_cast<int64_t>(u) * VEC) * mx_size(T)));
@@ -270,8 +278,10 @@ template <int T, int VEC>
 __global__ void __launch_bounds__(256, 5) combine_kernel(const MoveArgs a) {
     const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
     if (i >= a.total) return;
-    const int64_t t = i / a.units;
-    const int64_t c = (i - t * a.units) * VEC;
+    int64_t t;
+    uint32_t u;
+    place(a, i, t, u);
+    const int64_t c = static_cast<int64_t>(u) * VEC;
     float sum[VEC] = {};
     for (uint32_t j0 = 0; j0 < a.fan; j0 += kRows) {
         float w[kRows];
@@ -289,10 +299,10 @@ __global__ void __launch_bounds__(256, 5) combine_kernel(const MoveArgs a) {
 #pragma unroll
         for (int j = 0; j < kRows; ++j) {
             if (row[j] < 0) continue;
-            float u[VEC];
-            spread<T, VEC>(v[j], u);
+            float x[VEC];
+            spread<T, VEC>(v[j], x);
 #pragma unroll
-            for (int q = 0; q < VEC; ++q) sum[q] = __fmaf_rn(w[j], u[q], sum[q]);
+            for (int q = 0; q < VEC; ++q) sum[q] = __fmaf_rn(w[j], x[q], sum[q]);
         }
     }
     store_vec<T, VEC>(a.out, t * a.W + c, sum);
@@ -419,8 +429,8 @@ int bad_stride(const char *what) {
 template <int T>
 int launch_move(cudaStream_t s, MoveArgs &a, bool gather, int64_t tokens, bool vec, const char *what) {
     constexpr int kVec = 16 / mx_size(T);
-    a.units = vec ? a.W / kVec : a.W;
-    a.total = tokens * a.units;
+    a.units = Divisor::of(vec ? a.W / kVec : a.W);
+    a.total = tokens * a.units.d;
     const int64_t blocks = (a.total + 255) / 256;
     if (blocks > 0x7FFFFFFFll) {
         set_error(std::string(what) + ": too many elements");

@@ -450,21 +450,21 @@ __global__ void __launch_bounds__(128) turn_kernel(const TurnArgs a) {
 struct ValueArgs {
     const uint8_t *codes, *scales;
     void *out;
-    uint32_t K, KB, KT, units;  // units: of a row, runs of 16 values or of eight blocks
-    int64_t total;              // rows * units
-    uint32_t matrix_rows, matrix_tiles;
+    uint32_t K, KB, KT;
+    Divisor units;              // of a row: runs of 16 values or a warp's steps
+    uint32_t total;             // rows * units
+    Divisor matrix_rows;
+    uint32_t matrix_tiles;
     bool wide;                  // rows of out are 32-byte aligned
 };
 
 // Rows that are 16-byte aligned: 16 values a thread, 8 bytes of codes, a scale byte, 32 (64) bytes out.
 template <int T>
 __global__ void __launch_bounds__(256) values_kernel(const ValueArgs a) {
-    const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+    const uint32_t i = blockIdx.x * 256 + threadIdx.x;
     if (i >= a.total) return;
-    const int64_t r = i / a.units;
-    const uint32_t h = static_cast<uint32_t>(i - r * a.units);
-    const int64_t b = r / a.matrix_rows;
-    const int64_t sr = b * a.matrix_tiles * 128 + (r - b * a.matrix_rows);
+    const uint32_t row = a.units(i), h = i - row * a.units.d, b = a.matrix_rows(row);
+    const int64_t r = row, sr = static_cast<int64_t>(b) * a.matrix_tiles * 128 + (row - b * a.matrix_rows.d);
     const uint2 code = __ldg(reinterpret_cast<const uint2 *>(a.codes + r * a.KB * 16 + h * 8));
     const float s = mx_scale(__ldg(a.scales + mx_scale_word(sr, h >> 3, a.KT) + ((h >> 1) & 3)));
     Run<T> out;
@@ -483,29 +483,56 @@ __global__ void __launch_bounds__(256) values_kernel(const ValueArgs a) {
     store_run<T>(static_cast<uint8_t *>(a.out) + r * a.K * mx_size(T), h * 16, out, a.wide);
 }
 
-// Rows of any length: a warp reads eight blocks of a row one after another, a value a lane, so that
-// neighbouring lanes write neighbouring values.
+// Rows of any length and alignment: a lane makes the values of one 16-byte word of the output, which
+// begins anywhere in a row's blocks, so its codes come out of two words by a funnel shift and its scales
+// from the lanes that hold the warp's blocks'; a row's first and last values leave one by one.
+// [5120, 4097] fp32: a value a lane takes 25 us.
 template <int T>
 __global__ void __launch_bounds__(256) odd_values_kernel(const ValueArgs a) {
-    const int64_t i = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
+    constexpr int kPer = 16 / mx_size(T), kSteps = 4;
+    const uint32_t i = blockIdx.x * 8 + (threadIdx.x >> 5);
     const int lane = threadIdx.x & 31;
     if (i >= a.total) return;
-    const int64_t r = i / a.units;
-    const uint32_t b0 = static_cast<uint32_t>(i - r * a.units) * 8;
-    const int64_t m = r / a.matrix_rows;
-    const int64_t sr = m * a.matrix_tiles * 128 + (r - m * a.matrix_rows);
+    const uint32_t unit_row = a.units(i), m = a.matrix_rows(unit_row);
+    const int64_t r = unit_row, sr = static_cast<int64_t>(m) * a.matrix_tiles * 128 + (unit_row - m * a.matrix_rows.d);
     const uint8_t *codes = a.codes + r * a.KB * 16;
-    // lane j holds the scale of block j (of eight)
-    const uint32_t mine = min(b0 + (lane & 7), a.KB - 1);
-    const float scale = mx_scale(__ldg(a.scales + mx_scale_word(sr, mine >> 2, a.KT) + (mine & 3)));
-    codes += b0 * 16 + (lane >> 1);
-    const int shift = (lane & 1) * 4;
-    const int64_t at = r * a.K + b0 * 32 + lane;
-    const uint32_t left = a.K - b0 * 32;
+    uint8_t *row = static_cast<uint8_t *>(a.out) + r * a.K * mx_size(T);
+    const int lead = static_cast<int>((reinterpret_cast<uintptr_t>(row) & 15) / mx_size(T));  // values of the first word that are the row before's
+    const int K = static_cast<int>(a.K);
+    int c = (static_cast<int>(i - unit_row * a.units.d) * kSteps * 32 + lane) * kPer - lead;
+    // all steps' loads before the first is used
+    uint32_t lo[kSteps], hi[kSteps], e[kSteps];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        const float s = __shfl_sync(0xFFFFFFFFu, scale, j);
-        if (j * 32 + lane < left) mx_store1<T>(a.out, at + j * 32, __fmul_rn(mx_value(__ldg(codes + j * 16) >> shift), s));
+    for (int step = 0; step < kSteps; ++step) {
+        const int at = c + step * 32 * kPer;
+        const int first = max(__shfl_sync(0xFFFFFFFFu, at, 0), 0) >> 5;  // the warp's first block of the step; it has nine at most
+        const uint32_t mine = min(static_cast<uint32_t>(first + lane), a.KB - 1), word = static_cast<uint32_t>(max(at, 0)) >> 3;
+        e[step] = __ldg(a.scales + mx_scale_word(sr, mine >> 2, a.KT) + (mine & 3));
+        lo[step] = __ldg(reinterpret_cast<const uint32_t *>(codes) + min(word, a.KB * 4 - 1));
+        hi[step] = __ldg(reinterpret_cast<const uint32_t *>(codes) + min(word + 1, a.KB * 4 - 1));
+    }
+#pragma unroll
+    for (int step = 0; step < kSteps; ++step, c += 32 * kPer) {
+        const int first = max(__shfl_sync(0xFFFFFFFFu, c, 0), 0) >> 5;
+        const float scale = mx_scale(e[step]);
+        const float s0 = __shfl_sync(0xFFFFFFFFu, scale, (max(c, 0) >> 5) - first);
+        const float s1 = __shfl_sync(0xFFFFFFFFu, scale, (max(c + kPer - 1, 0) >> 5) - first);
+        if (c >= 0 && c + kPer <= K) {
+            const uint32_t x = __funnelshift_r(lo[step], hi[step], (c & 7) * 4);
+            const int other = 32 - (c & 31);  // values from here on are the next block's
+            float v[kPer];
+#pragma unroll
+            for (int q = 0; q < kPer; ++q) v[q] = __fmul_rn(mx_value(x >> (4 * q)), q < other ? s0 : s1);
+            uint4 o;
+            if constexpr (T == kMxF32) o = make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
+            else o = make_uint4(mx_join<T>(v[0], v[1]), mx_join<T>(v[2], v[3]), mx_join<T>(v[4], v[5]), mx_join<T>(v[6], v[7]));
+            *reinterpret_cast<uint4 *>(row + static_cast<int64_t>(c) * mx_size(T)) = o;
+        } else {
+            for (int q = max(c, 0); q < min(c + kPer, K); ++q) {
+                const uint32_t byte = __ldg(codes + (q >> 1));
+                mx_store1<T>(row, q, __fmul_rn(mx_value(q & 1 ? byte >> 4 : byte), (q >> 5) == (max(c, 0) >> 5) ? s0 : s1));
+            }
+        }
     }
 }
 
@@ -839,17 +866,19 @@ int xpuint8_mxfp4_dequantize_stream(const void *stream, const uint8_t *codes,
     a.K = static_cast<uint32_t>(K);
     a.KB = static_cast<uint32_t>((K + 31) / 32);
     a.KT = (a.KB + 3) / 4;
-    a.matrix_rows = static_cast<uint32_t>(matrix_rows);
+    a.matrix_rows = Divisor::of(static_cast<uint32_t>(matrix_rows));
     a.matrix_tiles = static_cast<uint32_t>((matrix_rows + 127) / 128);
     const bool vec = aligned(out, 16) && (K * mx_size(type)) % 16 == 0 && K % 16 == 0;
     a.wide = aligned(out, 32) && (K * mx_size(type)) % 32 == 0;
-    a.units = static_cast<uint32_t>(vec ? K / 16 : (K + 255) / 256);
-    a.total = rows * a.units;
-    const int64_t blocks = vec ? (a.total + 255) / 256 : (a.total + 7) / 8;
-    if (blocks > 0x7FFFFFFFll) {
-        set_error("mxfp4: too many values");
+    const int64_t span = 4 * 32 * (16 / mx_size(type));  // values of a warp, and up to a word's more before the row
+    const int64_t units = vec ? K / 16 : (K + 16 / mx_size(type) - 1 + span - 1) / span;
+    if (rows * units > 0x7FFFFFF0ll) {
+        set_error("mxfp4: rows x runs of 16 values must be below 2^31");
         return 2;
     }
+    a.units = Divisor::of(static_cast<uint32_t>(units));
+    a.total = static_cast<uint32_t>(rows * units);
+    const int64_t blocks = vec ? (a.total + 255ll) / 256 : (a.total + 7ll) / 8;
     cudaStream_t s = as_stream(stream);
     const uint32_t grid = static_cast<uint32_t>(blocks);
     switch (type * 2 + (vec ? 1 : 0)) {
