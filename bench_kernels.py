@@ -3,6 +3,8 @@
     python bench_kernels.py gemm --M 2048 --N 10240 --K 1280 --iters 20
     python bench_kernels.py rotate_quant --M 65536 --K 4096
     python bench_kernels.py linear | ffn | dx | dw | quantize_row | dequant | ...
+    python bench_kernels.py mx4_mm | mx4_linear | mx4_train | mx4_quantize | mx4_columns | mx4_values
+    python bench_kernels.py experts_linear | experts_route --M 16384 --K 2048 --experts 128 --top 8
     python bench_kernels.py suite [--iters N]   (every shape of SUITE, timing only)
 
 Inputs are seeded and generated on the device; each case launches its kernel
@@ -25,6 +27,7 @@ import torch
 
 sys.path.insert(0, os.path.join(os.path.dirname(os.path.abspath(__file__)), "oko-xpu-kernels_b200"))
 
+import xpu_kernels as xk  # noqa: E402
 from xpu_kernels.int8 import ops  # noqa: E402
 from xpu_kernels.int8._lib import _lib, _ptr, _stream  # noqa: E402
 
@@ -85,12 +88,17 @@ def main(argv=None):
     ap = argparse.ArgumentParser()
     ap.add_argument("case", choices=["gemm", "gemm_raw", "gemm_nn", "gemm_tn", "geglu",
                                      "rotate_quant", "rotate", "linear", "ffn", "dx", "dw",
-                                     "quantize_row", "colquant", "rope", "dequant", "dequant_act"])
+                                     "quantize_row", "colquant", "rope", "dequant", "dequant_act",
+                                     "mx4_mm", "mx4_linear", "mx4_train", "mx4_quantize", "mx4_columns",
+                                     "mx4_values", "experts_linear", "experts_route"])
     ap.add_argument("--M", type=int, default=2048)
     ap.add_argument("--N", type=int, default=10240)
     ap.add_argument("--K", type=int, default=1280)
     ap.add_argument("--iters", type=int, default=20)
     ap.add_argument("--sets", type=int, default=2)
+    ap.add_argument("--plain", action="store_true", help="mx4_*: without the rotation")
+    ap.add_argument("--experts", type=int, default=8)
+    ap.add_argument("--top", type=int, default=2, help="experts_*: experts of a token")
     ap.add_argument("--colscale", action="store_true",
                     help="quantize_row: with a column scale (the form linear_dx_int8 runs)")
     ap.add_argument("--act", type=int, default=4,
@@ -256,6 +264,64 @@ def main(argv=None):
                 ops.linear_dw_int8(dy, xq, xs)
         t = _time(fn, a.iters, st)
         res = {"case": a.case, "ms": t, "TOPS": 2.0 * M * N * K / (t * 1e-3) / 1e12}
+    elif a.case.startswith("mx4_"):
+        rotate = not a.plain
+        X = [bf(M, K) for _ in range(S)]
+        flops = 2.0 * M * N * K
+        if a.case in ("mx4_mm", "mx4_linear"):
+            W = [xk.prepare_weight_mxfp4(bf(N, K, s=0.02), rotate) for _ in range(S)]
+            Q = [xk.quantize_mxfp4(x, rotate=rotate) for x in X]
+
+            def fn(i):
+                j = i % S
+                if a.case == "mx4_mm":
+                    xk.mxfp4_mm(Q[j], W[j])
+                else:
+                    xk.linear_mxfp4(X[j], W[j], rotate=rotate)
+            nbytes = 0.53125 * (M + N) * K + 2 * M * N
+        elif a.case == "mx4_train":
+            W = [bf(N, K, s=0.02).requires_grad_() for _ in range(S)]
+            DY = [bf(M, N, s=1e-3) for _ in range(S)]
+            X = [x.requires_grad_() for x in X]
+
+            def fn(i):
+                j = i % S
+                torch.autograd.grad(xk.mxfp4_linear(X[j], W[j], rotate=rotate), (X[j], W[j]), DY[j])
+            flops, nbytes = 3 * flops, 4 * (M * K + N * K + M * N)
+        else:
+            Q = [xk.quantize_mxfp4(x) for x in X]
+
+            def fn(i):
+                j = i % S
+                if a.case == "mx4_values":
+                    xk.dequantize_mxfp4(Q[j])
+                else:
+                    xk.quantize_mxfp4(X[j], rotate=rotate and a.case == "mx4_quantize",
+                                      transpose=a.case == "mx4_columns")
+            flops, nbytes = 0.0, 2.53125 * M * K
+        t = _time(fn, a.iters, st)
+        res = {"case": a.case, "rotate": rotate, "ms": t, "GBps": nbytes / (t * 1e-3) / 1e9}
+        if flops:
+            res["TFLOPS"] = flops / (t * 1e-3) / 1e12
+    elif a.case.startswith("experts_"):
+        ids = torch.rand(M, a.experts, generator=g, device=dev).topk(a.top, dim=1).indices
+        plan = xk.expert_sort(ids, a.experts)
+        X = [bf(M, K) for _ in range(S)]
+        if a.case == "experts_linear":
+            w = xk.prepare_weight_mxfp4(bf(a.experts, N, K, s=0.02))
+
+            def fn(i):
+                xk.expert_linear_mxfp4(X[i % S], w, plan)
+            t = _time(fn, a.iters, st)
+            res = {"case": a.case, "ms": t, "TFLOPS": 2.0 * M * a.top * N * K / (t * 1e-3) / 1e12}
+        else:
+            weights = torch.rand(M, a.top, generator=g, device=dev)
+
+            def fn(i):
+                xk.expert_combine(xk.expert_gather(X[i % S], xk.expert_sort(ids, a.experts)), weights, plan)
+            t = _time(fn, a.iters, st)
+            res = {"case": a.case, "ms": t, "GBps": 4.0 * M * K * (1 + a.top) / (t * 1e-3) / 1e9}
+        res.update({"experts": a.experts, "top": a.top})
     res.update({"M": M, "N": N, "K": K})
     print(json.dumps(res))
 

@@ -6,7 +6,7 @@ current CUDA device and judged against a stated gate.  The seeded problem
 reference self-test's contract (python/xpu_kernels/int8/selftest.py:52-56 for
 the shapes and scales, :157-163 for the thresholds); the checks marked "new"
 cover what this build adds (the exact int8 GEMM, the fused qkv split, the int8
-weight gradient, the bounded-wait fault word).  ``run_checks`` returns one
+weight gradient, the MXFP4 linears and experts, the bounded-wait fault word).  ``run_checks`` returns one
 record per check; ``selftest`` prints them and returns True when all pass.
 """
 
@@ -182,6 +182,40 @@ def _trainable(p):
     return (fwd, dw), fwd and dw
 
 
+def _mxfp4_product(p):
+    from .. import mxfp4
+    a, b = mxfp4.quantize_mxfp4(p.x, rotate=True), mxfp4.prepare_weight_mxfp4(p.w)
+    values = [mxfp4.dequantize_mxfp4(q, dtype=torch.float32).double() for q in (a, b)]
+    r = _rel(mxfp4.mxfp4_mm(a, b, dtype=torch.float32).double(), values[0] @ values[1].t())
+    return r, r < 1e-6
+
+
+def _mxfp4_linear(p):
+    from .. import mxfp4
+    ref = p.x.float() @ p.w.float().t()
+    r = _rel(mxfp4.linear_mxfp4(p.x, mxfp4.prepare_weight_mxfp4(p.w)), ref)
+    return r, r < 0.25
+
+
+def _mxfp4_experts(p):
+    from .. import experts, mxfp4
+    e, ff = 4, 256
+    g = torch.Generator(device=p.dev).manual_seed(1)
+    ids = torch.rand(p.M, e, generator=g, device=p.dev).topk(2, dim=1).indices
+    weights = torch.rand(p.M, 2, generator=g, device=p.dev)
+    up = mxfp4.prepare_weight_mxfp4(torch.randn(e, 2 * ff, p.K, generator=g, device=p.dev) * 0.05)
+    down = mxfp4.prepare_weight_mxfp4(torch.randn(e, p.K, ff, generator=g, device=p.dev) * 0.05)
+    out = experts.expert_ffn_mxfp4(p.x, ids, weights, up, down)
+    ref = torch.zeros(p.M, p.K, device=p.dev)
+    for i in range(e):  # each expert on all tokens, by the dense linears
+        mats = [mxfp4.MXFP4(m.codes[i], m.scales[i], m.shape[1:]) for m in (up, down)]
+        gate, value = mxfp4.linear_mxfp4(p.x, mats[0]).chunk(2, dim=1)
+        y = mxfp4.linear_mxfp4(torch.nn.functional.silu(gate) * value, mats[1])
+        ref += (weights * (ids == i)).sum(1, keepdim=True) * y.float()
+    r = _rel(out, ref.to(torch.bfloat16))
+    return r, r < 5e-3
+
+
 def _fault_word(p):
     torch.cuda.synchronize(p.dev)
     word = L.load().xpuint8_fault_status(0)
@@ -214,6 +248,11 @@ CHECKS: List[Check] = [
     Check("int8 dW", "relative error vs the bf16 dW < 0.04", "new", _dw_int8),
     Check("trainable linear", "forward == the INT8 model's; dW == the bf16 model's",
           "selftest.py:162-163", _trainable),
+    Check("MXFP4 product", "== the fp64 product of the held values, relative error < 1e-6", "new",
+          _mxfp4_product),
+    Check("MXFP4 linear vs fp32 matmul", "relative error < 0.25 (4-bit operands)", "new", _mxfp4_linear),
+    Check("MXFP4 experts' network", "== every expert's dense linears, relative error < 5e-3", "new",
+          _mxfp4_experts),
     Check("device fault word", "no bounded wait gave up", "new", _fault_word),
 ]
 
