@@ -557,6 +557,22 @@ __global__ void __launch_bounds__(PairCfg<BN>::kThreads, 1)
 
 // -------------------------------------------------------------------------------------- few kernel
 
+// Waits until the count at `at` in shared memory is over `n`; bounded as mbar_wait is.
+__device__ __forceinline__ bool count_wait(uint32_t at, int n, int *fault, int site) {
+    const uint64_t t0 = global_timer_ns();
+    for (uint32_t it = 1; it < kWaitMaxIters; ++it) {
+        int v;
+        asm volatile("ld.acquire.cta.shared::cta.b32 %0, [%1];" : "=r"(v) : "r"(at) : "memory");
+        if (v > n) return true;
+        if ((it & 255u) == 0u) {
+            if (*reinterpret_cast<volatile int *>(fault) != 0) return false;
+            if (global_timer_ns() - t0 > kWaitTimeoutNs) break;
+        }
+    }
+    atomicCAS(fault, 0, site);
+    return false;
+}
+
 struct FewArgs {
     void *out;
     int64_t ldo;
@@ -600,7 +616,9 @@ struct FewMaps {
 // FUSE: the drain's warps first make the tokens' operand themselves: eight half-warps take pairs of
 // rows of a k-block (a 256-value group), quantize them, behind the rotation or not, straight into
 // the swizzled stage and its scale tiles, and arrive on the stage's FULL barrier beside the TMA
-// unit's bytes.  Every CTA repeats that for its share of K, which the weight's bytes hide while the
+// unit's bytes.  They learn that a stage is free from a count that the producer keeps of the k-blocks
+// whose stage it has found empty: a slot's next task may lie two turns of the ring on (one pair of
+// rows, four stages), where the parity of EMPTY can't tell the turn.  Every CTA repeats that for its share of K, which the weight's bytes hide while the
 // tokens are few, and one launch and the operand's way through memory are saved.
 template <int T, int FUSE>
 __global__ void __launch_bounds__(kFewThreads, 2)
@@ -650,9 +668,11 @@ __global__ void __launch_bounds__(kFewThreads, 2)
     auto EMPTY = [&](int s) { return bar0 + 8u * (kFewMaxStages + s); };
     const uint32_t done = bar0 + 8u * (2 * kFewMaxStages);
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 2 * kFewMaxStages + 1);
+    const uint32_t freed = smem_u32(tmem_slot + 1);  // FUSE: k-blocks whose stage is free
     const int pairs = (count + 1) / 2;  // FUSE: row pairs of a k-block
 
     if (threadIdx.x == 0) {
+        tmem_slot[1] = 0;
         for (int s = 0; s < kFewMaxStages; ++s) {
             mbar_init(FULL(s), FUSE == kFuseNone ? 1 : 1 + pairs);
             mbar_init(EMPTY(s), 1);
@@ -696,6 +716,7 @@ __global__ void __launch_bounds__(kFewThreads, 2)
         for (int kb = k0; kb < k1; ++kb) {
             if (!warp_wait(EMPTY(stage), ph ^ 1u, fault, 111)) break;
             if (elect_one()) {
+                if (FUSE != kFuseNone) asm volatile("st.release.cta.shared::cta.b32 [%0], %1;" ::"r"(freed), "r"(issued + 1) : "memory");
                 mbar_expect_tx(FULL(stage), FUSE == kFuseNone ? stage_bytes : w_bytes + kScaleBlock);
                 const uint32_t at = ring + stage * stage_bytes;
                 if (static_cast<int>(issued) >= pre) load_w(stage, kb);
@@ -786,7 +807,7 @@ __global__ void __launch_bounds__(kFewThreads, 2)
                 A = bring(2 * rp, kb);
                 B = bring(2 * rp + 1, kb);
             }
-            if (mine) ok = mbar_wait(EMPTY(stage), ((local / stages) & 1) ^ 1u, fault, 113);
+            if (mine) ok = count_wait(freed, local, fault, 113);
             ok = __all_sync(0xFFFFFFFFu, ok);
             if (mine && ok) {
                 const uint32_t at = ring + stage * stage_bytes + w_bytes, sx = at + x_bytes + kScaleBlock;

@@ -307,6 +307,22 @@ def test_rows_quantised_in_the_product_are_the_quantiser_s(gpu, tokens, top):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("tokens", [30, 60])
+def test_one_or_two_rows_an_expert_over_a_long_contraction(gpu, tokens):
+    """More k-blocks a CTA than its ring of stages takes in two turns: each is made once, in its turn."""
+    ids = (torch.arange(tokens, dtype=torch.int32, device=DEV) % 30).reshape(-1, 1)
+    plan = xk.expert_sort(ids, 30)
+    x = torch.randn((tokens, 4104), device=DEV).to(torch.bfloat16)
+    wq = xk.prepare_weight_mxfp4((torch.randn((30, 1280, 4096), device=DEV) * 0.02).to(torch.bfloat16))
+    aligned, other = x[:, :4096].contiguous(), torch.empty(tokens * 4097, dtype=torch.bfloat16, device=DEV)
+    odd = other.as_strided((tokens, 4096), (4097, 1))  # rows that are quantised before the product
+    odd.copy_(aligned)
+    want = xk.expert_linear_mxfp4(odd, wq, plan)
+    for _ in range(3):
+        assert torch.equal(xk.expert_linear_mxfp4(aligned, wq, plan), want)
+
+
+@pytest.mark.gpu
 def test_the_network(gpu):
     """The whole path against the same steps in 64 bits between its 4-bit roundings, within what
     codes that move at bf16 roundings of the intermediate can change (a step is at most a third of a

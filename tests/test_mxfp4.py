@@ -327,6 +327,19 @@ def test_tokens_quantised_in_the_product_are_the_quantiser_s(gpu, m):
             assert torch.equal(xk.linear_mxfp4(x, wq, rotate=rotate), want)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("m", [1, 2, 3, 8])
+@pytest.mark.parametrize("n,k,rotate", [(19200, 4096, True), (7790, 12160, False), (19200, 2100, False)])
+def test_tokens_over_a_contraction_of_several_turns(gpu, m, n, k, rotate):
+    """More k-blocks a CTA than its ring of stages takes in two turns: each is made once, in its turn."""
+    for dtype in TYPES:
+        x, w = rand((m, k), m, dtype).to(DEV), (torch.randn((n, k), device=DEV) * 0.02).to(dtype)
+        wq = xk.prepare_weight_mxfp4(w, rotate=rotate)
+        want = xk.mxfp4_mm(xk.quantize_mxfp4(x, rotate=rotate), wq, dtype=dtype)
+        for _ in range(3):
+            assert torch.equal(xk.linear_mxfp4(x, wq, rotate=rotate), want)
+
+
 # ------------------------------------------------------------------------------ streams and graphs
 
 @pytest.mark.gpu
