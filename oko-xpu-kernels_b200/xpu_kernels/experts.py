@@ -15,9 +15,9 @@ them have the largest size they can need.
 from __future__ import annotations
 
 import torch
-from torch.autograd.function import once_differentiable
 
-from .mxfp4 import _TYPES, _check_rotate, _entry, _launch, _rows, _scratch, _type, _wanted
+from . import mxfp4
+from .mxfp4 import _check_rotate, _load, _type
 
 
 class ExpertPlan:
@@ -30,7 +30,7 @@ class ExpertPlan:
     routing of these sizes.
     """
 
-    __slots__ = ("num_experts", "tokens", "top", "rows", "max_tiles", "_buffer", "_at", "_index")
+    __slots__ = ("num_experts", "tokens", "top", "rows", "max_tiles", "_buffer", "_index")
 
     # the arrays follow one another in one buffer and become tensors when asked for
     @property
@@ -76,23 +76,12 @@ def expert_sort(ids, num_experts):
         raise ValueError(f"num_experts must be 1 to 1024, got {num_experts}")
     if not ids.is_contiguous():
         ids = ids.contiguous()
-    e = num_experts
     plan = ExpertPlan()
-    plan.num_experts, plan.tokens, plan._index = e, shape[0], index
+    plan.num_experts, plan.tokens, plan._index = num_experts, shape[0], index
     plan.top = shape[1] if len(shape) == 2 else 1
     n = plan.rows = plan.tokens * plan.top
-    plan.max_tiles = n // 128 + min(e, n)
-    work = _entry("expert_sort_workspace_bytes")(n, e)
-    if work < 0:
-        raise ValueError(f"expert_sort: too many slots ({n})")
-    buffer = plan._buffer = torch.empty(3 * n + 2 * (e + 1) + work // 4, dtype=torch.int32, device=ids.device)
-    at = buffer.data_ptr()
-    p, o = at + 12 * n, 4 * (e + 1)
-    plan._at = (at, at + 4 * n, at + 8 * n, p, p + o)
-    if n:
-        _launch("expert_sort", index, ids.data_ptr(), size, n, e, *plan._at, p + 2 * o)
-    else:
-        buffer.zero_()
+    plan.max_tiles = n // 128 + min(num_experts, n)
+    plan._buffer = (mxfp4._native or _load()).sort(ids, num_experts)
     return plan
 
 
@@ -101,78 +90,14 @@ def _same_device(index, plan, x, what):
         raise ValueError(f"{what} is on {x.device} and the plan on {plan._buffer.device}")
 
 
-def _gather(x, plan):
-    t = _type(x, "x")
-    x, ldx = _rows(x)
-    w = x.shape[1]
-    out = x.new_empty((plan.rows, w))
-    if w and plan.rows:
-        _launch("expert_gather", plan._index, x.data_ptr(), t, ldx, out.data_ptr(), plan._at[1], plan._at[2],
-                plan.tokens, plan.top, w)
-    return out
-
-
-def _combine(y, weights, plan):
-    t = _type(y, "y")
-    y, ldy = _rows(y)
-    w = y.shape[1]
-    out = y.new_empty((plan.tokens, w))
-    if w and plan.rows:
-        _launch("expert_combine", plan._index, y.data_ptr(), t, ldy, None if weights is None else weights.data_ptr(),
-                out.data_ptr(), plan._at[1], plan._at[2], plan.tokens, plan.top, w)
-    else:
-        out.zero_()
-    return out
-
-
-class _GatherFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, plan):
-        ctx.plan = plan
-        return _gather(x, plan)
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dy):
-        return _combine(dy, None, ctx.plan), None
-
-
-class _CombineFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, y, weights, plan):
-        ctx.plan = plan
-        ctx.save_for_backward(y, weights)
-        return _combine(y, weights, plan)
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dy):
-        y, weights = ctx.saved_tensors
-        plan = ctx.plan
-        dy, ld_dy = _rows(dy)
-        y, ld_y = _rows(y)
-        w = y.shape[1]
-        grad_y = y.new_empty((plan.rows, w))
-        grad_w = weights.new_empty((plan.tokens, plan.top))
-        if w and plan.rows:
-            _launch("expert_combine_grad", plan._index, dy.data_ptr(), _TYPES[y.dtype], ld_dy, y.data_ptr(), ld_y,
-                    weights.data_ptr(), grad_y.data_ptr(), grad_w.data_ptr(), plan._at[1], plan._at[2], plan.tokens,
-                    plan.top, w)
-        else:
-            grad_w.zero_()
-        return grad_y, grad_w, None
-
-
 def expert_gather(x, plan):
     """``x`` [T, W] -> its rows in the plan's order [T * k, W]; zero rows for slots of no expert.
     Differentiable: the gradient of a token is the sum of its rows'."""
     if x.dim() != 2 or x.shape[0] != plan.tokens:
         raise ValueError(f"x must be [{plan.tokens}, W], got {tuple(x.shape)}")
     _same_device(x.get_device(), plan, x, "x")
-    if x.requires_grad and torch.is_grad_enabled():
-        _type(x, "x")
-        return _GatherFn.apply(x, plan)
-    return _gather(x, plan)
+    _type(x, "x")
+    return (mxfp4._native or _load()).gather(x, plan._buffer, plan.tokens, plan.top, plan.num_experts)
 
 
 def expert_combine(y, weights, plan):
@@ -189,10 +114,8 @@ def expert_combine(y, weights, plan):
         raise TypeError(f"weights must be floating point, got {weights.dtype}")
     if weights.dtype != torch.float32 or weights.shape != shape or not weights.is_contiguous():
         weights = weights.to(torch.float32).reshape(shape).contiguous()
-    if (y.requires_grad or weights.requires_grad) and torch.is_grad_enabled():
-        _type(y, "y")
-        return _CombineFn.apply(y, weights, plan)
-    return _combine(y, weights, plan)
+    _type(y, "y")
+    return (mxfp4._native or _load()).combine(y, weights, plan._buffer, plan.tokens, plan.top, plan.num_experts)
 
 
 # ------------------------------------------------------------------------------ the experts' product
@@ -220,85 +143,24 @@ def expert_linear_mxfp4(x, w, plan, *, rotate=True, sorted=False):
     Rows of no expert are zero.
     """
     _check_product(x, w.shape, plan, rotate, sorted)
-    t = _type(x, "x")
+    _type(x, "x")
     if w._index != plan._index:
         raise ValueError(f"the weight is on {w.device} and the plan on {plan._buffer.device}")
-    if x.requires_grad:
-        x = x.detach()
-    e, n, k = w.shape
-    rows = plan.rows
-    x, ldx = _rows(x)
-    out = x.new_empty((rows, n))
-    if rows and n:
-        p = x.data_ptr()
-        # up to 128 aligned rows are quantised inside the product, without scratch
-        work = None
-        if rows > 128 or p % 16 or ldx * x.element_size() % 16:
-            work = _scratch(_entry("mxfp4_expert_linear_workspace_bytes")(rows, plan.max_tiles, k), x.device)
-        _launch("mxfp4_expert_linear", plan._index, p, t, ldx, w._cp, w._sp, out.data_ptr(),
-                None if work is None else work.data_ptr(), *plan._at, plan.tokens, plan.top, plan.max_tiles, n, k, e,
-                1 if rotate else 0, 1 if sorted else 0)
-    return out
-
-
-class _ExpertLinearFn(torch.autograd.Function):
-    """As the MXFP4 linear's, expert by expert: dx from dy and w along N, dw from dy and the rows of x
-    along each expert's own rows."""
-
-    @staticmethod
-    def forward(ctx, x, w, plan, rotate, in_order, want):
-        e, n, k = w.shape
-        w = w.contiguous()
-        x2, ldx = _rows(x)
-        rows, device = plan.rows, x.device
-        y = x2.new_empty((rows, n))
-        flags = (1 if rotate else 0, 1 if in_order else 0)
-        if n:
-            saved = _scratch(_entry("mxfp4_expert_train_saved_workspace_bytes")(plan.max_tiles, n, k, e, want), device) if want else None
-            work = _scratch(_entry("mxfp4_expert_train_workspace_bytes")(rows, plan.max_tiles, n, k, e), device)
-            _launch("mxfp4_expert_train", plan._index, x2.data_ptr(), _TYPES[x.dtype], ldx, w.data_ptr(), _TYPES[w.dtype],
-                    y.data_ptr(), None if saved is None else saved.data_ptr(), work.data_ptr(), *plan._at, plan.tokens, plan.top,
-                    plan.max_tiles, n, k, e, *flags, want)
-            if saved is not None:
-                ctx.save_for_backward(saved)
-        ctx.plan, ctx.sizes, ctx.like = plan, (e, n, k, want, flags), (x.dtype, w.dtype)
-        return y
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dy):
-        plan = ctx.plan
-        e, n, k, want, flags = ctx.sizes
-        x_type, w_type = ctx.like
-        need = ctx.needs_input_grad
-        dy, ld = _rows(dy)
-        device = dy.device
-        rows = plan.rows
-        dx = torch.empty((rows if flags[1] else plan.tokens, k), dtype=x_type, device=device) if need[0] else None
-        dw = torch.empty((e, n, k), dtype=w_type, device=device) if need[1] else None
-        if n and (need[0] or need[1]):
-            saved, = ctx.saved_tensors
-            have = (1 if need[0] else 0) | (2 if need[1] else 0)
-            w_code = _TYPES[w_type]
-            work = _scratch(_entry("mxfp4_expert_grad_workspace_bytes")(rows, plan.max_tiles, n, k, e, w_code, *flags, have), device)
-            _launch("mxfp4_expert_grad", plan._index, dy.data_ptr(), _TYPES[x_type], ld, saved.data_ptr(),
-                    dx.data_ptr() if need[0] else None, dw.data_ptr() if need[1] else None, w_code, work.data_ptr(),
-                    *plan._at, plan.tokens, plan.top, plan.max_tiles, n, k, e, *flags, want)
-        elif need[0]:
-            dx.zero_()
-        return dx, dw, None, None, None, None
+    return (mxfp4._native or _load()).expert_linear(x, w._cp, w._sp, w.shape[1], plan._buffer, plan.tokens, plan.top,
+                                                    plan.num_experts, rotate, sorted)
 
 
 def mxfp4_expert_linear(x, w, plan, *, rotate=True, sorted=False):
     """:func:`expert_linear_mxfp4` with its gradients: ``w`` [E, N, K] stays in its own type (bf16,
-    fp16, fp32) and is quantised on every call, as are the gradients' operands."""
+    fp16, fp32) and is quantised on every call, as are the gradients' operands: as the linear's, expert by
+    expert, dx from dy and w along N, dw from dy and the rows of x along each expert's own rows."""
     _check_product(x, w.shape, plan, rotate, sorted)
     _type(x, "x")
     _type(w, "w")
     _same_device(w.get_device(), plan, w, "w")
     if plan.rows == 0:
         return x.reshape(0, x.shape[1]) @ w.sum(0).to(x.dtype).T
-    return _ExpertLinearFn.apply(x, w, plan, rotate, sorted, _wanted(x, w))
+    return (mxfp4._native or _load()).expert_train(x, w, plan._buffer, plan.tokens, plan.top, rotate, sorted)
 
 
 def expert_ffn_mxfp4(x, ids, weights, up, down, *, rotate=True):

@@ -16,34 +16,28 @@ The kernels run on torch's current stream; nothing here synchronises.
 
 from __future__ import annotations
 
-import torch
-from torch.autograd.function import once_differentiable
+import ctypes
 
-from .int8._lib import _err, _lib
+import torch
+
+from .int8._lib import _lib
 
 _TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
-_raw_stream = torch._C._cuda_getCurrentRawStream
-_current = torch._C._cuda_getDevice
-_entries = {}
+_native = None
 
 
-def _entry(name):
-    fn = _entries.get(name)
-    if fn is None:
-        fn = _entries[name] = getattr(_lib(), "xpuint8_" + name)
-    return fn
-
-
-def _launch(name, index, *args):
-    """The C entry xpuint8_<name>_stream on the current stream of device `index`; raises what it reports."""
-    fn = _entry(name + "_stream")
-    if index == _current():
-        rc = fn(_raw_stream(index), *args)
-    else:
-        with torch.cuda.device(index):
-            rc = fn(_raw_stream(index), *args)
-    if rc:
-        _err(_lib(), name)
+def _load():
+    """The torch binding over the loaded library (csrc/binding.cpp)."""
+    global _native
+    lib = _lib()
+    try:
+        from . import _native as module
+    except ImportError as exc:
+        raise RuntimeError(f"the torch binding is not usable ({exc}); build it with `make -C oko-xpu-kernels_b200/csrc` "
+                           "or __graft_entry__.build()") from exc
+    module.bind({name: ctypes.cast(getattr(lib, "xpuint8_" + name), ctypes.c_void_p).value for name in module.names()})
+    _native = module
+    return module
 
 
 def _type(x, what):
@@ -54,20 +48,6 @@ def _type(x, what):
     if not x.is_cuda:
         raise TypeError(f"{what} must be a CUDA tensor, got {x.device}")
     return t
-
-
-def _rows(x):
-    """x [R, K] with unit column stride (a copy where it has none), and its row stride."""
-    if x.is_contiguous():
-        return x, x.shape[1]
-    r, k = x.shape
-    if k != 1 and x.stride(1) != 1 or r > 1 and x.stride(0) < k:
-        return x.contiguous(), k
-    return x, (x.stride(0) if r > 1 else k)
-
-
-def _scratch(n, device):
-    return torch.empty(n, dtype=torch.uint8, device=device)
 
 
 def _check_rotate(k, rotate):
@@ -111,17 +91,15 @@ class MXFP4:
         self._cp, self._sp = codes.data_ptr(), scales.data_ptr()
 
     @classmethod
-    def _empty(cls, shape, device, index):
-        """An unwritten matrix: codes and scales in one buffer, made into tensors when asked for."""
+    def _of(cls, buffer, shape, index):
+        """The matrix whose codes and then scales are in `buffer`; they become tensors when asked for."""
         r, k = shape[-2:]
         n = shape[0] if len(shape) == 3 else 1
-        at = (n * r * ((k + 31) // 32 * 16) + 255) // 256 * 256
         q = cls.__new__(cls)
-        q._buffer = torch.empty(at + n * ((r + 127) // 128) * ((k + 127) // 128) * 512, dtype=torch.uint8,
-                                device=device)
-        q.shape, q._codes, q._scales, q._at, q._index = tuple(shape), None, None, at, index
-        q._cp = q._buffer.data_ptr()
-        q._sp = q._cp + at
+        q.shape, q._buffer, q._codes, q._scales, q._index = tuple(shape), buffer, None, None, index
+        q._at = (n * r * ((k + 31) // 32 * 16) + 255) // 256 * 256
+        q._cp = buffer.data_ptr()
+        q._sp = q._cp + q._at
         return q
 
     @property
@@ -154,32 +132,15 @@ def quantize_mxfp4(x, *, rotate=False, transpose=False):
     type.  ``transpose`` gives the MXFP4 of ``x``'s transpose instead, blocks along R.
     """
     shape = x.shape
-    if len(shape) == 2:
-        r, k = shape
-        n = 1
-    elif len(shape) == 3:
-        n, r, k = shape
-    else:
+    if len(shape) not in (2, 3):
         raise ValueError(f"x must be [R, K] or [E, R, K], got {tuple(shape)}")
     if transpose and rotate:
         raise ValueError("rotate goes along K: transpose quantises along the other axis")
-    if rotate and k % 256:
-        _check_rotate(k, rotate)
-    t = _type(x, "x")
-    if len(shape) == 2:
-        x, ldx = _rows(x)
-    else:
-        x, ldx = x.contiguous(), k
-    index = x.get_device()
-    if transpose:
-        q = MXFP4._empty((*shape[:-2], k, r), x.device, index)
-        if n and r and k:
-            _launch("mxfp4_quantize_columns", index, x.data_ptr(), t, ldx, q._cp, q._sp, r, k, n, None, None, 0, 0)
-    else:
-        q = MXFP4._empty(shape, x.device, index)
-        if n and r and k:
-            _launch("mxfp4_quantize", index, x.data_ptr(), t, ldx, q._cp, q._sp, None, n * r, k, r, 1 if rotate else 0)
-    return q
+    if rotate and shape[-1] % 256:
+        _check_rotate(shape[-1], rotate)
+    _type(x, "x")
+    buffer = (_native or _load()).quantize(x.detach() if x.requires_grad else x, rotate, transpose)
+    return MXFP4._of(buffer, (*shape[:-2], shape[-1], shape[-2]) if transpose else shape, x.get_device())
 
 
 def dequantize_mxfp4(q, dtype=torch.bfloat16):
@@ -189,12 +150,8 @@ def dequantize_mxfp4(q, dtype=torch.bfloat16):
         raise TypeError(f"dtype must be bfloat16, float16 or float32, got {dtype}")
     if q._index < 0:
         raise TypeError(f"q must be on a CUDA device, got {q.device}")
-    out = torch.empty(q.shape, dtype=dtype, device=q._buffer.device if q._codes is None else q._codes.device)
-    n = out.numel()
-    if n:
-        r, k = q.shape[-2:]
-        _launch("mxfp4_dequantize", q._index, q._cp, q._sp, out.data_ptr(), t, n // k, k, r)
-    return out
+    buffer = q._buffer if q._codes is None else q._codes
+    return (_native or _load()).dequantize(q._cp, q._sp, q.shape[-2], t, buffer, q.shape)
 
 
 def prepare_weight_mxfp4(w, rotate=True):
@@ -202,15 +159,9 @@ def prepare_weight_mxfp4(w, rotate=True):
     return quantize_mxfp4(w.detach(), rotate=rotate)
 
 
-def _bias(bias, n, device):
-    if bias is None:
-        return None
-    if bias.numel() != n:
+def _check_bias(bias, n):
+    if bias is not None and bias.numel() != n:
         raise ValueError(f"bias has {bias.numel()} values; expected N={n}")
-    b = bias.detach()
-    if b.dtype != torch.float32 or b.device != device or not b.is_contiguous():
-        b = b.to(device=device, dtype=torch.float32).contiguous()
-    return b.clone() if b.data_ptr() % 16 else b
 
 
 def mxfp4_mm(a, b, bias=None, dtype=torch.bfloat16):
@@ -227,13 +178,8 @@ def mxfp4_mm(a, b, bias=None, dtype=torch.bfloat16):
         raise ValueError(f"a is on {a.device} and b on {b.device}")
     if a._index < 0:
         raise TypeError(f"a and b must be on a CUDA device, got {a.device}")
-    device = a.device
-    bias = _bias(bias, n, device)
-    out = torch.empty((m, n), dtype=dtype, device=device)
-    if m and n:
-        _launch("mxfp4_mm", a._index, a._cp, a._sp, b._cp, b._sp, None if bias is None else bias.data_ptr(),
-                out.data_ptr(), t, n, m, n, k)
-    return out
+    _check_bias(bias, n)
+    return (_native or _load()).mm(a._cp, a._sp, b._cp, b._sp, bias, t, m, n, k, a._buffer if a._codes is None else a._codes)
 
 
 def linear_mxfp4(x, w, bias=None, *, rotate=True):
@@ -251,82 +197,21 @@ def linear_mxfp4(x, w, bias=None, *, rotate=True):
     n, k = w.shape
     if rotate and k % 256:
         _check_rotate(k, rotate)
-    t = _type(x, "x")
-    if x.requires_grad:
-        x = x.detach()
-    x2, ldx = _rows(x if len(shape) == 2 else x.reshape(-1, k))
-    m = x2.shape[0]
+    _type(x, "x")
     if bias is not None:
-        bias = _bias(bias, n, x.device)
-    out = x2.new_empty((m, n))
-    if m and n:
-        p = x2.data_ptr()
-        # up to 8 aligned rows are quantised inside the product, without scratch
-        work = None
-        if m > 8 or p % 16 or ldx * x2.element_size() % 16:
-            work = _scratch(_entry("mxfp4_linear_workspace_bytes")(m, k), x.device)
-        _launch("mxfp4_linear", index, p, t, ldx, w._cp, w._sp, None if bias is None else bias.data_ptr(),
-                out.data_ptr(), None if work is None else work.data_ptr(), m, n, k, 1 if rotate else 0)
-    return out if len(shape) == 2 else out.reshape(*shape[:-1], n)
-
-
-class _Mxfp4LinearFn(torch.autograd.Function):
-    """y = Q(x) Q(w)^T with both operands quantised along K; the gradients' products quantise their
-    operands along their own contractions, dy and w along N for dx, dy and x along the rows for dw
-    (straight through the roundings).  What is kept is in 4 bits: x and w along those axes, where
-    their gradient is wanted."""
-
-    @staticmethod
-    def forward(ctx, x, w, bias, rotate, want):
-        n, k = w.shape
-        x2, ldx = _rows(x.reshape(-1, k))
-        w2, ldw = _rows(w)
-        m, device, index = x2.shape[0], x.device, x.get_device()
-        y = x2.new_empty((m, n))
-        saved = None
-        if m and n:
-            if want:
-                saved = _scratch(_entry("mxfp4_train_saved_workspace_bytes")(m, n, k, want), device)
-            work = _scratch(_entry("mxfp4_train_workspace_bytes")(m, n, k), device)
-            b = _bias(bias, n, device)
-            _launch("mxfp4_train", index, x2.data_ptr(), _TYPES[x.dtype], ldx, w2.data_ptr(), _TYPES[w.dtype], ldw,
-                    None if b is None else b.data_ptr(), y.data_ptr(), None if saved is None else saved.data_ptr(),
-                    work.data_ptr(), m, n, k, 1 if rotate else 0, want)
-        if saved is not None:
-            ctx.save_for_backward(saved)
-        ctx.sizes = (m, n, k, want, rotate)
-        ctx.like = (x.dtype, w.dtype, None if bias is None else bias.dtype, x.shape)
-        return y.reshape(*x.shape[:-1], n)
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dy):
-        m, n, k, want, rotate = ctx.sizes
-        x_type, w_type, bias_type, shape = ctx.like
-        need = ctx.needs_input_grad
-        dy2, ld = _rows(dy.reshape(-1, n))
-        device = dy.device
-        dx = torch.empty((m, k), dtype=x_type, device=device) if need[0] else None
-        dw = torch.empty((n, k), dtype=w_type, device=device) if need[1] else None
-        if m and n and (need[0] or need[1]):
-            saved, = ctx.saved_tensors
-            have = (1 if need[0] else 0) | (2 if need[1] else 0)
-            w_code = _TYPES[w_type]
-            work = _scratch(_entry("mxfp4_grad_workspace_bytes")(m, n, k, w_code, 1 if rotate else 0, have), device)
-            _launch("mxfp4_grad", dy.get_device(), dy2.data_ptr(), _TYPES[x_type], ld, saved.data_ptr(),
-                    dx.data_ptr() if need[0] else None, dw.data_ptr() if need[1] else None, w_code, work.data_ptr(),
-                    m, n, k, 1 if rotate else 0, want)
-        else:
-            for g in (dx, dw):
-                if g is not None:
-                    g.zero_()
-        db = dy2.sum(dim=0, dtype=torch.float32).to(bias_type) if need[2] else None
-        return (None if dx is None else dx.reshape(shape)), dw, db, None, None
+        _check_bias(bias, n)
+    return (_native or _load()).linear(x, w._cp, w._sp, n, bias, rotate)
 
 
 def mxfp4_linear(x, w, bias=None, *, rotate=True):
     """The MXFP4 linear with its gradients: ``x`` [.., K], ``w`` [N, K] (bf16, fp16, fp32), both
-    quantised on every call; ``dx`` and ``dw`` are MXFP4 products too, ``dbias`` is a sum."""
+    quantised on every call; ``dx`` and ``dw`` are MXFP4 products too, ``dbias`` is a sum.
+
+    y = Q(x) Q(w)^T with both operands quantised along K.  The gradients' products quantise their
+    operands along their own contractions, dy and w along N for dx, dy and x along the rows for dw
+    (straight through the roundings).  What is kept between the two is in 4 bits: x and w along those
+    axes, where their gradient is wanted.
+    """
     if w.dim() != 2 or x.shape[-1] != w.shape[1]:
         raise ValueError(f"x has {x.shape[-1]} columns and the weight is {tuple(w.shape)}")
     _type(x, "x")
@@ -336,12 +221,8 @@ def mxfp4_linear(x, w, bias=None, *, rotate=True):
     if w.shape[1] == 0:
         raise ValueError("mxfp4_linear needs K of at least 1")
     _check_rotate(w.shape[1], rotate)
-    return _Mxfp4LinearFn.apply(x, w, bias, rotate, _wanted(x, w))
-
-
-def _wanted(x, w):
-    """Which gradients a backward call may ask for: bit 0 x's, bit 1 w's."""
-    return (1 if x.requires_grad else 0) | (2 if w.requires_grad else 0) if torch.is_grad_enabled() else 0
+    _check_bias(bias, w.shape[0])
+    return (_native or _load()).train(x, w, bias, rotate)
 
 
 class Mxfp4Linear(torch.nn.Module):
