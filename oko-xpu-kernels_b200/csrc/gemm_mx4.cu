@@ -134,7 +134,7 @@ struct PairCfg {
     static constexpr int kStages = BN == 256 ? 5 : 7;
     static constexpr int kEpiWarps = 8;
     static constexpr int kThreads = 64 + 32 * kEpiWarps;
-    static constexpr int kEpiBytes = kEpiWarps * 2 * 2048;
+    static constexpr int kEpiBytes = kEpiWarps * 4096;  // 32 rows of 128 bytes a warp
     static constexpr int kCumBytes = (kMaxExperts + 4) * 4;  // the experts' tiles, and up to 16 bytes
     static constexpr int kBarAt = kStages * kStageBytes + kEpiBytes + kCumBytes;
     static_assert(kBarAt % 16 == 0 && kStageBytes % 1024 == 0, "alignment of the barriers and tiles");
@@ -221,34 +221,38 @@ __device__ __forceinline__ Tile pair_tile(const PairArgs &a, const int32_t *s_cu
     return t;
 }
 
-// one row's 32 columns straight from registers: rows of a tile that the TMA store must not touch
-template <int T>
-__device__ __forceinline__ void store_row(const PairArgs &a, int64_t row, int n, const float (&v)[32]) {
+// one row's columns of a box straight from registers: rows of a tile that the TMA store must not touch
+template <int T, int W>
+__device__ __forceinline__ void store_row(const PairArgs &a, int64_t row, int n, const float (&v)[W]) {
     uint8_t *p = static_cast<uint8_t *>(a.out) + (row * a.ldo + n) * mx_size(T);
-    if (a.vec_out && n + 32 <= a.N) {
+    if (a.vec_out && n + W <= a.N) {
         if constexpr (T == kMxF32) {
 #pragma unroll
-            for (int q = 0; q < 8; ++q)
+            for (int q = 0; q < W / 4; ++q)
                 reinterpret_cast<uint4 *>(p)[q] = make_uint4(__float_as_uint(v[4 * q]), __float_as_uint(v[4 * q + 1]), __float_as_uint(v[4 * q + 2]), __float_as_uint(v[4 * q + 3]));
         } else {
 #pragma unroll
-            for (int q = 0; q < 4; ++q)
+            for (int q = 0; q < W / 8; ++q)
                 reinterpret_cast<uint4 *>(p)[q] = make_uint4(mx_join<T>(v[8 * q], v[8 * q + 1]), mx_join<T>(v[8 * q + 2], v[8 * q + 3]), mx_join<T>(v[8 * q + 4], v[8 * q + 5]), mx_join<T>(v[8 * q + 6], v[8 * q + 7]));
         }
         return;
     }
 #pragma unroll
-    for (int t = 0; t < 32; ++t)
+    for (int t = 0; t < W; ++t)
         if (n + t < a.N) mx_store1<T>(p, t, v[t]);
 }
 
-__device__ __forceinline__ uint32_t stage_addr(uint32_t buf, int row, int c) { return buf + row * 64 + ((c ^ ((row >> 1) & 3)) << 4); }
+__device__ __forceinline__ uint32_t stage_addr(uint32_t buf, int row, int c) { return buf + row * 128 + ((c ^ (row & 7)) << 4); }
 
 // A CTA pair: each CTA holds 128 of the tile's 256 rows of A, half of its BN rows of B, its own
 // rows' scales and all of B's scales.
 //   warp 0     TMA producer of its CTA; both CTAs' bytes complete on the leader's FULL barrier
 //   warp 1     TMEM; in the leader the scale copies and MMAs of the pair
 //   warps 2-9  drain: TMEM lanes 32 (w % 4) .., half of the tile's columns each
+// The tensor cores bound it while the contraction is long: 8192 x 14336 x 4096 to bf16 takes 190 us alone
+// (5.1 PFLOP/s; 0.32 us a k-block and 2.4 us a tile for the hand-over and the first chunk's drain),
+// 223 us under a lasting load, where the 1 kW power limit holds the clock at 1.54 GHz.  Short ones
+// are bound by that time a tile: 4096 x 5120 x 1280 21.2 us to bf16, 28 to fp32.
 template <int BN, int T>
 __global__ void __launch_bounds__(PairCfg<BN>::kThreads, 1)
     pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
@@ -443,10 +447,14 @@ __global__ void __launch_bounds__(PairCfg<BN>::kThreads, 1)
     } else {
         // ---------------------------------------------------------- drain (both CTAs)
         const int quarter = warp & 3, half = (warp - 2) >> 2;
-        constexpr int kChunks = BN / 64;  // 32-column chunks of this warp's half
-        const uint32_t bufs = sEpi + (warp - 2) * 4096;
+        // Columns of a box, 128 bytes a row: with rows of 64 bytes and two buffers a warp 8192 x 14336 x
+        // 1024 takes 90.7 us against 87.0, and 191.2 against 190.3 at K 4096; two buffers of 128-byte rows
+        // leave room for four stages only (85.1 and 192.9)
+        constexpr int W = T == kMxF32 ? 32 : 64;
+        constexpr int kChunks = BN / 2 / W;       // boxes of this warp's half
+        const uint32_t buf = sEpi + (warp - 2) * 4096;
         const uint32_t tempty0 = peer_smem(TEMPTY(0), 0), over0 = peer_smem(OVER(0), 0);
-        int bsel = 0, count = 0;
+        int count = 0;
         pdl_wait();
         auto hand_over = [&](uint32_t local, uint32_t remote) {
             tc_fence_before();
@@ -472,25 +480,27 @@ __global__ void __launch_bounds__(PairCfg<BN>::kThreads, 1)
             for (int i = 0; i < kChunks; ++i) {
                 // the columns that both accumulators use come first: the last of the first
                 // accumulator, the first of the second
-                const int c = half * (BN / 2) + 32 * (acc ? i : kChunks - 1 - i);
+                const int c = half * (BN / 2) + W * (acc ? i : kChunks - 1 - i);
                 const int n = t.n0 + c;
-                float v[32];
+                float v[W];
                 if (t.nk > 0) {
-                    uint32_t r[32];
-                    tmem_ld32(taddr + c, r);
-                    tmem_wait_ld(r);
+                    uint32_t r[W];
+                    tmem_ld32(taddr + c, *reinterpret_cast<uint32_t(*)[32]>(r));
+                    if constexpr (W == 64) tmem_ld32(taddr + c + 32, *reinterpret_cast<uint32_t(*)[32]>(r + W - 32));
+                    tmem_wait_ld(*reinterpret_cast<uint32_t(*)[32]>(r));
+                    if constexpr (W == 64) tmem_wait_ld(*reinterpret_cast<uint32_t(*)[32]>(r + W - 32));
                     if (BN == 256 && i == 0 && half == (acc ^ 1)) hand_over(OVER(acc), over0 + 8u * acc);
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]);
+                    for (int j = 0; j < W; ++j) v[j] = __uint_as_float(r[j]);
                 } else {
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) v[j] = 0.f;
+                    for (int j = 0; j < W; ++j) v[j] = 0.f;
                 }
                 if (n >= args.N || left <= 0) continue;
                 if (args.bias) {
-                    if (n + 32 <= args.N) {
+                    if (n + W <= args.N) {
 #pragma unroll
-                        for (int j = 0; j < 32; j += 4) {
+                        for (int j = 0; j < W; j += 4) {
                             const float4 b = __ldg(reinterpret_cast<const float4 *>(args.bias + n + j));
                             v[j] += b.x;
                             v[j + 1] += b.y;
@@ -499,36 +509,30 @@ __global__ void __launch_bounds__(PairCfg<BN>::kThreads, 1)
                         }
                     } else {
 #pragma unroll
-                        for (int j = 0; j < 32; ++j)
+                        for (int j = 0; j < W; ++j)
                             if (n + j < args.N) v[j] += __ldg(args.bias + n + j);
                     }
                 }
                 if (!tma) {
-                    if (lane < left) store_row<T>(args, t.out_row + row0 + lane, n, v);
+                    if (lane < left) store_row<T, W>(args, t.out_row + row0 + lane, n, v);
                     continue;
                 }
-                constexpr int kStores = T == kMxF32 ? 2 : 1;  // boxes of 64 bytes a row
+                if (lane == 0) bulk_wait_read<0>();  // the buffer's last store has read it
+                __syncwarp();
 #pragma unroll
-                for (int h = 0; h < kStores; ++h) {
-                    if (lane == 0) bulk_wait_read<1>();  // the buffer's last store has read it
-                    __syncwarp();
-                    const uint32_t buf = bufs + bsel * 2048;
-#pragma unroll
-                    for (int q = 0; q < 4; ++q) {
-                        if constexpr (T == kMxF32)
-                            st_shared_v4(stage_addr(buf, lane, q), __float_as_uint(v[16 * h + 4 * q]), __float_as_uint(v[16 * h + 4 * q + 1]),
-                                         __float_as_uint(v[16 * h + 4 * q + 2]), __float_as_uint(v[16 * h + 4 * q + 3]));
-                        else
-                            st_shared_v4(stage_addr(buf, lane, q), mx_join<T>(v[8 * q], v[8 * q + 1]), mx_join<T>(v[8 * q + 2], v[8 * q + 3]),
-                                         mx_join<T>(v[8 * q + 4], v[8 * q + 5]), mx_join<T>(v[8 * q + 6], v[8 * q + 7]));
-                    }
-                    fence_async_smem();
-                    __syncwarp();
-                    if (lane == 0) {
-                        if (n + 16 * h < args.N || kStores == 1) tma_store_2d(&tmOut, buf, n + 16 * h, static_cast<int>(t.out_row + row0));
-                        bulk_commit();
-                    }
-                    bsel ^= 1;
+                for (int q = 0; q < 8; ++q) {
+                    if constexpr (T == kMxF32)
+                        st_shared_v4(stage_addr(buf, lane, q), __float_as_uint(v[4 * q]), __float_as_uint(v[4 * q + 1]),
+                                     __float_as_uint(v[4 * q + 2]), __float_as_uint(v[4 * q + 3]));
+                    else
+                        st_shared_v4(stage_addr(buf, lane, q), mx_join<T>(v[8 * q], v[8 * q + 1]), mx_join<T>(v[8 * q + 2], v[8 * q + 3]),
+                                     mx_join<T>(v[8 * q + 4], v[8 * q + 5]), mx_join<T>(v[8 * q + 6], v[8 * q + 7]));
+                }
+                fence_async_smem();
+                __syncwarp();
+                if (lane == 0) {
+                    tma_store_2d(&tmOut, buf, n, static_cast<int>(t.out_row + row0));
+                    bulk_commit();
                 }
             }
             if (t.nk > 0) {
@@ -618,8 +622,11 @@ struct FewMaps {
 // the swizzled stage and its scale tiles, and arrive on the stage's FULL barrier beside the TMA
 // unit's bytes.  They learn that a stage is free from a count that the producer keeps of the k-blocks
 // whose stage it has found empty: a slot's next task may lie two turns of the ring on (one pair of
-// rows, four stages), where the parity of EMPTY can't tell the turn.  Every CTA repeats that for its share of K, which the weight's bytes hide while the
-// tokens are few, and one launch and the operand's way through memory are saved.
+// rows, four stages), where the parity of EMPTY can't tell the turn.  Every CTA repeats that for its
+// share of K, which the weight's bytes hide while the tokens are few, and one launch and the
+// operand's way through memory are saved.
+// One row of 4096 bf16, rotated, against 14336: 7.0 us, 4.4 TB/s of the weight; of that the launch and
+// the rotation take 2 to 3 us, and 224 CTAs fill 148 SMs unevenly.
 template <int T, int FUSE>
 __global__ void __launch_bounds__(kFewThreads, 2)
     few_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmSW,
@@ -926,7 +933,7 @@ bool out_map(CUtensorMap *m, void *out, int type, int64_t rows, int64_t cols, in
     const CUtensorMapDataType dt = type == kMxF32   ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
                                    : type == kMxF16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
                                                     : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
-    return make_map(m, out, cols, rows, ldo * mx_size(type), type == kMxF32 ? 16 : 32, 32, dt, CU_TENSOR_MAP_SWIZZLE_64B);
+    return make_map(m, out, cols, rows, ldo * mx_size(type), type == kMxF32 ? 32 : 64, 32, dt, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
 template <int BN, int T>
