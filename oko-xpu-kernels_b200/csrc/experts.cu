@@ -11,10 +11,10 @@
 // Beside the order the sort gives each slot's row among rows padded to whole 128-row tiles an
 // expert (the tiles of MXFP4 scales): tiles[e] is the first tile of expert e.
 //
-// Gather, combine and the gradient move bytes: each element is read and written once, 16 bytes a
-// thread and access where the rows' alignment allows it.
+// Gather, combine and the gradient move bytes: each element is read and written once.
 #include <cuda_runtime.h>
 
+#include <cstring>
 #include <string>
 #include <type_traits>
 
@@ -198,94 +198,121 @@ struct MoveArgs {
     const float *weights;      // combine: [tokens, fan] or null
     const int32_t *positions, *scale_rows;
     int64_t total;             // tokens * units
-    Divisor units;             // vectors of a row
+    Divisor units;             // threads of a row
     uint32_t fan, W;
 };
 
-// vector i: its token and place in the row
+// A row is read and written in accesses of A bytes: 16 where the rows' alignment allows it, else 8, 4, or
+// an element.  Of the narrow ones a thread takes several, which lie a row's threads apart, so that
+// neighbouring lanes touch neighbouring bytes and a slot's place is looked up once for all of them
+// (16384 tokens, 4 rows each of 2047 bf16: gather 87 us where one element a thread takes 143, combine
+// 147 against 350, the gradient 170 against 353; rows of 2046 67, 71 and 129 us, of 2048 54, 53 and 115).
+template <int T, int A>
+struct Access {
+    using Word = typename std::conditional<A == 16, uint4, typename std::conditional<A == 8, uint2, typename std::conditional<A == 4, uint32_t, uint16_t>::type>::type>::type;
+    static constexpr int kValues = A / mx_size(T);
+    static constexpr int kCount = A == 16 ? 1 : A == 8 ? 2 : 4;             // a thread's accesses
+    static constexpr int kSums = A == 16 ? 1 : A == 8 ? 4 : A == 4 ? 8 : 4;  // in combine
+};
+template <int T, int A>
+__device__ __forceinline__ typename Access<T, A>::Word load_word(const void *p, int64_t at) {
+    return __ldcs(reinterpret_cast<const typename Access<T, A>::Word *>(static_cast<const uint8_t *>(p) + at * mx_size(T)));
+}
+template <int T, int A>
+__device__ __forceinline__ void store_word(void *p, int64_t at, const typename Access<T, A>::Word &w) {
+    __stcs(reinterpret_cast<typename Access<T, A>::Word *>(static_cast<uint8_t *>(p) + at * mx_size(T)), w);
+}
+// an access's values in 32 bits, and back
+template <int T, int A>
+__device__ __forceinline__ void spread(const typename Access<T, A>::Word &w, float *v) {
+    if constexpr (A >= 8) {
+        uint32_t u[A / 4];
+        memcpy(u, &w, A);
+#pragma unroll
+        for (int q = 0; q < A / 4; ++q) {
+            if constexpr (T == kMxF32) v[q] = __uint_as_float(u[q]);
+            else mx_split<T>(u[q], v[2 * q], v[2 * q + 1]);
+        }
+    } else if constexpr (T == kMxF32) {
+        v[0] = __uint_as_float(w);
+    } else if constexpr (A == 4) {
+        mx_split<T>(w, v[0], v[1]);
+    } else {
+        float none;
+        mx_split<T>(w, v[0], none);
+    }
+}
+template <int T, int A>
+__device__ __forceinline__ typename Access<T, A>::Word join(const float *v) {
+    if constexpr (A >= 8) {
+        typename Access<T, A>::Word w;
+        uint32_t u[A / 4];
+#pragma unroll
+        for (int q = 0; q < A / 4; ++q) {
+            if constexpr (T == kMxF32) u[q] = __float_as_uint(v[q]);
+            else u[q] = mx_join<T>(v[2 * q], v[2 * q + 1]);
+        }
+        memcpy(&w, u, A);
+        return w;
+    } else if constexpr (T == kMxF32) {
+        return __float_as_uint(v[0]);
+    } else if constexpr (A == 4) {
+        return mx_join<T>(v[0], v[1]);
+    } else {
+        return static_cast<uint16_t>(mx_join<T>(v[0], 0.f));
+    }
+}
+
+// thread i: its token and its place in the row
 __device__ __forceinline__ void place(const MoveArgs &a, int64_t i, int64_t &t, uint32_t &u) {
     t = a.total < 0x7FFFFFFF ? a.units(static_cast<uint32_t>(i)) : i / a.units.d;
     u = static_cast<uint32_t>(i - t * a.units.d);
 }
 
-// One thread: one vector of VEC elements of a token, read once and written to the token's rows.  Memory
-// bounds it: 16384 tokens, 8 rows each of 2048 bf16, 604 MB in 97 us, 6.2 TB/s.
-template <int T, int VEC>
+// One thread: its accesses of a token, read once and written to the token's rows.  Memory bounds it:
+// 16384 tokens, 8 rows each of 2048 bf16, 604 MB in 97 us, 6.2 TB/s.
+template <int T, int A>
 __global__ void __launch_bounds__(256) gather_kernel(const MoveArgs a) {
+    using C = Access<T, A>;
+    constexpr int U = C::kCount;
     const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
     if (i >= a.total) return;
     int64_t t;
     uint32_t u;
     place(a, i, t, u);
-    constexpr int kBytes = VEC * mx_size(T);
-    using Word = typename std::conditional<kBytes == 16, uint4, typename std::conditional<kBytes == 4, uint32_t, uint16_t>::type>::type;
-    const Word v = __ldg(reinterpret_cast<const Word *>(static_cast<const uint8_t *>(a.in) + (t * a.ld_in + static_cast<int64_t>(u) * VEC) * mx_size(T)));
-    const Word zero{};
+    const uint32_t step = a.units.d * C::kValues, c = u * C::kValues;
+    typename C::Word v[U];
+#pragma unroll
+    for (int q = 0; q < U; ++q)
+        if (U == 1 || c + q * step < a.W) v[q] = load_word<T, A>(a.in, t * a.ld_in + c + q * step);
+    const typename C::Word zero{};
 #pragma unroll 4
     for (uint32_t j = 0; j < a.fan; ++j) {
         const int64_t slot = t * a.fan + j;
         const int64_t row = __ldg(a.positions + slot);
         const bool taken = __ldg(a.scale_rows + slot) >= 0;
-        *reinterpret_cast<Word *>(static_cast<uint8_t *>(a.out) + (row * a.W + static_cast<int64_t>(u) * VEC) * mx_size(T)) = taken ? v : zero;
-    }
-}
-
-// VEC values as loaded (one, or 16 bytes of them), and in 32 bits
-template <int T, int VEC>
-struct VecWord {
-    using type = uint4;
-};
-template <int T>
-struct VecWord<T, 1> {
-    using type = float;
-};
-template <int T, int VEC>
-__device__ __forceinline__ typename VecWord<T, VEC>::type load_word(const void *p, int64_t at) {
-    if constexpr (VEC == 1) return mx_load1<T>(p, at);
-    else return __ldcs(reinterpret_cast<const uint4 *>(static_cast<const uint8_t *>(p) + at * mx_size(T)));
-}
-template <int T, int VEC>
-__device__ __forceinline__ void spread(const typename VecWord<T, VEC>::type &w, float (&v)[VEC]) {
-    if constexpr (VEC == 1) {
-        v[0] = w;
-    } else {
-        const uint32_t u[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            if constexpr (T == kMxF32) v[q] = __uint_as_float(u[q]);
-            else mx_split<T>(u[q], v[2 * q], v[2 * q + 1]);
-        }
-    }
-}
-template <int T, int VEC>
-__device__ __forceinline__ void store_vec(void *p, int64_t at, const float (&v)[VEC]) {
-    if constexpr (VEC == 1) {
-        mx_store1<T>(p, at, v[0]);
-    } else {
-        uint32_t u[4];
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            if constexpr (T == kMxF32) u[q] = __float_as_uint(v[q]);
-            else u[q] = mx_join<T>(v[2 * q], v[2 * q + 1]);
-        }
-        __stcs(reinterpret_cast<uint4 *>(static_cast<uint8_t *>(p) + at * mx_size(T)), make_uint4(u[0], u[1], u[2], u[3]));
+        for (int q = 0; q < U; ++q)
+            if (U == 1 || c + q * step < a.W) store_word<T, A>(a.out, row * a.W + c + q * step, taken ? v[q] : zero);
     }
 }
 
 constexpr int kFan = 8;   // choices whose products a gradient keeps at a time
 constexpr int kRows = 4;  // rows whose loads are in flight together
 
-// One thread: one vector of a token's sum.  Four rows' loads at a time and five CTAs an SM: with eight
+// One thread: its accesses of a token's sum.  Four rows' loads at a time and five CTAs an SM: with eight
 // and three the same bytes take 119 us instead of 96 (16384 tokens, 8 rows each of 2048 bf16: 6.3 TB/s).
-template <int T, int VEC>
-__global__ void __launch_bounds__(256, 5) combine_kernel(const MoveArgs a) {
+template <int T, int A>
+__global__ void __launch_bounds__(256, A == 16 ? 5 : A == 2 ? 4 : 3) combine_kernel(const MoveArgs a) {
+    using C = Access<T, A>;
+    constexpr int U = C::kSums, E = C::kValues;
     const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
     if (i >= a.total) return;
     int64_t t;
     uint32_t u;
     place(a, i, t, u);
-    const int64_t c = static_cast<int64_t>(u) * VEC;
-    float sum[VEC] = {};
+    const uint32_t step = a.units.d * E, c = u * E;
+    float sum[U * E] = {};
     for (uint32_t j0 = 0; j0 < a.fan; j0 += kRows) {
         float w[kRows];
         int32_t row[kRows];
@@ -295,20 +322,27 @@ __global__ void __launch_bounds__(256, 5) combine_kernel(const MoveArgs a) {
             row[j] = j0 + j < a.fan && __ldg(a.scale_rows + slot) >= 0 ? __ldg(a.positions + slot) : -1;
             w[j] = row[j] >= 0 && a.weights ? __ldg(a.weights + slot) : 1.f;
         }
-        typename VecWord<T, VEC>::type v[kRows];
+        typename C::Word v[kRows][U];
 #pragma unroll
         for (int j = 0; j < kRows; ++j)
-            if (row[j] >= 0) v[j] = load_word<T, VEC>(a.in, row[j] * a.ld_in + c);
+#pragma unroll
+            for (int q = 0; q < U; ++q)
+                if (row[j] >= 0 && (U == 1 || c + q * step < a.W)) v[j][q] = load_word<T, A>(a.in, row[j] * a.ld_in + c + q * step);
 #pragma unroll
         for (int j = 0; j < kRows; ++j) {
             if (row[j] < 0) continue;
-            float x[VEC];
-            spread<T, VEC>(v[j], x);
 #pragma unroll
-            for (int q = 0; q < VEC; ++q) sum[q] = __fmaf_rn(w[j], x[q], sum[q]);
+            for (int q = 0; q < U; ++q) {
+                float x[E];
+                spread<T, A>(v[j][q], x);
+#pragma unroll
+                for (int e = 0; e < E; ++e) sum[q * E + e] = __fmaf_rn(w[j], x[e], sum[q * E + e]);
+            }
         }
     }
-    store_vec<T, VEC>(a.out, t * a.W + c, sum);
+#pragma unroll
+    for (int q = 0; q < U; ++q)
+        if (U == 1 || c + q * step < a.W) store_word<T, A>(a.out, t * a.W + c + q * step, join<T, A>(sum + q * E));
 }
 
 struct GradArgs {
@@ -321,14 +355,17 @@ struct GradArgs {
     uint32_t fan, W;
 };
 
-constexpr int kGradThreads = 256;
 
 // One CTA a token: its dy is read once for eight choices, whose rows are read once for the product
-// and the sum's terms.  The sums go lane by lane, then warp by warp, in a fixed order.  Four CTAs an SM:
-// 190 us for 16384 tokens, 8 rows each of 2048 bf16 (1.14 GB, 6.0 TB/s), 232 with two.
-template <int T, int VEC>
-__global__ void __launch_bounds__(kGradThreads, 4) combine_grad_kernel(const GradArgs a) {
-    __shared__ float s_sum[kFan][kGradThreads / 32];
+// and the sum's terms.  The sums go lane by lane, then warp by warp, in a fixed order.  Four CTAs of
+// 256 threads an SM: 190 us for 16384 tokens, 8 rows each of 2048 bf16 (1.14 GB, 6.0 TB/s), 232 with two.
+// Narrow rows go to CTAs of 64 threads (4 rows of 256 fp32 or 300 bf16 a token: below 48 us, the host's
+// time, in place of 63 and 90).
+template <int T, int A, int THREADS>
+__global__ void __launch_bounds__(THREADS, (A == 16 ? 4 : 3) * 256 / THREADS) combine_grad_kernel(const GradArgs a) {
+    using C = Access<T, A>;
+    constexpr int U = C::kCount, E = C::kValues;
+    __shared__ float s_sum[kFan][THREADS / 32];
     const int64_t t = blockIdx.x;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     for (uint32_t j0 = 0; j0 < a.fan; j0 += kFan) {
@@ -348,29 +385,40 @@ __global__ void __launch_bounds__(kGradThreads, 4) combine_grad_kernel(const Gra
                 n = j + 1;
             }
         }
-        for (int64_t c = threadIdx.x * VEC; c < a.W; c += kGradThreads * VEC) {
-            float d[VEC];
-            spread<T, VEC>(load_word<T, VEC>(a.dy, t * a.ld_dy + c), d);
+        constexpr uint32_t step = THREADS * E;
+        for (uint32_t c = threadIdx.x * E; c < a.W; c += step * U) {
+            typename C::Word dw[U];
+#pragma unroll
+            for (int q = 0; q < U; ++q)
+                if (U == 1 || c + q * step < a.W) dw[q] = load_word<T, A>(a.dy, t * a.ld_dy + c + q * step);
 #pragma unroll
             for (int h = 0; h < kFan; h += kRows) {
                 if (h >= n) break;
-                typename VecWord<T, VEC>::type v[kRows];
+                typename C::Word v[kRows][U];
 #pragma unroll
                 for (int j = 0; j < kRows; ++j)
-                    if (h + j < n && row[h + j] >= 0) v[j] = load_word<T, VEC>(a.rows, row[h + j] * a.ld_rows + c);
+#pragma unroll
+                    for (int q = 0; q < U; ++q)
+                        if (h + j < n && row[h + j] >= 0 && (U == 1 || c + q * step < a.W)) v[j][q] = load_word<T, A>(a.rows, row[h + j] * a.ld_rows + c + q * step);
 #pragma unroll
                 for (int j = 0; j < kRows; ++j) {
                     if (h + j >= n) break;
                     const bool taken = row[h + j] >= 0;
-                    float u[VEC], g[VEC];
-                    if (taken) {
-                        spread<T, VEC>(v[j], u);
+                    const int64_t at = static_cast<int64_t>(taken ? row[h + j] : ~row[h + j]) * a.W + c;
 #pragma unroll
-                        for (int q = 0; q < VEC; ++q) dot[h + j] = __fmaf_rn(d[q], u[q], dot[h + j]);
+                    for (int q = 0; q < U; ++q) {
+                        if (U > 1 && c + q * step >= a.W) break;
+                        float d[E], u[E], g[E];
+                        spread<T, A>(dw[q], d);
+                        if (taken) {
+                            spread<T, A>(v[j][q], u);
+#pragma unroll
+                            for (int e = 0; e < E; ++e) dot[h + j] = __fmaf_rn(d[e], u[e], dot[h + j]);
+                        }
+#pragma unroll
+                        for (int e = 0; e < E; ++e) g[e] = taken ? __fmul_rn(w[h + j], d[e]) : 0.f;
+                        store_word<T, A>(a.grad_rows, at + q * step, join<T, A>(g));
                     }
-#pragma unroll
-                    for (int q = 0; q < VEC; ++q) g[q] = taken ? __fmul_rn(w[h + j], d[q]) : 0.f;
-                    store_vec<T, VEC>(a.grad_rows, static_cast<int64_t>(taken ? row[h + j] : ~row[h + j]) * a.W + c, g);
                 }
             }
         }
@@ -384,7 +432,7 @@ __global__ void __launch_bounds__(kGradThreads, 4) combine_grad_kernel(const Gra
         if (threadIdx.x < kFan && j0 + threadIdx.x < a.fan) {
             float sum = 0.f;
 #pragma unroll
-            for (int q = 0; q < kGradThreads / 32; ++q) sum = __fadd_rn(sum, s_sum[threadIdx.x][q]);
+            for (int q = 0; q < THREADS / 32; ++q) sum = __fadd_rn(sum, s_sum[threadIdx.x][q]);
             a.grad_weights[t * a.fan + j0 + threadIdx.x] = sum;
         }
         __syncthreads();
@@ -429,10 +477,22 @@ int bad_stride(const char *what) {
     return 2;
 }
 
-template <int T>
-int launch_move(cudaStream_t s, MoveArgs &a, bool gather, int64_t tokens, bool vec, const char *what) {
-    constexpr int kVec = 16 / mx_size(T);
-    a.units = Divisor::of(vec ? a.W / kVec : a.W);
+// the widest access for these rows: 16 bytes, 8, 4, or an element's
+int access(int type, std::initializer_list<const void *> values, std::initializer_list<int64_t> strides) {
+    const int es = mx_size(type);
+    for (const int n : {16, 8, 4}) {
+        bool ok = true;
+        for (const void *p : values) ok = ok && aligned(p, n);
+        for (const int64_t ld : strides) ok = ok && ld * es % n == 0;
+        if (ok) return n;
+    }
+    return es;
+}
+
+template <int T, int A>
+int launch_move(cudaStream_t s, MoveArgs &a, bool gather, int64_t tokens, const char *what) {
+    const int each = Access<T, A>::kValues * (gather ? Access<T, A>::kCount : Access<T, A>::kSums);
+    a.units = Divisor::of((a.W + each - 1) / each);
     a.total = tokens * a.units.d;
     const int64_t blocks = (a.total + 255) / 256;
     if (blocks > 0x7FFFFFFFll) {
@@ -440,31 +500,41 @@ int launch_move(cudaStream_t s, MoveArgs &a, bool gather, int64_t tokens, bool v
         return 2;
     }
     const uint32_t grid = static_cast<uint32_t>(blocks);
-    if (gather) {
-        if (vec) gather_kernel<T, kVec><<<grid, 256, 0, s>>>(a);
-        else gather_kernel<T, 1><<<grid, 256, 0, s>>>(a);
-    } else {
-        if (vec) combine_kernel<T, kVec><<<grid, 256, 0, s>>>(a);
-        else combine_kernel<T, 1><<<grid, 256, 0, s>>>(a);
-    }
+    if (gather) gather_kernel<T, A><<<grid, 256, 0, s>>>(a);
+    else combine_kernel<T, A><<<grid, 256, 0, s>>>(a);
     return launch_status(what);
+}
+template <int T>
+int launch_move(cudaStream_t s, MoveArgs &a, bool gather, int64_t tokens, int bytes, const char *what) {
+    if (bytes == 16) return launch_move<T, 16>(s, a, gather, tokens, what);
+    if (bytes == 8) return launch_move<T, 8>(s, a, gather, tokens, what);
+    if constexpr (T != kMxF32)
+        if (bytes == 2) return launch_move<T, 2>(s, a, gather, tokens, what);
+    return launch_move<T, 4>(s, a, gather, tokens, what);
 }
 
 int move(cudaStream_t s, MoveArgs &a, int type, bool gather, int64_t tokens, const char *what) {
-    const int es = mx_size(type);
-    const bool vec = aligned(a.in, 16) && aligned(a.out, 16) && (a.ld_in * es) % 16 == 0 &&
-                     (static_cast<int64_t>(a.W) * es) % 16 == 0;
+    const int bytes = access(type, {a.in, a.out}, {a.ld_in, a.W});
     switch (type) {
-        case kMxBf16: return launch_move<kMxBf16>(s, a, gather, tokens, vec, what);
-        case kMxF16: return launch_move<kMxF16>(s, a, gather, tokens, vec, what);
-        default: return launch_move<kMxF32>(s, a, gather, tokens, vec, what);
+        case kMxBf16: return launch_move<kMxBf16>(s, a, gather, tokens, bytes, what);
+        case kMxF16: return launch_move<kMxF16>(s, a, gather, tokens, bytes, what);
+        default: return launch_move<kMxF32>(s, a, gather, tokens, bytes, what);
     }
 }
 
+template <int T, int A>
+void launch_grad(cudaStream_t s, const GradArgs &a, int64_t tokens) {
+    // rows that 64 threads take at once are left to them
+    const uint32_t grid = static_cast<uint32_t>(tokens);
+    if (a.W <= 64 * Access<T, A>::kValues * Access<T, A>::kCount) combine_grad_kernel<T, A, 64><<<grid, 64, 0, s>>>(a);
+    else combine_grad_kernel<T, A, 256><<<grid, 256, 0, s>>>(a);
+}
 template <int T>
-void launch_grad(cudaStream_t s, const GradArgs &a, int64_t tokens, bool vec) {
-    if (vec) combine_grad_kernel<T, 16 / mx_size(T)><<<static_cast<uint32_t>(tokens), kGradThreads, 0, s>>>(a);
-    else combine_grad_kernel<T, 1><<<static_cast<uint32_t>(tokens), kGradThreads, 0, s>>>(a);
+void launch_grad(cudaStream_t s, const GradArgs &a, int64_t tokens, int bytes) {
+    if (bytes == 16) launch_grad<T, 16>(s, a, tokens);
+    else if (bytes == 8) launch_grad<T, 8>(s, a, tokens);
+    else if (bytes == 4) launch_grad<T, 4>(s, a, tokens);
+    else if constexpr (T != kMxF32) launch_grad<T, 2>(s, a, tokens);
 }
 
 }  // namespace
@@ -591,14 +661,12 @@ int xpuint8_expert_combine_grad_stream(const void *stream, const void *dy, int32
     a.scale_rows = scale_rows;
     a.fan = static_cast<uint32_t>(fan);
     a.W = static_cast<uint32_t>(width);
-    const int es = mx_size(type);
-    const bool vec = aligned(dy, 16) && aligned(rows, 16) && aligned(grad_rows, 16) &&
-                     (ld_dy * es) % 16 == 0 && (ld_rows * es) % 16 == 0 && (width * es) % 16 == 0;
+    const int bytes = access(type, {dy, rows, grad_rows}, {ld_dy, ld_rows, width});
     cudaStream_t s = as_stream(stream);
     switch (type) {
-        case kMxBf16: launch_grad<kMxBf16>(s, a, tokens, vec); break;
-        case kMxF16: launch_grad<kMxF16>(s, a, tokens, vec); break;
-        default: launch_grad<kMxF32>(s, a, tokens, vec); break;
+        case kMxBf16: launch_grad<kMxBf16>(s, a, tokens, bytes); break;
+        case kMxF16: launch_grad<kMxF16>(s, a, tokens, bytes); break;
+        default: launch_grad<kMxF32>(s, a, tokens, bytes); break;
     }
     return launch_status("expert_combine_grad");
 }

@@ -5,7 +5,9 @@ The B200-native build of the reference package's INT8 half
 sm_100a CUDA kernels (rotate+quantize, a tcgen05 int8 GEMM with fused dequant
 and GEGLU epilogues, the row quantizers and the backward) and this torch-only
 binding.  The flat namespace below is the INT8 API (the same names are
-available as ``xpu_kernels.int8.<name>``).  The reference's Triton half (norm,
+available as ``xpu_kernels.int8.<name>``), the MXFP4 linear beside it
+(:mod:`xpu_kernels.mxfp4`) and mixtures of experts over MXFP4 weights
+(:mod:`xpu_kernels.experts`).  The reference's Triton half (norm,
 rope, attention, NF4) is not part of this build.
 
 Run ``python -m xpu_kernels`` to self-test the library on this machine.

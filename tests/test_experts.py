@@ -91,7 +91,8 @@ def test_sort_of_ids_past_32_bits_and_of_none(gpu):
 
 # --------------------------------------------------------------------------------- gather, combine
 
-MOVES = [(1, 1, 1, 1, 0), (1, 8, 64, 4096, 0), (5, 2, 3, 33, 0.3), (300, 3, 7, 136, 0.1), (2000, 9, 40, 250, 0.05), (64, 2, 4, 2056, 1.0)]
+MOVES = [(1, 1, 1, 1, 0), (1, 8, 64, 4096, 0), (5, 2, 3, 33, 0.3), (300, 3, 7, 136, 0.1), (2000, 9, 40, 250, 0.05), (64, 2, 4, 2056, 1.0),
+         (200, 3, 7, 300, 0.1), (33, 2, 4, 1028, 0.2), (50, 5, 9, 2050, 0.1), (50, 10, 12, 4097, 0.1)]
 
 
 @pytest.mark.gpu
