@@ -121,7 +121,6 @@ struct PairArgs {
     int b_tiles;                      // rows: 128-row scale tiles of each expert's B
     int64_t rows;                     // rows: D's rows, the ones of no expert among them
     int tma_out;                      // D can be stored by the TMA unit
-    int vec_out;                      // D's rows are 16-byte aligned
     int b_early;                      // B is not written by the kernel before this one
 };
 
@@ -221,28 +220,60 @@ __device__ __forceinline__ Tile pair_tile(const PairArgs &a, const int32_t *s_cu
     return t;
 }
 
-// one row's columns of a box straight from registers: rows of a tile that the TMA store must not touch
-template <int T, int W>
-__device__ __forceinline__ void store_row(const PairArgs &a, int64_t row, int n, const float (&v)[W]) {
-    uint8_t *p = static_cast<uint8_t *>(a.out) + (row * a.ldo + n) * mx_size(T);
-    if (a.vec_out && n + W <= a.N) {
-        if constexpr (T == kMxF32) {
-#pragma unroll
-            for (int q = 0; q < W / 4; ++q)
-                reinterpret_cast<uint4 *>(p)[q] = make_uint4(__float_as_uint(v[4 * q]), __float_as_uint(v[4 * q + 1]), __float_as_uint(v[4 * q + 2]), __float_as_uint(v[4 * q + 3]));
-        } else {
-#pragma unroll
-            for (int q = 0; q < W / 8; ++q)
-                reinterpret_cast<uint4 *>(p)[q] = make_uint4(mx_join<T>(v[8 * q], v[8 * q + 1]), mx_join<T>(v[8 * q + 2], v[8 * q + 3]), mx_join<T>(v[8 * q + 4], v[8 * q + 5]), mx_join<T>(v[8 * q + 6], v[8 * q + 7]));
-        }
-        return;
-    }
-#pragma unroll
-    for (int t = 0; t < W; ++t)
-        if (n + t < a.N) mx_store1<T>(p, t, v[t]);
-}
-
 __device__ __forceinline__ uint32_t stage_addr(uint32_t buf, int row, int c) { return buf + row * 128 + ((c ^ (row & 7)) << 4); }
+
+// A box in shared memory (32 rows of 128 bytes, as the TMA store takes it) to `rows` rows of the output
+// from column n on, where the TMA unit can't: rows that aren't 16-byte aligned, or strips that another
+// matrix's rows follow.  A warp writes a row at a time, 4 bytes a lane; a 16-bit row that begins
+// between two words goes one value on, its first and last by themselves.  The loops take rows of one
+// parity, so that nothing in them branches: 4096 x 5122 x 1280 to bf16 takes 28 us so, 41 where
+// each row asks, 209 where each lane stores a row of its own, and 21 by TMA where N is 5120.
+template <int T>
+__device__ __forceinline__ void store_box(const PairArgs &a, uint32_t buf, int64_t row, int rows, int n, int lane) {
+    const int left = a.N - n;  // columns that exist
+    uint8_t *out = static_cast<uint8_t *>(a.out) + (row * a.ldo + n) * mx_size(T);
+    const int64_t pitch = a.ldo * mx_size(T);
+    auto word = [&](int r, int w) {  // 4-byte word w of row r
+        uint32_t v;
+        asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(stage_addr(buf, r, w >> 2) + (w & 3) * 4));
+        return v;
+    };
+    if (a.tma_out && left * mx_size(T) >= 128) {  // four rows at a time, 16 bytes a lane
+#pragma unroll 1
+        for (int r = lane >> 3; r < rows; r += 4) {
+            uint32_t w[4];
+            asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(stage_addr(buf, r, lane & 7)));
+            *reinterpret_cast<uint4 *>(out + r * pitch + (lane & 7) * 16) = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+    } else if (T == kMxF32) {
+        uint8_t *p = out + lane * 4;
+        if (lane < left)
+#pragma unroll 8
+            for (int r = 0; r < rows; ++r, p += pitch) *reinterpret_cast<uint32_t *>(p) = word(r, lane);
+    } else if (left < 64) {
+#pragma unroll 1
+        for (int r = 0; r < rows; ++r)
+            for (int c = lane; c < left; c += 32) reinterpret_cast<uint16_t *>(out + r * pitch)[c] = static_cast<uint16_t>(word(r, c >> 1) >> (16 * (c & 1)));
+    } else {
+        const int stride = pitch & 2 ? 2 : 1;  // rows of the same parity
+        for (int first = 0; first < stride; ++first) {
+            uint8_t *p = out + first * pitch + lane * 4;
+            if ((reinterpret_cast<uintptr_t>(p) & 2) == 0) {
+#pragma unroll 8
+                for (int r = first; r < rows; r += stride, p += stride * pitch) *reinterpret_cast<uint32_t *>(p) = word(r, lane);
+            } else {
+                const bool inner = lane < 31, edge = lane == 0 || lane == 31;
+                uint8_t *e = p + (lane ? 2 : 0);
+#pragma unroll 8
+                for (int r = first; r < rows; r += stride, p += stride * pitch, e += stride * pitch) {
+                    const uint32_t v = word(r, lane), next = word(r, (lane + 1) & 31);
+                    if (inner) *reinterpret_cast<uint32_t *>(p + 2) = __byte_perm(v, next, 0x5432);
+                    if (edge) *reinterpret_cast<uint16_t *>(e) = static_cast<uint16_t>(lane ? v >> 16 : v);
+                }
+            }
+        }
+    }
+}
 
 // A CTA pair: each CTA holds 128 of the tile's 256 rows of A, half of its BN rows of B, its own
 // rows' scales and all of B's scales.
@@ -513,10 +544,6 @@ __global__ void __launch_bounds__(PairCfg<BN>::kThreads, 1)
                             if (n + j < args.N) v[j] += __ldg(args.bias + n + j);
                     }
                 }
-                if (!tma) {
-                    if (lane < left) store_row<T, W>(args, t.out_row + row0 + lane, n, v);
-                    continue;
-                }
                 if (lane == 0) bulk_wait_read<0>();  // the buffer's last store has read it
                 __syncwarp();
 #pragma unroll
@@ -528,9 +555,12 @@ __global__ void __launch_bounds__(PairCfg<BN>::kThreads, 1)
                         st_shared_v4(stage_addr(buf, lane, q), mx_join<T>(v[8 * q], v[8 * q + 1]), mx_join<T>(v[8 * q + 2], v[8 * q + 3]),
                                      mx_join<T>(v[8 * q + 4], v[8 * q + 5]), mx_join<T>(v[8 * q + 6], v[8 * q + 7]));
                 }
-                fence_async_smem();
+                if (tma) fence_async_smem();
                 __syncwarp();
-                if (lane == 0) {
+                if (!tma) {
+                    store_box<T>(args, buf, t.out_row + row0, min(left, 32), n, lane);
+                    __syncwarp();
+                } else if (lane == 0) {
                     tma_store_2d(&tmOut, buf, n, static_cast<int>(t.out_row + row0));
                     bulk_commit();
                 }
@@ -1026,8 +1056,7 @@ int run_pair(cudaStream_t s, PairArgs a, const Operand &A, const Operand &B, int
         return 2;
     }
     const int es = mx_size(type);
-    a.vec_out = (reinterpret_cast<uintptr_t>(a.out) & 15) == 0 && (a.ldo * es) % 16 == 0;
-    a.tma_out = a.vec_out;
+    a.tma_out = (reinterpret_cast<uintptr_t>(a.out) & 15) == 0 && (a.ldo * es) % 16 == 0;
     PairMaps m{};
     if (!code_map(&m.a, A, 128) || !code_map(&m.b, B, bn / 2) || !scale_map(&m.sa, A, 1) || !scale_map(&m.sb, B, bn / 128)) return 2;
     if (a.tma_out && !out_map(&m.out, a.out, type, out_rows, a.N, a.ldo)) return 2;
@@ -1197,15 +1226,15 @@ int mx4_expert_token_mm(cudaStream_t s, const void *x, int64_t ldx, const int32_
 }
 
 int mx4_expert_mm(cudaStream_t s, const uint8_t *a_codes, const uint8_t *a_scales, const uint8_t *b_codes, const uint8_t *b_scales,
-                  void *out, int type, const int32_t *offsets, const int32_t *tiles, int64_t rows, int64_t max_tiles, int64_t N,
-                  int64_t K, int64_t experts) {
+                  void *out, int type, int64_t ldo, const int32_t *offsets, const int32_t *tiles, int64_t rows, int64_t max_tiles,
+                  int64_t N, int64_t K, int64_t experts) {
     const Operand A{a_codes, a_scales, rows, K, max_tiles};
     const Operand B{b_codes, b_scales, experts * N, K, experts * ((N + 127) / 128)};
     // by the mean rows of an expert: 64 experts of 2816 x 2048 take 50 us at 32 rows against the pairs'
     // 57, 56 against 57 at 48, 63 against 57 at 64; 8 of 5632 x 2048 13.8 against 18.2, 15.9 against
     // 18.4, 19.2 against 18.5
     if (rows <= experts * 48) {
-        FewArgs a = few_args(out, N, rows, N, K);
+        FewArgs a = few_args(out, ldo, rows, N, K);
         a.mode = kRows;
         a.offsets = offsets;
         a.tiles = tiles;
@@ -1214,7 +1243,7 @@ int mx4_expert_mm(cudaStream_t s, const uint8_t *a_codes, const uint8_t *a_scale
     }
     PairArgs a{};
     a.out = out;
-    a.ldo = N;
+    a.ldo = ldo;
     a.M = static_cast<int>(rows);
     a.N = static_cast<int>(N);
     set_k(K, a.nk, a.last_steps);
@@ -1286,7 +1315,7 @@ int xpuint8_mxfp4_expert_mm_stream(const void *stream, const uint8_t *a_codes,
         set_error("mxfp4_expert_mm: offsets and tiles, 1 to 1024 experts, experts x N below 2^31, at most 65535 tiles");
         return 2;
     }
-    return mx4_expert_mm(as_stream(stream), a_codes, a_scales, b_codes, b_scales, out, type, offsets, tiles, rows, max_tiles, N, K, experts);
+    return mx4_expert_mm(as_stream(stream), a_codes, a_scales, b_codes, b_scales, out, type, N, offsets, tiles, rows, max_tiles, N, K, experts);
 }
 
 int xpuint8_mxfp4_expert_dw_stream(const void *stream, const uint8_t *a_codes,

@@ -31,9 +31,10 @@ struct Mx4Both {
     int64_t experts = 0, max_tiles = 0, fan = 0;
 };
 int mx4_quantize_both(cudaStream_t s, const Mx4Both &b);
-// out [rows, K] = fp32 rows (or, with positions, the sums of each token's rows), rotated where asked,
-// rounded once to `type`
-int mx4_turn(cudaStream_t s, const float *x, void *out, int type, int64_t rows, int64_t K, const int32_t *positions,
+// out [rows, K] = fp32 rows (or, with positions, the sums of each token's rows), rounded once to `type`: rotated
+// (K a multiple of 256, the rows contiguous); else x's rows are `ldx` apart, a multiple of 4, and only
+// sums are wanted
+int mx4_turn(cudaStream_t s, const float *x, int64_t ldx, void *out, int type, int64_t rows, int64_t K, const int32_t *positions,
              const int32_t *scale_rows, int64_t fan, bool rotate);
 
 // ------------------------------------------------------------------------------ products (gemm_mx4.cu)
@@ -41,8 +42,8 @@ int mx4_turn(cudaStream_t s, const float *x, void *out, int type, int64_t rows, 
 int mx4_mm(cudaStream_t s, const uint8_t *a_codes, const uint8_t *a_scales, const uint8_t *b_codes, const uint8_t *b_scales,
            const float *bias, void *out, int type, int64_t ldo, int64_t M, int64_t N, int64_t K, bool b_early);
 int mx4_expert_mm(cudaStream_t s, const uint8_t *a_codes, const uint8_t *a_scales, const uint8_t *b_codes, const uint8_t *b_scales,
-                  void *out, int type, const int32_t *offsets, const int32_t *tiles, int64_t rows, int64_t max_tiles, int64_t N,
-                  int64_t K, int64_t experts);
+                  void *out, int type, int64_t ldo, const int32_t *offsets, const int32_t *tiles, int64_t rows, int64_t max_tiles,
+                  int64_t N, int64_t K, int64_t experts);
 int mx4_expert_dw(cudaStream_t s, const uint8_t *a_codes, const uint8_t *a_scales, const uint8_t *b_codes, const uint8_t *b_scales,
                   void *out, int type, const int32_t *tiles, int64_t max_tiles, int64_t M, int64_t N, int64_t experts);
 // few tokens quantised inside the product: x [M, K] of the output's type, M <= kMx4Tokens

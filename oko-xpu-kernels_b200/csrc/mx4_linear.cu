@@ -115,11 +115,14 @@ GradWork grad_work(Scratch &s, int64_t M, int64_t N, int64_t K, int w_type, int 
     if ((want & 2) && rotate) g.dw = s.take(N * K * size_of(w_type));
     return g;
 }
+// fp32 rows that are summed afterwards: 16-byte aligned, for the product's stores and the sum's loads (22544
+// rows of 850: 54 and 66 us packed)
+int64_t sum_pitch(int64_t K) { return (K + 3) / 4 * 4; }
 GradWork expert_grad_work(Scratch &s, int64_t rows, int64_t max_tiles, int64_t N, int64_t K, int64_t experts, int w_type, bool turn_dx, int rotate, int want) {
     GradWork g{};
     if (want & 1) g.rows = take_rows(s, rows, max_tiles, N);
     if (want & 2) g.cols = take(s, N, max_tiles * 128);
-    if ((want & 1) && turn_dx) g.dx = reinterpret_cast<float *>(s.take(rows * K * 4));
+    if ((want & 1) && turn_dx) g.dx = reinterpret_cast<float *>(s.take(rows * sum_pitch(K) * 4));
     if ((want & 2) && rotate) g.dw = s.take(experts * N * K * size_of(w_type));
     return g;
 }
@@ -254,7 +257,7 @@ int xpuint8_mxfp4_grad_stream(const void *stream, const void *dy, int32_t type, 
         void *to = rotate ? static_cast<void *>(g.dx) : dx;
         if (int rc = mx4_mm(s, g.rows.codes, g.rows.scales, t.w.codes, t.w.scales, nullptr, to, rotate ? 2 : type, K, M, K, N, true)) return rc;
         if (rotate)
-            if (int rc = mx4_turn(s, g.dx, dx, type, M, K, nullptr, nullptr, 1, true)) return rc;
+            if (int rc = mx4_turn(s, g.dx, K, dx, type, M, K, nullptr, nullptr, 1, true)) return rc;
     }
     if (want_w) {
         void *to = rotate ? static_cast<void *>(g.dw) : dw;
@@ -296,7 +299,7 @@ int xpuint8_mxfp4_expert_linear_stream(const void *stream, const void *x, int32_
     if (int rc = mx4_quantize_sorted(s, x, type, ldx, q.codes, q.scales, nullptr, sorted ? order : nullptr, positions, scale_rows,
                                      sorted ? rows : tokens, sorted ? 1 : fan, K, rotate != 0))
         return rc;
-    return mx4_expert_mm(s, q.codes, q.scales, w_codes, w_scales, out, type, offsets, tiles, rows, max_tiles, N, K, experts);
+    return mx4_expert_mm(s, q.codes, q.scales, w_codes, w_scales, out, type, N, offsets, tiles, rows, max_tiles, N, K, experts);
 }
 
 int64_t xpuint8_mxfp4_expert_train_saved_workspace_bytes(int64_t max_tiles, int64_t N, int64_t K, int64_t experts, int32_t want) {
@@ -369,7 +372,7 @@ int xpuint8_mxfp4_expert_train_stream(const void *stream, const void *x, int32_t
                                             sorted ? rows : tokens, sorted ? 1 : fan, K, rotate != 0)) {
         return rc;
     }
-    return mx4_expert_mm(s, xq.codes, xq.scales, wq.codes, wq.scales, out, type, offsets, tiles, rows, max_tiles, N, K, experts);
+    return mx4_expert_mm(s, xq.codes, xq.scales, wq.codes, wq.scales, out, type, N, offsets, tiles, rows, max_tiles, N, K, experts);
 }
 
 int64_t xpuint8_mxfp4_expert_grad_workspace_bytes(int64_t rows, int64_t max_tiles, int64_t N, int64_t K, int64_t experts,
@@ -424,9 +427,9 @@ int xpuint8_mxfp4_expert_grad_stream(const void *stream, const void *dy, int32_t
     }
     if (want_x) {
         void *to = turn_dx ? static_cast<void *>(g.dx) : dx;
-        if (int rc = mx4_expert_mm(s, g.rows.codes, g.rows.scales, t.w.codes, t.w.scales, to, turn_dx ? 2 : type, offsets, tiles, rows, max_tiles, K, N, experts)) return rc;
+        if (int rc = mx4_expert_mm(s, g.rows.codes, g.rows.scales, t.w.codes, t.w.scales, to, turn_dx ? 2 : type, turn_dx ? sum_pitch(K) : K, offsets, tiles, rows, max_tiles, K, N, experts)) return rc;
         if (turn_dx)
-            if (int rc = mx4_turn(s, g.dx, dx, type, sorted ? rows : tokens, K, sorted ? nullptr : positions, sorted ? nullptr : scale_rows, sorted ? 1 : fan, rotate != 0)) return rc;
+            if (int rc = mx4_turn(s, g.dx, sum_pitch(K), dx, type, sorted ? rows : tokens, K, sorted ? nullptr : positions, sorted ? nullptr : scale_rows, sorted ? 1 : fan, rotate != 0)) return rc;
     }
     if (want_w) {
         void *to = rotate ? static_cast<void *>(g.dw) : dw;

@@ -395,18 +395,21 @@ __global__ void __launch_bounds__(kBothThreads, T == kMxF32 ? 2 : ROT ? 4 : 3) q
 
 struct TurnArgs {
     const float *x;              // [rows, K], or the experts' rows that are summed
+    int64_t ldx;                 // sums: elements between x's rows, a multiple of 4
     void *out;                   // [rows, K]
     uint32_t groups, G, K;
+    int64_t total;               // sums: rows * units
+    Divisor units;               // sums: threads of a row
     const int32_t *positions, *scale_rows;  // experts: [rows, fan], or null
     uint32_t fan;
-    bool wide, wide_out;         // rows of x and out are 32-byte aligned
+    bool wide, vec_out, wide_out;  // rows of x are 32-byte aligned, of out 16 and 32
 };
 
 // fp32 rows, or the sums of each token's rows, turned back by the rotation and rounded once.  8192 tokens,
 // two rows of 2048 each, 168 MB: 34.5 us, 4.9 TB/s, by the rotation's instructions.
-template <int T, bool ROT, bool VEC>
+template <int T>
 __global__ void __launch_bounds__(128) turn_kernel(const TurnArgs a) {
-    __shared__ __align__(128) uint8_t tiles[ROT ? 8 * kSlotBytes : 16];
+    __shared__ __align__(128) uint8_t tiles[8 * kSlotBytes];
     const int slot = threadIdx.x >> 4, l = threadIdx.x & 15;
     const uint32_t f0 = (blockIdx.x * 8u + slot) * 2u;
     const uint32_t r0 = f0 / a.G, g0 = f0 - r0 * a.G;
@@ -415,12 +418,12 @@ __global__ void __launch_bounds__(128) turn_kernel(const TurnArgs a) {
         Run<kMxF32> v = zero_run<kMxF32>();
         if (!ok) return v;
         const uint32_t c = g * 256 + l * 16;
-        if (!a.positions) return load_run<kMxF32, VEC>(a.x + static_cast<int64_t>(r) * a.K, c, a.K, a.wide);
+        if (!a.positions) return load_run<kMxF32, true>(a.x + static_cast<int64_t>(r) * a.K, c, a.K, a.wide);
 #pragma unroll 2
         for (uint32_t j = 0; j < a.fan; ++j) {
             const int64_t at = static_cast<int64_t>(r) * a.fan + j;
             if (__ldg(a.scale_rows + at) < 0) continue;
-            const Run<kMxF32> u = load_run<kMxF32, VEC>(a.x + static_cast<int64_t>(__ldg(a.positions + at)) * a.K, c, a.K, a.wide);
+            const Run<kMxF32> u = load_run<kMxF32, true>(a.x + static_cast<int64_t>(__ldg(a.positions + at)) * a.K, c, a.K, a.wide);
 #pragma unroll
             for (int t = 0; t < 16; ++t) v.w[t] = __float_as_uint(__fadd_rn(__uint_as_float(v.w[t]), __uint_as_float(u.w[t])));
         }
@@ -428,30 +431,68 @@ __global__ void __launch_bounds__(128) turn_kernel(const TurnArgs a) {
     };
     const bool ok0 = f0 < a.groups, ok1 = f0 + 1 < a.groups;
     Run<kMxF32> A = bring(ok0, r0, g0), B = bring(ok1, r1, g1);
-    if constexpr (ROT) {
-        const uint32_t tile = smem_u32(tiles) + slot * kSlotBytes;
-        rotate_to_shared<kMxF32>(A, B, tile, l);
-        split_pairs<kMxF32>(pairs_from_shared<kMxF32>(tile, l), A, B);
-    }
+    const uint32_t tile = smem_u32(tiles) + slot * kSlotBytes;
+    rotate_to_shared<kMxF32>(A, B, tile, l);
+    split_pairs<kMxF32>(pairs_from_shared<kMxF32>(tile, l), A, B);
     auto put = [&](uint32_t r, uint32_t g, const Run<kMxF32> &v) {
         uint8_t *row = static_cast<uint8_t *>(a.out) + static_cast<int64_t>(r) * a.K * mx_size(T);
         const uint32_t c = g * 256 + l * 16;
-        if (VEC && c + 16 <= a.K) {
-            Run<T> o;
+        if (!a.vec_out) {
 #pragma unroll
-            for (int t = 0; t < Run<T>::kWords; ++t) {
-                if constexpr (T == kMxF32) o.w[t] = v.w[t];
-                else o.w[t] = mx_join<T>(__uint_as_float(v.w[2 * t]), __uint_as_float(v.w[2 * t + 1]));
-            }
-            store_run<T>(row, c, o, a.wide_out);
-        } else {
-#pragma unroll
-            for (int t = 0; t < 16; ++t)
-                if (c + t < a.K) mx_store1<T>(row, c + t, __uint_as_float(v.w[t]));
+            for (int t = 0; t < 16; ++t) mx_store1<T>(row, c + t, __uint_as_float(v.w[t]));
+            return;
         }
+        Run<T> o;
+#pragma unroll
+        for (int t = 0; t < Run<T>::kWords; ++t) {
+            if constexpr (T == kMxF32) o.w[t] = v.w[t];
+            else o.w[t] = mx_join<T>(__uint_as_float(v.w[2 * t]), __uint_as_float(v.w[2 * t + 1]));
+        }
+        store_run<T>(row, c, o, a.wide_out);
     };
     if (ok0) put(r0, g0, A);
     if (ok1) put(r1, g1, B);
+}
+
+// The sums of each token's fp32 rows, in the order of its choices, rounded once.  A thread takes U accesses
+// of E values, a row's threads apart, so that lanes touch neighbouring bytes; E is 4 where the output's rows
+// allow it.
+template <int T, int E>
+__global__ void __launch_bounds__(256) sum_kernel(const TurnArgs a) {
+    constexpr int U = E == 4 ? 2 : 8;
+    const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+    if (i >= a.total) return;
+    const int64_t r = a.total < 0x7FFFFFFF ? a.units(static_cast<uint32_t>(i)) : i / a.units.d;
+    const uint32_t step = a.units.d * E, c = static_cast<uint32_t>(i - r * a.units.d) * E;
+    float sum[U * E] = {};
+#pragma unroll 2
+    for (uint32_t j = 0; j < a.fan; ++j) {
+        const int64_t at = r * a.fan + j;
+        if (__ldg(a.scale_rows + at) < 0) continue;
+        const float *x = a.x + __ldg(a.positions + at) * a.ldx + c;
+#pragma unroll
+        for (int q = 0; q < U; ++q) {
+            if (c + q * step >= a.K) break;
+            if constexpr (E == 4) {
+                const float4 v = __ldg(reinterpret_cast<const float4 *>(x + q * step));
+                sum[4 * q] = __fadd_rn(sum[4 * q], v.x);
+                sum[4 * q + 1] = __fadd_rn(sum[4 * q + 1], v.y);
+                sum[4 * q + 2] = __fadd_rn(sum[4 * q + 2], v.z);
+                sum[4 * q + 3] = __fadd_rn(sum[4 * q + 3], v.w);
+            } else {
+                sum[q] = __fadd_rn(sum[q], __ldg(x + q * step));
+            }
+        }
+    }
+    uint8_t *out = static_cast<uint8_t *>(a.out) + (r * a.K + c) * mx_size(T);
+#pragma unroll
+    for (int q = 0; q < U; ++q) {
+        if (c + q * step >= a.K) break;
+        uint8_t *p = out + static_cast<int64_t>(q) * step * mx_size(T);
+        if constexpr (E == 1) mx_store1<T>(p, 0, sum[q]);
+        else if constexpr (T == kMxF32) *reinterpret_cast<float4 *>(p) = make_float4(sum[4 * q], sum[4 * q + 1], sum[4 * q + 2], sum[4 * q + 3]);
+        else *reinterpret_cast<uint2 *>(p) = make_uint2(mx_join<T>(sum[4 * q], sum[4 * q + 1]), mx_join<T>(sum[4 * q + 2], sum[4 * q + 3]));
+    }
 }
 
 struct ValueArgs {
@@ -604,11 +645,11 @@ int launch_both(cudaStream_t s, const BothArgs &a, dim3 grid, bool rotate, bool 
 }
 
 template <int T>
-void launch_turn(cudaStream_t s, const TurnArgs &a, bool rotate, bool vec) {
-    const uint32_t grid = (a.groups + 15) / 16;
-    if (rotate) turn_kernel<T, true, true><<<grid, 128, 0, s>>>(a);  // K % 256 == 0: rows are aligned
-    else if (vec) turn_kernel<T, false, true><<<grid, 128, 0, s>>>(a);
-    else turn_kernel<T, false, false><<<grid, 128, 0, s>>>(a);
+void launch_turn(cudaStream_t s, const TurnArgs &a, bool rotate, int each) {
+    const uint32_t sums = static_cast<uint32_t>((a.total + 255) / 256);
+    if (rotate) turn_kernel<T><<<(a.groups + 15) / 16, 128, 0, s>>>(a);
+    else if (each == 4) sum_kernel<T, 4><<<sums, 256, 0, s>>>(a);
+    else sum_kernel<T, 1><<<sums, 256, 0, s>>>(a);
 }
 
 }  // namespace
@@ -727,14 +768,17 @@ int mx4_quantize_both(cudaStream_t s, const Mx4Both &b) {
     }
 }
 
-int mx4_turn(cudaStream_t s, const float *x, void *out, int type, int64_t rows, int64_t K, const int32_t *positions,
+int mx4_turn(cudaStream_t s, const float *x, int64_t ldx, void *out, int type, int64_t rows, int64_t K, const int32_t *positions,
              const int32_t *scale_rows, int64_t fan, bool rotate) {
     TurnArgs a{};
     a.x = x;
+    a.ldx = ldx;
     a.out = out;
     a.G = static_cast<uint32_t>((K + 255) / 256);
     a.K = static_cast<uint32_t>(K);
-    if (rows * a.G > 0x7FFFFFF0ll) {
+    a.units = Divisor::of(static_cast<uint32_t>((K + 7) / 8));  // eight values a thread
+    a.total = rows * a.units.d;
+    if (rows * a.G > 0x7FFFFFF0ll || (a.total + 255) / 256 > 0x7FFFFFFFll) {
         set_error("mxfp4: rows x 256-groups must be below 2^31");
         return 2;
     }
@@ -742,13 +786,14 @@ int mx4_turn(cudaStream_t s, const float *x, void *out, int type, int64_t rows, 
     a.positions = positions;
     a.scale_rows = scale_rows;
     a.fan = static_cast<uint32_t>(fan);
-    a.wide = aligned(x, 32) && K % 8 == 0;
-    a.wide_out = aligned(out, 32) && (K * mx_size(type)) % 32 == 0;
-    const bool vec = aligned(x, 16) && aligned(out, 16) && (K * mx_size(type)) % 16 == 0 && K % 4 == 0;
+    a.wide = aligned(x, 32);
+    a.vec_out = aligned(out, 16);
+    a.wide_out = aligned(out, 32);
+    const int e = K % 4 == 0 && aligned(out, 4 * mx_size(type)) ? 4 : 1;
     switch (type) {
-        case kMxBf16: launch_turn<kMxBf16>(s, a, rotate, vec); break;
-        case kMxF16: launch_turn<kMxF16>(s, a, rotate, vec); break;
-        default: launch_turn<kMxF32>(s, a, rotate, vec); break;
+        case kMxBf16: launch_turn<kMxBf16>(s, a, rotate, e); break;
+        case kMxF16: launch_turn<kMxF16>(s, a, rotate, e); break;
+        default: launch_turn<kMxF32>(s, a, rotate, e); break;
     }
     return launch_status("mxfp4_turn");
 }
