@@ -226,8 +226,9 @@ __device__ __forceinline__ uint32_t stage_addr(uint32_t buf, int row, int c) { r
 // from column n on, where the TMA unit can't: rows that aren't 16-byte aligned, or strips that another
 // matrix's rows follow.  A warp writes a row at a time, 4 bytes a lane; a 16-bit row that begins
 // between two words goes one value on, its first and last by themselves.  The loops take rows of one
-// parity, so that nothing in them branches: 4096 x 5122 x 1280 to bf16 takes 28 us so, 41 where
-// each row asks, 209 where each lane stores a row of its own, and 21 by TMA where N is 5120.
+// parity, so that nothing in them branches: 4096 x 5122 x 1280 to bf16 takes 28 us so and 5121 columns
+// 32, 41 where each row asks, 209 where each lane stores a row of its own, and 21 by TMA where N is
+// 5120.
 template <int T>
 __device__ __forceinline__ void store_box(const PairArgs &a, uint32_t buf, int64_t row, int rows, int n, int lane) {
     const int left = a.N - n;  // columns that exist
@@ -255,18 +256,47 @@ __device__ __forceinline__ void store_box(const PairArgs &a, uint32_t buf, int64
         for (int r = 0; r < rows; ++r)
             for (int c = lane; c < left; c += 32) reinterpret_cast<uint16_t *>(out + r * pitch)[c] = static_cast<uint16_t>(word(r, c >> 1) >> (16 * (c & 1)));
     } else {
-        const int stride = pitch & 2 ? 2 : 1;  // rows of the same parity
-        for (int first = 0; first < stride; ++first) {
+        // rows of one parity: all of them, or every other one
+        const int by = pitch & 2 ? 2 : 1;
+        const int64_t step = by * pitch;
+#pragma unroll 1
+        for (int first = 0; first < by; ++first) {
+            const int count = (rows - first + by - 1) >> (by - 1);
             uint8_t *p = out + first * pitch + lane * 4;
+            int r = first;
             if ((reinterpret_cast<uintptr_t>(p) & 2) == 0) {
+                if (by == 1)
 #pragma unroll 8
-                for (int r = first; r < rows; r += stride, p += stride * pitch) *reinterpret_cast<uint32_t *>(p) = word(r, lane);
+                    for (r = 0; r < rows; ++r, p += pitch) *reinterpret_cast<uint32_t *>(p) = word(r, lane);
+                else
+#pragma unroll 8
+                    for (r = first; r < rows; r += 2, p += step) *reinterpret_cast<uint32_t *>(p) = word(r, lane);
             } else {
                 const bool inner = lane < 31, edge = lane == 0 || lane == 31;
                 uint8_t *e = p + (lane ? 2 : 0);
-#pragma unroll 8
-                for (int r = first; r < rows; r += stride, p += stride * pitch, e += stride * pitch) {
-                    const uint32_t v = word(r, lane), next = word(r, (lane + 1) & 31);
+                int k = 0;  // eight rows' loads before their stores
+#pragma unroll 1
+                for (; k + 8 <= count; k += 8) {
+                    uint32_t v[8], w[8];
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) v[j] = word(r + j * by, lane);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) w[j] = __byte_perm(v[j], __shfl_down_sync(0xFFFFFFFFu, v[j], 1), 0x5432);
+                    if (inner) {
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) *reinterpret_cast<uint32_t *>(p + 2 + j * step) = w[j];
+                    }
+                    if (edge) {
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) *reinterpret_cast<uint16_t *>(e + j * step) = static_cast<uint16_t>(lane ? v[j] >> 16 : v[j]);
+                    }
+                    r += 8 * by;
+                    p += 8 * step;
+                    e += 8 * step;
+                }
+#pragma unroll 1
+                for (; k < count; ++k, r += by, p += step, e += step) {
+                    const uint32_t v = word(r, lane), next = __shfl_down_sync(0xFFFFFFFFu, v, 1);
                     if (inner) *reinterpret_cast<uint32_t *>(p + 2) = __byte_perm(v, next, 0x5432);
                     if (edge) *reinterpret_cast<uint16_t *>(e) = static_cast<uint16_t>(lane ? v >> 16 : v);
                 }
