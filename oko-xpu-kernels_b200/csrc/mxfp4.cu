@@ -179,6 +179,27 @@ __global__ void __launch_bounds__(128) quantize_columns_kernel(const ColumnArgs 
             w[i] = Word{};
             if (r0 + i < end) w[i] = __ldg(reinterpret_cast<const Word *>(x + (static_cast<int64_t>(r0 + i) * a.ldx + c) * mx_size(T)));
         }
+    } else if (!VEC && T != kMxF32 && blockIdx.x * 64 + 66 <= a.cols && r0 + 32 <= end) {
+        // a row that begins between two words: the words one value on, whose first the lane before has
+        // (lane 0 reads its own): [9001, 4001] 22 us, 38 where each value is read by itself
+        const uint8_t *p = x + (static_cast<int64_t>(r0) * a.ldx + c) * 2;
+        const int64_t pitch = a.ldx * 2;
+        const uint32_t o0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(p)) & 2, o1 = (o0 + static_cast<uint32_t>(pitch)) & 2;
+        uint32_t own[32], v[32];
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+            const uint8_t *q = p + i * pitch;
+            v[i] = __ldg(reinterpret_cast<const uint32_t *>(q + (i & 1 ? o1 : o0)));
+            own[i] = 0;
+            if (lane == 0) own[i] = __ldg(reinterpret_cast<const uint16_t *>(q));
+        }
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+            uint32_t up = __shfl_up_sync(0xFFFFFFFFu, v[i], 1);
+            if (lane == 0) up = own[i] << 16;
+            const uint32_t u = (i & 1 ? o1 : o0) ? __byte_perm(up, v[i], 0x5432) : v[i];
+            if constexpr (T != kMxF32) w[i] = u;
+        }
     } else {
 #pragma unroll
         for (int i = 0; i < 32; ++i) {
