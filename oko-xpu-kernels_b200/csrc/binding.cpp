@@ -312,7 +312,7 @@ struct ExpertLinearFn : torch::autograd::Function<ExpertLinearFn> {
 // ------------------------------------------------------------------------ from and to Python objects
 
 const Tensor &tensor(PyObject *o) {
-    if (!THPVariable_Check(o)) throw std::invalid_argument("a tensor was expected");
+    TORCH_CHECK_TYPE(THPVariable_Check(o), "a tensor was expected");
     return THPVariable_Unpack(o);
 }
 Tensor tensor_or_none(PyObject *o) { return o == Py_None ? Tensor() : tensor(o); }
@@ -335,7 +335,7 @@ uint8_t *address(PyObject *o) {
 template <Tensor (*F)(PyObject *const *), Py_ssize_t N>
 PyObject *wrapped(PyObject *, PyObject *const *args, Py_ssize_t n) {
     HANDLE_TH_ERRORS
-    if (n != N) throw std::invalid_argument("wrong number of arguments");
+    TORCH_CHECK_VALUE(n == N, "wrong number of arguments");
     return THPVariable_Wrap(F(args));
     END_HANDLE_TH_ERRORS
 }

@@ -375,6 +375,15 @@ def test_a_captured_linear_replays(gpu, m):
 
 # ---------------------------------------------------------------------------------------- refusals
 
+def test_the_binding_takes_entries_that_the_library_has():
+    from xpu_kernels import _native
+    from xpu_kernels.int8 import _lib as L
+    assert {"xpuint8_" + name for name in _native.names()} - {"xpuint8_last_error"} <= set(L._signatures())
+    for call in (_native.quantize, _native.linear, _native.sort):
+        with pytest.raises(ValueError, match="arguments"):
+            call(1)
+
+
 def test_a_matrix_checks_its_buffers():
     codes, scales = torch.zeros((4, 32), dtype=torch.uint8), torch.zeros((1, 1, 32, 16), dtype=torch.uint8)
     assert xk.MXFP4(codes, scales, (4, 64)).shape == (4, 64)
