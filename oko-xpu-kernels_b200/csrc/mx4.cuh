@@ -73,16 +73,6 @@ __device__ __forceinline__ void mx_unpack2(uint32_t byte, float &lo, float &hi) 
         : "=f"(lo), "=f"(hi) : "r"(h));
 }
 
-// 16-bit and 32-bit element conversions
-template <int T>
-__device__ __forceinline__ float mx_load1(const void *p, int64_t i) {
-    if constexpr (T == kMxF32) return __ldg(static_cast<const float *>(p) + i);
-    const uint16_t h = __ldg(static_cast<const uint16_t *>(p) + i);
-    if constexpr (T == kMxBf16) return bf16_bits_to_f32(h);
-    float f;
-    asm("cvt.f32.f16 %0, %1;" : "=f"(f) : "h"(h));
-    return f;
-}
 // the two values of a 32-bit word of a 16-bit type
 template <int T>
 __device__ __forceinline__ void mx_split(uint32_t w, float &lo, float &hi) {
