@@ -7,10 +7,10 @@
 //   grad           dx = Q(dy) Q(w^T)^T, dw = Q(dy^T) Q(x^T)^T, each turned back where x and w were rotated
 //   expert_*       the same by expert, rows in the plan's order
 //
-// A rotated dx goes from the product to the rotation in fp32, and is rounded once: as a sum over a
-// token's experts it would be rounded three times otherwise (the error against 64 bits 1.9 times one
-// rounding's, measured).  dw is rounded to its type before the rotation and after (1.2 times): its
-// bytes, one matrix an expert, count more.
+// Rotated gradients go from the product to the rotation in fp32, and are rounded once.  Rounded to their
+// type before the rotation as well, dw's error against 64 bits is 1.41 times one rounding's (two
+// independent ones) and a dx summed over a token's experts 1.9 times; and a group's value before the
+// rotation can be 16 times the largest after it, which fp16 may not hold.
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -104,26 +104,25 @@ TrainWork train_work(Scratch &s, int64_t M, int64_t N, int64_t K) { return {take
 
 struct GradWork {
     Codes rows, cols;
-    float *dx;
-    uint8_t *dw;
+    float *dx, *dw;
 };
-GradWork grad_work(Scratch &s, int64_t M, int64_t N, int64_t K, int w_type, int rotate, int want) {
+GradWork grad_work(Scratch &s, int64_t M, int64_t N, int64_t K, int rotate, int want) {
     GradWork g{};
     if (want & 1) g.rows = take(s, M, N);
     if (want & 2) g.cols = take(s, N, M);
     if ((want & 1) && rotate) g.dx = reinterpret_cast<float *>(s.take(M * K * 4));
-    if ((want & 2) && rotate) g.dw = s.take(N * K * size_of(w_type));
+    if ((want & 2) && rotate) g.dw = reinterpret_cast<float *>(s.take(N * K * 4));
     return g;
 }
 // fp32 rows that are summed afterwards: 16-byte aligned, for the product's stores and the sum's loads (22544
 // rows of 850: 54 and 66 us packed)
 int64_t sum_pitch(int64_t K) { return (K + 3) / 4 * 4; }
-GradWork expert_grad_work(Scratch &s, int64_t rows, int64_t max_tiles, int64_t N, int64_t K, int64_t experts, int w_type, bool turn_dx, int rotate, int want) {
+GradWork expert_grad_work(Scratch &s, int64_t rows, int64_t max_tiles, int64_t N, int64_t K, int64_t experts, bool turn_dx, int rotate, int want) {
     GradWork g{};
     if (want & 1) g.rows = take_rows(s, rows, max_tiles, N);
     if (want & 2) g.cols = take(s, N, max_tiles * 128);
     if ((want & 1) && turn_dx) g.dx = reinterpret_cast<float *>(s.take(rows * sum_pitch(K) * 4));
-    if ((want & 2) && rotate) g.dw = s.take(experts * N * K * size_of(w_type));
+    if ((want & 2) && rotate) g.dw = reinterpret_cast<float *>(s.take(experts * N * K * 4));
     return g;
 }
 
@@ -219,10 +218,10 @@ int xpuint8_mxfp4_train_stream(const void *stream, const void *x, int32_t type, 
     return mx4_mm(s, q.x.codes, q.x.scales, q.w.codes, q.w.scales, bias, out, type, N, M, N, K, true);
 }
 
-int64_t xpuint8_mxfp4_grad_workspace_bytes(int64_t M, int64_t N, int64_t K, int32_t w_type, int32_t rotate, int32_t want) {
+int64_t xpuint8_mxfp4_grad_workspace_bytes(int64_t M, int64_t N, int64_t K, int32_t /*w_type*/, int32_t rotate, int32_t want) {
     if (M < 0 || N <= 0 || K <= 0) return -1;
     Scratch s(nullptr);
-    grad_work(s, M, N, K, w_type, rotate, want);
+    grad_work(s, M, N, K, rotate, want);
     return s.at;
 }
 
@@ -241,7 +240,7 @@ int xpuint8_mxfp4_grad_stream(const void *stream, const void *dy, int32_t type, 
     Scratch keep(const_cast<void *>(saved)), work(workspace);
     const TrainSaved t = train_saved(keep, M, N, K, want);
     const int have = (want_x ? 1 : 0) | (want_w ? 2 : 0);
-    const GradWork g = grad_work(work, M, N, K, w_type, rotate, have);
+    const GradWork g = grad_work(work, M, N, K, rotate, have);
     Mx4Both b;
     b.x = dy;
     b.type = type;
@@ -261,9 +260,9 @@ int xpuint8_mxfp4_grad_stream(const void *stream, const void *dy, int32_t type, 
     }
     if (want_w) {
         void *to = rotate ? static_cast<void *>(g.dw) : dw;
-        if (int rc = mx4_mm(s, g.cols.codes, g.cols.scales, t.x.codes, t.x.scales, nullptr, to, w_type, K, N, K, M, true)) return rc;
+        if (int rc = mx4_mm(s, g.cols.codes, g.cols.scales, t.x.codes, t.x.scales, nullptr, to, rotate ? 2 : w_type, K, N, K, M, true)) return rc;
         if (rotate)
-            if (int rc = mx4_quantize_rows(s, g.dw, w_type, K, nullptr, nullptr, dw, N, K, N, true)) return rc;
+            if (int rc = mx4_turn(s, g.dw, K, dw, w_type, N, K, nullptr, nullptr, 1, true)) return rc;
     }
     return 0;
 }
@@ -376,10 +375,10 @@ int xpuint8_mxfp4_expert_train_stream(const void *stream, const void *x, int32_t
 }
 
 int64_t xpuint8_mxfp4_expert_grad_workspace_bytes(int64_t rows, int64_t max_tiles, int64_t N, int64_t K, int64_t experts,
-                                                  int32_t w_type, int32_t rotate, int32_t sorted, int32_t want) {
+                                                  int32_t /*w_type*/, int32_t rotate, int32_t sorted, int32_t want) {
     if (rows < 0 || max_tiles < 0 || N <= 0 || K <= 0 || experts <= 0) return -1;
     Scratch s(nullptr);
-    expert_grad_work(s, rows, max_tiles, N, K, experts, w_type, rotate || !sorted, rotate, want);
+    expert_grad_work(s, rows, max_tiles, N, K, experts, rotate || !sorted, rotate, want);
     return s.at;
 }
 
@@ -405,7 +404,7 @@ int xpuint8_mxfp4_expert_grad_stream(const void *stream, const void *dy, int32_t
     const TrainSaved t = expert_saved(keep, max_tiles, N, K, experts, want);
     const bool turn_dx = rotate || !sorted;
     const int have = (want_x ? 1 : 0) | (want_w ? 2 : 0);
-    const GradWork g = expert_grad_work(work, rows, max_tiles, N, K, experts, w_type, turn_dx, rotate, have);
+    const GradWork g = expert_grad_work(work, rows, max_tiles, N, K, experts, turn_dx, rotate, have);
     if (want_w) {
         Mx4Both b;
         b.x = dy;
@@ -433,9 +432,9 @@ int xpuint8_mxfp4_expert_grad_stream(const void *stream, const void *dy, int32_t
     }
     if (want_w) {
         void *to = rotate ? static_cast<void *>(g.dw) : dw;
-        if (int rc = mx4_expert_dw(s, g.cols.codes, g.cols.scales, t.x.codes, t.x.scales, to, w_type, tiles, max_tiles, N, K, experts)) return rc;
+        if (int rc = mx4_expert_dw(s, g.cols.codes, g.cols.scales, t.x.codes, t.x.scales, to, rotate ? 2 : w_type, tiles, max_tiles, N, K, experts)) return rc;
         if (rotate)
-            if (int rc = mx4_quantize_rows(s, g.dw, w_type, K, nullptr, nullptr, dw, experts * N, K, experts * N, true)) return rc;
+            if (int rc = mx4_turn(s, g.dw, K, dw, w_type, experts * N, K, nullptr, nullptr, 1, true)) return rc;
     }
     return 0;
 }

@@ -377,6 +377,68 @@ def test_no_tokens(gpu):
     assert xk.expert_combine(y, torch.zeros((0, 2), device=DEV), plan).shape == (0, 32)
 
 
+# ------------------------------------------------------------------ the experts' gradients, rounded once
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("in_order", [False, True])
+@pytest.mark.parametrize("rotate", [False, True])
+@pytest.mark.parametrize("tokens,top,experts,n,k,dropped", [(7, 3, 9, 80, 256, 0.2), (300, 2, 3, 130, 512, 0.1), (150, 4, 4, 272, 256, 0)])
+def test_expert_gradients_are_rounded_once(gpu, tokens, top, experts, n, k, dropped, rotate, in_order, dtype):
+    """Against the formulas with one rounding to the type: the products' rows stay in fp32 up to a
+    token's sum and the rotation back."""
+    ids = routing(tokens, top, experts, 8, dropped)
+    plan = xk.expert_sort(torch.from_numpy(ids).to(DEV), experts)
+    order, _, offsets, _, _ = X.sort(ids, experts)
+    x, w = rand((tokens * top if in_order else tokens, k), 1, dtype), rand((experts, n, k), 2, dtype, 0.1)
+    dy = rand((tokens * top, n), 3, dtype, 0.1)
+    xd, wd = x.to(DEV).requires_grad_(), w.to(DEV).requires_grad_()
+    y = xk.mxfp4_expert_linear(xd, wd, plan, rotate=rotate, sorted=in_order)
+    dx, dw = torch.autograd.grad(y, (xd, wd), dy.to(DEV))
+    t = turned if rotate else (lambda v: v)
+    xs = f64(t(x)) if in_order else f64(t(x))[order // top]
+    d = f64(dy)
+    h = np.abs(O.hadamard_matrix().astype(np.float64))
+    groups = lambda v: (v.reshape(-1, 256) @ h).reshape(v.shape)  # noqa: E731
+
+    def one_rounding(got, ref, inner):
+        """`inner`: what is lost in 32 bits before the rotation (at most ten additions one after
+        another, sixteen allowed, each off by 2^-24 of a group's sum)."""
+        if rotate:
+            ref, inner = O.rotate_groups_dense_f64(ref), groups(inner) + 16 * 2.0 ** -24 * groups(np.abs(ref) + inner)
+        check(got, ref, 0 * ref, 0, dtype, inner * (1 + ROUND[dtype]))
+
+    gx, lost = np.zeros((tokens * top, k)), np.zeros((tokens * top, k))
+    for e in range(experts):
+        r = slice(offsets[e], offsets[e + 1])
+        we = f64(t(w[e]))
+        gx[r], spread = X.product(X.rounded(d[r]), X.rounded(we.T))
+        lost[r] = (n / 64 + 10) * 2.0 ** -23 * spread + 2.0 ** -24 * np.abs(gx[r])
+        if offsets[e] == offsets[e + 1]:
+            assert not f64(dw[e]).any()
+            continue
+        ref, spread = X.product(X.rounded(d[r].T), X.rounded(xs[r].T))
+        one_rounding(dw[e], ref, ((offsets[e + 1] - offsets[e]) / 64 + 10) * 2.0 ** -23 * spread + 2.0 ** -24 * np.abs(ref))
+    if in_order:
+        one_rounding(dx, gx, lost)
+    else:
+        one = np.ones((tokens, top))
+        total = X.combine(np.abs(gx) + lost, one, ids, experts)
+        one_rounding(dx, X.combine(gx, one, ids, experts), X.combine(lost, one, ids, experts) + top * 2.0 ** -24 * total)
+
+
+@pytest.mark.gpu
+def test_a_rotated_expert_gradient_keeps_fp16_s_range(gpu):
+    """A group of dw whose values are all 6144 is one value of 98304 before the rotation back, which
+    fp16 does not hold."""
+    sign = torch.from_numpy(O.hadamard_matrix()[37] * 16)
+    plan = xk.expert_sort(torch.tensor([[1]], device=DEV), 2)
+    x = (sign * 1024).to(torch.float16).reshape(1, 256).to(DEV)  # 16384 at place 37 of its rotation
+    w = torch.zeros((2, 3, 256), dtype=torch.float16, device=DEV, requires_grad=True)
+    dw, = torch.autograd.grad(xk.mxfp4_expert_linear(x, w, plan), w, torch.full((1, 3), 6.0, dtype=torch.float16, device=DEV))
+    assert torch.equal(dw[1].cpu(), (sign * 6144).to(torch.float16).expand(3, 256)) and not dw[0].any()
+
+
 # ---------------------------------------------------------------------------------------- refusals
 
 def test_ids_are_checked_before_the_device():

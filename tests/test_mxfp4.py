@@ -340,6 +340,43 @@ def test_tokens_over_a_contraction_of_several_turns(gpu, m, n, k, rotate):
             assert torch.equal(xk.linear_mxfp4(x, wq, rotate=rotate), want)
 
 
+# ---------------------------------------------------------------------- gradients turned back
+
+def turned_back(ref, spread, terms):
+    """A product turned back by the rotation, and what 32 bits lose before the one rounding to the
+    gradient's type: the running sums, the product's rounding to fp32, and the rotation's additions (at
+    most ten one after another, sixteen allowed, each off by 2^-24 of a group's sum)."""
+    h = np.abs(O.hadamard_matrix().astype(np.float64))
+    groups = lambda v: (v.reshape(-1, 256) @ h).reshape(v.shape)  # noqa: E731
+    inner = terms * 2.0 ** -23 * spread + 2.0 ** -24 * np.abs(ref)
+    return O.rotate_groups_dense_f64(ref), groups(inner) + 16 * 2.0 ** -24 * groups(np.abs(ref) + inner)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("m,n,k", [(1, 16, 256), (300, 272, 512), (513, 96, 768)])
+def test_a_rotated_gradient_is_rounded_once(gpu, m, n, k, dtype):
+    x, w, dy = rand((m, k), 1, dtype), rand((n, k), 2, dtype, 0.02), rand((m, n), 3, dtype, 0.1)
+    args = [v.to(DEV).requires_grad_() for v in (x, w)]
+    dx, dw = torch.autograd.grad(xk.mxfp4_linear(*args), args, dy.to(DEV))
+    xr, wr, d = f64(turned(x)), f64(turned(w)), f64(dy)
+    for got, product, contraction in ((dx, X.product(X.rounded(d), X.rounded(wr.T)), n), (dw, X.product(X.rounded(d.T), X.rounded(xr.T)), m)):
+        ref, extra = turned_back(*product, contraction / 64 + 10)
+        check(got, ref, 0 * ref, contraction, dtype, extra * (1 + ROUND[dtype]))
+
+
+@pytest.mark.gpu
+def test_a_rotated_gradient_keeps_fp16_s_range(gpu):
+    """A group of dw whose values are all 6144 is one value of 98304 before the rotation back, which
+    fp16 does not hold."""
+    sign = torch.from_numpy(O.hadamard_matrix()[37] * 16)
+    x = (sign * 1024).to(torch.float16).reshape(1, 256)  # 16384 at place 37 of its rotation
+    w = torch.zeros((3, 256), dtype=torch.float16)
+    xd, wd = x.to(DEV).requires_grad_(), w.to(DEV).requires_grad_()
+    dw, = torch.autograd.grad(xk.mxfp4_linear(xd, wd), wd, torch.full((1, 3), 6.0, dtype=torch.float16, device=DEV))
+    assert torch.equal(dw.cpu(), (sign * 6144).to(torch.float16).expand(3, 256))
+
+
 # ------------------------------------------------------------------------------ streams and graphs
 
 @pytest.mark.gpu
