@@ -18,6 +18,7 @@
 #include <c10/cuda/CUDAStream.h>
 
 #include <cstdint>
+#include <functional>
 #include <stdexcept>
 #include <string>
 
@@ -370,10 +371,25 @@ Tensor py_mm(PyObject *const *a) {
     return out;
 }
 
-// (x, codes, scales, n, bias or None, rotate)
-Tensor py_linear(PyObject *const *a) {
-    const Tensor &x = tensor(a[0]);
-    const int64_t n = integer(a[3]), k = x.size(-1), rotate = flag(a[5]);
+bool differentiates(const Tensor &x) { return x.defined() && x.requires_grad() && at::GradMode::is_enabled(); }
+
+// A product over a weight held in 4 bits has no backward, but its result depends on what asks for a
+// gradient.  So it joins the graph as a node that refuses: left out, a loss that reaches the same tensor by
+// another way as well gets a wrong gradient without a word.
+struct FrozenFn : torch::autograd::Function<FrozenFn> {
+    static Tensor forward(AutogradContext *ctx, const Tensor &, const std::optional<Tensor> &, const std::function<Tensor()> &product, const std::string &refusal) {
+        ctx->saved_data["refusal"] = refusal;
+        return product();
+    }
+    static variable_list backward(AutogradContext *ctx, variable_list) { throw std::runtime_error(ctx->saved_data["refusal"].toStringRef()); }
+};
+Tensor frozen(const Tensor &x, const Tensor &bias, const std::function<Tensor()> &product, const char *refusal) {
+    if (!differentiates(x) && !differentiates(bias)) return product();
+    return FrozenFn::apply(x, bias.defined() ? std::optional<Tensor>(bias) : std::nullopt, product, std::string(refusal));
+}
+
+Tensor linear(const Tensor &x, const uint8_t *codes, const uint8_t *scales, int64_t n, const Tensor &bias_in, bool rotate) {
+    const int64_t k = x.size(-1);
     at::AutoDispatchBelowADInplaceOrView below;
     int64_t ldx;
     const Tensor x2 = rows(x.dim() == 2 ? x : x.reshape({-1, k}), ldx);
@@ -386,11 +402,21 @@ Tensor py_linear(PyObject *const *a) {
         // up to 8 rows of whole 16-byte words are quantised inside the product, without scratch
         Tensor work;
         if (m > 8 || reinterpret_cast<uintptr_t>(x2.data_ptr()) % 16 || ldx * x2.element_size() % 16) work = scratch(lib.mxfp4_linear_workspace_bytes(m, k), x);
-        const Tensor bias = prepared_bias(tensor_or_none(a[4]), x);
-        check(lib.mxfp4_linear_stream(on.stream, x2.data_ptr(), type_of(x), ldx, address(a[1]), address(a[2]), bias_of(bias), out.data_ptr(), bytes(work), m, n, k, rotate),
-              "mxfp4_linear");
+        const Tensor bias = prepared_bias(bias_in, x);
+        check(lib.mxfp4_linear_stream(on.stream, x2.data_ptr(), type_of(x), ldx, codes, scales, bias_of(bias), out.data_ptr(), bytes(work), m, n, k, rotate), "mxfp4_linear");
     }
     return out;
+}
+
+// (x, codes, scales, n, bias or None, rotate)
+Tensor py_linear(PyObject *const *a) {
+    const Tensor &x = tensor(a[0]);
+    const Tensor bias = tensor_or_none(a[4]);
+    const uint8_t *codes = address(a[1]), *scales = address(a[2]);
+    const int64_t n = integer(a[3]);
+    const bool rotate = flag(a[5]);
+    return frozen(x, bias, [&] { return linear(x, codes, scales, n, bias, rotate); },
+                  "linear_mxfp4 has no backward, its weight is held in 4 bits: train with mxfp4_linear, or call it under torch.no_grad()");
 }
 
 // (x, w, bias or None, rotate)
@@ -402,8 +428,6 @@ Tensor py_train(PyObject *const *a) {
 }
 
 Tensor py_sort(PyObject *const *a) { return sorted_plan(tensor(a[0]), integer(a[1])); }
-
-bool differentiates(const Tensor &x) { return x.requires_grad() && at::GradMode::is_enabled(); }
 
 // (x, buffer, tokens, top, experts)
 Tensor py_gather(PyObject *const *a) {
@@ -419,13 +443,11 @@ Tensor py_combine(PyObject *const *a) {
     return differentiates(y) || differentiates(w) ? CombineFn::apply(y, w, p.buffer, p.tokens, p.top, p.experts) : combine(y, w, p);
 }
 
-// (x, codes, scales, n, buffer, tokens, top, experts, rotate, sorted)
-Tensor py_expert_linear(PyObject *const *a) {
+Tensor expert_linear(const Tensor &in, const uint8_t *codes, const uint8_t *scales, int64_t n, const Plan &p, bool rotate, bool sorted) {
     at::AutoDispatchBelowADInplaceOrView below;
     int64_t ldx;
-    const Tensor x = rows(tensor(a[0]), ldx);
-    const int64_t n = integer(a[3]), k = x.size(1);
-    const Plan p{tensor(a[4]), integer(a[5]), integer(a[6]), integer(a[7])};
+    const Tensor x = rows(in, ldx);
+    const int64_t k = x.size(1);
     Tensor out = empty({p.slots(), n}, x.scalar_type(), x);
     if (p.slots() && n) {
         On on(x);
@@ -433,11 +455,22 @@ Tensor py_expert_linear(PyObject *const *a) {
         Tensor work;
         if (p.slots() > 128 || reinterpret_cast<uintptr_t>(x.data_ptr()) % 16 || ldx * x.element_size() % 16)
             work = scratch(lib.mxfp4_expert_linear_workspace_bytes(p.slots(), p.max_tiles(), k), x);
-        check(lib.mxfp4_expert_linear_stream(on.stream, x.data_ptr(), type_of(x), ldx, address(a[1]), address(a[2]), out.data_ptr(), bytes(work), p.order(), p.positions(),
-                                             p.scale_rows(), p.offsets(), p.tiles(), p.tokens, p.top, p.max_tiles(), n, k, p.experts, flag(a[8]), flag(a[9])),
+        check(lib.mxfp4_expert_linear_stream(on.stream, x.data_ptr(), type_of(x), ldx, codes, scales, out.data_ptr(), bytes(work), p.order(), p.positions(), p.scale_rows(),
+                                             p.offsets(), p.tiles(), p.tokens, p.top, p.max_tiles(), n, k, p.experts, rotate, sorted),
               "mxfp4_expert_linear");
     }
     return out;
+}
+
+// (x, codes, scales, n, buffer, tokens, top, experts, rotate, sorted)
+Tensor py_expert_linear(PyObject *const *a) {
+    const Tensor &x = tensor(a[0]);
+    const uint8_t *codes = address(a[1]), *scales = address(a[2]);
+    const int64_t n = integer(a[3]);
+    const Plan p{tensor(a[4]), integer(a[5]), integer(a[6]), integer(a[7])};
+    const bool rotate = flag(a[8]), sorted = flag(a[9]);
+    return frozen(x, Tensor(), [&] { return expert_linear(x, codes, scales, n, p, rotate, sorted); },
+                  "expert_linear_mxfp4 has no backward, its weights are held in 4 bits: train with mxfp4_expert_linear, or call it under torch.no_grad()");
 }
 
 // (x, w, buffer, tokens, top, rotate, sorted)

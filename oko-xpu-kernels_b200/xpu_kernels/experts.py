@@ -140,7 +140,8 @@ def expert_linear_mxfp4(x, w, plan, *, rotate=True, sorted=False):
 
     ``x`` [T, K] holds the tokens, each quantised once and taken to its rows; with ``sorted`` it holds
     the plan's rows [T * k, K].  ``w`` is the MXFP4 stack [E, N, K] of :func:`prepare_weight_mxfp4`.
-    Rows of no expert are zero.
+    Rows of no expert are zero.  For serving: a backward pass that reaches the result raises
+    (:func:`mxfp4_expert_linear` has gradients).
     """
     _check_product(x, w.shape, plan, rotate, sorted)
     _type(x, "x")
@@ -167,7 +168,8 @@ def expert_ffn_mxfp4(x, ids, weights, up, down, *, rotate=True):
     """The experts' SwiGLU network: ``x`` [T, K] -> [T, K].
 
     ``ids`` and ``weights`` [T, k] are the router's; ``up`` is the MXFP4 stack [E, 2 F, K] with rows
-    ``[gate | up]``, ``down`` [E, K, F].
+    ``[gate | up]``, ``down`` [E, K, F].  For serving: ``weights`` may ask for a gradient, which
+    :func:`expert_combine` gives, but a backward pass to ``x`` raises (:func:`expert_linear_mxfp4`).
     """
     plan = expert_sort(ids, up.shape[0])
     gate, value = expert_linear_mxfp4(x, up, plan, rotate=rotate).chunk(2, dim=1)

@@ -186,7 +186,8 @@ def linear_mxfp4(x, w, bias=None, *, rotate=True):
     """The MXFP4 linear: ``x`` [.., K] (bf16, fp16, fp32) -> [.., N] of x's type.
 
     ``w`` is the :class:`MXFP4` weight [N, K] of :func:`prepare_weight_mxfp4`, ``rotate`` what it was
-    prepared with.  ``bias`` is added in 32 bits before the one rounding.
+    prepared with.  ``bias`` is added in 32 bits before the one rounding.  For serving: a backward pass
+    that reaches the result raises (:func:`mxfp4_linear` has gradients).
     """
     shape = x.shape
     if len(w.shape) != 2 or shape[-1] != w.shape[1]:
@@ -226,7 +227,7 @@ def mxfp4_linear(x, w, bias=None, *, rotate=True):
 
 
 class Mxfp4Linear(torch.nn.Module):
-    """``nn.Linear`` for serving with a prepared MXFP4 weight."""
+    """``nn.Linear`` for serving with a prepared MXFP4 weight (:func:`linear_mxfp4`: no gradients)."""
 
     def __init__(self, w, bias=None, *, rotate=True):
         super().__init__()

@@ -439,6 +439,40 @@ def test_a_rotated_expert_gradient_keeps_fp16_s_range(gpu):
     assert torch.equal(dw[1].cpu(), (sign * 6144).to(torch.float16).expand(3, 256)) and not dw[0].any()
 
 
+# --------------------------------------------------------------------- what has no gradient says so
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("tokens", [5, 200])
+def test_frozen_experts_have_no_backward_and_say_so(gpu, tokens):
+    ids = torch.from_numpy(routing(tokens, 2, 4, 5, 0.1)).to(DEV)
+    plan = xk.expert_sort(ids, 4)
+    x, weights = rand((tokens, 256), 1).to(DEV), torch.softmax(rand((tokens, 2), 2, torch.float32), -1).to(DEV)
+    up = xk.prepare_weight_mxfp4(rand((4, 512, 256), 3, scale=0.05).to(DEV))
+    down = xk.prepare_weight_mxfp4(rand((4, 256, 256), 4, scale=0.05).to(DEV))
+    want = xk.expert_linear_mxfp4(x, up, plan)
+    xg = x.clone().requires_grad_()
+    y = xk.expert_linear_mxfp4(xg, up, plan)
+    assert torch.equal(y, want) and y.requires_grad and not want.requires_grad
+    for loss in (y.sum(), xk.expert_linear_mxfp4(xg, up, plan).sum() + xg.sum()):
+        with pytest.raises(RuntimeError, match="mxfp4_expert_linear"):
+            torch.autograd.grad(loss, xg)
+    with torch.no_grad():
+        assert not xk.expert_linear_mxfp4(xg, up, plan).requires_grad
+    # the network: the router's gradient is there, a token's is refused
+    wg = weights.clone().requires_grad_()
+    out = xk.expert_ffn_mxfp4(x, ids, wg, up, down)
+    assert torch.equal(out, xk.expert_ffn_mxfp4(x, ids, weights, up, down))
+    gw, = torch.autograd.grad(out, wg, torch.ones_like(out))
+    h = xk.expert_linear_mxfp4(x, up, plan).chunk(2, dim=1)
+    y = xk.expert_linear_mxfp4(torch.nn.functional.silu(h[0]) * h[1], down, plan, sorted=True)
+    again = weights.clone().requires_grad_()
+    assert torch.equal(gw, torch.autograd.grad(xk.expert_combine(y, again, plan), again, torch.ones_like(out))[0])
+    out = xk.expert_ffn_mxfp4(xg, ids, wg, up, down)
+    assert torch.equal(torch.autograd.grad(out.sum(), wg, retain_graph=True)[0], gw)
+    with pytest.raises(RuntimeError, match="mxfp4_expert_linear"):
+        (out + xg).sum().backward()
+
+
 # ---------------------------------------------------------------------------------------- refusals
 
 def test_ids_are_checked_before_the_device():

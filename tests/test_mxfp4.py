@@ -377,6 +377,31 @@ def test_a_rotated_gradient_keeps_fp16_s_range(gpu):
     assert torch.equal(dw.cpu(), (sign * 6144).to(torch.float16).expand(3, 256))
 
 
+# --------------------------------------------------------------------- what has no gradient says so
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m", [1, 40])
+def test_a_frozen_weight_s_linear_has_no_backward_and_says_so(gpu, m):
+    x, bias = rand((m, 256), 1).to(DEV), rand((96,), 3, torch.float32).to(DEV)
+    w = xk.prepare_weight_mxfp4(rand((96, 256), 2).to(DEV))
+    want = xk.linear_mxfp4(x, w, bias)
+    assert not want.requires_grad
+    for xg, bg in ((x.clone().requires_grad_(), bias), (x, bias.clone().requires_grad_()), (x.clone().requires_grad_(), None)):
+        at = xg if xg.requires_grad else bg
+        y = xk.linear_mxfp4(xg, w, bg)
+        assert y.requires_grad and (bg is None or torch.equal(y, want))
+        with pytest.raises(RuntimeError, match="mxfp4_linear"):
+            torch.autograd.grad(y.sum(), at, retain_graph=True)
+        with pytest.raises(RuntimeError, match="mxfp4_linear"):  # beside another way to the same tensor
+            torch.autograd.grad(y.sum() + at.sum(), at)
+        with torch.no_grad():
+            assert not xk.linear_mxfp4(xg, w, bg).requires_grad
+    module = xk.Mxfp4Linear(w, bias)
+    with pytest.raises(RuntimeError, match="mxfp4_linear"):
+        module(x.clone().requires_grad_()).sum().backward()
+    assert torch.equal(module(x), want)
+
+
 # ------------------------------------------------------------------------------ streams and graphs
 
 @pytest.mark.gpu
