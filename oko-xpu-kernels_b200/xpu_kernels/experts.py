@@ -101,12 +101,12 @@ def expert_gather(x, plan):
 
 
 def expert_combine(y, weights, plan):
-    """``y`` [T * k, W] in the plan's order and ``weights`` [T, k] -> [T, W]: each token's rows times
-    its weights, summed in 32 bits.  Differentiable in both."""
+    """``y`` [T * k, W] in the plan's order and ``weights`` [T, k] (or [T * k], a value a slot) -> [T, W]:
+    each token's rows times its weights, summed in 32 bits.  Differentiable in both."""
     if y.dim() != 2 or y.shape[0] != plan.rows:
         raise ValueError(f"y must be [{plan.rows}, W], got {tuple(y.shape)}")
     shape = (plan.tokens, plan.top)
-    if weights.shape != shape and weights.numel() != plan.rows:
+    if weights.shape != shape and weights.shape != (plan.rows,):
         raise ValueError(f"weights must be [{plan.tokens}, {plan.top}], got {tuple(weights.shape)}")
     _same_device(y.get_device(), plan, y, "y")
     _same_device(weights.get_device(), plan, weights, "weights")

@@ -186,6 +186,19 @@ def test_offsets_past_32_bits(gpu):
     assert back[:, -1].tolist() == list(range(1, tokens + 1))
 
 
+@pytest.mark.gpu
+def test_weights_are_by_token_and_choice(gpu):
+    plan = xk.expert_sort(torch.zeros((4, 2), dtype=torch.int32, device=DEV), 4)
+    y, w = rand((8, 64), 1).to(DEV), rand((4, 2), 2, torch.float32).to(DEV)
+    want = xk.expert_combine(y, w, plan)
+    assert torch.equal(xk.expert_combine(y, w.reshape(8), plan), want)  # a value a slot
+    for wrong in (w.T, w.T.contiguous(), w.reshape(1, 8), w.reshape(8, 1), w.reshape(2, 2, 2)):
+        with pytest.raises(ValueError, match=r"weights must be \[4, 2\]"):
+            xk.expert_combine(y, wrong, plan)
+    one = xk.expert_sort(torch.zeros(8, dtype=torch.int32, device=DEV), 4)
+    assert torch.equal(xk.expert_combine(y, w.reshape(8), one), xk.expert_combine(y, w.reshape(8, 1), one))
+
+
 # --------------------------------------------------------------------------- the experts' product
 
 #: tokens, top, experts, N, K, dropped, the experts that are chosen from (None: all)
