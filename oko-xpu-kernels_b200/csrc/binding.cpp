@@ -336,7 +336,7 @@ uint8_t *address(PyObject *o) {
 template <Tensor (*F)(PyObject *const *), Py_ssize_t N>
 PyObject *wrapped(PyObject *, PyObject *const *args, Py_ssize_t n) {
     HANDLE_TH_ERRORS
-    TORCH_CHECK_VALUE(n == N, "wrong number of arguments");
+    TORCH_CHECK_VALUE(n == N, "expected ", N, " arguments, got ", n);
     return THPVariable_Wrap(F(args));
     END_HANDLE_TH_ERRORS
 }

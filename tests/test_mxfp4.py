@@ -446,6 +446,15 @@ def test_the_binding_takes_entries_that_the_library_has():
             call(1)
 
 
+def test_the_binding_formats_its_errors():
+    """By streams, which crash in a module that is linked with a C++ runtime of its own."""
+    from xpu_kernels import _native
+    with pytest.raises(ValueError, match="expected 3 arguments, got 1"):
+        _native.quantize(1)
+    with pytest.raises(ValueError, match="expected 2 arguments, got 0"):
+        _native.sort()
+
+
 def test_a_matrix_checks_its_buffers():
     codes, scales = torch.zeros((4, 32), dtype=torch.uint8), torch.zeros((1, 1, 32, 16), dtype=torch.uint8)
     assert xk.MXFP4(codes, scales, (4, 64)).shape == (4, 64)
