@@ -327,10 +327,32 @@ bool flag(PyObject *o) {
     if (v < 0) throw py::error_already_set();
     return v;
 }
-uint8_t *address(PyObject *o) {
+void *address(PyObject *o) {
     void *p = PyLong_AsVoidPtr(o);
     if (!p && PyErr_Occurred()) throw py::error_already_set();
-    return static_cast<uint8_t *>(p);
+    return p;
+}
+
+// An MXFP4 matrix [r, k], or a stack of n: two objects from Python, its codes and its scales, or the buffer
+// that holds both and where the scales begin.  Looked at on every call, never kept as addresses: who holds the
+// tensors can give them other memory.
+struct Matrix {
+    const uint8_t *codes, *scales;
+};
+const uint8_t *held(const char *what, const Tensor &t, int64_t at, int64_t bytes, const Tensor &like) {
+    TORCH_CHECK_VALUE(t.scalar_type() == at::kByte && t.is_contiguous() && t.device() == like.device() && t.numel() >= at + bytes &&
+                          static_cast<int64_t>(t.storage().nbytes()) >= t.storage_offset() + at + bytes,
+                      "the ", what, " of an MXFP4 matrix were changed: expected ", bytes, " contiguous bytes on ", like.device());
+    return bytes ? static_cast<const uint8_t *>(t.data_ptr()) + at : nullptr;
+}
+Matrix matrix(PyObject *codes, PyObject *scales, int64_t n, int64_t r, int64_t k, const Tensor &like) {
+    const int64_t code_bytes = n * r * ((k + 31) / 32) * 16, scale_bytes = n * ((r + 127) / 128) * ((k + 127) / 128) * 512;
+    const Tensor &c = tensor(codes);
+    if (PyLong_Check(scales)) return {held("codes", c, 0, code_bytes, like), held("scales", c, integer(scales), scale_bytes, like)};
+    const Tensor &s = tensor(scales);
+    TORCH_CHECK_VALUE(c.numel() == code_bytes && s.numel() == scale_bytes, "the codes or the scales of an MXFP4 matrix were changed: expected ", code_bytes, " and ",
+                      scale_bytes, " bytes, got ", c.numel(), " and ", s.numel());
+    return {held("codes", c, 0, code_bytes, like), held("scales", s, 0, scale_bytes, like)};
 }
 
 template <Tensor (*F)(PyObject *const *), Py_ssize_t N>
@@ -343,30 +365,33 @@ PyObject *wrapped(PyObject *, PyObject *const *args, Py_ssize_t n) {
 
 Tensor py_quantize(PyObject *const *a) { return quantize(tensor(a[0]), flag(a[1]), flag(a[2])); }
 
-// (codes, scales, rows of a matrix, type, a tensor on the device, shape)
+// (codes, scales, type, shape)
 Tensor py_dequantize(PyObject *const *a) {
-    const int64_t each = integer(a[2]), type = integer(a[3]);
-    const Tensor &like = tensor(a[4]);
+    const Tensor &like = tensor(a[0]);
+    const int64_t type = integer(a[2]);
     std::vector<int64_t> shape;
-    for (Py_ssize_t i = 0; i < PyTuple_GET_SIZE(a[5]); ++i) shape.push_back(integer(PyTuple_GET_ITEM(a[5], i)));
+    for (Py_ssize_t i = 0; i < PyTuple_GET_SIZE(a[3]); ++i) shape.push_back(integer(PyTuple_GET_ITEM(a[3], i)));
+    const int64_t each = shape[shape.size() - 2], k = shape.back();
     Tensor out = empty(shape, scalar_type(type), like);
     const int64_t n = out.numel();
     if (n) {
+        const Matrix q = matrix(a[0], a[1], n / k / each, each, k, like);
         On on(like);
-        check(lib.mxfp4_dequantize_stream(on.stream, address(a[0]), address(a[1]), out.data_ptr(), type, n / shape.back(), shape.back(), each), "mxfp4_dequantize");
+        check(lib.mxfp4_dequantize_stream(on.stream, q.codes, q.scales, out.data_ptr(), type, n / k, k, each), "mxfp4_dequantize");
     }
     return out;
 }
 
-// (a codes, a scales, b codes, b scales, bias or None, type, m, n, k, a tensor on the device)
+// (a codes, a scales, b codes, b scales, bias or None, type, m, n, k)
 Tensor py_mm(PyObject *const *a) {
     const int64_t type = integer(a[5]), m = integer(a[6]), n = integer(a[7]), k = integer(a[8]);
-    const Tensor &like = tensor(a[9]);
+    const Tensor &like = tensor(a[0]);
     Tensor out = empty({m, n}, scalar_type(type), like);
     if (m && n) {
+        const Matrix p = matrix(a[0], a[1], 1, m, k, like), q = matrix(a[2], a[3], 1, n, k, like);
         On on(like);
         const Tensor bias = prepared_bias(tensor_or_none(a[4]), like);
-        check(lib.mxfp4_mm_stream(on.stream, address(a[0]), address(a[1]), address(a[2]), address(a[3]), bias_of(bias), out.data_ptr(), type, n, m, n, k), "mxfp4_mm");
+        check(lib.mxfp4_mm_stream(on.stream, p.codes, p.scales, q.codes, q.scales, bias_of(bias), out.data_ptr(), type, n, m, n, k), "mxfp4_mm");
     }
     return out;
 }
@@ -388,7 +413,7 @@ Tensor frozen(const Tensor &x, const Tensor &bias, const std::function<Tensor()>
     return FrozenFn::apply(x, bias.defined() ? std::optional<Tensor>(bias) : std::nullopt, product, std::string(refusal));
 }
 
-Tensor linear(const Tensor &x, const uint8_t *codes, const uint8_t *scales, int64_t n, const Tensor &bias_in, bool rotate) {
+Tensor linear(const Tensor &x, const Matrix &w, int64_t n, const Tensor &bias_in, bool rotate) {
     const int64_t k = x.size(-1);
     at::AutoDispatchBelowADInplaceOrView below;
     int64_t ldx;
@@ -403,7 +428,7 @@ Tensor linear(const Tensor &x, const uint8_t *codes, const uint8_t *scales, int6
         Tensor work;
         if (m > 8 || reinterpret_cast<uintptr_t>(x2.data_ptr()) % 16 || ldx * x2.element_size() % 16) work = scratch(lib.mxfp4_linear_workspace_bytes(m, k), x);
         const Tensor bias = prepared_bias(bias_in, x);
-        check(lib.mxfp4_linear_stream(on.stream, x2.data_ptr(), type_of(x), ldx, codes, scales, bias_of(bias), out.data_ptr(), bytes(work), m, n, k, rotate), "mxfp4_linear");
+        check(lib.mxfp4_linear_stream(on.stream, x2.data_ptr(), type_of(x), ldx, w.codes, w.scales, bias_of(bias), out.data_ptr(), bytes(work), m, n, k, rotate), "mxfp4_linear");
     }
     return out;
 }
@@ -412,10 +437,10 @@ Tensor linear(const Tensor &x, const uint8_t *codes, const uint8_t *scales, int6
 Tensor py_linear(PyObject *const *a) {
     const Tensor &x = tensor(a[0]);
     const Tensor bias = tensor_or_none(a[4]);
-    const uint8_t *codes = address(a[1]), *scales = address(a[2]);
     const int64_t n = integer(a[3]);
+    const Matrix w = matrix(a[1], a[2], 1, n, x.size(-1), x);
     const bool rotate = flag(a[5]);
-    return frozen(x, bias, [&] { return linear(x, codes, scales, n, bias, rotate); },
+    return frozen(x, bias, [&] { return linear(x, w, n, bias, rotate); },
                   "linear_mxfp4 has no backward, its weight is held in 4 bits: train with mxfp4_linear, or call it under torch.no_grad()");
 }
 
@@ -443,7 +468,7 @@ Tensor py_combine(PyObject *const *a) {
     return differentiates(y) || differentiates(w) ? CombineFn::apply(y, w, p.buffer, p.tokens, p.top, p.experts) : combine(y, w, p);
 }
 
-Tensor expert_linear(const Tensor &in, const uint8_t *codes, const uint8_t *scales, int64_t n, const Plan &p, bool rotate, bool sorted) {
+Tensor expert_linear(const Tensor &in, const Matrix &w, int64_t n, const Plan &p, bool rotate, bool sorted) {
     at::AutoDispatchBelowADInplaceOrView below;
     int64_t ldx;
     const Tensor x = rows(in, ldx);
@@ -455,7 +480,7 @@ Tensor expert_linear(const Tensor &in, const uint8_t *codes, const uint8_t *scal
         Tensor work;
         if (p.slots() > 128 || reinterpret_cast<uintptr_t>(x.data_ptr()) % 16 || ldx * x.element_size() % 16)
             work = scratch(lib.mxfp4_expert_linear_workspace_bytes(p.slots(), p.max_tiles(), k), x);
-        check(lib.mxfp4_expert_linear_stream(on.stream, x.data_ptr(), type_of(x), ldx, codes, scales, out.data_ptr(), bytes(work), p.order(), p.positions(), p.scale_rows(),
+        check(lib.mxfp4_expert_linear_stream(on.stream, x.data_ptr(), type_of(x), ldx, w.codes, w.scales, out.data_ptr(), bytes(work), p.order(), p.positions(), p.scale_rows(),
                                              p.offsets(), p.tiles(), p.tokens, p.top, p.max_tiles(), n, k, p.experts, rotate, sorted),
               "mxfp4_expert_linear");
     }
@@ -465,11 +490,11 @@ Tensor expert_linear(const Tensor &in, const uint8_t *codes, const uint8_t *scal
 // (x, codes, scales, n, buffer, tokens, top, experts, rotate, sorted)
 Tensor py_expert_linear(PyObject *const *a) {
     const Tensor &x = tensor(a[0]);
-    const uint8_t *codes = address(a[1]), *scales = address(a[2]);
     const int64_t n = integer(a[3]);
     const Plan p{tensor(a[4]), integer(a[5]), integer(a[6]), integer(a[7])};
+    const Matrix w = matrix(a[1], a[2], p.experts, n, x.size(1), x);
     const bool rotate = flag(a[8]), sorted = flag(a[9]);
-    return frozen(x, Tensor(), [&] { return expert_linear(x, codes, scales, n, p, rotate, sorted); },
+    return frozen(x, Tensor(), [&] { return expert_linear(x, w, n, p, rotate, sorted); },
                   "expert_linear_mxfp4 has no backward, its weights are held in 4 bits: train with mxfp4_expert_linear, or call it under torch.no_grad()");
 }
 
@@ -487,7 +512,7 @@ PyObject *py_bind(PyObject *, PyObject *dict) {
     {                                                                                          \
         PyObject *v = PyDict_GetItemString(dict, #name);                                       \
         if (!v) throw std::runtime_error("the library has no entry " #name);                   \
-        lib.name = reinterpret_cast<decltype(lib.name)>(reinterpret_cast<void *>(address(v))); \
+        lib.name = reinterpret_cast<decltype(lib.name)>(address(v)); \
     }
     ENTRIES(BIND)
     Py_RETURN_NONE;
@@ -504,7 +529,7 @@ PyObject *py_names(PyObject *, PyObject *) {
 }
 
 #define FAST(name, n) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void *>(&wrapped<py_##name, n>)), METH_FASTCALL, nullptr}
-PyMethodDef methods[] = {FAST(quantize, 3), FAST(dequantize, 6), FAST(mm, 10), FAST(linear, 6), FAST(train, 4), FAST(sort, 2), FAST(gather, 5), FAST(combine, 6),
+PyMethodDef methods[] = {FAST(quantize, 3), FAST(dequantize, 4), FAST(mm, 9), FAST(linear, 6), FAST(train, 4), FAST(sort, 2), FAST(gather, 5), FAST(combine, 6),
                          FAST(expert_linear, 10), FAST(expert_train, 7), {"bind", py_bind, METH_O, nullptr}, {"names", py_names, METH_NOARGS, nullptr},
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_native", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

@@ -145,9 +145,10 @@ def expert_linear_mxfp4(x, w, plan, *, rotate=True, sorted=False):
     """
     _check_product(x, w.shape, plan, rotate, sorted)
     _type(x, "x")
-    if w._index != plan._index:
+    codes, scales = w._held
+    if codes.get_device() != plan._index:
         raise ValueError(f"the weight is on {w.device} and the plan on {plan._buffer.device}")
-    return (mxfp4._native or _load()).expert_linear(x, w._cp, w._sp, w.shape[1], plan._buffer, plan.tokens, plan.top,
+    return (mxfp4._native or _load()).expert_linear(x, codes, scales, w.shape[1], plan._buffer, plan.tokens, plan.top,
                                                     plan.num_experts, rotate, sorted)
 
 

@@ -64,7 +64,7 @@ class MXFP4:
     aligned, so they can be saved and loaded as they are.
     """
 
-    __slots__ = ("shape", "_codes", "_scales", "_buffer", "_at", "_cp", "_sp", "_index")
+    __slots__ = ("shape", "_codes", "_scales", "_buffer", "_at")
 
     def __init__(self, codes, scales, shape):
         if len(shape) == 2:
@@ -81,26 +81,34 @@ class MXFP4:
         if codes.shape != want_codes or scales.shape != want_scales:
             raise ValueError(f"an MXFP4 matrix {tuple(shape)} has codes {want_codes} and scales {want_scales}, "
                              f"got {tuple(codes.shape)} and {tuple(scales.shape)}")
-        index = codes.get_device()
-        if index != scales.get_device():
+        if codes.get_device() != scales.get_device():
             raise ValueError(f"codes are on {codes.device} and scales on {scales.device}")
         if not codes.is_contiguous() or not scales.is_contiguous():
             raise ValueError("codes and scales must be contiguous")
         self.shape = tuple(shape)
-        self._codes, self._scales, self._index = codes, scales, index
-        self._cp, self._sp = codes.data_ptr(), scales.data_ptr()
+        self._codes, self._scales, self._buffer, self._at = codes, scales, None, 0
 
     @classmethod
-    def _of(cls, buffer, shape, index):
+    def _of(cls, buffer, shape):
         """The matrix whose codes and then scales are in `buffer`; they become tensors when asked for."""
         r, k = shape[-2:]
         n = shape[0] if len(shape) == 3 else 1
         q = cls.__new__(cls)
-        q.shape, q._buffer, q._codes, q._scales, q._index = tuple(shape), buffer, None, None, index
+        q.shape, q._buffer, q._codes, q._scales = tuple(shape), buffer, None, None
         q._at = (n * r * ((k + 31) // 32 * 16) + 255) // 256 * 256
-        q._cp = buffer.data_ptr()
-        q._sp = q._cp + q._at
         return q
+
+    # What the binding takes: the codes and the scales, or, before either became a tensor, the buffer and
+    # where its scales begin.  Addresses are taken at the call alone.
+    @property
+    def _held(self):
+        if self._codes is None and self._scales is None:
+            return self._buffer, self._at
+        return self.codes, self.scales
+
+    @property
+    def _index(self):
+        return self._held[0].get_device()
 
     @property
     def codes(self):
@@ -140,7 +148,7 @@ def quantize_mxfp4(x, *, rotate=False, transpose=False):
         _check_rotate(shape[-1], rotate)
     _type(x, "x")
     buffer = (_native or _load()).quantize(x.detach() if x.requires_grad else x, rotate, transpose)
-    return MXFP4._of(buffer, (*shape[:-2], shape[-1], shape[-2]) if transpose else shape, x.get_device())
+    return MXFP4._of(buffer, (*shape[:-2], shape[-1], shape[-2]) if transpose else shape)
 
 
 def dequantize_mxfp4(q, dtype=torch.bfloat16):
@@ -150,8 +158,7 @@ def dequantize_mxfp4(q, dtype=torch.bfloat16):
         raise TypeError(f"dtype must be bfloat16, float16 or float32, got {dtype}")
     if q._index < 0:
         raise TypeError(f"q must be on a CUDA device, got {q.device}")
-    buffer = q._buffer if q._codes is None else q._codes
-    return (_native or _load()).dequantize(q._cp, q._sp, q.shape[-2], t, buffer, q.shape)
+    return (_native or _load()).dequantize(*q._held, t, q.shape)
 
 
 def prepare_weight_mxfp4(w, rotate=True):
@@ -174,12 +181,13 @@ def mxfp4_mm(a, b, bias=None, dtype=torch.bfloat16):
     t = _TYPES.get(dtype)
     if t is None:
         raise TypeError(f"dtype must be bfloat16, float16 or float32, got {dtype}")
-    if a._index != b._index:
+    index = a._index
+    if index != b._index:
         raise ValueError(f"a is on {a.device} and b on {b.device}")
-    if a._index < 0:
+    if index < 0:
         raise TypeError(f"a and b must be on a CUDA device, got {a.device}")
     _check_bias(bias, n)
-    return (_native or _load()).mm(a._cp, a._sp, b._cp, b._sp, bias, t, m, n, k, a._buffer if a._codes is None else a._codes)
+    return (_native or _load()).mm(*a._held, *b._held, bias, t, m, n, k)
 
 
 def linear_mxfp4(x, w, bias=None, *, rotate=True):
@@ -192,8 +200,8 @@ def linear_mxfp4(x, w, bias=None, *, rotate=True):
     shape = x.shape
     if len(w.shape) != 2 or shape[-1] != w.shape[1]:
         raise ValueError(f"x has {shape[-1]} columns and the weight is {w.shape}")
-    index = x.get_device()
-    if index != w._index:
+    codes, scales = w._held
+    if x.get_device() != codes.get_device():
         raise ValueError(f"x is on {x.device} and the weight on {w.device}")
     n, k = w.shape
     if rotate and k % 256:
@@ -201,7 +209,7 @@ def linear_mxfp4(x, w, bias=None, *, rotate=True):
     _type(x, "x")
     if bias is not None:
         _check_bias(bias, n)
-    return (_native or _load()).linear(x, w._cp, w._sp, n, bias, rotate)
+    return (_native or _load()).linear(x, codes, scales, n, bias, rotate)
 
 
 def mxfp4_linear(x, w, bias=None, *, rotate=True):

@@ -486,6 +486,22 @@ def test_frozen_experts_have_no_backward_and_say_so(gpu, tokens):
         (out + xg).sum().backward()
 
 
+@pytest.mark.gpu
+def test_the_experts_weights_are_read_where_their_tensors_are(gpu):
+    plan = xk.expert_sort(torch.from_numpy(routing(9, 2, 3, 5)).to(DEV), 3)
+    x = rand((9, 256), 1).to(DEV)
+    q, other = (xk.prepare_weight_mxfp4(rand((3, 96, 256), seed).to(DEV)) for seed in (2, 3))
+    want = xk.expert_linear_mxfp4(x, other, plan)
+    q.codes.data, q.scales.data = other.codes.clone(), other.scales.clone()
+    assert torch.equal(xk.expert_linear_mxfp4(x, q, plan), want)
+    q.codes.untyped_storage().resize_(0)
+    with pytest.raises(ValueError, match="codes"):
+        xk.expert_linear_mxfp4(x, q, plan)
+    q.codes.data = other.codes[:2]
+    with pytest.raises(ValueError, match="codes"):
+        xk.expert_linear_mxfp4(x, q, plan)
+
+
 # ---------------------------------------------------------------------------------------- refusals
 
 def test_ids_are_checked_before_the_device():

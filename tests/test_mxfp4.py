@@ -402,6 +402,57 @@ def test_a_frozen_weight_s_linear_has_no_backward_and_says_so(gpu, m):
     assert torch.equal(module(x), want)
 
 
+# ------------------------------------------------------------------------- matrices whose memory changes
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("made", ["by the quantiser", "from tensors"])
+def test_a_matrix_is_read_where_its_tensors_are(gpu, made):
+    x = rand((5, 256), 1).to(DEV)
+    first, other = (xk.prepare_weight_mxfp4(rand((96, 256), seed).to(DEV)) for seed in (2, 3))
+    want, values = xk.linear_mxfp4(x, other), xk.dequantize_mxfp4(other)
+    product = xk.mxfp4_mm(other, other)
+    q = first if made == "by the quantiser" else xk.MXFP4(first.codes.clone(), first.scales.clone(), first.shape)
+    q.codes.data = other.codes.clone()
+    q.scales.set_(other.scales.clone())
+    assert torch.equal(xk.linear_mxfp4(x, q), want) and torch.equal(xk.dequantize_mxfp4(q), values)
+    assert torch.equal(xk.mxfp4_mm(q, q), product)
+    calls = (lambda: xk.linear_mxfp4(x, q), lambda: xk.dequantize_mxfp4(q), lambda: xk.mxfp4_mm(q, other), lambda: xk.mxfp4_mm(other, q))
+    codes = q.codes.clone()
+
+    def refused():
+        for call in calls:
+            with pytest.raises(ValueError, match="codes|is on|are on"):
+                call()
+
+    q.codes.untyped_storage().resize_(0)
+    refused()
+    for wrong in (codes[:95], codes.to(torch.int16), codes.T, torch.zeros((97, 128), dtype=torch.uint8, device=DEV)):
+        q.codes.data = wrong
+        refused()
+    q.codes.data = codes.cpu()
+    with pytest.raises((ValueError, TypeError)):
+        xk.linear_mxfp4(x, q)
+    q.codes.data = codes
+    assert torch.equal(xk.linear_mxfp4(x, q), want)
+
+
+@pytest.mark.gpu
+def test_copies_of_a_matrix_are_their_own(gpu):
+    import copy
+    import io
+    x, q = rand((5, 256), 1).to(DEV), xk.prepare_weight_mxfp4(rand((96, 256), 2).to(DEV))
+    want = xk.linear_mxfp4(x, q)
+    file = io.BytesIO()
+    torch.save(q, file)
+    copies = [copy.deepcopy(q), torch.load(io.BytesIO(file.getvalue()), weights_only=False)]
+    q.codes, q.scales
+    copies.append(copy.deepcopy(q))
+    q.codes.zero_()
+    q.scales.zero_()
+    for c in copies:
+        assert c.shape == q.shape and torch.equal(xk.linear_mxfp4(x, c), want)
+
+
 # ------------------------------------------------------------------------------ streams and graphs
 
 @pytest.mark.gpu
