@@ -10,6 +10,7 @@
 // C entries report is raised.
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/extension.h>
 
@@ -396,7 +397,10 @@ Tensor py_mm(PyObject *const *a) {
     return out;
 }
 
-bool differentiates(const Tensor &x) { return x.defined() && x.requires_grad() && at::GradMode::is_enabled(); }
+// In either mode; forward-mode tangents are refused by the nodes' apply, where they would be lost below it.
+bool differentiates(const Tensor &x) {
+    return x.defined() && ((x.requires_grad() && at::GradMode::is_enabled()) || torch::autograd::isFwGradDefined(x));
+}
 
 // A product over a weight held in 4 bits has no backward, but its result depends on what asks for a
 // gradient.  So it joins the graph as a node that refuses: left out, a loss that reaches the same tensor by

@@ -487,6 +487,21 @@ def test_frozen_experts_have_no_backward_and_say_so(gpu, tokens):
 
 
 @pytest.mark.gpu
+def test_forward_mode_is_refused(gpu):
+    from torch.autograd import forward_ad as fw
+    plan = xk.expert_sort(torch.zeros((4, 2), dtype=torch.int32, device=DEV), 2)
+    x, y, weights = rand((4, 64), 1).to(DEV), rand((8, 64), 2).to(DEV), torch.ones((4, 2), device=DEV)
+    w = xk.quantize_mxfp4(rand((2, 32, 64), 3).to(DEV))
+    with fw.dual_level():
+        dual = lambda v: fw.make_dual(v, torch.ones_like(v))  # noqa: E731
+        for call in (lambda: xk.expert_gather(dual(x), plan), lambda: xk.expert_combine(dual(y), weights, plan),
+                     lambda: xk.expert_combine(y, dual(weights), plan), lambda: xk.expert_linear_mxfp4(dual(x), w, plan, rotate=False),
+                     lambda: xk.mxfp4_expert_linear(dual(x), torch.ones((2, 32, 64), device=DEV), plan, rotate=False)):
+            with pytest.raises(RuntimeError, match="jvp|forward AD"):
+                call()
+
+
+@pytest.mark.gpu
 def test_the_experts_weights_are_read_where_their_tensors_are(gpu):
     plan = xk.expert_sort(torch.from_numpy(routing(9, 2, 3, 5)).to(DEV), 3)
     x = rand((9, 256), 1).to(DEV)

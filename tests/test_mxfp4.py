@@ -402,6 +402,21 @@ def test_a_frozen_weight_s_linear_has_no_backward_and_says_so(gpu, m):
     assert torch.equal(module(x), want)
 
 
+@pytest.mark.gpu
+def test_forward_mode_is_refused(gpu):
+    from torch.autograd import forward_ad as fw
+    x, w = rand((4, 64), 1).to(DEV), xk.quantize_mxfp4(rand((32, 64), 2).to(DEV))
+    bias = torch.zeros(32, device=DEV)
+    with fw.dual_level():
+        dual = lambda v: fw.make_dual(v, torch.ones_like(v))  # noqa: E731
+        for call in (lambda: xk.linear_mxfp4(dual(x), w, rotate=False), lambda: xk.linear_mxfp4(x, w, dual(bias), rotate=False),
+                     lambda: xk.mxfp4_linear(dual(x), torch.ones_like(x), rotate=False)):
+            with pytest.raises(RuntimeError, match="jvp|forward AD"):
+                call()
+            with torch.no_grad(), pytest.raises(RuntimeError, match="jvp|forward AD"):
+                call()
+
+
 # ------------------------------------------------------------------------- matrices whose memory changes
 
 @pytest.mark.gpu
