@@ -161,7 +161,7 @@ def mxfp4_expert_linear(x, w, plan, *, rotate=True, sorted=False):
     _type(w, "w")
     _same_device(w.get_device(), plan, w, "w")
     if plan.rows == 0:
-        return x.reshape(0, x.shape[1]) @ w.sum(0).to(x.dtype).T
+        return x[:0] @ w[0].to(x.dtype).T
     return (mxfp4._native or _load()).expert_train(x, w, plan._buffer, plan.tokens, plan.top, rotate, sorted)
 
 

@@ -452,6 +452,20 @@ def test_a_rotated_expert_gradient_keeps_fp16_s_range(gpu):
     assert torch.equal(dw[1].cpu(), (sign * 6144).to(torch.float16).expand(3, 256)) and not dw[0].any()
 
 
+@pytest.mark.gpu
+def test_tokens_without_a_choice(gpu):
+    plan = xk.expert_sort(torch.zeros((5, 0), dtype=torch.int64, device=DEV), 3)
+    x, w = rand((5, 64), 1).to(DEV).requires_grad_(), rand((3, 32, 64), 2).to(DEV).requires_grad_()
+    for rows, in_order in ((x, False), (x[:0], True)):
+        y = xk.mxfp4_expert_linear(rows, w, plan, rotate=False, sorted=in_order)
+        assert y.shape == (0, 32) and y.dtype == x.dtype
+        dx, dw = torch.autograd.grad(y, (x, w), torch.zeros_like(y))
+        assert dx.shape == x.shape and dw.shape == w.shape and not dx.any() and not dw.any()
+    assert xk.expert_linear_mxfp4(x.detach(), xk.quantize_mxfp4(w), plan, rotate=False).shape == (0, 32)
+    out = xk.expert_combine(xk.expert_gather(x, plan), torch.zeros((5, 0), device=DEV), plan)
+    assert out.shape == (5, 64) and not out.any() and not torch.autograd.grad(out.sum(), x)[0].any()
+
+
 # --------------------------------------------------------------------- what has no gradient says so
 
 @pytest.mark.gpu
