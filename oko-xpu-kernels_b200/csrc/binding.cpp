@@ -149,7 +149,7 @@ struct LinearFn : torch::autograd::Function<LinearFn> {
         const int64_t m = s[0], n = s[1], k = s[2], want = s[4];
         const bool need_x = ctx->needs_input_grad(0), need_w = ctx->needs_input_grad(1), need_b = s[7] >= 0 && ctx->needs_input_grad(2);
         int64_t ld;
-        const Tensor dy = rows(grads[0].reshape({-1, n}), ld);
+        const Tensor dy = rows(grads[0].reshape({m, n}), ld);
         Tensor dx, dw, db;
         if (need_x) dx = empty(shape, scalar_type(s[5]), dy);
         if (need_w) dw = empty({n, k}, scalar_type(s[6]), dy);

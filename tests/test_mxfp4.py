@@ -340,6 +340,17 @@ def test_tokens_over_a_contraction_of_several_turns(gpu, m, n, k, rotate):
             assert torch.equal(xk.linear_mxfp4(x, wq, rotate=rotate), want)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("m,n", [(4, 0), (0, 6), (0, 0)])
+def test_empty_sizes_have_gradients(gpu, m, n):
+    x, w, bias = (torch.zeros(s, device=DEV, requires_grad=True) for s in ((2, m, 256), (n, 256), (n,)))
+    y = xk.mxfp4_linear(x, w, bias)
+    assert y.shape == (2, m, n)
+    grads = torch.autograd.grad(y, (x, w, bias), torch.zeros_like(y))
+    for g, v in zip(grads, (x, w, bias)):
+        assert g.shape == v.shape and not g.any()
+
+
 # ---------------------------------------------------------------------- gradients turned back
 
 def turned_back(ref, spread, terms):
