@@ -140,6 +140,10 @@ struct LinearFn : torch::autograd::Function<LinearFn> {
         }
         if (saved.defined()) ctx->save_for_backward({saved});
         ctx->saved_data["s"] = std::vector<int64_t>{m, n, k, rotate, want, type_of(x), type_of(w), bias.defined() ? static_cast<int64_t>(bias.scalar_type()) : -1};
+        if (bias.defined() && bias.requires_grad()) {
+            ctx->saved_data["b"] = bias.sizes().vec();
+            ctx->saved_data["d"] = bias.device();
+        }
         return y;
     }
 
@@ -162,7 +166,10 @@ struct LinearFn : torch::autograd::Function<LinearFn> {
             if (need_x) dx.zero_();
             if (need_w) dw.zero_();
         }
-        if (need_b) db = dy.sum(at::IntArrayRef{0}, false, at::kFloat).to(static_cast<at::ScalarType>(s[7]));
+        if (need_b) {  // as the bias is: any shape of n values, any type, any device
+            db = dy.sum(at::IntArrayRef{0}, false, at::kFloat).reshape(ctx->saved_data["b"].toIntVector());
+            db = db.to(ctx->saved_data["d"].toDevice(), static_cast<at::ScalarType>(s[7]));
+        }
         return once({dx, dw, db, Tensor(), Tensor()}, grads);
     }
 };

@@ -351,6 +351,19 @@ def test_empty_sizes_have_gradients(gpu, m, n):
         assert g.shape == v.shape and not g.any()
 
 
+@pytest.mark.gpu
+def test_a_bias_s_gradient_is_the_bias_s_own(gpu):
+    """Of its shape, its type and its device: any bias that the forward call takes."""
+    x, w, dy = rand((7, 64), 1).to(DEV), rand((48, 64), 2).to(DEV), rand((7, 48), 3).to(DEV)
+    want = dy.float().sum(0)
+    for bias in (torch.zeros(48), torch.zeros((1, 48), device=DEV), torch.zeros((48, 1), device=DEV, dtype=torch.float16)):
+        bias.requires_grad_()
+        y = xk.mxfp4_linear(x, w, bias, rotate=False)
+        g, = torch.autograd.grad(y, bias, dy)
+        assert g.shape == bias.shape and g.dtype == bias.dtype and g.device == bias.device
+        assert torch.equal(g.reshape(-1), want.to(device=bias.device, dtype=bias.dtype))
+
+
 # ---------------------------------------------------------------------- gradients turned back
 
 def turned_back(ref, spread, terms):
