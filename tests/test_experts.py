@@ -390,6 +390,66 @@ def test_no_tokens(gpu):
     assert xk.expert_combine(y, torch.zeros((0, 2), device=DEV), plan).shape == (0, 32)
 
 
+# ----------------------------------------------------------------------------- many tiles a CTA pair
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("tokens,in_order,n,k,rotate", [(8192, False, 2816, 2048, True), (4500, True, 2816, 2048, True), (8192, True, 2305, 2000, False),
+                                                        (4500, False, 2820, 1999, False)])
+def test_products_of_many_tiles(gpu, tokens, in_order, n, k, rotate, dtype):
+    """More tiles a CTA pair than it has accumulators, two experts without rows among the others, several
+    k-blocks an expert in dw, and operands of two and four 32-row steps a CTA of the kernel that
+    quantises along both axes.  Against 64-bit products of operands quantised one axis at a time."""
+    experts, top = 8, 2
+    rows = tokens * top
+    ids = torch.from_numpy(routing(tokens, top, experts, 8, 0.05, used=[0, 1, 3, 4, 6, 7])).to(DEV)
+    plan = xk.expert_sort(ids, experts)
+    offsets = plan.offsets.tolist()
+    x, w, dy = rand((rows if in_order else tokens, k), 1, dtype), rand((experts, n, k), 2, dtype, 0.1), rand((rows, n), 3, dtype, 0.1).to(DEV)
+    xd, wd = x.to(DEV).requires_grad_(), w.to(DEV).requires_grad_()
+    y = xk.mxfp4_expert_linear(xd, wd, plan, rotate=rotate, sorted=in_order)
+    dx, dw = torch.autograd.grad(y, (xd, wd), dy)
+    assert torch.equal(y, xk.mxfp4_expert_linear(xd, wd, plan, rotate=rotate, sorted=in_order))
+    xr, wr = (turned(v).to(DEV) if rotate else v.to(DEV) for v in (x, w))
+    xs = xr if in_order else xr[plan.order.long() // top]
+    h = torch.from_numpy(O.hadamard_matrix()).to(DEV).double()
+
+    def held(v, transpose=False):
+        return xk.dequantize_mxfp4(xk.quantize_mxfp4(v, transpose=transpose), dtype=torch.float32).double()
+
+    def groups(v, m):
+        return (v.reshape(-1, 256) @ m).reshape(v.shape)
+
+    def within(got, ref, lost):
+        """`lost`: what 32 bits lose before the rotation back, if there is one, and the one rounding."""
+        if rotate and got is not y:
+            ref, lost = groups(ref, h), groups(lost, h.abs()) + 16 * 2.0 ** -24 * groups(ref.abs() + lost, h.abs())
+        off = (got.double() - ref).abs() - lost * (1 + ROUND[dtype]) - ROUND[dtype] * ref.abs() - SMALL[dtype]
+        assert bool((off <= 0).all()), f"{int((off > 0).sum())} past the bound, by {float(off.max())}"
+
+    def product(a, b, terms):
+        ref = a @ b.T
+        return ref, (terms / 64 + 10) * 2.0 ** -23 * (a.abs() @ b.abs().T) + 2.0 ** -24 * ref.abs()
+
+    want, lost = (torch.zeros((rows, n), dtype=torch.float64, device=DEV) for _ in range(2))
+    gx, lost_x = (torch.zeros((rows, k), dtype=torch.float64, device=DEV) for _ in range(2))
+    for e in range(experts):
+        r = slice(offsets[e], offsets[e + 1])
+        if r.start == r.stop:
+            assert not dw[e].any()
+            continue
+        want[r], lost[r] = product(held(xs[r]), held(wr[e]), k)
+        gx[r], lost_x[r] = product(held(dy[r]), held(wr[e], True), n)
+        within(dw[e], *product(held(dy[r], True), held(xs[r], True), r.stop - r.start))
+    within(y, want, lost)
+    if not in_order:
+        taken = torch.arange(rows, device=DEV) < offsets[-1]
+        token = plan.order.long()[taken] // top
+        gx, lost_x, size = (torch.zeros((tokens, k), dtype=torch.float64, device=DEV).index_add_(0, token, v[taken]) for v in (gx, lost_x, gx.abs() + lost_x))
+        lost_x = lost_x + top * 2.0 ** -24 * size
+    within(dx, gx, lost_x)
+
+
 # ------------------------------------------------------------------ the experts' gradients, rounded once
 
 @pytest.mark.gpu

@@ -364,6 +364,64 @@ def test_a_bias_s_gradient_is_the_bias_s_own(gpu):
         assert torch.equal(g.reshape(-1), want.to(device=bias.device, dtype=bias.dtype))
 
 
+# ----------------------------------------------------------------------------- many tiles a CTA pair
+
+def held(q):
+    """What q stands for, in 64 bits on the GPU."""
+    return xk.dequantize_mxfp4(q, dtype=torch.float32).double()
+
+
+def check_gpu(got, ref, spread, k, dtype):
+    bound = ((k / 64 + 10) * 2.0 ** -23) * spread + ROUND[dtype] * (ref.abs() + spread * 2.0 ** -20) + SMALL[dtype]
+    off = (got.double() - ref).abs() - bound
+    assert got.shape == ref.shape and bool((off <= 0).all()), f"{int((off > 0).sum())} past the bound, by {float(off.max())}"
+
+
+#: 17 x 20 (21) tiles of 256 x 256, 15 x 9 of 256 x 128 and 149 of 256 x 128 on 74 pairs, with fewer k-blocks a tile
+#: than stages, as many, and more; N across the columns that both accumulators use; odd rows of the output
+MANY_TILES = [(4097, 5120, 64, True), (4097, 5121, 288, False), (4097, 5120, 1280, True), (4097, 5121, 1280, True), (4097, 5118, 2560, False),
+              (3840, 1152, 1280, True), (38017, 120, 320, False)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m,n,k,with_bias", MANY_TILES)
+def test_products_of_many_tiles(gpu, m, n, k, with_bias):
+    g = torch.Generator(device=DEV).manual_seed(m + n + k)
+    a, b = (xk.quantize_mxfp4(torch.randn((r, k), generator=g, device=DEV)) for r in (m, n))
+    bias = torch.randn(n, generator=g, device=DEV) if with_bias else None
+    va, vb = held(a), held(b)
+    ref, spread = va @ vb.T, va.abs() @ vb.abs().T
+    if with_bias:
+        ref, spread = ref + bias.double(), spread + bias.double().abs()
+    for dtype in TYPES:
+        y = xk.mxfp4_mm(a, b, bias, dtype=dtype)
+        check_gpu(y, ref, spread, k, dtype)
+        for _ in range(5):
+            assert torch.equal(xk.mxfp4_mm(a, b, bias, dtype=dtype), y)
+
+
+# ------------------------------------------------------------------ operands quantised along both axes
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("m,n,k,rotate", [(4097, 200, 5120, True), (4100, 200, 5100, False), (8200, 130, 4096, True), (8129, 130, 4095, False),
+                                          (130, 4097, 5120, True), (130, 8200, 4099, False)])
+def test_large_operands_are_the_single_quantisers_(gpu, m, n, k, rotate, dtype):
+    """x and w large enough for two and four 32-row steps a CTA of the kernel that quantises along both
+    axes: the products' bits are those of operands quantised one axis at a time."""
+    x, w, dy = rand((m, k), 1, dtype), rand((n, k), 2, dtype, 0.02), rand((m, n), 3, dtype, 0.1).to(DEV)
+    xd, wd = x.to(DEV).requires_grad_(), w.to(DEV).requires_grad_()
+    y = xk.mxfp4_linear(xd, wd, rotate=rotate)
+    dx, dw = torch.autograd.grad(y, (xd, wd), dy)
+    xr, wr = (turned(v).to(DEV) if rotate else v.to(DEV) for v in (x, w))
+    quant = xk.quantize_mxfp4
+    assert torch.equal(y, xk.mxfp4_mm(quant(xr), quant(wr), dtype=dtype))
+    want_dx = xk.mxfp4_mm(quant(dy), quant(wr, transpose=True), dtype=torch.float32 if rotate else dtype)
+    want_dw = xk.mxfp4_mm(quant(dy, transpose=True), quant(xr, transpose=True), dtype=torch.float32 if rotate else dtype)
+    for got, want in ((dx, want_dx), (dw, want_dw)):
+        assert torch.equal(got.cpu(), turned(want.cpu()).to(dtype) if rotate else want.cpu())
+
+
 # ---------------------------------------------------------------------- gradients turned back
 
 def turned_back(ref, spread, terms):
