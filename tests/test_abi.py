@@ -61,3 +61,17 @@ def test_the_python_binding_declares_every_entry_point():
 def test_group_size_needs_no_device(lib):
     lib.xpuint8_convrot_groupsize.restype = ctypes.c_int
     assert lib.xpuint8_convrot_groupsize() == 256
+
+
+@pytest.mark.parametrize("torch", [False, True])
+def test_the_library_builds_with_and_without_torch(tmp_path, torch):
+    """A C caller has nvcc but no torch: the library is built and the binding left out with a message."""
+    import subprocess
+    python = tmp_path / "python"
+    python.write_text(f'#!/bin/sh\ncase "$1" in -c) exit {0 if torch else 1};; *) touch "$3";; esac\n')
+    python.chmod(0o755)
+    binding = tmp_path / "_native.so"
+    made = subprocess.run(["make", "-C", os.path.join(ROOT, "oko-xpu-kernels_b200", "csrc"), "NVCC=true", f"PYTHON={python}", f"BUILD={tmp_path}/build",
+                           f"OUT={tmp_path}/lib.so", f"BINDING={binding}"], capture_output=True, text=True)
+    assert made.returncode == 0, made.stderr
+    assert binding.exists() == torch and ("left out" in made.stdout) == (not torch)
