@@ -531,7 +531,8 @@ __global__ void __launch_bounds__(PairCfg<BN>::kThreads, 1)
             const int left = t.rows - row0;                                // rows of this warp that exist
             const int acc = count & 1;
             if (t.nk > 0) {
-                if (!mbar_wait(TFULL(acc), (count >> 1) & 1, fault, 105)) break;
+                // one answer for the warp: the TMEM loads and the cluster barrier below are .aligned
+                if (!warp_wait(TFULL(acc), (count >> 1) & 1, fault, 105)) break;
                 tc_fence_after();
             }
             const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + static_cast<uint32_t>(acc ? C::kAccCol1 : 0);

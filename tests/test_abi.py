@@ -75,3 +75,13 @@ def test_the_library_builds_with_and_without_torch(tmp_path, torch):
                            f"OUT={tmp_path}/lib.so", f"BINDING={binding}"], capture_output=True, text=True)
     assert made.returncode == 0, made.stderr
     assert binding.exists() == torch and ("left out" in made.stdout) == (not torch)
+
+
+def test_the_mxfp4_products_wait_by_whole_warps():
+    """A wait that gives up may do so on some lanes only, and what follows in these kernels wants all of
+    them: every wait goes through the one that gives all lanes the same answer."""
+    text = open(os.path.join(ROOT, "oko-xpu-kernels_b200", "csrc", "gemm_mx4.cu")).read()
+    text = re.sub(r"//.*", "", text)
+    wait = re.search(r"bool warp_wait\(.*?\n}\n", text, flags=re.S).group()
+    assert "__all_sync(0xFFFFFFFFu, mbar_wait(" in wait
+    assert not re.search(r"\bmbar_wait\(", text.replace(wait, ""))
