@@ -20,7 +20,7 @@
  * Return codes: 0 ok; 1 no usable device; 2 bad size, null pointer or
  * misalignment; 3 K (or the FFN inner width) not a multiple of 256; 4
  * unsupported group count (K > 32768); 5 kernel launch failure; 6 bad
- * activation id.  The message is in xpuint8_last_error() (per thread).
+ * activation id; 7 an earlier MXFP4 product gave up a wait on the device.  The message is in xpuint8_last_error() (per thread).
  */
 #ifndef XPU_INT8_H
 #define XPU_INT8_H
@@ -231,6 +231,12 @@ int xpuint8_fault_status(int32_t reset);
  * reference, whose failure model is the return code and last-error text
  * (src/xpuint8.cpp:47-50). */
 int xpuint8_wait_probe(int64_t limit_ns, int32_t site, int64_t *elapsed_ns);
+
+/* The same for the MXFP4 products' wait, in their fault word: after it they are
+ * refused (code 7), as after a wait of their own that gave up and left an
+ * output incomplete, until xpuint8_fault_status(1).  A replayed graph is not
+ * refused: its caller asks xpuint8_fault_status. */
+int xpuint8_mxfp4_wait_probe(int64_t limit_ns, int32_t site);
 
 /* The N-sharded INT8 linear with its output all-gather fused into the GEMM
  * (BASELINE config C5's large-weight variant; the reference has no

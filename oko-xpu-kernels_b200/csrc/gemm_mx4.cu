@@ -23,12 +23,13 @@
 // instruction descriptor names.
 //
 // Every mbarrier wait is bounded (common.cuh: mbar_wait); on a timeout the kernel records the site
-// in g_mx4_fault, drains its own TMA loads and MMAs, frees its TMEM and returns.  No load uses
-// cluster multicast.
+// in g_mx4_fault and in the host's word, drains its own TMA loads and MMAs, frees its TMEM and returns;
+// its output is not complete, and the next call is refused.  No load uses cluster multicast.
 #include <cuda.h>
 
 #include <algorithm>
 #include <atomic>
+#include <mutex>
 #include <string>
 
 #include "internal.h"
@@ -80,14 +81,28 @@ __device__ __forceinline__ void umma_mx4(uint32_t d, uint64_t a, uint64_t b, uin
             : "memory");
 }
 
+// Where a wait that gives up leaves its site (0: one that gave up because another had): the device's word,
+// which makes the other waits give up too, and the host's, which the next call reads.  Not inlined: in the
+// few-row kernel, whose CTAs are short, the code itself costs time (16 tokens, 4 of 64 experts 28.5 us, 29.9 inlined).
+__device__ __noinline__ void record_fault(int *word, int *host, int site) {
+    if (site) atomicCAS(word, 0, site);
+    const int first = *reinterpret_cast<volatile int *>(word);
+    *reinterpret_cast<volatile int *>(host) = first ? first : 196;
+    __threadfence_system();
+}
+struct Fault {
+    int *word, *host;
+    __device__ __forceinline__ void at(int site) const { record_fault(word, host, site); }
+};
+
 // bounded wait that ignores other threads' faults: only to drain this CTA's own asynchronous work
-__device__ __forceinline__ void drain_wait(uint32_t bar, uint32_t parity) {
+__device__ __forceinline__ void drain_wait(uint32_t bar, uint32_t parity, const Fault &fault) {
     const uint64_t t0 = global_timer_ns();
     for (uint32_t it = 0; it < kWaitMaxIters; ++it) {
         if (mbar_try_wait(bar, parity)) return;
         if ((it & 255u) == 0u && global_timer_ns() - t0 > kWaitTimeoutNs) break;
     }
-    atomicCAS(&g_mx4_fault, 0, 199);
+    fault.at(199);
 }
 
 // one lane of a converged warp
@@ -97,8 +112,10 @@ __device__ __forceinline__ bool elect_one() {
     return p != 0;
 }
 // mbar_wait by a whole warp: the same answer in every lane
-__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, int *fault, int site) {
-    return __all_sync(0xFFFFFFFFu, mbar_wait(bar, parity, fault, site));
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, const Fault &fault, int site, uint64_t timeout_ns = kWaitTimeoutNs) {
+    if (__all_sync(0xFFFFFFFFu, mbar_wait(bar, parity, fault.word, site, timeout_ns))) return true;
+    fault.at(0);
+    return false;
 }
 
 // ------------------------------------------------------------------------------------- pair kernel
@@ -122,6 +139,7 @@ struct PairArgs {
     int64_t rows;                     // rows: D's rows, the ones of no expert among them
     int tma_out;                      // D can be stored by the TMA unit
     int b_early;                      // B is not written by the kernel before this one
+    int *host_fault;
 };
 
 template <int BN>
@@ -323,7 +341,7 @@ __global__ void __launch_bounds__(PairCfg<BN>::kThreads, 1)
     constexpr int STAGES = C::kStages;
     extern __shared__ __align__(1024) uint8_t smem[];
     if (smem_u32(smem) & 1023u) {  // the 128-byte swizzle's alignment; the same in both CTAs
-        if (threadIdx.x == 0) atomicCAS(&g_mx4_fault, 0, 198);
+        if (threadIdx.x == 0) Fault{&g_mx4_fault, args.host_fault}.at(198);
         return;
     }
     const uint32_t sA = smem_u32(smem);
@@ -344,7 +362,7 @@ __global__ void __launch_bounds__(PairCfg<BN>::kThreads, 1)
     static_assert(8 * (2 * STAGES + 8) <= 256, "barriers");
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    int *fault = &g_mx4_fault;
+    const Fault fault{&g_mx4_fault, args.host_fault};
     const uint32_t rank = cluster_rank();
     const bool leader = rank == 0;
     const int pair = static_cast<int>(cluster_index()), npairs = static_cast<int>(cluster_count());
@@ -446,7 +464,7 @@ __global__ void __launch_bounds__(PairCfg<BN>::kThreads, 1)
         // every load has landed once the MMAs that read it are done
         for (uint32_t s = 0; s < static_cast<uint32_t>(STAGES) && s < issued; ++s) {
             const uint32_t last = s + ((issued - 1 - s) / STAGES) * STAGES;
-            drain_wait(EMPTY(s), (last / STAGES) & 1u);
+            drain_wait(EMPTY(s), (last / STAGES) & 1u, fault);
         }
     } else if (warp == 1) {
         if (leader) {
@@ -503,7 +521,7 @@ __global__ void __launch_bounds__(PairCfg<BN>::kThreads, 1)
             }
             if (elect_one()) umma_commit_pair(final_bar);
             __syncwarp();
-            drain_wait(final_bar, 0);
+            drain_wait(final_bar, 0, fault);
         }
     } else {
         // ---------------------------------------------------------- drain (both CTAs)
@@ -623,18 +641,21 @@ __global__ void __launch_bounds__(PairCfg<BN>::kThreads, 1)
 // -------------------------------------------------------------------------------------- few kernel
 
 // Waits until the count at `at` in shared memory is over `n`; bounded as mbar_wait is.
-__device__ __forceinline__ bool count_wait(uint32_t at, int n, int *fault, int site) {
+__device__ __forceinline__ bool count_wait(uint32_t at, int n, const Fault &fault, int site) {
     const uint64_t t0 = global_timer_ns();
     for (uint32_t it = 1; it < kWaitMaxIters; ++it) {
         int v;
         asm volatile("ld.acquire.cta.shared::cta.b32 %0, [%1];" : "=r"(v) : "r"(at) : "memory");
         if (v > n) return true;
         if ((it & 255u) == 0u) {
-            if (*reinterpret_cast<volatile int *>(fault) != 0) return false;
+            if (*reinterpret_cast<volatile int *>(fault.word) != 0) {
+                fault.at(0);
+                return false;
+            }
             if (global_timer_ns() - t0 > kWaitTimeoutNs) break;
         }
     }
-    atomicCAS(fault, 0, site);
+    fault.at(site);
     return false;
 }
 
@@ -656,6 +677,7 @@ struct FewArgs {
     const int32_t *order;            // FUSE, rows: row r is slot order[r]'s token (fan > 0) or x's row r
     int fan;
     int vec_out;                     // four neighbouring outputs are aligned to their bytes
+    int *host_fault;
 };
 
 enum Fuse { kFuseNone = 0, kFusePlain = 1, kFuseRotate = 2 };
@@ -695,14 +717,14 @@ __global__ void __launch_bounds__(kFewThreads, 2)
     using C = FewCfg<FUSE>;
     extern __shared__ __align__(1024) uint8_t smem[];
     if (smem_u32(smem) & 1023u) {
-        if (threadIdx.x == 0) atomicCAS(&g_mx4_fault, 0, 197);
+        if (threadIdx.x == 0) Fault{&g_mx4_fault, args.host_fault}.at(197);
         return;
     }
     uint32_t splits;
     asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(splits));
     const uint32_t rank = cluster_rank();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    int *fault = &g_mx4_fault;
+    const Fault fault{&g_mx4_fault, args.host_fault};
     const int nb = blockIdx.x / static_cast<int>(splits);
     int e = 0, x_row, x_sf = blockIdx.y, count;
     if (args.mode == kRows) {
@@ -801,7 +823,7 @@ __global__ void __launch_bounds__(kFewThreads, 2)
         const uint32_t n = static_cast<uint32_t>(stages);
         for (uint32_t s = 0; s < n && s < issued; ++s) {
             const uint32_t last = s + ((issued - 1 - s) / n) * n;
-            drain_wait(EMPTY(s), (last / n) & 1u);
+            drain_wait(EMPTY(s), (last / n) & 1u, fault);
         }
     } else if (warp == 1) {
         const uint32_t idesc[2] = {idesc_mx4(128, nt, 0), idesc_mx4(128, nt, 1)};
@@ -833,7 +855,7 @@ __global__ void __launch_bounds__(kFewThreads, 2)
         }
         if (elect_one()) umma_commit(done);
         __syncwarp();
-        drain_wait(done, 0);
+        drain_wait(done, 0, fault);
     } else if constexpr (FUSE != kFuseNone) {
         // task t: k-block k0 + t / pairs, rows 2 (t % pairs) and the next; eight slots, task by task,
         // so every stage is freed by k-blocks whose tasks come earlier
@@ -975,7 +997,49 @@ __global__ void __launch_bounds__(kFewThreads, 2)
     cluster_sync();  // the others have read this CTA's parts
 }
 
+// One warp waits on a barrier that nothing arrives on: the products' own wait, made to give up.
+__global__ void wait_probe_kernel(uint64_t limit_ns, int site, int *host_fault) {
+    __shared__ __align__(8) uint64_t bar;
+    const uint32_t b = smem_u32(&bar);
+    if (threadIdx.x == 0) {
+        mbar_init(b, 1);
+        fence_mbar_init();
+    }
+    __syncwarp();
+    warp_wait(b, 0, Fault{&g_mx4_fault, host_fault}, site, limit_ns);
+}
+
 // -------------------------------------------------------------------------------------------- host
+
+// The host's fault word: memory of this library's that the devices write, zero while no wait has given up.
+// Its mapping is asked for at every launch, so that a reset of the device only costs another registration.
+alignas(4096) volatile int g_host_fault[1024];
+
+// the devices' address of it, or null with the error recorded
+int *host_fault() {
+    void *host = const_cast<int *>(g_host_fault), *p = nullptr;
+    if (cudaHostGetDevicePointer(&p, host, 0) == cudaSuccess) return static_cast<int *>(p);
+    cudaGetLastError();
+    static std::mutex one;
+    const std::lock_guard<std::mutex> lock(one);
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;  // no part of a graph that may be being captured
+    cudaThreadExchangeStreamCaptureMode(&mode);
+    cudaHostRegister(host, sizeof(g_host_fault), cudaHostRegisterPortable | cudaHostRegisterMapped);
+    cudaThreadExchangeStreamCaptureMode(&mode);
+    cudaGetLastError();
+    if (cudaHostGetDevicePointer(&p, host, 0) == cudaSuccess) return static_cast<int *>(p);
+    launch_status("mxfp4 (the fault word's registration)");
+    return nullptr;
+}
+
+// 0, or 7 with the error recorded: outputs since the fault are not complete
+int earlier_fault() {
+    const int site = g_host_fault[0];
+    if (!site) return 0;
+    set_error("mxfp4: an earlier product gave up a wait on the device (site " + std::to_string(site) +
+              "); outputs since then are not complete.  xpuint8_fault_status(1) clears it");
+    return 7;
+}
 
 struct Operand {
     const uint8_t *codes, *scales;
@@ -1066,6 +1130,8 @@ int launch_pair_type(cudaStream_t s, const PairMaps &m, const PairArgs &a, int64
 
 // `a` complete but for the tile counts; max_m: 256-row tiles (rows: at most)
 int run_pair(cudaStream_t s, PairArgs a, const Operand &A, const Operand &B, int type, int64_t out_rows, int64_t max_m) {
+    if (int rc = earlier_fault()) return rc;
+    if (!(a.host_fault = host_fault())) return 5;
     // 256 or 128 columns a tile, by the rounds that the pairs take.  A k-block takes 0.32 us at 256
     // columns and nearly as long at 128 (0.9 of it: an MMA's time hardly depends on its columns), and a
     // tile costs its hand-over and the end of its drain, 7.5 k-blocks' time at 256 columns and 5 at
@@ -1128,6 +1194,8 @@ int launch_few(cudaStream_t s, const CUtensorMap &w, const CUtensorMap &sw, cons
 // X tokens (null where they are quantised in the kernel), W weight rows; slots: 128-token tiles (rows:
 // at most)
 int run_few(cudaStream_t s, FewArgs a, const Operand *X, const Operand &W, int type, int64_t slots, int fuse) {
+    if (int rc = earlier_fault()) return rc;
+    if (!(a.host_fault = host_fault())) return 5;
     if (slots > 65535) {
         set_error("mxfp4_mm: too many token tiles");
         return 2;
@@ -1311,9 +1379,11 @@ int mx4_fault_status(int reset) {
         set_error("could not read the MXFP4 product's fault word");
         return -1;
     }
+    if (!v) v = g_host_fault[0];  // another device's
     if (reset && v) {
         const int zero = 0;
         cudaMemcpyToSymbol(g_mx4_fault, &zero, sizeof(int));
+        g_host_fault[0] = 0;
     }
     return v;
 }
@@ -1323,6 +1393,20 @@ int mx4_fault_status(int reset) {
 using namespace xpuint8;
 
 extern "C" {
+
+int xpuint8_mxfp4_wait_probe(int64_t limit_ns, int32_t site) {
+    if (site == 0) {
+        set_error("mxfp4_wait_probe: the site must not be 0");
+        return 2;
+    }
+    int *const host = host_fault();
+    if (!host) return 5;
+    // at least 1 us, at most the products' own limit
+    const int64_t limit = std::min(std::max<int64_t>(limit_ns, 1000), static_cast<int64_t>(kWaitTimeoutNs));
+    wait_probe_kernel<<<1, 32>>>(static_cast<uint64_t>(limit), site, host);
+    if (const int rc = launch_status("mxfp4_wait_probe")) return rc;
+    return cudaStreamSynchronize(nullptr) == cudaSuccess ? 0 : launch_status("mxfp4_wait_probe");
+}
 
 int xpuint8_mxfp4_mm_stream(const void *stream, const uint8_t *a_codes, const uint8_t *a_scales,
                             const uint8_t *b_codes, const uint8_t *b_scales, const float *bias,

@@ -94,6 +94,7 @@ def _signatures():
         "xpuint8_ipc_close": [vp],
         "xpuint8_ipc_free": [vp],
         "xpuint8_linear_noalloc_stream": [vp] * 6 + [i64] * 3 + [i32],
+        "xpuint8_mxfp4_wait_probe": [i64, i32],
         "xpuint8_mxfp4_quantize_stream": [vp, vp, i32, i64] + [vp] * 3 + [i64] * 3 + [i32],
         "xpuint8_mxfp4_quantize_sorted_stream": [vp, vp, i32, i64] + [vp] * 6 + [i64] * 3 + [i32],
         "xpuint8_mxfp4_quantize_columns_stream": [vp, vp, i32, i64, vp, vp] + [i64] * 3 + [vp] * 2

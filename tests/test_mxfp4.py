@@ -550,6 +550,56 @@ def test_copies_of_a_matrix_are_their_own(gpu):
         assert c.shape == q.shape and torch.equal(xk.linear_mxfp4(x, c), want)
 
 
+# ------------------------------------------------------------------------------ a wait that gives up
+
+@pytest.mark.gpu
+def test_products_after_a_fault_are_refused_until_it_is_cleared(gpu):
+    """One wait of the products' own runs out on a barrier that nothing arrives on; what would be left
+    unwritten since then is an error, not a result."""
+    from xpu_kernels.int8 import _lib as L
+    lib = L.load()
+    x, w, dy = rand((40, 256), 1).to(DEV), rand((96, 256), 2).to(DEV), rand((40, 96), 3).to(DEV)
+    q, ids = xk.prepare_weight_mxfp4(w), torch.zeros((40, 1), dtype=torch.int32, device=DEV)
+    stack, plan = xk.prepare_weight_mxfp4(w[None]), xk.expert_sort(ids, 1)
+    xg = x.clone().requires_grad_()
+    y = xk.mxfp4_linear(xg, w)
+    calls = [lambda: xk.linear_mxfp4(x, q), lambda: xk.linear_mxfp4(x[:1], q), lambda: xk.mxfp4_mm(q, q), lambda: xk.expert_linear_mxfp4(x, stack, plan),
+             lambda: xk.mxfp4_expert_linear(x, w[None], plan), lambda: torch.autograd.grad(y, xg, dy, retain_graph=True)[0]]
+    want = [call() for call in calls]
+    assert lib.xpuint8_mxfp4_wait_probe(200_000, 0) == 2
+    assert lib.xpuint8_mxfp4_wait_probe(200_000, 77) == 0
+    for call in calls:
+        with pytest.raises(RuntimeError, match=r"gave up a wait on the device \(site 77\)"):
+            call()
+    xk.dequantize_mxfp4(q)  # no product
+    assert lib.xpuint8_fault_status(0) == 77 and lib.xpuint8_fault_status(1) == 77 and lib.xpuint8_fault_status(0) == 0
+    for call, value in zip(calls, want):
+        assert torch.equal(call(), value)
+
+
+@pytest.mark.gpu
+def test_the_first_product_may_be_a_captured_one(gpu):
+    """Its preparations on the host are no part of the graph."""
+    import os
+    import subprocess
+    import sys
+    code = """
+import torch, xpu_kernels as xk
+x = torch.ones((3, 256), device="cuda", dtype=torch.bfloat16)
+w = xk.prepare_weight_mxfp4(torch.ones((32, 256), device="cuda", dtype=torch.bfloat16))
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    y = xk.linear_mxfp4(x, w)
+graph.replay()
+torch.cuda.synchronize()
+assert torch.equal(y, xk.linear_mxfp4(x, w)) and y[0, 0] == 256
+"""
+    path = os.pathsep.join([os.path.dirname(os.path.dirname(xk.__file__)), os.environ.get("PYTHONPATH", "")])
+    done = subprocess.run([sys.executable, "-c", code], env={**os.environ, "PYTHONPATH": path}, capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0, done.stderr
+
+
 # ------------------------------------------------------------------------------ streams and graphs
 
 @pytest.mark.gpu
