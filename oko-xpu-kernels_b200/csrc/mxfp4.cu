@@ -355,7 +355,7 @@ __global__ void __launch_bounds__(kBothThreads, T == kMxF32 ? 2 : ROT ? 4 : 3) q
                 if (one) *reinterpret_cast<uint32_t *>(scales) = q.w0;
                 if (two) *reinterpret_cast<uint32_t *>(scales + 16) = q.w1;
             }
-            codes += a.KB * 512;
+            codes += static_cast<int64_t>(a.KB) * 512;
             scales += 4;
         }
         __syncwarp();

@@ -159,6 +159,20 @@ def test_offsets_past_32_bits(gpu):
     assert torch.equal(xk.dequantize_mxfp4(q)[-3:], xk.dequantize_mxfp4(xk.quantize_mxfp4(tail)))
 
 
+@pytest.mark.gpu
+def test_rows_of_codes_whose_steps_pass_32_bits(gpu):
+    """32 rows of codes are 2^32 bytes: the second 32-row step of the kernel that quantises along both axes."""
+    k = 2 ** 28
+    x, w = torch.zeros((1, k), dtype=torch.bfloat16, device=DEV), torch.zeros((33, k), dtype=torch.bfloat16, device=DEV)
+    x[0, 5], x[0, 7], w[0, 5], w[32, 7] = 2, 3, 1, 1
+    y = xk.mxfp4_linear(x.requires_grad_(), w, rotate=False)
+    want = torch.zeros(33)
+    want[0], want[32] = 2, 3
+    assert torch.equal(y[0].float().cpu(), want)
+    del x, w, y
+    torch.cuda.empty_cache()
+
+
 # ------------------------------------------------------------------------------------- products
 
 PRODUCTS = [(1, 1, 1), (1, 128, 256), (1, 300, 4096), (2, 77, 100), (16, 128, 32), (17, 129, 288), (33, 64, 544),
