@@ -96,5 +96,5 @@ __all__ = [
     "MXFP4", "Mxfp4Linear", "TrainableMxfp4Linear", "dequantize_mxfp4", "linear_mxfp4",
     "mxfp4_linear", "mxfp4_mm", "prepare_weight_mxfp4", "quantize_mxfp4",
     "ExpertPlan", "expert_combine", "expert_ffn_mxfp4", "expert_gather", "expert_linear_mxfp4",
-    "expert_sort", "expert_ffn_mxfp4", "mxfp4_expert_linear",
+    "expert_sort", "mxfp4_expert_linear",
 ]
